@@ -20,6 +20,8 @@ __all__ = [
     "attn_sharded",
     "shard_range", "set_split", "set_schedule", "plan_split", "plan_schedule", "query_split",
     "set_correction",
+    "PagedCache", "BlockPool", "BlockPlan", "CacheBatch", "block_tables", "block_trim",
+    "cache_append", "attn_cached",
 ]
 
 ERR = {
@@ -82,11 +84,22 @@ def lib() -> ctypes.CDLL:
                                          ctypes.POINTER(ctypes.c_double)]
         L.attn_plan_split.argtypes = [ll, i, ll, i, ctypes.POINTER(i), llp, llp]
         L.attn_query_split.argtypes = [i, i, i, i, i, i, i, ctypes.POINTER(i), llp, llp, u64p]
+        f, ull = ctypes.c_float, ctypes.c_ulonglong
+        L.attn_block_tables.argtypes = [vp, vp, i, vp, i, ll, vp, vp, i, i, vp, vp, vp, i, vp, vp,
+                                        vp]
+        L.attn_block_trim.argtypes = [vp, vp, i, vp, i, ll, vp, vp, i, i, vp, vp, vp, vp]
+        L.attn_cache_append.argtypes = [vp, ll, ll, vp, ll, ll, vp, i, i, i, i, vp, vp, vp, vp, i,
+                                        i, i, vp]
+        L.attn_cached.argtypes = [vp, ll, ll, vp, ll, ll, i, i, i, i, i, vp, vp, vp, vp, i, i, i,
+                                  vp, i, ll, vp, vp, i, i, i, f, vp, ull, vp]
+        L.attn_cached_workspace.argtypes = [i, i, i, i, ctypes.POINTER(ull)]
         for name in ("attn_fwd", "attn_fwd_padded", "attn_fwd_profiled", "attn_fwd_sharded",
                      "attn_shard_range", "attn_get_status", "attn_query_config",
                      "attn_profile_layout", "attn_debug_fault", "attn_version",
                      "attn_set_split", "attn_plan_split", "attn_query_split",
-                     "attn_set_schedule", "attn_plan_schedule", "attn_set_correction"):
+                     "attn_set_schedule", "attn_plan_schedule", "attn_set_correction",
+                     "attn_block_tables", "attn_block_trim", "attn_cache_append", "attn_cached",
+                     "attn_cached_workspace"):
             getattr(L, name).restype = ctypes.c_int
         _lib = L
     return _lib
@@ -283,3 +296,17 @@ def shard_range(units: int, n_dev: int, g: int) -> tuple[int, int]:
     _check(lib().attn_shard_range(units, n_dev, g, ctypes.byref(b), ctypes.byref(e)),
            "attn_shard_range")
     return b.value, e.value
+
+
+_CACHE_NAMES = ("PagedCache", "BlockPool", "BlockPlan", "CacheBatch", "block_tables", "block_trim",
+                "cache_append", "attn_cached")
+
+
+def __getattr__(name):
+    # The cache's face needs torch, which this module imports only in calls.
+    if name in _CACHE_NAMES:
+        from . import cache
+        for n in _CACHE_NAMES:
+            globals()[n] = getattr(cache, n)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -1,0 +1,390 @@
+"""A paged cache of keys and values held in 8 bits, and attention over it.
+
+Python face of the cache entry points of the C ABI (include/attnprof.h):
+
+  block_tables   block tables and slot maps of a step from request lengths
+  block_trim     blocks of ended or shortened requests back to the pool
+  cache_append   keys and values of new tokens quantised into the cache
+  attn_cached    attention of each request's newest tokens over its cache
+
+and CacheBatch, which runs them together for the requests of a server.  All
+work is asynchronous on `stream` (default: the current stream of the tensors'
+device), never synchronises, and can be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _check, lib
+
+__all__ = ["PagedCache", "BlockPool", "BlockPlan", "CacheBatch", "block_tables", "block_trim",
+           "cache_append", "attn_cached", "BLOCK_SIZES", "BLOCKS", "MAX_BATCH"]
+
+BLOCK_SIZES = (16, 32, 64, 128)
+#: Values of the status word that block_tables and block_trim write.
+BLOCKS = {"OK": 0, "POOL": 1, "ROW": 2, "SLOTS": 3, "NEGATIVE": 4}
+MAX_BATCH = 16384
+_CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_workspace_bytes: dict = {}
+
+
+class _On:
+    """The device and stream of a call: makes the device current inside."""
+    __slots__ = ("index", "stream", "other", "guard")
+
+    def __init__(self, device, stream):
+        self.index = device.index
+        now = torch.cuda.current_device()
+        if stream is None:
+            self.other = None
+            self.stream = torch.cuda.current_stream(device).cuda_stream
+        else:
+            if stream.device != device:
+                raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+            self.other = stream
+            self.stream = stream.cuda_stream
+        self.guard = torch.cuda.device(device) if now != self.index else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return self.stream
+
+    def __exit__(self, *a):
+        if self.guard is not None:
+            self.guard.__exit__(*a)
+
+    def empty(self, shape, dtype, device):
+        """A new tensor for work on this stream, also used by the current one."""
+        if self.other is None:
+            return torch.empty(shape, dtype=dtype, device=device)
+        with torch.cuda.stream(self.other):
+            x = torch.empty(shape, dtype=dtype, device=device)
+        x.record_stream(torch.cuda.current_stream(device))
+        return x
+
+
+def _ints(name, t, device, shape):
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{name} must be int32")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of shape {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _table(tables, device, batch):
+    if tables.dtype is not torch.int32:
+        raise TypeError("tables must be int32")
+    if tables.device != device:
+        raise ValueError(f"tables must be on {device}")
+    if tables.dim() != 2 or tables.shape[0] != batch:
+        raise ValueError(f"tables must be [{batch}, width]")
+    width = tables.shape[1]
+    if (width > 1 and tables.stride(1) != 1) or (batch > 1 and tables.stride(0) < width):
+        raise ValueError("rows of tables must be contiguous and may not overlap")
+    return tables.data_ptr(), width, tables.stride(0) if batch > 1 else width
+
+
+class PagedCache:
+    """Keys and values of one layer in a pool of blocks.
+
+    k, v: codes [num_blocks, kv_heads, block_size, D], float8_e4m3fn or int8;
+    k_scale, v_scale: float32 [num_blocks, kv_heads], all contiguous CUDA
+    tensors of one device.  A code c of block b, head h stands for
+    c * scale[b, h].  The object holds the tensors and nothing else."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "num_blocks", "kv_heads", "block_size", "dim",
+                 "device", "code", "ptrs")
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v must share one [num_blocks, kv_heads, block_size, D] shape "
+                             "and dtype")
+        if k.dtype not in _CODES:
+            raise TypeError(f"unsupported codes {k.dtype} (float8_e4m3fn or int8)")
+        self.num_blocks, self.kv_heads, self.block_size, self.dim = k.shape
+        if self.block_size not in BLOCK_SIZES:
+            raise ValueError(f"block_size {self.block_size} is not one of {BLOCK_SIZES}")
+        if self.dim not in (64, 128):
+            raise ValueError(f"D = {self.dim} is not 64 or 128")
+        if not k.is_cuda:
+            raise ValueError("k must be a CUDA tensor")
+        for name, t in (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.device != k.device:
+                raise ValueError(f"{name} must be on {k.device}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if t.dtype is not torch.float32:
+                raise TypeError(f"{name} must be float32")
+            if t.shape != k.shape[:2]:
+                raise ValueError(f"{name} must be [num_blocks, kv_heads]")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device, self.code = k.device, _CODES[k.dtype]
+        self.ptrs = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+
+    @classmethod
+    def empty(cls, num_blocks: int, kv_heads: int, dim: int, *, block_size: int = 32,
+              dtype=torch.float8_e4m3fn, device="cuda"):
+        """A cache that holds nothing yet."""
+        shape = (num_blocks, kv_heads, block_size, dim)
+        k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        ks, vs = (torch.ones(shape[:2], dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs)
+
+
+class BlockPool:
+    """The free blocks of a pool: the stack free[0 : free_count[0]] of block
+    ids (int32, capacity = the number of blocks)."""
+
+    __slots__ = ("free", "free_count", "block_size", "num_blocks", "device")
+
+    def __init__(self, free, free_count, block_size: int):
+        if not free.is_cuda or free.dim() != 1 or free.numel() == 0:
+            raise ValueError("free must be a CUDA tensor [num_blocks]")
+        if block_size not in BLOCK_SIZES:
+            raise ValueError(f"block_size {block_size} is not one of {BLOCK_SIZES}")
+        self.device, self.num_blocks, self.block_size = free.device, free.numel(), block_size
+        _ints("free", free, self.device, free.shape)
+        _ints("free_count", free_count, self.device, (1,))
+        self.free, self.free_count = free, free_count
+
+    @classmethod
+    def full(cls, num_blocks: int, block_size: int, device="cuda"):
+        """All blocks free, block 0 on top."""
+        free = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=device)
+        return cls(free, torch.full((1,), num_blocks, dtype=torch.int32, device=device),
+                   block_size)
+
+
+class BlockPlan:
+    """What block_tables writes: kv_lens [batch], starts [batch + 1], slots
+    [tokens] and the status word [1] (BLOCKS), all int32."""
+
+    __slots__ = ("kv_lens", "starts", "slots", "status")
+
+    def __init__(self, kv_lens, starts, slots, status):
+        self.kv_lens, self.starts, self.slots, self.status = kv_lens, starts, slots, status
+
+    @classmethod
+    def empty(cls, batch: int, tokens: int, device="cuda"):
+        new = lambda n: torch.empty(n, dtype=torch.int32, device=device)  # noqa: E731
+        return cls(new(batch), new(batch + 1), new(tokens), new(1))
+
+
+def block_tables(pool: BlockPool, lens, new_lens, tables, tokens: int, *, plan=None,
+                 free_left=None, stream=None) -> BlockPlan:
+    """Blocks, slots and lengths of one step: request r holds lens[r] tokens
+    and gets new_lens[r] more.  New blocks come from the pool and are written
+    into `tables` [batch, width]; the rest goes into `plan` (a new one by
+    default; its kv_lens may be `lens`).  `tokens` is the length of the slot
+    map, at least the number of new tokens; behind them slots are -1.
+    pool.free_count becomes what is left, or keeps its value if free_left
+    takes it.  All or nothing: plan.status tells (on the device) whether the
+    pool, the table rows and the slot map were large enough."""
+    device, batch = pool.device, lens.shape[0]
+    on = _On(device, stream)
+    if plan is None:
+        plan = BlockPlan(on.empty(batch, torch.int32, device),
+                         on.empty(batch + 1, torch.int32, device),
+                         on.empty(tokens, torch.int32, device), on.empty(1, torch.int32, device))
+    if free_left is None:
+        free_left = pool.free_count
+    t, width, stride = _table(tables, device, batch)
+    args = (_ints("lens", lens, device, (batch,)), _ints("new_lens", new_lens, device, (batch,)),
+            batch, t, width, stride, pool.free.data_ptr(), pool.free_count.data_ptr(),
+            pool.num_blocks, pool.block_size, _ints("plan.kv_lens", plan.kv_lens, device, (batch,)),
+            _ints("plan.starts", plan.starts, device, (batch + 1,)),
+            _ints("plan.slots", plan.slots, device, (tokens,)), tokens,
+            _ints("free_left", free_left, device, (1,)),
+            _ints("plan.status", plan.status, device, (1,)))
+    with on as s:
+        _check(lib().attn_block_tables(*args, s), "attn_block_tables")
+    return plan
+
+
+def block_trim(pool: BlockPool, lens, keep, tables, *, lens_left=None, free_left=None,
+               status=None, stream=None):
+    """Request r keeps its first min(lens[r], keep[r]) tokens; the blocks
+    behind them go back to the pool.  Writes lens_left (default: `lens`
+    itself) and free_left (default: pool.free_count); returns the status word
+    [1] (BLOCKS; anything but OK: nothing was changed)."""
+    device, batch = pool.device, lens.shape[0]
+    on = _On(device, stream)
+    if lens_left is None:
+        lens_left = lens
+    if free_left is None:
+        free_left = pool.free_count
+    if status is None:
+        status = on.empty(1, torch.int32, device)
+    t, width, stride = _table(tables, device, batch)
+    args = (_ints("lens", lens, device, (batch,)), _ints("keep", keep, device, (batch,)), batch, t,
+            width, stride, pool.free.data_ptr(), pool.free_count.data_ptr(), pool.num_blocks,
+            pool.block_size, _ints("lens_left", lens_left, device, (batch,)),
+            _ints("free_left", free_left, device, (1,)), _ints("status", status, device, (1,)))
+    with on as s:
+        _check(lib().attn_block_trim(*args, s), "attn_block_trim")
+    return status
+
+
+def _rows(name, x, device, heads, dim):
+    """Checks a [tokens, heads, D] tensor; its dtype code."""
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {x.dtype} of {name} (float16 or bfloat16)")
+    if x.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    if x.dim() != 3 or x.shape[2] != dim or (heads and x.shape[1] != heads):
+        raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {dim}]")
+    if x.stride(2) != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    return _DTYPES[x.dtype]
+
+
+def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
+    """Writes k and v [tokens, kv_heads, D] (float16 or bfloat16; slices of a
+    larger projection are fine) into the cache at `slots` [tokens] int32.
+
+    A block's scale per head is the least power of two that holds its largest
+    number; it grows when new tokens need that, and the block's older codes are
+    rounded again.  Negative slots (padding) are skipped.  A number that is not
+    finite makes that block's k_scale NaN for its head.  The tokens of one
+    block follow each other with ascending slots (as block_tables gives them),
+    and no block appears twice."""
+    device = cache.device
+    kind = _rows("k", k, device, cache.kv_heads, cache.dim)
+    if _rows("v", v, device, cache.kv_heads, cache.dim) != kind or v.shape != k.shape:
+        raise ValueError("k and v must share one shape and dtype")
+    tokens = k.shape[0]
+    slot_ptr = _ints("slots", slots, device, (tokens,))
+    kc, vc, ks, vs = cache.ptrs
+    k_token, k_head, _ = k.stride()
+    v_token, v_head, _ = v.stride()
+    with _On(device, stream) as s:
+        _check(lib().attn_cache_append(
+            k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, slot_ptr, tokens,
+            cache.kv_heads, cache.dim, kind, kc, vc, ks, vs, cache.code, cache.num_blocks,
+            cache.block_size, s), "attn_cache_append")
+
+
+def _workspace(index, heads, kv_heads, dim, max_new):
+    key = (index, heads, kv_heads, dim, max_new)
+    n = _workspace_bytes.get(key)
+    if n is None:
+        out = ctypes.c_ulonglong()
+        _check(lib().attn_cached_workspace(heads, kv_heads, dim, max_new, ctypes.byref(out)),
+               "attn_cached_workspace")
+        n = _workspace_bytes[key] = out.value
+    return n
+
+
+def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
+                causal: bool = True, scale: float | None = None, out=None, workspace=None,
+                stream=None):
+    """Attention of each request's newest tokens over its cache; returns out.
+
+    q, out: [tokens, heads, D], heads a multiple of the cache's; rows
+    starts[r] .. starts[r + 1) are the last tokens of request r, whose
+    kv_lens[r] tokens lie in the blocks tables[r] (they are in the cache
+    already).  Row i of n sees the first kv_lens[r] - n + i + 1 tokens (causal)
+    or all of them; a row that sees none becomes 0.  max_new: the most rows of
+    any request.  scale: of the scores, 1 / sqrt(D) by default.  Rows of `out`
+    behind starts[-1] are left as they were (with out=None: undefined).
+    workspace: a uint8 tensor to use instead of a new one per call; calls that
+    may overlap on the GPU need one each."""
+    device = cache.device
+    kind = _rows("q", q, device, 0, cache.dim)
+    tokens, heads, dim = q.shape
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError(f"{heads} heads are not a multiple of the cache's {cache.kv_heads}")
+    if scale is not None and not scale > 0:
+        raise ValueError("scale must be positive")
+    if max_new < 0:
+        raise ValueError("max_new must not be negative")
+    batch = kv_lens.shape[0]
+    t, width, stride = _table(tables, device, batch)
+    lens_ptr = _ints("kv_lens", kv_lens, device, (batch,))
+    starts_ptr = _ints("starts", starts, device, (batch + 1,))
+    on = _On(device, stream)
+    if out is None:
+        out = on.empty(q.shape, q.dtype, device)
+    elif _rows("out", out, device, heads, dim) != kind or out.shape != q.shape:
+        raise ValueError("out must have the shape and dtype of q")
+    q_token, q_head, _ = q.stride()
+    o_token, o_head, _ = out.stride()
+    kc, vc, ks, vs = cache.ptrs
+    with on as s:
+        if workspace is None:
+            need = _workspace(on.index, heads, cache.kv_heads, dim, max_new)
+            workspace = on.empty(need, torch.uint8, device)
+        else:
+            if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+                raise TypeError("workspace must be a contiguous uint8 tensor")
+            if workspace.device != device:
+                raise ValueError(f"workspace must be on {device}")
+            need = workspace.numel()
+        _check(lib().attn_cached(
+            q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head, tokens, heads,
+            cache.kv_heads, dim, kind, kc, vc, ks, vs, cache.code, cache.num_blocks,
+            cache.block_size, t, width, stride, lens_ptr, starts_ptr, batch, max_new,
+            1 if causal else 0, 0.0 if scale is None else scale, workspace.data_ptr(), need, s),
+            "attn_cached")
+    return out
+
+
+class CacheBatch:
+    """The requests of a server: `rows` of them, each with a table row of up to
+    max_len tokens, over one pool of blocks shared by any number of layers.
+
+    A step is advance() once, then attend() for each layer:
+
+        batch = CacheBatch(BlockPool.full(num_blocks, 32), rows=64, max_len=8192)
+        cache = [PagedCache.empty(num_blocks, 8, 128) for _ in layers]
+        batch.advance(new_lens, tokens=q.shape[0])
+        for each layer: o = batch.attend(cache[i], q, k, v, max_new=1)
+        batch.trim(keep)        # ended requests: 0, refused drafts: fewer
+
+    q, k, v hold the new tokens of all requests, request after request;
+    padding may follow the last one.  Nothing waits for the GPU: `status` holds
+    the last advance()'s word (BLOCKS) there.  Where it is not OK the step has
+    no tokens: nothing is appended, and attend() leaves its output alone."""
+
+    def __init__(self, pool: BlockPool, rows: int, max_len: int):
+        device, bs = pool.device, pool.block_size
+        if rows <= 0 or max_len <= 0:
+            raise ValueError("rows and max_len must be positive")
+        self.pool = pool
+        self.lens = torch.zeros(rows, dtype=torch.int32, device=device)
+        self.tables = torch.full((rows, -(-max_len // bs)), -1, dtype=torch.int32, device=device)
+        self.starts = torch.zeros(rows + 1, dtype=torch.int32, device=device)
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.trim_status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.plan = None
+
+    def advance(self, new_lens, tokens: int, *, stream=None) -> BlockPlan:
+        """new_lens[r] tokens more for request r, in a slot map of `tokens`."""
+        if self.plan is None or self.plan.slots.shape[0] != tokens:
+            slots = _On(self.pool.device, stream).empty(tokens, torch.int32, self.pool.device)
+            self.plan = BlockPlan(self.lens, self.starts, slots, self.status)
+        return block_tables(self.pool, self.lens, new_lens, self.tables, tokens, plan=self.plan,
+                            stream=stream)
+
+    def attend(self, cache: PagedCache, q, k, v, *, max_new: int, causal: bool = True,
+               scale: float | None = None, out=None, stream=None):
+        """Appends k and v of the step's tokens, then attends with q."""
+        if self.plan is None:
+            raise RuntimeError("advance() first")
+        if cache.block_size != self.pool.block_size or cache.num_blocks != self.pool.num_blocks:
+            raise ValueError("the cache's blocks are not the pool's")
+        cache_append(cache, k, v, self.plan.slots, stream=stream)
+        return attn_cached(q, cache, self.tables, self.lens, self.starts, max_new=max_new,
+                           causal=causal, scale=scale, out=out, stream=stream)
+
+    def trim(self, keep, *, stream=None):
+        """Requests keep their first keep[r] tokens; returns the status word."""
+        return block_trim(self.pool, self.lens, keep, self.tables, status=self.trim_status,
+                          stream=stream)

@@ -1,0 +1,348 @@
+// Block tables and slot maps on the GPU, from the requests' lengths.
+//
+// attn_block_tables gives every request the blocks that its new tokens need
+// and writes each new token's slot; attn_block_trim takes back the blocks
+// behind the tokens that a request keeps.  The pool's free blocks are a stack:
+// free_blocks[0 .. free_count), taken from and returned to the top.
+//
+// The mathematics is two prefix sums over the requests (new tokens, blocks)
+// and a search of them per token and per block.  It moves a few words a
+// request and 4 bytes a token, so a call is bound by its launch and by the
+// chain of loads, scan and stores (a few microseconds), not by bandwidth.
+// Therefore one launch of one thread-block cluster: every CTA scans all
+// requests into its own shared memory (that repeats a few KB of L2 reads,
+// where a second launch or a global counter would cost more), a cluster
+// barrier ends the reading, and then all threads of the cluster write.  The
+// barrier makes in-place calls (kv_lens = lens, free_left = free_count) safe
+// without any scratch memory, atomics or order between CTAs.
+#include "cache.cuh"
+#include "ptx.cuh"
+
+namespace attnprof {
+namespace cache {
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr int kClusterCtas = 8;
+
+struct Counts {
+  long long tokens, blocks;
+};
+
+// Exclusive prefix of (tokens, blocks) over the CTA's threads, plus `carry`;
+// *total becomes carry + the sum over all threads.
+__device__ __forceinline__ Counts scan_threads(Counts v, Counts carry, Counts* total,
+                                               Counts* warp_sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Counts in = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long a = __shfl_up_sync(~0u, in.tokens, d), b = __shfl_up_sync(~0u, in.blocks, d);
+    if (lane >= d) {
+      in.tokens += a;
+      in.blocks += b;
+    }
+  }
+  __syncthreads();  // warp_sum of an earlier call has been read
+  if (lane == 31) warp_sum[warp] = in;
+  __syncthreads();
+  if (warp == 0) {
+    Counts w = lane < kThreads / 32 ? warp_sum[lane] : Counts{0, 0};
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long a = __shfl_up_sync(~0u, w.tokens, d), b = __shfl_up_sync(~0u, w.blocks, d);
+      if (lane >= d) {
+        w.tokens += a;
+        w.blocks += b;
+      }
+    }
+    if (lane < kThreads / 32) warp_sum[lane] = w;
+  }
+  __syncthreads();
+  const Counts before = warp > 0 ? warp_sum[warp - 1] : Counts{0, 0};
+  const Counts all = warp_sum[kThreads / 32 - 1];
+  *total = Counts{carry.tokens + all.tokens, carry.blocks + all.blocks};
+  return Counts{carry.tokens + before.tokens + in.tokens - v.tokens,
+                carry.blocks + before.blocks + in.blocks - v.blocks};
+}
+
+// Largest r with first[r] <= x, for first[0] = 0 <= x (n >= 1 entries).
+__device__ __forceinline__ int last_at_most(const int* first, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void end_of_reading(int ctas) {
+  if (ctas > 1)
+    ptx::cluster_sync();
+  else
+    __syncthreads();
+}
+
+struct TablesParams {
+  const int *lens, *new_lens, *free_blocks, *free_count;
+  int *tables, *kv_lens, *starts, *slots, *free_left, *status;
+  long long table_stride;
+  int batch, width, tokens, num_blocks, shift;
+};
+
+__global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) {
+  extern __shared__ int sm[];
+  int* start = sm;                      // [batch] first new token of a request
+  int* first = sm + p.batch;            // [batch] rank of its first new block
+  int* len = sm + 2 * p.batch;          // [batch] tokens held before
+  __shared__ Counts warp_sum[kThreads / 32];
+  const int ctas = static_cast<int>(gridDim.x);
+  const int mask = (1 << p.shift) - 1;
+
+  Counts total{0, 0};
+  int bad = 0;  // bit 0: a row of the table is too short, bit 1: a negative number
+  for (int base = 0; base < p.batch; base += kThreads) {
+    const int r = base + static_cast<int>(threadIdx.x);
+    Counts v{0, 0};
+    int l = 0;
+    if (r < p.batch) {
+      l = p.lens[r];
+      const int n = p.new_lens[r];
+      if (l < 0 || n < 0) {
+        bad |= 2;
+        l = 0;
+      } else {
+        const long long after = (static_cast<long long>(l) + n + mask) >> p.shift;
+        if (after > p.width || static_cast<long long>(l) + n > INT_MAX) bad |= 1;
+        v = Counts{n, after - ((static_cast<long long>(l) + mask) >> p.shift)};
+      }
+    }
+    const Counts at = scan_threads(v, total, &total, warp_sum);
+    if (r < p.batch) {  // (kept only where the call is carried out, so that they fit)
+      start[r] = static_cast<int>(at.tokens);
+      first[r] = static_cast<int>(at.blocks);
+      len[r] = l;
+    }
+  }
+  const int count = *p.free_count;
+  bad = (__syncthreads_or(bad & 1) ? 1 : 0) | (__syncthreads_or(bad & 2) ? 2 : 0);
+  int status = ATTN_BLOCKS_OK;
+  if (count < 0 || count > p.num_blocks || total.blocks > count) status = ATTN_BLOCKS_POOL;
+  if (bad & 1) status = ATTN_BLOCKS_ROW;
+  if (total.tokens > p.tokens) status = ATTN_BLOCKS_SLOTS;
+  if (bad & 2) status = ATTN_BLOCKS_NEGATIVE;
+  const bool ok = status == ATTN_BLOCKS_OK;
+  const int used = ok ? static_cast<int>(total.tokens) : 0;
+  const int taken = ok ? static_cast<int>(total.blocks) : 0;
+
+  end_of_reading(ctas);
+
+  const int me = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
+  const int all = ctas * kThreads;
+  // The step's lengths and the pool's count: one thread each.
+  for (int r = me; r < p.batch; r += all) {
+    // (p.lens may be p.kv_lens: len[] has it where it is not negative)
+    if (ok) {
+      const int end = r + 1 < p.batch ? start[r + 1] : used;
+      p.kv_lens[r] = len[r] + (end - start[r]);
+      p.starts[r] = start[r];
+    } else {
+      if (p.kv_lens != p.lens) p.kv_lens[r] = p.lens[r];
+      p.starts[r] = 0;
+    }
+  }
+  if (me == 0) {
+    p.starts[p.batch] = used;
+    *p.free_left = count - taken;
+    *p.status = status;
+  }
+  // New blocks into the tables.
+  for (int j = me; j < taken; j += all) {
+    const int r = last_at_most(first, p.batch, j);
+    const int column = ((len[r] + mask) >> p.shift) + (j - first[r]);
+    p.tables[r * p.table_stride + column] = p.free_blocks[count - 1 - j];
+  }
+  // Slots, four tokens a thread: one search, then a walk.  A block that the
+  // request holds already is read from its table row, a new one from the free
+  // list (not from the table, which other threads are writing).
+  const bool wide = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0;
+  for (long long t0 = 4ll * me; t0 < p.tokens; t0 += 4ll * all) {
+    int out[4] = {-1, -1, -1, -1};
+    if (t0 < used) {
+      int r = last_at_most(start, p.batch, static_cast<int>(t0));
+      int block_rank = -1, id = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = static_cast<int>(t0) + i;
+        if (t >= used) break;
+        while (r + 1 < p.batch && start[r + 1] <= t) {
+          ++r;
+          block_rank = -1;
+        }
+        const int pos = len[r] + (t - start[r]);
+        const int b = pos >> p.shift;
+        if (b != block_rank) {
+          const int held = (len[r] + mask) >> p.shift;
+          id = b < held ? p.tables[r * p.table_stride + b]
+                        : p.free_blocks[count - 1 - (first[r] + b - held)];
+          block_rank = b;
+        }
+        // An id that is not a block of the pool gives no slot.
+        if (id >= 0 && id < p.num_blocks) out[i] = (id << p.shift) + (pos & mask);
+      }
+    }
+    if (wide && t0 + 3 < p.tokens) {
+      *reinterpret_cast<int4*>(p.slots + t0) = make_int4(out[0], out[1], out[2], out[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t0 + i < p.tokens) p.slots[t0 + i] = out[i];
+    }
+  }
+}
+
+struct TrimParams {
+  const int *lens, *keep, *tables, *free_count;
+  int *free_blocks, *lens_left, *free_left, *status;
+  long long table_stride;
+  int batch, width, num_blocks, shift;
+};
+
+__global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
+  extern __shared__ int sm[];
+  int* first = sm;              // [batch] rank of the first block given back
+  int* left = sm + p.batch;     // [batch] tokens kept
+  __shared__ Counts warp_sum[kThreads / 32];
+  const int ctas = static_cast<int>(gridDim.x);
+  const int mask = (1 << p.shift) - 1;
+
+  Counts total{0, 0};
+  int bad = 0;
+  for (int base = 0; base < p.batch; base += kThreads) {
+    const int r = base + static_cast<int>(threadIdx.x);
+    Counts v{0, 0};
+    int l = 0;
+    if (r < p.batch) {
+      l = p.lens[r];
+      const int k = p.keep[r];
+      if (l < 0 || k < 0) bad |= 2;
+      const long long held = (static_cast<long long>(max(l, 0)) + mask) >> p.shift;
+      if (held > p.width) bad |= 1;
+      l = max(0, min(l, k));
+      v.blocks = held - ((static_cast<long long>(l) + mask) >> p.shift);
+    }
+    const Counts at = scan_threads(v, total, &total, warp_sum);
+    if (r < p.batch) {
+      first[r] = static_cast<int>(at.blocks);
+      left[r] = l;
+    }
+  }
+  const int count = *p.free_count;
+  bad = (__syncthreads_or(bad & 1) ? 1 : 0) | (__syncthreads_or(bad & 2) ? 2 : 0);
+  int status = ATTN_BLOCKS_OK;
+  // More blocks than the pool has: some were given back before.
+  if (count < 0 || count + total.blocks > p.num_blocks) status = ATTN_BLOCKS_POOL;
+  if (bad & 1) status = ATTN_BLOCKS_ROW;
+  if (bad & 2) status = ATTN_BLOCKS_NEGATIVE;
+  const bool ok = status == ATTN_BLOCKS_OK;
+  const int back = ok ? static_cast<int>(total.blocks) : 0;
+
+  end_of_reading(ctas);
+
+  const int me = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
+  const int all = ctas * kThreads;
+  for (int r = me; r < p.batch; r += all) {
+    if (ok)
+      p.lens_left[r] = left[r];
+    else if (p.lens_left != p.lens)
+      p.lens_left[r] = p.lens[r];
+  }
+  if (me == 0) {
+    *p.free_left = count + back;
+    *p.status = status;
+  }
+  for (int j = me; j < back; j += all) {
+    const int r = last_at_most(first, p.batch, j);
+    const int column = ((left[r] + mask) >> p.shift) + (j - first[r]);
+    p.free_blocks[count + j] = p.tables[r * p.table_stride + column];
+  }
+}
+
+// One CTA where 4 entries a thread do all of the writing, else a cluster.
+int ctas_for(long long entries) { return entries > 4 * kThreads ? kClusterCtas : 1; }
+
+template <typename P>
+int launch_cluster(void (*kern)(P), const P& p, int ctas, size_t smem, cudaStream_t st) {
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(smem)) != cudaSuccess)
+    return ATTN_ERR_RESOURCE;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
+}
+
+int shift_of(int block_size) {
+  int s = 0;
+  while ((1 << s) < block_size) ++s;
+  return s;
+}
+
+int check_batch(int batch, int width, long long table_stride, int num_blocks, int block_size) {
+  if (!block_size_ok(block_size)) return ATTN_ERR_UNSUPPORTED;
+  if (batch < 0 || width < 0 || table_stride < width || num_blocks <= 0)
+    return ATTN_ERR_INVALID_ARG;
+  if (static_cast<long long>(num_blocks) * block_size > INT_MAX) return ATTN_ERR_INVALID_ARG;
+  if (batch > ATTN_BLOCKS_MAX_BATCH) return ATTN_ERR_UNSUPPORTED;
+  return ATTN_OK;
+}
+
+}  // namespace
+}  // namespace cache
+}  // namespace attnprof
+
+using namespace attnprof::cache;
+
+extern "C" int attn_block_tables(const int* lens, const int* new_lens, int batch, int* tables,
+                                 int width, long long table_stride, const int* free_blocks,
+                                 const int* free_count, int num_blocks, int block_size,
+                                 int* kv_lens, int* starts, int* slots, int tokens,
+                                 int* free_left, int* status, void* stream) {
+  const int rc = check_batch(batch, width, table_stride, num_blocks, block_size);
+  if (rc != ATTN_OK) return rc;
+  if (tokens < 0) return ATTN_ERR_INVALID_ARG;
+  if (!free_blocks || !free_count || !starts || !free_left || !status) return ATTN_ERR_INVALID_ARG;
+  if (batch > 0 && (!lens || !new_lens || !kv_lens)) return ATTN_ERR_INVALID_ARG;
+  if ((batch > 0 && width > 0 && !tables) || (tokens > 0 && !slots)) return ATTN_ERR_INVALID_ARG;
+  TablesParams p{lens,    new_lens, free_blocks, free_count,   tables, kv_lens, starts,     slots,
+                 free_left, status, table_stride, batch,       width,  tokens,  num_blocks, shift_of(block_size)};
+  return launch_cluster(tables_kernel, p, ctas_for(tokens), 3ull * sizeof(int) * batch,
+                        static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int attn_block_trim(const int* lens, const int* keep, int batch, const int* tables,
+                               int width, long long table_stride, int* free_blocks,
+                               const int* free_count, int num_blocks, int block_size,
+                               int* lens_left, int* free_left, int* status, void* stream) {
+  const int rc = check_batch(batch, width, table_stride, num_blocks, block_size);
+  if (rc != ATTN_OK) return rc;
+  if (!free_blocks || !free_count || !free_left || !status) return ATTN_ERR_INVALID_ARG;
+  if (batch > 0 && (!lens || !keep || !lens_left)) return ATTN_ERR_INVALID_ARG;
+  if (batch > 0 && width > 0 && !tables) return ATTN_ERR_INVALID_ARG;
+  TrimParams p{lens,      keep,   tables,       free_count, free_blocks, lens_left,
+               free_left, status, table_stride, batch,      width,       num_blocks,
+               shift_of(block_size)};
+  const long long most = static_cast<long long>(batch) * width;
+  return launch_cluster(trim_kernel, p, ctas_for(most < num_blocks ? most : num_blocks),
+                        2ull * sizeof(int) * batch, static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,109 @@
+// The paged cache held in 8 bits: its layout, its two codes and its argument
+// checks, shared by the kernels that fill it and the ones that read it.
+//
+// A pool of num_blocks blocks of block_size tokens (16, 32, 64 or 128):
+//   K, V codes   [num_blocks, kv_heads, block_size, D] bytes, D = 64 or 128
+//   K, V scales  [num_blocks, kv_heads] f32; a code c stands for c * scale
+// so the tokens of one (block, head) lie in one piece of block_size * D bytes
+// and share one scale.  Token `pos` of request r lies in block
+// tables[r][pos / block_size] at offset pos % block_size.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <cstdint>
+#include <type_traits>
+
+#include "attnprof.h"
+
+namespace attnprof {
+namespace cache {
+
+constexpr int kLeastExponent = -100;  // of a block's power-of-two scale
+
+inline bool code_ok(int code) { return code == ATTN_CODE_E4M3 || code == ATTN_CODE_INT8; }
+inline bool dtype_ok(int dtype) { return dtype == ATTN_DTYPE_F16 || dtype == ATTN_DTYPE_BF16; }
+inline bool block_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs == 128; }
+inline bool aligned(const void* p, unsigned n) {
+  return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
+}
+
+// Shape checks common to every call on a pool; ATTN_OK or an error.
+inline int check_pool(int num_blocks, int kv_heads, int block_size, int D, int code) {
+  if (!code_ok(code) || !block_size_ok(block_size) || (D != 64 && D != 128))
+    return ATTN_ERR_UNSUPPORTED;
+  if (num_blocks <= 0 || kv_heads <= 0) return ATTN_ERR_INVALID_ARG;
+  // A slot (block * block_size + offset) is a 32-bit number.
+  if (static_cast<long long>(num_blocks) * block_size > INT_MAX) return ATTN_ERR_INVALID_ARG;
+  return ATTN_OK;
+}
+
+#ifdef __CUDACC__
+// ---------------------------------------------------------------------------
+// Codes.  E4M3 is the 8-bit float of 4 exponent and 3 mantissa bits (largest
+// 448); INT8 is a whole number in [-127, 127].  Both are held exactly by f16.
+// ---------------------------------------------------------------------------
+template <int CODE>
+struct Code;
+
+template <>
+struct Code<ATTN_CODE_E4M3> {
+  static constexpr float kLargest = 448.f;
+  // Two codes (in the low 16 bits) to two f16.
+  static __device__ __forceinline__ uint32_t half2_lo(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}"
+        : "=r"(r)
+        : "r"(w));
+    return r;
+  }
+  static __device__ __forceinline__ uint32_t half2_hi(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
+        : "=r"(r)
+        : "r"(w));
+    return r;
+  }
+  // Two numbers rounded to the nearest code (ties to even), a in the low byte.
+  static __device__ __forceinline__ uint32_t encode2(float a, float b) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+    return r;
+  }
+};
+
+template <>
+struct Code<ATTN_CODE_INT8> {
+  static constexpr float kLargest = 127.f;
+  // 1024 + u is an f16 whose low byte is u: the bytes with their sign bit
+  // flipped are u = code + 128, so code = (1024 + u) - 1152, exact in f16.
+  static __device__ __forceinline__ uint32_t biased(uint32_t w, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w ^ 0x80808080u), "r"(0x64646464u), "r"(sel));
+    const __half2 h = __hsub2(*reinterpret_cast<__half2*>(&r), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ uint32_t half2_lo(uint32_t w) { return biased(w, 0x4140); }
+  static __device__ __forceinline__ uint32_t half2_hi(uint32_t w) { return biased(w, 0x4342); }
+  static __device__ __forceinline__ uint32_t encode2(float a, float b) {
+    const int i = max(-127, min(127, __float2int_rn(a)));
+    const int j = max(-127, min(127, __float2int_rn(b)));
+    return (static_cast<uint32_t>(i) & 0xffu) | ((static_cast<uint32_t>(j) & 0xffu) << 8);
+  }
+};
+
+__device__ __forceinline__ float2 half2_to_float2(uint32_t h) {
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+
+// 2^e for e in [-126, 127].
+__device__ __forceinline__ float power_of_two(int e) {
+  return __int_as_float((e + 127) << 23);
+}
+#endif  // __CUDACC__
+
+}  // namespace cache
+}  // namespace attnprof

@@ -1,0 +1,270 @@
+// attn_cache_append: keys and values of new tokens into a paged cache held in
+// 8 bits, with one power-of-two scale for each (block, head) of K and of V.
+//
+// Per (block, head) that the call writes into, with a = max |x| over its new
+// tokens there: e = the least exponent >= -100 with a <= C * 2^e (C = 448 for
+// e4m3, 127 for int8); the scale becomes 2^e where the call writes the block's
+// first slot, else max(old scale, 2^e).  Where it grew, the codes in front of
+// the call's first slot are rounded again to the new scale; then the new
+// tokens' codes are round_to_nearest_even(x / scale).  With powers of two that
+// is a shift of the exponent: e4m3 codes move exactly unless they fall into
+// the subnormals, and every product here is exact in f32 before the one
+// rounding to 8 bits.
+//
+// A number that is not finite cannot be held: its code is 0, and the block's K
+// scale becomes NaN for that head (whichever of k and v had it), until the
+// block is written from its first slot again.  Scores against such a block are
+// NaN for the rows that see it, and masked ones are dropped before they reach
+// a sum; a NaN among the values would instead spread to masked rows as 0 * NaN.
+//
+// Tokens that follow each other into one block (`a run`) share its scale, so
+// the unit of work is one run and one head: one warp, half of it on K and half
+// on V, so that both halves can see whether the other met a number that is not
+// finite.  A warp looks at `chunk` consecutive tokens and takes the runs that
+// begin there: one token where that gives enough warps, else a block's worth,
+// which leaves few warps without a run when prompts come in.
+// It reads 2 bytes and writes 1 per element, plus 8 bytes a run and head.
+#include "cache.cuh"
+
+namespace attnprof {
+namespace cache {
+namespace {
+
+constexpr int kWarps = 4;
+
+struct AppendParams {
+  const void *k, *v;
+  const int* slots;
+  uint8_t *kc, *vc;
+  float *ks, *vs;
+  long long k_token, k_head, v_token, v_head;  // strides in elements
+  int tokens, heads, num_slots, shift, chunk;
+};
+
+template <typename T>
+struct Bits;
+template <>
+struct Bits<__half> {
+  static constexpr uint32_t kInf = 0x7c00u;
+  static __device__ __forceinline__ float2 to_float2(uint32_t w) {
+    return __half22float2(*reinterpret_cast<__half2*>(&w));
+  }
+  static __device__ __forceinline__ float to_float(uint32_t b) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(b)));
+  }
+};
+template <>
+struct Bits<__nv_bfloat16> {
+  static constexpr uint32_t kInf = 0x7f80u;
+  static __device__ __forceinline__ float2 to_float2(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ float to_float(uint32_t b) { return __uint_as_float(b << 16); }
+};
+
+// Both halves of each word: those that are not finite become 0; `bad` gathers
+// whether there were any.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w, uint32_t& bad) {
+  const uint32_t m = __vcmpgeu2(w & 0x7fff7fffu, Bits<T>::kInf * 0x10001u);
+  bad |= m;
+  return w & ~m;
+}
+
+// The least e >= kLeastExponent with a <= C * 2^e (a >= 0, finite).
+template <int CODE>
+__device__ __forceinline__ int exponent_for(float a) {
+  const int bits = __float_as_int(a);
+  const int e2 = (bits >> 23) - 127;  // a = 1.m * 2^e2 (a subnormal a ends at the bound)
+  const int m = bits & 0x7fffff;
+  // C = 1.75 * 2^8 and 1.984375 * 2^6
+  const int e = CODE == ATTN_CODE_E4M3 ? e2 - 8 + (m > 0x600000 ? 1 : 0)
+                                       : e2 - 6 + (m > 0x7e0000 ? 1 : 0);
+  return max(e, kLeastExponent);
+}
+
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams p) {
+  constexpr int kLanes = D / 8;              // lanes on one token's row: 16 bytes each
+  constexpr int kRows = 16 / kLanes;         // tokens a half warp takes at once
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool is_v = lane >= 16;
+  const int sub = (lane & 15) / kLanes;      // which of the kRows tokens
+  const int part = (lane & 15) % kLanes;     // which 8 elements of the row
+  const int bs = 1 << p.shift;
+  const int head = static_cast<int>(blockIdx.y);
+  const long long begin = (static_cast<long long>(blockIdx.x) * kWarps + warp) * p.chunk;
+  const long long end = min(begin + p.chunk, static_cast<long long>(p.tokens));
+
+  const T* x = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.v_head : p.k_head) +
+               8 * part;
+  const long long x_token = is_v ? p.v_token : p.k_token;
+  uint8_t* codes = is_v ? p.vc : p.kc;
+  float* scales = is_v ? p.vs : p.ks;
+
+  auto slot_at = [&](long long t) {
+    const int s = p.slots[t];
+    return s >= 0 && s < p.num_slots ? s : -1;
+  };
+
+  for (long long t0 = begin; t0 < end;) {
+    // The next token that begins a run: one with a slot, into which the token
+    // before does not lead.
+    int mine = -1;
+    if (t0 + lane < end) {
+      mine = slot_at(t0 + lane);
+      if (mine >= 0 && (mine & (bs - 1)) > 0 && t0 + lane > 0 &&
+          slot_at(t0 + lane - 1) == mine - 1)
+        mine = -1;
+    }
+    const unsigned heads_of_runs = __ballot_sync(~0u, mine >= 0);
+    if (heads_of_runs == 0) {
+      t0 += 32;
+      continue;
+    }
+    const int skip = __ffs(heads_of_runs) - 1;
+    const int slot = __shfl_sync(~0u, mine, skip);
+    const int off = slot & (bs - 1);
+    t0 += skip;
+    // The run: following tokens with following slots of the same block.
+    const int most = static_cast<int>(min(static_cast<long long>(bs - off), p.tokens - t0));
+    int n = 1;
+    while (n < most) {
+      const int i = n + lane;
+      const unsigned next = __ballot_sync(~0u, i < most && p.slots[t0 + i] == slot + i);
+      n += next == ~0u ? 32 : __ffs(~next) - 1;
+      if (next != ~0u) break;
+    }
+    const long long block_head = static_cast<long long>(slot >> p.shift) * p.heads + head;
+    float* scale_at = scales + block_head;
+    uint8_t* rows = codes + (block_head << p.shift) * D;
+    const float old = off > 0 ? *scale_at : 0.f;
+
+    // Largest |x| of the run, as bits: for finite numbers these order alike.
+    uint32_t top = 0, bad = 0;
+    const T* xr = x + t0 * x_token;
+#pragma unroll 4
+    for (int i = sub; i < n; i += kRows) {
+      const uint4 w = *reinterpret_cast<const uint4*>(xr + i * x_token);
+      const uint32_t a = finite_only<T>(w.x, bad), b = finite_only<T>(w.y, bad);
+      const uint32_t c = finite_only<T>(w.z, bad), d = finite_only<T>(w.w, bad);
+      top = __vmaxu2(top, __vmaxu2(__vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu),
+                                   __vmaxu2(c & 0x7fff7fffu, d & 0x7fff7fffu)));
+    }
+    top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
+    const bool any_bad = __any_sync(~0u, bad != 0);
+
+    const float want = power_of_two(exponent_for<CODE>(Bits<T>::to_float(top)));
+    const bool dead = off > 0 && old != old;  // a NaN scale stays until the block is begun anew
+    const float now = (off > 0 && old > want) ? old : want;
+    const bool grew = off > 0 && !dead && now > old;
+    __syncwarp();  // every lane has read the old scale
+    if ((lane & 15) == 0) *scale_at = ((any_bad && !is_v) || dead) ? __int_as_float(0x7fffffff) : now;
+
+    // Dividing by `now`: by its reciprocal where that is exact.
+    const bool pow2 = (__float_as_int(now) & 0x7fffff) == 0;
+    const float inv = pow2 ? 1.f / now : 0.f;
+    auto scaled = [&](float f) { return pow2 ? f * inv : f / now; };
+
+    if (grew) {  // codes in front of the run, to the new scale
+      const float r = old / now;
+      for (int i = sub; i < off; i += kRows) {
+        uint2* at = reinterpret_cast<uint2*>(rows + static_cast<long long>(i) * D + 8 * part);
+        uint2 c = *at;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&c);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float2 a = half2_to_float2(Code<CODE>::half2_lo(w[j]));
+          const float2 b = half2_to_float2(Code<CODE>::half2_hi(w[j]));
+          w[j] = Code<CODE>::encode2(a.x * r, a.y * r) | (Code<CODE>::encode2(b.x * r, b.y * r) << 16);
+        }
+        *at = c;
+      }
+    }
+#pragma unroll 4
+    for (int i = sub; i < n; i += kRows) {
+      uint4 w = *reinterpret_cast<const uint4*>(xr + i * x_token);
+      uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+      uint2 c;
+      uint32_t e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = Bits<T>::to_float2(finite_only<T>(u[j], bad));
+        e[j] = Code<CODE>::encode2(scaled(f.x), scaled(f.y));
+      }
+      c.x = e[0] | (e[1] << 16);
+      c.y = e[2] | (e[3] << 16);
+      *reinterpret_cast<uint2*>(rows + static_cast<long long>(off + i) * D + 8 * part) = c;
+    }
+    t0 += n;
+  }
+}
+
+template <typename T, int CODE, int D>
+int launch(const AppendParams& p0, cudaStream_t st) {
+  AppendParams p = p0;
+  // One token a warp up to some 16 warps an SM; beyond that a block's worth,
+  // since most tokens then follow others into their block.
+  const long long warps = static_cast<long long>(p.tokens) * p.heads;
+  p.chunk = warps <= 148 * 16 ? 1 : 1 << p.shift;
+  const long long groups = (static_cast<long long>(p.tokens) + p.chunk - 1) / p.chunk;
+  const dim3 grid(static_cast<unsigned>((groups + kWarps - 1) / kWarps),
+                  static_cast<unsigned>(p.heads));
+  append_kernel<T, CODE, D><<<grid, 32 * kWarps, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
+}
+
+template <typename T, int CODE>
+int launch_d(const AppendParams& p, int D, cudaStream_t st) {
+  return D == 64 ? launch<T, CODE, 64>(p, st) : launch<T, CODE, 128>(p, st);
+}
+
+template <typename T>
+int launch_code(const AppendParams& p, int D, int code, cudaStream_t st) {
+  return code == ATTN_CODE_E4M3 ? launch_d<T, ATTN_CODE_E4M3>(p, D, st)
+                                : launch_d<T, ATTN_CODE_INT8>(p, D, st);
+}
+
+}  // namespace
+}  // namespace cache
+}  // namespace attnprof
+
+using namespace attnprof::cache;
+
+extern "C" int attn_cache_append(const void* k, long long k_token_stride, long long k_head_stride,
+                                 const void* v, long long v_token_stride, long long v_head_stride,
+                                 const int* slots, int tokens, int kv_heads, int D, int dtype,
+                                 void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                                 int code, int num_blocks, int block_size, void* stream) {
+  const int rc = check_pool(num_blocks, kv_heads, block_size, D, code);
+  if (rc != ATTN_OK) return rc;
+  if (!dtype_ok(dtype)) return ATTN_ERR_UNSUPPORTED;
+  if (tokens < 0 || kv_heads > 65535) return ATTN_ERR_INVALID_ARG;
+  if (tokens == 0) return ATTN_OK;
+  if (!k || !v || !slots || !k_codes || !v_codes || !k_scale || !v_scale)
+    return ATTN_ERR_INVALID_ARG;
+  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_codes, 16) || !aligned(v_codes, 16) ||
+      ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) != 0)
+    return ATTN_ERR_MISALIGNED;
+  AppendParams p{};
+  p.k = k;
+  p.v = v;
+  p.slots = slots;
+  p.kc = static_cast<uint8_t*>(k_codes);
+  p.vc = static_cast<uint8_t*>(v_codes);
+  p.ks = k_scale;
+  p.vs = v_scale;
+  p.k_token = k_token_stride;
+  p.k_head = k_head_stride;
+  p.v_token = v_token_stride;
+  p.v_head = v_head_stride;
+  p.tokens = tokens;
+  p.heads = kv_heads;
+  p.num_slots = num_blocks * block_size;
+  p.shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == ATTN_DTYPE_F16 ? launch_code<__half>(p, D, code, st)
+                                 : launch_code<__nv_bfloat16>(p, D, code, st);
+}

@@ -1,0 +1,41 @@
+// Attention over the paged 8-bit cache: what its kernels share.
+#pragma once
+
+#include "cache.cuh"
+
+namespace attnprof {
+namespace cache {
+
+struct CachedParams {
+  const void* q;
+  void* out;
+  const uint8_t *kc, *vc;
+  const float *ks, *vs;
+  const int *tables, *kv_lens, *starts;
+  long long q_token, q_head, o_token, o_head, table_stride;
+  int tokens, heads, kv_heads, group, batch, num_blocks, shift, capacity, causal;
+  float scale_log2;  // score scale * log2(e)
+  // Requests of more than `rows_most` query rows a kv head (tokens * group)
+  // belong to the other kernel: the split one takes those up to it, the tiled
+  // one those above it.
+  long long rows_most;
+  float* ws;
+};
+
+// A request as the kernels see it, with every number brought into range.
+struct Request {
+  int start, n, kv;  // first query row, rows, tokens in the cache
+};
+
+__device__ __forceinline__ Request request_at(const CachedParams& p, int r) {
+  const int a = min(max(p.starts[r], 0), p.tokens);
+  const int b = min(max(p.starts[r + 1], 0), p.tokens);
+  return Request{a, max(b - a, 0), min(max(p.kv_lens[r], 0), p.capacity)};
+}
+
+int launch_split(const CachedParams& p, int D, int dtype, int code, int max_new, void* ws,
+                 unsigned long long ws_bytes, cudaStream_t st);
+int split_workspace(int group, int D, int max_new, unsigned long long* bytes);
+
+}  // namespace cache
+}  // namespace attnprof

@@ -243,6 +243,122 @@ int attn_query_split(int B, int H, int S, int D, int dtype, int BM, int BN, int*
 int attn_fwd_noalloc(const void* Q, const void* K, const void* V, void* O, int B, int H, int S,
                      int D, int dtype, int BM, int BN, void* stream);
 
+/*
+ * A paged cache held in 8 bits, and attention over it.
+ *
+ * A pool holds num_blocks blocks of block_size tokens (16, 32, 64 or 128):
+ *   k_codes, v_codes  [num_blocks, kv_heads, block_size, D] bytes, D 64 or 128
+ *   k_scale, v_scale  [num_blocks, kv_heads] f32
+ * A code c of block b and head h stands for c * scale[b][h].  Codes are e4m3
+ * (8-bit float, largest 448) or int8 (whole numbers in [-127, 127]).  Request
+ * r holds its token `pos` in block tables[r][pos / block_size] at offset
+ * pos % block_size, the slot block * block_size + offset of the pool.  A row
+ * of `tables` has `width` entries and begins table_stride entries after the
+ * row before; entries behind a request's last block mean nothing and are not
+ * read.  Pool sizes whose slots do not fit 31 bits are refused; addresses are
+ * computed in 64 bits.  The reference has no cache: its attention takes dense
+ * K and V (tuning/attn_test.cu:1665-1691).
+ */
+#define ATTN_CODE_E4M3 0
+#define ATTN_CODE_INT8 1
+
+/* Values of the status word that attn_block_tables and attn_block_trim write
+ * (on the device, in stream order).  Unless it is OK the call has changed
+ * nothing; where several apply, the largest is given. */
+#define ATTN_BLOCKS_OK 0
+#define ATTN_BLOCKS_POOL 1     /* too few free blocks; trim: more blocks than the pool has */
+#define ATTN_BLOCKS_ROW 2      /* a request needs more blocks than its table row holds     */
+#define ATTN_BLOCKS_SLOTS 3    /* more new tokens than the slot map holds                  */
+#define ATTN_BLOCKS_NEGATIVE 4 /* a negative number of tokens                              */
+#define ATTN_BLOCKS_MAX_BATCH 16384
+
+/*
+ * attn_block_tables -- the block tables and slot maps of one step, built on
+ * the GPU.  Request r holds lens[r] tokens and gets new_lens[r] more (either
+ * may be 0).  The blocks that this needs come from the top of the stack
+ * free_blocks[0 .. *free_count) (capacity num_blocks), in the order of the
+ * requests.  Writes
+ *   tables      the new blocks' entries
+ *   kv_lens     [batch] lens + new_lens
+ *   starts      [batch + 1] first new token of each request, then their sum
+ *   slots       [tokens] slot of every new token; -1 behind the last one (and
+ *               where a table or the free list holds no block of the pool)
+ *   free_left   [1] free blocks left (the list itself is not changed)
+ *   status      [1] ATTN_BLOCKS_*.  When it is not OK: tables unchanged,
+ *               kv_lens = lens, starts 0, slots -1, free_left = free_count
+ * kv_lens may be lens and free_left may be free_count; no other arrays may
+ * overlap.  Asynchronous; needs no scratch, so it can be captured and replayed.
+ * batch at most ATTN_BLOCKS_MAX_BATCH.
+ */
+int attn_block_tables(const int* lens, const int* new_lens, int batch, int* tables, int width,
+                      long long table_stride, const int* free_blocks, const int* free_count,
+                      int num_blocks, int block_size, int* kv_lens, int* starts, int* slots,
+                      int tokens, int* free_left, int* status, void* stream);
+
+/*
+ * attn_block_trim -- requests give blocks back: request r keeps its first
+ * min(lens[r], keep[r]) tokens (0 when it has ended, fewer than lens[r] when
+ * drafted tokens were refused), and the blocks behind them go onto the stack
+ * in the order of the requests.  Writes free_blocks, lens_left [batch]
+ * (may be lens), free_left (may be free_count) and status; when that is not
+ * OK, lens_left = lens and the stack is unchanged.  The tables keep their
+ * entries, which mean nothing behind lens_left.  A block that several requests
+ * share must be given back by one of them only.
+ */
+int attn_block_trim(const int* lens, const int* keep, int batch, const int* tables, int width,
+                    long long table_stride, int* free_blocks, const int* free_count,
+                    int num_blocks, int block_size, int* lens_left, int* free_left, int* status,
+                    void* stream);
+
+/*
+ * attn_cache_append -- k and v of `tokens` new tokens ([tokens, kv_heads, D],
+ * f16 or bf16, strides in elements and multiples of 8) quantised into the
+ * slots given (a slot that is negative or not in the pool is skipped: padded
+ * batches).  The scale of a (block, head) is a power of two, the least one of
+ * at least 2^-100 that brings the new tokens' largest |x| into the code's
+ * range; a block that is not written from its first slot keeps its scale if
+ * that is larger, and otherwise its codes in front of the new tokens are
+ * rounded again to the larger scale.  New codes are rounded to nearest even.
+ * A number that is not finite makes the block's k_scale NaN for that head
+ * (and its own code 0), so that rows attending to the block become NaN and no
+ * others, until the block is written from its first slot again.
+ * The tokens of one block must follow each other in the call with ascending
+ * slots, as attn_block_tables gives them; a block must not appear twice.
+ */
+int attn_cache_append(const void* k, long long k_token_stride, long long k_head_stride,
+                      const void* v, long long v_token_stride, long long v_head_stride,
+                      const int* slots, int tokens, int kv_heads, int D, int dtype, void* k_codes,
+                      void* v_codes, float* k_scale, float* v_scale, int code, int num_blocks,
+                      int block_size, void* stream);
+
+/*
+ * attn_cached -- attention of each request's newest tokens over its cache.
+ * q and out are [tokens, heads, D] (f16 or bf16, strides in elements and
+ * multiples of 8); the rows of request r are starts[r] .. starts[r + 1), at
+ * most max_new of them, and stand for its last tokens.  Query head h reads
+ * kv head h / (heads / kv_heads).  With causal != 0, row i of n sees the first
+ * kv_lens[r] - n + i + 1 tokens, else all kv_lens[r].  scale multiplies the
+ * scores (0: 1 / sqrt(D)).  A row that sees no token becomes 0.  Rows behind
+ * starts[batch] are left as they were.  Scales must be positive; V scales and
+ * the codes of tokens held must be finite numbers.  What lies in slots that
+ * hold no token is never used, whatever it is.  kv_lens is taken as at most
+ * width * block_size, starts as within [0, tokens]; a table entry that is no
+ * block of the pool is left out.
+ * workspace: 16-byte aligned, attn_cached_workspace(...) bytes, needs no
+ * initial value; calls that may overlap need one each.  Asynchronous.
+ */
+int attn_cached(const void* q, long long q_token_stride, long long q_head_stride, void* out,
+                long long out_token_stride, long long out_head_stride, int tokens, int heads,
+                int kv_heads, int D, int dtype, const void* k_codes, const void* v_codes,
+                const float* k_scale, const float* v_scale, int code, int num_blocks,
+                int block_size, const int* tables, int width, long long table_stride,
+                const int* kv_lens, const int* starts, int batch, int max_new, int causal,
+                float scale, void* workspace, unsigned long long workspace_bytes, void* stream);
+
+/* Workspace bytes of attn_cached on the current device, whatever the lengths. */
+int attn_cached_workspace(int heads, int kv_heads, int D, int max_new,
+                          unsigned long long* bytes);
+
 /* Human-readable text for a return code.  Never NULL. */
 const char* attn_error_string(int code);
 

@@ -1,0 +1,123 @@
+"""Argument checks of the paged cache: every call here is refused on the host
+(or has nothing to do), so no GPU is needed."""
+import ctypes
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+P = 4096  # an address that is aligned and never read
+
+
+def call(engine, name, order, good, **change):
+    a = {**good, **change}
+    assert set(change) <= set(good)
+    return getattr(engine.lib(), name)(*[a[k] for k in order])
+
+
+TABLES = dict(lens=P, new_lens=P, batch=4, tables=P, width=8, table_stride=8, free=P,
+              free_count=P, num_blocks=64, block_size=16, kv_lens=P, starts=P, slots=P, tokens=9,
+              free_left=P, status=P, stream=None)
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"block_size": 8}, "UNSUPPORTED"), ({"block_size": 48}, "UNSUPPORTED"),
+    ({"batch": 16385}, "UNSUPPORTED"), ({"batch": -1}, "INVALID_ARG"),
+    ({"width": -1}, "INVALID_ARG"), ({"table_stride": 7}, "INVALID_ARG"),
+    ({"num_blocks": 0}, "INVALID_ARG"), ({"num_blocks": 2 ** 27}, "INVALID_ARG"),
+    ({"tokens": -1}, "INVALID_ARG"),
+    *[({k: None}, "INVALID_ARG") for k in ("lens", "new_lens", "tables", "free", "free_count",
+                                           "kv_lens", "starts", "slots", "free_left", "status")],
+])
+def test_block_tables_refusals(engine, change, code):
+    assert call(engine, "attn_block_tables", TABLES, TABLES, **change) == engine.ERR[code]
+
+
+TRIM = dict(lens=P, keep=P, batch=4, tables=P, width=8, table_stride=8, free=P, free_count=P,
+            num_blocks=64, block_size=16, lens_left=P, free_left=P, status=P, stream=None)
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"block_size": 24}, "UNSUPPORTED"), ({"batch": 16385}, "UNSUPPORTED"),
+    ({"batch": -2}, "INVALID_ARG"), ({"table_stride": 3}, "INVALID_ARG"),
+    ({"num_blocks": -1}, "INVALID_ARG"),
+    *[({k: None}, "INVALID_ARG") for k in ("lens", "keep", "tables", "free", "free_count",
+                                           "lens_left", "free_left", "status")],
+])
+def test_block_trim_refusals(engine, change, code):
+    assert call(engine, "attn_block_trim", TRIM, TRIM, **change) == engine.ERR[code]
+
+
+APPEND = dict(k=P, k_token=256, k_head=128, v=P, v_token=256, v_head=128, slots=P, tokens=5,
+              kv_heads=2, D=128, dtype=0, k_codes=P, v_codes=P, k_scale=P, v_scale=P, code=0,
+              num_blocks=64, block_size=16, stream=None)
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"D": 96}, "UNSUPPORTED"), ({"dtype": 2}, "UNSUPPORTED"), ({"code": 2}, "UNSUPPORTED"),
+    ({"block_size": 256}, "UNSUPPORTED"), ({"tokens": -1}, "INVALID_ARG"),
+    ({"kv_heads": 0}, "INVALID_ARG"), ({"kv_heads": 65536}, "INVALID_ARG"),
+    ({"num_blocks": 2 ** 27}, "INVALID_ARG"), ({"k": P + 8}, "MISALIGNED"),
+    ({"v": P + 2}, "MISALIGNED"), ({"k_codes": P + 8}, "MISALIGNED"),
+    ({"k_token": 260}, "MISALIGNED"), ({"v_head": 4}, "MISALIGNED"),
+    *[({k: None}, "INVALID_ARG") for k in ("k", "v", "slots", "k_codes", "v_codes", "k_scale",
+                                           "v_scale")],
+])
+def test_cache_append_refusals(engine, change, code):
+    assert call(engine, "attn_cache_append", APPEND, APPEND, **change) == engine.ERR[code]
+
+
+def test_cache_append_of_nothing(engine):
+    assert call(engine, "attn_cache_append", APPEND, APPEND, tokens=0, k=None) == 0
+
+
+ATTN = dict(q=P, q_token=512, q_head=128, out=P, o_token=512, o_head=128, tokens=3, heads=4,
+            kv_heads=2, D=128, dtype=1, k_codes=P, v_codes=P, k_scale=P, v_scale=P, code=1,
+            num_blocks=64, block_size=32, tables=P, width=8, table_stride=8, kv_lens=P, starts=P,
+            batch=3, max_new=1, causal=1, scale=0.0, workspace=P, workspace_bytes=1 << 30,
+            stream=None)
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"D": 256}, "UNSUPPORTED"), ({"dtype": -1}, "UNSUPPORTED"), ({"code": 7}, "UNSUPPORTED"),
+    ({"block_size": 0}, "UNSUPPORTED"), ({"heads": 5}, "INVALID_ARG"),
+    ({"heads": 0}, "INVALID_ARG"), ({"kv_heads": -2}, "INVALID_ARG"),
+    ({"tokens": -1}, "INVALID_ARG"), ({"batch": -1}, "INVALID_ARG"),
+    ({"max_new": -1}, "INVALID_ARG"), ({"max_new": 2 ** 31 - 1}, "INVALID_ARG"),
+    ({"table_stride": 7}, "INVALID_ARG"), ({"scale": -1.0}, "INVALID_ARG"),
+    ({"scale": float("nan")}, "INVALID_ARG"), ({"scale": float("inf")}, "INVALID_ARG"),
+    ({"q": P + 8}, "MISALIGNED"), ({"out": P + 2}, "MISALIGNED"), ({"q_token": 516}, "MISALIGNED"),
+    ({"o_head": 132}, "MISALIGNED"), ({"workspace": P + 4}, "MISALIGNED"),
+    *[({k: None}, "INVALID_ARG") for k in ("q", "out", "k_codes", "v_codes", "k_scale", "v_scale",
+                                           "tables", "kv_lens", "starts", "workspace")],
+])
+def test_attn_cached_refusals(engine, change, code):
+    assert call(engine, "attn_cached", ATTN, ATTN, **change) == engine.ERR[code]
+
+
+@pytest.mark.parametrize("change", [{"tokens": 0}, {"batch": 0}, {"max_new": 0}])
+def test_attn_cached_of_nothing(engine, change):
+    assert call(engine, "attn_cached", ATTN, ATTN, q=None, **change) == 0
+
+
+@pytest.mark.parametrize("args,code", [((4, 3, 64, 1), "INVALID_ARG"), ((4, 0, 64, 1), "INVALID_ARG"),
+                                       ((4, 2, 80, 1), "UNSUPPORTED"), ((4, 2, 64, -1), "INVALID_ARG")])
+def test_workspace_refusals(engine, args, code):
+    out = ctypes.c_ulonglong()
+    assert engine.lib().attn_cached_workspace(*args, ctypes.byref(out)) == engine.ERR[code]
+    assert engine.lib().attn_cached_workspace(4, 2, 64, 1, None) == engine.ERR["INVALID_ARG"]
+
+
+def test_python_face_refuses_cpu_tensors_and_shapes(engine):
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.int8)
+    s = torch.ones(4, 2)
+    with pytest.raises(ValueError, match="CUDA"):
+        engine.PagedCache(k, k, s, s)
+    with pytest.raises(TypeError):
+        engine.PagedCache(k.half(), k.half(), s, s)
+    with pytest.raises(ValueError):
+        engine.PagedCache(k[:, :, :8], k[:, :, :8], s, s)
+    with pytest.raises(ValueError):
+        engine.PagedCache(k, k[:2], s, s)
+    with pytest.raises(ValueError, match="CUDA"):
+        engine.BlockPool(torch.zeros(4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 16)
