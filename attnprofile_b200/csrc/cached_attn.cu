@@ -5,6 +5,10 @@
 
 using namespace attnprof::cache;
 
+namespace {
+constexpr long long kSplitRows = 64;
+}
+
 extern "C" int attn_cached(const void* q, long long q_token_stride, long long q_head_stride,
                            void* out, long long out_token_stride, long long out_head_stride,
                            int tokens, int heads, int kv_heads, int D, int dtype,
@@ -57,9 +61,21 @@ extern "C" int attn_cached(const void* q, long long q_token_stride, long long q_
   p.scale_log2 = static_cast<float>(
       (scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(D))) *
       1.4426950408889634);
-  p.rows_most = LLONG_MAX;
-  return launch_split(p, D, dtype, code, max_new, workspace, workspace_bytes,
-                      static_cast<cudaStream_t>(stream));
+  // Rows of one request and kv head: up to kSplitRows the keys' bytes are what
+  // counts and the split kernel reads them with every SM; above, the tiled one.
+  // A batch may hold both kinds (the lengths are on the GPU): then both run,
+  // each on its own requests.  A single request, or none that can be long,
+  // needs one launch.
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long most = static_cast<long long>(max_new) * p.group;
+  if (most <= kSplitRows) {
+    p.rows_most = LLONG_MAX;
+    return launch_split(p, D, dtype, code, max_new, workspace, workspace_bytes, st);
+  }
+  p.rows_most = batch == 1 ? 0 : kSplitRows;
+  const int rt = launch_tiled(p, D, dtype, code, st);
+  if (rt != ATTN_OK || batch == 1) return rt;
+  return launch_split(p, D, dtype, code, max_new, workspace, workspace_bytes, st);
 }
 
 extern "C" int attn_cached_workspace(int heads, int kv_heads, int D, int max_new,

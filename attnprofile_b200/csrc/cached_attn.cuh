@@ -35,6 +35,7 @@ __device__ __forceinline__ Request request_at(const CachedParams& p, int r) {
 
 int launch_split(const CachedParams& p, int D, int dtype, int code, int max_new, void* ws,
                  unsigned long long ws_bytes, cudaStream_t st);
+int launch_tiled(const CachedParams& p, int D, int dtype, int code, cudaStream_t st);
 int split_workspace(int group, int D, int max_new, unsigned long long* bytes);
 
 }  // namespace cache

@@ -1,0 +1,663 @@
+// Attention over the 8-bit cache for many query rows a request (prompts and
+// chunks of them): the tensor cores' rate bounds it, 4 D operations a visible
+// (row, key).
+//
+// One CTA takes 256 query rows (token x head of the group, so grouped heads
+// share every key and value) of one request and kv head: two tiles of 128 rows
+// whose softmax steps take turns, as in the dense kernel of this library.  Per
+// 128 keys:
+//   * a warpgroup reads the codes (through L2: the row tiles of a head follow
+//     each other), turns them into f16 and writes them into a ring of shared
+//     memory tiles in the tensor cores' 128-byte swizzle: 8 bits to 16 once for
+//     256 rows.  The codes of the next tile are on their way meanwhile.
+//   * one thread issues tcgen05.mma: S = Q K^T and O += P V, sums in tensor
+//     memory, P read from there too (it overwrites S);
+//   * a warpgroup per tile runs the online softmax, a thread a row, and moves O
+//     to a new maximum only when that grew by more than 2^8.
+//
+// Scales.  K's multiplies the scores in f32, 16 keys at a time (no block is
+// smaller).  V's must act before the sum over keys: V is held as code * s / r
+// * 2^7 (int8: 2^8) in f16, r being the largest V scale of the blocks that the
+// unit sees, found first.  For powers of two that is exact down to s = 2^-22 r
+// (code and factor only meet f16's end below), and what is lost below is under
+// 2^-32 of the largest value that block r could hold; other scales round V to
+// f16 once.  P is rounded to f16 as in the split kernel, held as 2^7 p with p
+// up to 2^8 between two moves of the maximum.  bf16 queries become f16 times
+// a power of two per row.
+#include "attn_kernel.cuh"
+#include "cached_attn.cuh"
+
+namespace attnprof {
+int* device_status_ptr();
+unsigned long long current_timeout_ns();
+
+namespace cache {
+namespace {
+
+constexpr int kBM = 128;                 // rows of a tile
+constexpr int kBN = 128;                 // keys of a step
+constexpr int kUnit = 2 * kBM;           // rows of a CTA
+constexpr int kThreads = 512;            // 2 softmax warpgroups, 1 converting, 1 with the issuer
+constexpr int kScaleRing = 8;            // steps whose K scales are kept (see convert_role)
+constexpr float kMove = 8.f;             // growth of the maximum (log2) that moves O
+constexpr float kLift = 7.f;             // P is held as 2^kLift p
+
+template <int D>
+struct Tile {
+  static constexpr int kBytes = kBN * D * 2;        // one tile in 16 bits
+  static constexpr int kBlock = kBN * 128;          // its 64-column blocks
+  static constexpr int kSlots = D == 128 ? 5 : 8;   // of the ring
+  static constexpr int kOffKv = 2 * kBytes;
+  static constexpr int kOffScale = kOffKv + kSlots * kBytes;        // [kScaleRing][12] f32
+  static constexpr int kOffBar = kOffScale + kScaleRing * 12 * 4;
+  static constexpr int kBars = 2 * kSlots + 2 + 2 + 4 + 2 + 1;
+  static constexpr int kOffMisc = kOffBar + 8 * kBars;
+  static constexpr int kSmem = kOffMisc + 32 + 1024;                // + alignment
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+// Barriers.
+template <int D>
+struct Bar {
+  static constexpr int kFull = 0;
+  static constexpr int kEmpty = Tile<D>::kSlots;
+  static constexpr int kQ = 2 * Tile<D>::kSlots;
+  static constexpr int kS = kQ + 2;
+  static constexpr int kP = kS + 2;       // [tile][part]
+  static constexpr int kO = kP + 4;
+  static constexpr int kDrain = kO + 2;
+};
+
+struct Unit {
+  Request rq;
+  int request, kvh, row0, rows_in, steps, kv_end;
+};
+
+struct TiledParams : CachedParams {
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+__device__ __forceinline__ long long units_of(const CachedParams& p, const Request& r) {
+  const long long rows = static_cast<long long>(r.n) * p.group;
+  return rows > p.rows_most ? p.kv_heads * ((rows + kUnit - 1) / kUnit) : 0;
+}
+
+// Tokens that a row sees.
+__device__ __forceinline__ int row_limit(const CachedParams& p, const Request& rq, int row) {
+  const int last = p.causal ? rq.kv - rq.n + row / p.group + 1 : rq.kv;
+  return min(max(last, 0), rq.kv);
+}
+
+// The unit of this CTA.  Units are taken from the last to the first, and
+// within a request the heads of a row tile follow each other: causal rows
+// that see most keys begin first, and neighbours share keys in L2.
+__device__ bool find_unit(const CachedParams& p, Unit& u) {
+  __shared__ long long warp_sum[kThreads / 32];
+  __shared__ long long where[2];
+  const int each = (p.batch + kThreads - 1) / kThreads;
+  const int first = static_cast<int>(threadIdx.x) * each;
+  long long sum = 0;
+  for (int r = first; r < min(first + each, p.batch); ++r) sum += units_of(p, request_at(p, r));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long in = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long a = __shfl_up_sync(~0u, in, d);
+    if (lane >= d) in += a;
+  }
+  if (lane == 31) warp_sum[warp] = in;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  const long long mine = before + in - sum;  // units in front of this thread's requests
+  const long long at = total - 1 - static_cast<long long>(blockIdx.x);
+  if (at < 0) return false;
+  if (at >= mine && at < mine + sum) {
+    long long b = mine;
+    int r = first;
+    for (;; ++r) {
+      const long long n = units_of(p, request_at(p, r));
+      if (at < b + n || r + 1 >= min(first + each, p.batch)) break;
+      b += n;
+    }
+    where[0] = r;
+    where[1] = at - b;
+  }
+  __syncthreads();
+  u.request = static_cast<int>(where[0]);
+  u.rq = request_at(p, u.request);
+  const int in_request = static_cast<int>(where[1]);
+  u.kvh = in_request % p.kv_heads;
+  u.row0 = in_request / p.kv_heads * kUnit;
+  u.rows_in = u.rq.n * p.group;
+  u.kv_end = row_limit(p, u.rq, min(u.row0 + kUnit, u.rows_in) - 1);
+  u.steps = (u.kv_end + kBN - 1) / kBN;
+  return true;
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z,
+                                             uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, __half2 b) {
+  const __half2 h = __hmul2(*reinterpret_cast<__half2*>(&a), b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ uint32_t half2_of(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ---------------------------------------------------------------------------
+// Converting warpgroup: items K_0, V_0, K_1, V_1, ... through the ring.
+// ---------------------------------------------------------------------------
+template <int CODE, int D>
+__device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase, uint8_t* sgen,
+                             const WaitCtx& w) {
+  using T = Tile<D>;
+  constexpr int kIters = D / 16;          // 16-byte pieces of codes a thread has of a tile
+  constexpr float kVLift = CODE == ATTN_CODE_E4M3 ? 128.f : 256.f;
+  auto bar = [&](int i) { return sbase + T::kOffBar + 8u * i; };
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
+  const int* table = p.tables + u.request * p.table_stride;
+  float* misc = reinterpret_cast<float*>(sgen + T::kOffMisc);
+  auto valid = [&](int id) { return id >= 0 && id < p.num_blocks; };
+
+  // The largest V scale in sight.
+  float ref = 0.f;
+  const int blocks = (u.kv_end + (1 << p.shift) - 1) >> p.shift;
+  for (int b = 32 * warp + lane; b < blocks; b += 128) {
+    const int id = table[b];
+    if (valid(id)) ref = fmaxf(ref, p.vs[static_cast<long long>(id) * p.kv_heads + u.kvh]);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) ref = fmaxf(ref, __shfl_xor_sync(~0u, ref, d));
+  if (lane == 0) misc[4 + warp] = ref;
+  ptx::named_bar_sync(1, 128);
+  ref = fmaxf(fmaxf(misc[4], misc[5]), fmaxf(misc[6], misc[7]));
+  if (!(ref > 0.f)) ref = 1.f;
+  if (warp == 0 && lane == 0) misc[2] = ref / kVLift;  // what O is multiplied by
+  const float to_v = kVLift / ref;
+
+  // Lane g < 8 holds what concerns keys 16 g .. 16 g + 15 of a step.
+  auto ids_of = [&](int j) {
+    const int key = j * kBN + 16 * lane;
+    if (j < u.steps && lane < 8 && key < u.rq.kv) {
+      const int id = table[key >> p.shift];
+      if (valid(id)) return id;
+    }
+    return -1;
+  };
+  // A thread's piece `it` of a tile: row and 16-byte piece of that row, so that
+  // global reads cover whole rows and, in the 16-bit tile, the 8 lanes of
+  // one shared memory pass hit 8 different 16-byte banks.
+  auto row_of = [&](int it) {
+    return D == 128 ? 16 * it + 4 * warp + 2 * (lane >> 4) + ((lane >> 2) & 1)
+                    : 32 * it + 8 * warp + (lane >> 2);
+  };
+  const int piece = D == 128 ? (lane & 3) + 4 * (((lane >> 2) ^ (lane >> 3)) & 1) : lane & 3;
+  auto group_of = [&](int it) { return D == 128 ? it : 2 * it + (warp >> 1); };
+
+  uint4 c[kIters];
+  auto load = [&](int it, int j, bool is_v, int ids) {
+    const int id = __shfl_sync(~0u, ids, group_of(it));
+    const int row = row_of(it), key = j * kBN + row;
+    c[it] = make_uint4(0, 0, 0, 0);
+    // (keys behind the last token may be any bits: masked in the scores, and
+    // zero among the values, where 0 * NaN would reach a sum)
+    if (id >= 0 && (!is_v || key < u.rq.kv)) {
+      const long long at =
+          (((static_cast<long long>(id) * p.kv_heads + u.kvh) << p.shift) +
+           (key & ((1 << p.shift) - 1))) * D + 16 * piece;
+      c[it] = __ldg(reinterpret_cast<const uint4*>((is_v ? p.vc : p.kc) + at));
+    }
+  };
+
+  int ids = ids_of(0), ids_next = ids_of(1);
+  float ks = 0.f, vs = 0.f;  // of this lane's group, for the step being converted
+  auto scales_of = [&](int id) {
+    const long long at = static_cast<long long>(id) * p.kv_heads + u.kvh;
+    ks = id >= 0 ? p.ks[at] * p.scale_log2 : -1.f;  // -1: not a block of the pool
+    vs = id >= 0 ? p.vs[at] * to_v : 0.f;
+  };
+  scales_of(ids);
+#pragma unroll
+  for (int it = 0; it < kIters; ++it) load(it, 0, false, ids);
+
+  for (int t = 0; t < 2 * u.steps; ++t) {
+    const bool is_v = (t & 1) != 0;
+    const int j = t >> 1;
+    const int slot = t % T::kSlots;
+    const bool ok = wait_bar(bar(Bar<D>::kEmpty + slot), ((t / T::kSlots) & 1) ^ 1, w, kSiteKvEmpty);
+    if (!__all_sync(~0u, ok)) return;
+    const uint32_t tile = sbase + T::kOffKv + slot * T::kBytes;
+    if (!is_v && warp == 0) {
+      // K scales of the step.  The place's last reader was the softmax of step
+      // j - kScaleRing; this slot came free after P V of a later step.
+      float* dst = reinterpret_cast<float*>(sgen + T::kOffScale) + (j % kScaleRing) * 12;
+      const bool hole = lane < 8 && ks == -1.f && j * kBN + 16 * lane < u.rq.kv;
+      const unsigned holes = __ballot_sync(~0u, hole);
+      if (lane < 8) dst[lane] = ks;
+      if (lane == 8) dst[8] = __uint_as_float(holes);
+    }
+    // The next item's codes replace this one's as they are used up.
+    const bool more = t + 1 < 2 * u.steps;
+    const int ids_load = is_v ? ids_next : ids;
+#pragma unroll
+    for (int it = 0; it < kIters; ++it) {
+      uint32_t h[8];
+      const uint32_t word[4] = {c[it].x, c[it].y, c[it].z, c[it].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        h[2 * i] = Code<CODE>::half2_lo(word[i]);
+        h[2 * i + 1] = Code<CODE>::half2_hi(word[i]);
+      }
+      if (is_v) {
+        const float f = __shfl_sync(~0u, vs, group_of(it));
+        if ((__float_as_int(f) & 0x7fffff) == 0) {  // a power of two (or 0)
+          const __half2 f2 = __float2half2_rn(f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[i] = mul_half2(h[i], f2);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 x = half2_to_float2(h[i]);
+            h[i] = half2_of(x.x * f, x.y * f);
+          }
+        }
+      }
+      if (more) load(it, (t + 1) >> 1, !is_v, ids_load);
+      const int row = row_of(it);
+      const uint32_t base = tile + (piece >> 2) * T::kBlock + row * 128;
+      const int k16 = (2 * piece) & 7;
+      st_shared_v4(base + (((k16) ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
+      st_shared_v4(base + (((k16 + 1) ^ (row & 7)) << 4), h[4], h[5], h[6], h[7]);
+    }
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar(Bar<D>::kFull + slot));
+    if (is_v) {
+      ids = ids_next;
+      scales_of(ids);
+      ids_next = ids_of(j + 2);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The issuer: one thread, both tiles' MMAs in turn.
+// ---------------------------------------------------------------------------
+template <int D>
+__device__ void mma_role(const Unit& u, uint32_t tmem, uint32_t sbase, const WaitCtx& w) {
+  using T = Tile<D>;
+  auto bar = [&](int i) { return sbase + T::kOffBar + 8u * i; };
+  constexpr uint32_t kIdescS = ptx::idesc_f16(kBM, kBN, false, false);
+  constexpr uint32_t kIdescPV = ptx::idesc_f16(kBM, D, false, true);
+  const int tiles = u.rows_in - u.row0 > kBM ? 2 : 1;
+  const int n = u.steps;
+  uint64_t qd[2];
+  for (int i = 0; i < 2; ++i) qd[i] = ptx::smem_desc_sw128(sbase + i * T::kBytes, 16, 1024);
+  const uint64_t kd0 = ptx::smem_desc_sw128(sbase + T::kOffKv, 16, 1024);
+  const uint64_t vd0 = ptx::smem_desc_sw128(sbase + T::kOffKv, T::kBlock, 1024);
+  auto slot_off = [](int t) { return static_cast<uint32_t>((t % T::kSlots) * T::kBytes) >> 4; };
+  auto ring_wait = [&](int t) {
+    const bool ok = wait_bar(bar(Bar<D>::kFull + t % T::kSlots), (t / T::kSlots) & 1, w, kSiteKvFull);
+    if (ok) ptx::tc_fence_after();
+    return ok;
+  };
+  auto issue_s = [&](int i, int t) {
+    const uint64_t kd = ptx::desc_add(kd0, slot_off(t));
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint32_t off = static_cast<uint32_t>((kk >> 2) * T::kBlock + (kk & 3) * 32) >> 4;
+      ptx::mma_ss(tmem + i * kBN, ptx::desc_add(qd[i], off), ptx::desc_add(kd, off), kIdescS,
+                  kk > 0 ? 1u : 0u);
+    }
+  };
+  auto issue_pv = [&](int i, int j, int t, int k0, int k1) {
+    const uint64_t vd = ptx::desc_add(vd0, slot_off(t));
+#pragma unroll
+    for (int kk = k0; kk < k1; ++kk)
+      ptx::mma_ts(tmem + 2 * kBN + i * D, tmem + i * kBN + kk * 8,
+                  ptx::desc_add(vd, static_cast<uint32_t>(kk * 2048) >> 4), kIdescPV,
+                  (j > 0 || kk > 0) ? 1u : 0u);
+  };
+
+  bool ok = n > 0 && ring_wait(0);
+  for (int i = 0; i < tiles && ok; ++i) {
+    if (!(ok = wait_bar(bar(Bar<D>::kQ + i), 0, w, kSiteQ))) break;
+    ptx::tc_fence_after();
+    issue_s(i, 0);
+    ptx::mma_commit(bar(Bar<D>::kS + i));
+  }
+  if (ok) ptx::mma_commit(bar(Bar<D>::kEmpty));
+  for (int j = 0; j < n && ok; ++j) {
+    const int tv = 2 * j + 1, tk = 2 * j + 2;
+    if (!(ok = ring_wait(tv))) break;
+    for (int i = 0; i < tiles && ok; ++i) {
+      if (!(ok = wait_bar(bar(Bar<D>::kP + 2 * i), j & 1, w, kSitePReady))) break;
+      ptx::tc_fence_after();
+      issue_pv(i, j, tv, 0, 6);
+      if (i == 0 && j + 1 < n && !(ok = ring_wait(tk))) break;
+      if (!(ok = wait_bar(bar(Bar<D>::kP + 2 * i + 1), j & 1, w, kSitePReady))) break;
+      ptx::tc_fence_after();
+      issue_pv(i, j, tv, 6, 8);
+      if (j + 1 < n) {
+        issue_s(i, tk);
+        ptx::mma_commit(bar(Bar<D>::kS + i));  // covers this step's P V too
+      } else {
+        ptx::mma_commit(bar(Bar<D>::kO + i));
+      }
+    }
+    if (!ok) break;
+    ptx::mma_commit(bar(Bar<D>::kEmpty + tv % T::kSlots));
+    if (j + 1 < n) ptx::mma_commit(bar(Bar<D>::kEmpty + tk % T::kSlots));
+  }
+  // Every MMA issued here has ended before tensor memory is freed.
+  ptx::mma_commit(bar(Bar<D>::kDrain));
+  const unsigned long long t0 = ptx::globaltimer_ns();
+  while (!ptx::mbar_try_wait(bar(Bar<D>::kDrain), 0)) {
+    if (ptx::globaltimer_ns() - t0 > w.timeout_ns) {
+      if (w.status) atomicCAS(w.status, 0, kDeviceTimeoutBase + kSiteDrain);
+      break;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Softmax warpgroup of tile i: a thread a row.
+// ---------------------------------------------------------------------------
+template <typename TQ, int D>
+__device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_t tmem,
+                             uint32_t sbase, const uint8_t* sgen, const WaitCtx& w) {
+  using T = Tile<D>;
+  auto bar = [&](int b) { return sbase + T::kOffBar + 8u * b; };
+  const int lane = threadIdx.x & 31, wi = (threadIdx.x >> 5) & 3;
+  const int r = 32 * wi + lane;                 // row of the tile, lane of tensor memory
+  const int row = u.row0 + i * kBM + r;
+  const bool live = row < u.rows_in;
+  const int tok = live ? row / p.group : 0;
+  const int head = u.kvh * p.group + (live ? row - tok * p.group : 0);
+  const int limit = live ? row_limit(p, u.rq, row) : 0;
+  const bool tile_there = u.row0 + i * kBM < u.rows_in;
+
+  // Q: this row to shared memory, in f16.
+  float row_f = 1.f;
+  if (tile_there && u.steps > 0) {
+    const TQ* q = static_cast<const TQ*>(p.q) + (u.rq.start + tok) * p.q_token + head * p.q_head;
+    if constexpr (std::is_same<TQ, __nv_bfloat16>::value) {
+      uint32_t top = 0;
+      if (live) {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 x = __ldg(reinterpret_cast<const uint4*>(q) + c);
+          top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                                       __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+        }
+      }
+      top = max(top & 0xffffu, top >> 16);
+      const int e = static_cast<int>(top >> 7) - 127;
+      if (top > 0 && e < 128) row_f = power_of_two(min(max(e - 14, -112), 112));
+    }
+    const float inv = 1.f / row_f;
+    const uint32_t base = sbase + i * T::kBytes + r * 128;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
+      if constexpr (std::is_same<TQ, __nv_bfloat16>::value) {
+        uint32_t* y = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          y[k] = half2_of(__uint_as_float(y[k] << 16) * inv,
+                          __uint_as_float(y[k] & 0xffff0000u) * inv);
+      }
+      st_shared_v4(base + (c >> 3) * T::kBlock + (((c & 7) ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
+    }
+    ptx::fence_proxy_async_smem();
+    ptx::mbar_arrive(bar(Bar<D>::kQ + i));
+  }
+
+  const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * wi) << 16);
+  const uint32_t s_col = i * kBN, o_col = 2 * kBN + i * D;
+  float m = -INFINITY, l = 0.f;  // maximum in log2 units, sum of 2^kLift p
+  bool ok = true;
+  for (int j = 0; j < u.steps && tile_there; ++j) {
+    ok = __all_sync(~0u, wait_bar(bar(Bar<D>::kS + i), j & 1, w, kSiteSFull));
+    if (!ok) break;
+    ptx::tc_fence_after();
+    uint32_t s[kBN];
+#pragma unroll
+    for (int c = 0; c < kBN / 32; ++c)
+      ptx::tmem_ld32(lane_base + s_col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+    const float* ks = reinterpret_cast<const float*>(sgen + T::kOffScale) + (j % kScaleRing) * 12;
+    const uint32_t holes = __float_as_uint(ks[8]);
+    const int lim = limit - j * kBN;  // columns below it are seen
+    ptx::tmem_wait_ld();
+    ptx::reg_fence(s);
+    if (__any_sync(~0u, lim < kBN) || holes != 0) {
+#pragma unroll
+      for (int c = 0; c < kBN; ++c)
+        if (c >= lim || ((holes >> (c / 16)) & 1u)) s[c] = __float_as_uint(-INFINITY);
+    }
+    // Factor of group g's scores.  That of a group which the row does not see
+    // may be anything (NaN): 1 keeps -inf there.  The least factor keeps
+    // -inf too, where ks * row_f may reach 0 (f16 products are below 2^32, so
+    // scores that small are 0 either way); NaN stays.
+    auto factor = [&](int g) {
+      float f = ks[g] * row_f;
+      if (f < 0x1p-90f) f = 0x1p-90f;
+      return (16 * g >= lim || ((holes >> g) & 1u)) ? 1.f : f;
+    };
+    float top = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < kBN / 16; ++g) {
+      float a[5];
+#pragma unroll
+      for (int k = 0; k < 5; ++k)
+        a[k] = ptx::fmax3(__uint_as_float(s[16 * g + 3 * k]), __uint_as_float(s[16 * g + 3 * k + 1]),
+                          __uint_as_float(s[16 * g + 3 * k + 2]));
+      const float b = ptx::fmax3(a[0], a[1], a[2]);
+      const float d = ptx::fmax3(a[3], a[4], __uint_as_float(s[16 * g + 15]));
+      top = fmaxf(top, fmaxf(b, d) * factor(g));
+    }
+    float alpha = 1.f;
+    bool move = false;
+    if (j == 0) {
+      m = top;
+    } else if (top - m > kMove) {
+      alpha = ptx::ex2_approx(m - top);
+      m = top;
+      move = true;
+    }
+    if (__any_sync(~0u, move)) {
+      // O holds the sum through the step before (S was issued behind its P V).
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        ptx::tmem_ld32(lane_base + o_col + 32 * c, o);
+        ptx::tmem_wait_ld();
+        ptx::reg_fence(o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+        ptx::tmem_st32(lane_base + o_col + 32 * c, o);
+      }
+    }
+    const float neg = m == -INFINITY ? 0.f : kLift - m;
+    const uint64_t neg2 = ptx::f2_pack(neg, neg);
+    uint64_t part[2] = {0ull, 0ull};
+#pragma unroll
+    for (int c = 0; c < kBN / 32; ++c) {
+      uint32_t pk[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int c0 = 32 * c + 2 * e;
+        const float f = factor(c0 / 16);
+        const uint64_t x2 = ptx::f2_fma(
+            ptx::f2_pack(__uint_as_float(s[c0]), __uint_as_float(s[c0 + 1])), ptx::f2_pack(f, f),
+            neg2);
+        float x0, x1;
+        ptx::f2_unpack(x2, x0, x1);
+        const float p0 = ptx::ex2_approx(x0), p1 = ptx::ex2_approx(x1);
+        part[e & 1] = ptx::f2_add(part[e & 1], ptx::f2_pack(p0, p1));
+        pk[e] = half2_of(p0, p1);
+      }
+      ptx::tmem_st16(lane_base + s_col + 16 * c, pk);
+      if (c == 2) {  // P V of 96 keys may begin
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(bar(Bar<D>::kP + 2 * i));
+      }
+    }
+    ptx::tmem_wait_st();
+    ptx::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar(Bar<D>::kP + 2 * i + 1));
+    float sa, sb, sc, sd;
+    ptx::f2_unpack(part[0], sa, sb);
+    ptx::f2_unpack(part[1], sc, sd);
+    l = l * alpha + ((sa + sb) + (sc + sd));
+  }
+
+  if (!tile_there || !ok) return;
+  float f = 0.f;
+  if (u.steps > 0) {
+    if (!__all_sync(~0u, wait_bar(bar(Bar<D>::kO + i), 0, w, kSiteODone))) return;
+    ptx::tc_fence_after();
+    if (m != -INFINITY || l != l)
+      f = reinterpret_cast<const float*>(sgen + T::kOffMisc)[2] / l;
+  }
+  TQ* out = static_cast<TQ*>(p.out) + (u.rq.start + tok) * p.o_token + head * p.o_head;
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    if (u.steps > 0) {
+      ptx::tmem_ld32(lane_base + o_col + 32 * c, o);
+      ptx::tmem_wait_ld();
+      ptx::reg_fence(o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = 0u;
+    }
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          y[e] = pack2<TQ>(__uint_as_float(o[8 * k + 2 * e]) * f,
+                           __uint_as_float(o[8 * k + 2 * e + 1]) * f);
+        *reinterpret_cast<uint4*>(out + 32 * c + 8 * k) = make_uint4(y[0], y[1], y[2], y[3]);
+      }
+    }
+  }
+}
+
+template <typename TQ, int CODE, int D>
+__global__ void __launch_bounds__(kThreads, 1) tiled_kernel(const TiledParams p) {
+#if defined(__CUDA_ARCH_FEAT_SM100_ALL)
+  using T = Tile<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;
+  uint8_t* sgen = smem_raw + (sbase - raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Unit u;
+  if (!find_unit(p, u)) return;
+
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + T::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + T::kOffMisc + 4);
+  if (threadIdx.x == 0) {
+    auto bar = [&](int i) { return sbase + T::kOffBar + 8u * i; };
+    for (int s = 0; s < T::kSlots; ++s) {
+      ptx::mbar_init(bar(Bar<D>::kFull + s), 4);
+      ptx::mbar_init(bar(Bar<D>::kEmpty + s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(bar(Bar<D>::kQ + i), kBM);
+      ptx::mbar_init(bar(Bar<D>::kS + i), 1);
+      ptx::mbar_init(bar(Bar<D>::kP + 2 * i), 4);
+      ptx::mbar_init(bar(Bar<D>::kP + 2 * i + 1), 4);
+      ptx::mbar_init(bar(Bar<D>::kO + i), 1);
+    }
+    ptx::mbar_init(bar(Bar<D>::kDrain), 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  if (warp == 12) {
+    ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const WaitCtx w{abort_flag, p.status, p.timeout_ns};
+
+  // Registers of the four warpgroups: 128 x (2 * 184 + 96 + 48) = 512 * 128.
+  if (warp < 8) {
+    ptx::setmaxnreg_inc<184>();
+    softmax_role<TQ, D>(p, u, warp >> 2, tmem, sbase, sgen, w);
+  } else if (warp < 12) {
+    ptx::setmaxnreg_dec<96>();
+    convert_role<CODE, D>(p, u, sbase, sgen, w);
+  } else {
+    ptx::setmaxnreg_dec<48>();
+    if (warp == 12 && lane == 0) mma_role<D>(u, tmem, sbase, w);
+    __syncwarp();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+#endif
+}
+
+template <typename TQ, int CODE, int D>
+int launch(const TiledParams& p, cudaStream_t st) {
+  auto kern = tiled_kernel<TQ, CODE, D>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<D>::kSmem) !=
+      cudaSuccess)
+    return ATTN_ERR_RESOURCE;
+  // Each request's rows end in at most one tile that is not full.
+  const long long units =
+      p.kv_heads * (static_cast<long long>(p.tokens) * p.group / kUnit + p.batch);
+  if (units > INT_MAX) return ATTN_ERR_INVALID_ARG;
+  kern<<<static_cast<unsigned>(units), kThreads, Tile<D>::kSmem, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
+}
+
+template <typename TQ, int CODE>
+int launch_d(const TiledParams& p, int D, cudaStream_t st) {
+  return D == 64 ? launch<TQ, CODE, 64>(p, st) : launch<TQ, CODE, 128>(p, st);
+}
+
+template <typename TQ>
+int launch_code(const TiledParams& p, int D, int code, cudaStream_t st) {
+  return code == ATTN_CODE_E4M3 ? launch_d<TQ, ATTN_CODE_E4M3>(p, D, st)
+                                : launch_d<TQ, ATTN_CODE_INT8>(p, D, st);
+}
+
+}  // namespace
+
+int launch_tiled(const CachedParams& q, int D, int dtype, int code, cudaStream_t st) {
+  TiledParams p;
+  static_cast<CachedParams&>(p) = q;
+  p.status = device_status_ptr();
+  if (p.status == nullptr) return ATTN_ERR_CUDA;
+  p.timeout_ns = current_timeout_ns();
+  return dtype == ATTN_DTYPE_F16 ? launch_code<__half>(p, D, code, st)
+                                 : launch_code<__nv_bfloat16>(p, D, code, st);
+}
+
+}  // namespace cache
+}  // namespace attnprof

@@ -101,6 +101,9 @@ static int dispatch(const void* Q, const void* K, const void* V, void* O, int B,
 // The key-split mode attn_set_split last stored.
 int current_split_mode() { return g_split_mode.load(); }
 
+// The bounded-wait limit that attn_set_timeout_ns last stored.
+unsigned long long current_timeout_ns() { return g_timeout_ns.load(); }
+
 // Launch with a caller-provided workspace and per-call tensor maps (no
 // device or host allocation, never the stream-ordered pool: a plan that
 // needs more than ws_bytes returns ATTN_ERR_SCRATCH_LIMIT); split_mode as
