@@ -31,49 +31,53 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _workspace_bytes: dict = {}
 
 
-class _On:
-    """The device and stream of a call: makes the device current inside."""
-    __slots__ = ("index", "stream", "other", "guard")
-
-    def __init__(self, device, stream):
-        self.index = device.index
-        now = torch.cuda.current_device()
-        if stream is None:
-            self.other = None
-            self.stream = torch.cuda.current_stream(device).cuda_stream
-        else:
-            if stream.device != device:
-                raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-            self.other = stream
-            self.stream = stream.cuda_stream
-        self.guard = torch.cuda.device(device) if now != self.index else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *a):
-        if self.guard is not None:
-            self.guard.__exit__(*a)
-
-    def empty(self, shape, dtype, device):
-        """A new tensor for work on this stream, also used by the current one."""
-        if self.other is None:
-            return torch.empty(shape, dtype=dtype, device=device)
-        with torch.cuda.stream(self.other):
-            x = torch.empty(shape, dtype=dtype, device=device)
-        x.record_stream(torch.cuda.current_stream(device))
-        return x
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
 
 
-def _ints(name, t, device, shape):
+# The same without building a Stream object (2 us less per call), where this
+# torch offers it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _stream(device, stream) -> int:
+    """The stream of a call (default: the current one of the tensors' device)."""
+    if stream is None:
+        return _raw_stream(device.index)
+    if stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+    return stream.cuda_stream
+
+
+def _call(name, device, *args):
+    """A C entry point with the tensors' device current."""
+    if torch.cuda.current_device() == device.index:
+        rc = getattr(lib(), name)(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib(), name)(*args)
+    if rc:
+        _check(rc, name)
+
+
+def _empty(shape, dtype, device, stream):
+    """A new tensor for work on `stream` that the current stream may use too."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        x = torch.empty(shape, dtype=dtype, device=device)
+    x.record_stream(torch.cuda.current_stream(device))
+    return x
+
+
+def _ints(name, t, device, n):
+    """Checks an int32 vector of n; its address."""
     if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous tensor of shape {tuple(shape)}")
+    if t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of shape ({n},)")
     return t.data_ptr()
 
 
@@ -82,12 +86,14 @@ def _table(tables, device, batch):
         raise TypeError("tables must be int32")
     if tables.device != device:
         raise ValueError(f"tables must be on {device}")
-    if tables.dim() != 2 or tables.shape[0] != batch:
+    shape = tables.shape
+    if len(shape) != 2 or shape[0] != batch:
         raise ValueError(f"tables must be [{batch}, width]")
-    width = tables.shape[1]
-    if (width > 1 and tables.stride(1) != 1) or (batch > 1 and tables.stride(0) < width):
+    width = shape[1]
+    row, one = tables.stride()
+    if (width > 1 and one != 1) or (batch > 1 and row < width):
         raise ValueError("rows of tables must be contiguous and may not overlap")
-    return tables.data_ptr(), width, tables.stride(0) if batch > 1 else width
+    return tables.data_ptr(), width, row if batch > 1 else width
 
 
 class PagedCache:
@@ -150,8 +156,8 @@ class BlockPool:
         if block_size not in BLOCK_SIZES:
             raise ValueError(f"block_size {block_size} is not one of {BLOCK_SIZES}")
         self.device, self.num_blocks, self.block_size = free.device, free.numel(), block_size
-        _ints("free", free, self.device, free.shape)
-        _ints("free_count", free_count, self.device, (1,))
+        _ints("free", free, self.device, free.numel())
+        _ints("free_count", free_count, self.device, 1)
         self.free, self.free_count = free, free_count
 
     @classmethod
@@ -188,23 +194,21 @@ def block_tables(pool: BlockPool, lens, new_lens, tables, tokens: int, *, plan=N
     takes it.  All or nothing: plan.status tells (on the device) whether the
     pool, the table rows and the slot map were large enough."""
     device, batch = pool.device, lens.shape[0]
-    on = _On(device, stream)
+    s = _stream(device, stream)
     if plan is None:
-        plan = BlockPlan(on.empty(batch, torch.int32, device),
-                         on.empty(batch + 1, torch.int32, device),
-                         on.empty(tokens, torch.int32, device), on.empty(1, torch.int32, device))
+        plan = BlockPlan(*(_empty(n, torch.int32, device, stream)
+                           for n in (batch, batch + 1, tokens, 1)))
     if free_left is None:
         free_left = pool.free_count
     t, width, stride = _table(tables, device, batch)
-    args = (_ints("lens", lens, device, (batch,)), _ints("new_lens", new_lens, device, (batch,)),
-            batch, t, width, stride, pool.free.data_ptr(), pool.free_count.data_ptr(),
-            pool.num_blocks, pool.block_size, _ints("plan.kv_lens", plan.kv_lens, device, (batch,)),
-            _ints("plan.starts", plan.starts, device, (batch + 1,)),
-            _ints("plan.slots", plan.slots, device, (tokens,)), tokens,
-            _ints("free_left", free_left, device, (1,)),
-            _ints("plan.status", plan.status, device, (1,)))
-    with on as s:
-        _check(lib().attn_block_tables(*args, s), "attn_block_tables")
+    _call("attn_block_tables", device, _ints("lens", lens, device, batch),
+          _ints("new_lens", new_lens, device, batch), batch, t, width, stride,
+          pool.free.data_ptr(), pool.free_count.data_ptr(), pool.num_blocks, pool.block_size,
+          _ints("plan.kv_lens", plan.kv_lens, device, batch),
+          _ints("plan.starts", plan.starts, device, batch + 1),
+          _ints("plan.slots", plan.slots, device, tokens), tokens,
+          _ints("free_left", free_left, device, 1), _ints("plan.status", plan.status, device, 1),
+          s)
     return plan
 
 
@@ -215,34 +219,36 @@ def block_trim(pool: BlockPool, lens, keep, tables, *, lens_left=None, free_left
     itself) and free_left (default: pool.free_count); returns the status word
     [1] (BLOCKS; anything but OK: nothing was changed)."""
     device, batch = pool.device, lens.shape[0]
-    on = _On(device, stream)
+    s = _stream(device, stream)
     if lens_left is None:
         lens_left = lens
     if free_left is None:
         free_left = pool.free_count
     if status is None:
-        status = on.empty(1, torch.int32, device)
+        status = _empty(1, torch.int32, device, stream)
     t, width, stride = _table(tables, device, batch)
-    args = (_ints("lens", lens, device, (batch,)), _ints("keep", keep, device, (batch,)), batch, t,
-            width, stride, pool.free.data_ptr(), pool.free_count.data_ptr(), pool.num_blocks,
-            pool.block_size, _ints("lens_left", lens_left, device, (batch,)),
-            _ints("free_left", free_left, device, (1,)), _ints("status", status, device, (1,)))
-    with on as s:
-        _check(lib().attn_block_trim(*args, s), "attn_block_trim")
+    _call("attn_block_trim", device, _ints("lens", lens, device, batch),
+          _ints("keep", keep, device, batch), batch, t, width, stride, pool.free.data_ptr(),
+          pool.free_count.data_ptr(), pool.num_blocks, pool.block_size,
+          _ints("lens_left", lens_left, device, batch), _ints("free_left", free_left, device, 1),
+          _ints("status", status, device, 1), s)
     return status
 
 
 def _rows(name, x, device, heads, dim):
-    """Checks a [tokens, heads, D] tensor; its dtype code."""
-    if x.dtype not in _DTYPES:
+    """Checks a [tokens, heads, D] tensor; its dtype code, shape and strides."""
+    kind = _DTYPES.get(x.dtype)
+    if kind is None:
         raise TypeError(f"unsupported dtype {x.dtype} of {name} (float16 or bfloat16)")
     if x.device != device:
         raise ValueError(f"{name} must be on {device}")
-    if x.dim() != 3 or x.shape[2] != dim or (heads and x.shape[1] != heads):
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != dim or (heads and shape[1] != heads):
         raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {dim}]")
-    if x.stride(2) != 1:
+    strides = x.stride()
+    if strides[2] != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    return _DTYPES[x.dtype]
+    return kind, shape, strides
 
 
 def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
@@ -256,28 +262,23 @@ def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
     block follow each other with ascending slots (as block_tables gives them),
     and no block appears twice."""
     device = cache.device
-    kind = _rows("k", k, device, cache.kv_heads, cache.dim)
-    if _rows("v", v, device, cache.kv_heads, cache.dim) != kind or v.shape != k.shape:
+    heads, dim = cache.kv_heads, cache.dim
+    kind, shape, (k_token, k_head, _) = _rows("k", k, device, heads, dim)
+    v_kind, v_shape, (v_token, v_head, _) = _rows("v", v, device, heads, dim)
+    if v_kind != kind or v_shape != shape:
         raise ValueError("k and v must share one shape and dtype")
-    tokens = k.shape[0]
-    slot_ptr = _ints("slots", slots, device, (tokens,))
-    kc, vc, ks, vs = cache.ptrs
-    k_token, k_head, _ = k.stride()
-    v_token, v_head, _ = v.stride()
-    with _On(device, stream) as s:
-        _check(lib().attn_cache_append(
-            k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head, slot_ptr, tokens,
-            cache.kv_heads, cache.dim, kind, kc, vc, ks, vs, cache.code, cache.num_blocks,
-            cache.block_size, s), "attn_cache_append")
+    tokens = shape[0]
+    _call("attn_cache_append", device, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token,
+          v_head, _ints("slots", slots, device, tokens), tokens, heads, dim, kind, *cache.ptrs,
+          cache.code, cache.num_blocks, cache.block_size, _stream(device, stream))
 
 
-def _workspace(index, heads, kv_heads, dim, max_new):
-    key = (index, heads, kv_heads, dim, max_new)
+def _workspace(device, heads, kv_heads, dim, max_new) -> int:
+    key = (device.index, heads, kv_heads, dim, max_new)
     n = _workspace_bytes.get(key)
     if n is None:
         out = ctypes.c_ulonglong()
-        _check(lib().attn_cached_workspace(heads, kv_heads, dim, max_new, ctypes.byref(out)),
-               "attn_cached_workspace")
+        _call("attn_cached_workspace", device, heads, kv_heads, dim, max_new, ctypes.byref(out))
         n = _workspace_bytes[key] = out.value
     return n
 
@@ -296,43 +297,42 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     behind starts[-1] are left as they were (with out=None: undefined).
     workspace: a uint8 tensor to use instead of a new one per call; calls that
     may overlap on the GPU need one each."""
-    device = cache.device
-    kind = _rows("q", q, device, 0, cache.dim)
-    tokens, heads, dim = q.shape
-    if heads == 0 or heads % cache.kv_heads:
-        raise ValueError(f"{heads} heads are not a multiple of the cache's {cache.kv_heads}")
-    if scale is not None and not scale > 0:
+    device, kv_heads, dim = cache.device, cache.kv_heads, cache.dim
+    kind, shape, (q_token, q_head, _) = _rows("q", q, device, 0, dim)
+    tokens, heads, _ = shape
+    if heads == 0 or heads % kv_heads:
+        raise ValueError(f"{heads} heads are not a multiple of the cache's {kv_heads}")
+    if scale is None:
+        scale = 0.0
+    elif not scale > 0:
         raise ValueError("scale must be positive")
     if max_new < 0:
         raise ValueError("max_new must not be negative")
     batch = kv_lens.shape[0]
     t, width, stride = _table(tables, device, batch)
-    lens_ptr = _ints("kv_lens", kv_lens, device, (batch,))
-    starts_ptr = _ints("starts", starts, device, (batch + 1,))
-    on = _On(device, stream)
+    lens_ptr = _ints("kv_lens", kv_lens, device, batch)
+    starts_ptr = _ints("starts", starts, device, batch + 1)
+    s = _stream(device, stream)
     if out is None:
-        out = on.empty(q.shape, q.dtype, device)
-    elif _rows("out", out, device, heads, dim) != kind or out.shape != q.shape:
-        raise ValueError("out must have the shape and dtype of q")
-    q_token, q_head, _ = q.stride()
-    o_token, o_head, _ = out.stride()
-    kc, vc, ks, vs = cache.ptrs
-    with on as s:
-        if workspace is None:
-            need = _workspace(on.index, heads, cache.kv_heads, dim, max_new)
-            workspace = on.empty(need, torch.uint8, device)
-        else:
-            if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
-                raise TypeError("workspace must be a contiguous uint8 tensor")
-            if workspace.device != device:
-                raise ValueError(f"workspace must be on {device}")
-            need = workspace.numel()
-        _check(lib().attn_cached(
-            q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head, tokens, heads,
-            cache.kv_heads, dim, kind, kc, vc, ks, vs, cache.code, cache.num_blocks,
-            cache.block_size, t, width, stride, lens_ptr, starts_ptr, batch, max_new,
-            1 if causal else 0, 0.0 if scale is None else scale, workspace.data_ptr(), need, s),
-            "attn_cached")
+        out = _empty(shape, q.dtype, device, stream)
+        o_token, o_head = heads * dim, dim
+    else:
+        o_kind, o_shape, (o_token, o_head, _) = _rows("out", out, device, heads, dim)
+        if o_kind != kind or o_shape != shape:
+            raise ValueError("out must have the shape and dtype of q")
+    if workspace is None:
+        need = _workspace(device, heads, kv_heads, dim, max_new)
+        workspace = _empty(need, torch.uint8, device, stream)
+    else:
+        if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+            raise TypeError("workspace must be a contiguous uint8 tensor")
+        if workspace.device != device:
+            raise ValueError(f"workspace must be on {device}")
+        need = workspace.numel()
+    _call("attn_cached", device, q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head,
+          tokens, heads, kv_heads, dim, kind, *cache.ptrs, cache.code, cache.num_blocks,
+          cache.block_size, t, width, stride, lens_ptr, starts_ptr, batch, max_new,
+          1 if causal else 0, scale, workspace.data_ptr(), need, s)
     return out
 
 
@@ -368,7 +368,7 @@ class CacheBatch:
     def advance(self, new_lens, tokens: int, *, stream=None) -> BlockPlan:
         """new_lens[r] tokens more for request r, in a slot map of `tokens`."""
         if self.plan is None or self.plan.slots.shape[0] != tokens:
-            slots = _On(self.pool.device, stream).empty(tokens, torch.int32, self.pool.device)
+            slots = _empty(tokens, torch.int32, self.pool.device, stream)
             self.plan = BlockPlan(self.lens, self.starts, slots, self.status)
         return block_tables(self.pool, self.lens, new_lens, self.tables, tokens, plan=self.plan,
                             stream=stream)

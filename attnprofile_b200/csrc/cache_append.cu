@@ -17,20 +17,23 @@
 // NaN for the rows that see it, and masked ones are dropped before they reach
 // a sum; a NaN among the values would instead spread to masked rows as 0 * NaN.
 //
-// Tokens that follow each other into one block (`a run`) share its scale, so
-// the unit of work is one run and one head: one warp, half of it on K and half
-// on V, so that both halves can see whether the other met a number that is not
-// finite.  A warp looks at `chunk` consecutive tokens and takes the runs that
-// begin there: one token where that gives enough warps, else a block's worth,
-// which leaves few warps without a run when prompts come in.
-// It reads 2 bytes and writes 1 per element, plus 8 bytes a run and head.
+// Tokens that follow each other into one block (a run) share its scale, so the
+// unit of work is one run and one head.  A CTA of eight warps looks at `chunk`
+// consecutive tokens of one head and takes the runs that begin there: a short
+// run (single tokens, drafts) by one warp, so that eight go at once, a longer
+// one by the whole CTA, which holds it in registers between finding its largest
+// number and rounding it: every number is read once, with all loads on their
+// way at the same time.  Half of each warp works on K and half on V, so that
+// both can see whether the other met a number that is not finite.
+// It reads 2 bytes and writes 1 per element, plus 8 bytes a run and head; long
+// prompts are bound by that traffic, single tokens by latency.
 #include "cache.cuh"
 
 namespace attnprof {
 namespace cache {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
 
 struct AppendParams {
   const void *k, *v;
@@ -83,17 +86,20 @@ __device__ __forceinline__ int exponent_for(float a) {
   return max(e, kLeastExponent);
 }
 
-template <typename T, int CODE, int D>
+template <typename T, int CODE, int D, int ITERS>
 __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams p) {
   constexpr int kLanes = D / 8;              // lanes on one token's row: 16 bytes each
   constexpr int kRows = 16 / kLanes;         // tokens a half warp takes at once
+  constexpr int kShort = 2 * kRows;          // tokens of a run that one warp takes
+  __shared__ uint32_t tops[2][kWarps];
+  __shared__ uint32_t bads[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool is_v = lane >= 16;
   const int sub = (lane & 15) / kLanes;      // which of the kRows tokens
   const int part = (lane & 15) % kLanes;     // which 8 elements of the row
   const int bs = 1 << p.shift;
   const int head = static_cast<int>(blockIdx.y);
-  const long long begin = (static_cast<long long>(blockIdx.x) * kWarps + warp) * p.chunk;
+  const long long begin = static_cast<long long>(blockIdx.x) * p.chunk;
   const long long end = min(begin + p.chunk, static_cast<long long>(p.tokens));
 
   const T* x = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.v_head : p.k_head) +
@@ -102,66 +108,60 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams 
   uint8_t* codes = is_v ? p.vc : p.kc;
   float* scales = is_v ? p.vs : p.ks;
 
-  auto slot_at = [&](long long t) {
-    const int s = p.slots[t];
-    return s >= 0 && s < p.num_slots ? s : -1;
-  };
-
-  for (long long t0 = begin; t0 < end;) {
-    // The next token that begins a run: one with a slot, into which the token
-    // before does not lead.
-    int mine = -1;
-    if (t0 + lane < end) {
-      mine = slot_at(t0 + lane);
-      if (mine >= 0 && (mine & (bs - 1)) > 0 && t0 + lane > 0 &&
-          slot_at(t0 + lane - 1) == mine - 1)
-        mine = -1;
-    }
-    const unsigned heads_of_runs = __ballot_sync(~0u, mine >= 0);
-    if (heads_of_runs == 0) {
-      t0 += 32;
-      continue;
-    }
-    const int skip = __ffs(heads_of_runs) - 1;
-    const int slot = __shfl_sync(~0u, mine, skip);
+  // One run: tokens t0 .. t0 + n into slots slot .. slot + n of one block.
+  // WHOLE: by all warps together, else by this warp alone.
+  auto run = [&](auto whole, long long t0, int n, int slot) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    constexpr int kIters = WHOLE ? ITERS : kShort / kRows;
+    constexpr int kStep = WHOLE ? kRows * kWarps : kRows;
+    const int row = (WHOLE ? warp * kRows : 0) + sub;
     const int off = slot & (bs - 1);
-    t0 += skip;
-    // The run: following tokens with following slots of the same block.
-    const int most = static_cast<int>(min(static_cast<long long>(bs - off), p.tokens - t0));
-    int n = 1;
-    while (n < most) {
-      const int i = n + lane;
-      const unsigned next = __ballot_sync(~0u, i < most && p.slots[t0 + i] == slot + i);
-      n += next == ~0u ? 32 : __ffs(~next) - 1;
-      if (next != ~0u) break;
-    }
     const long long block_head = static_cast<long long>(slot >> p.shift) * p.heads + head;
     float* scale_at = scales + block_head;
-    uint8_t* rows = codes + (block_head << p.shift) * D;
-    const float old = off > 0 ? *scale_at : 0.f;
+    uint8_t* rows = codes + (block_head << p.shift) * D + 8 * part;
 
+    uint4 w[kIters];
+#pragma unroll
+    for (int i = 0; i < kIters; ++i) {
+      w[i] = make_uint4(0, 0, 0, 0);
+      if (row + i * kStep < n)
+        w[i] = __ldcs(reinterpret_cast<const uint4*>(x + (t0 + row + i * kStep) * x_token));
+    }
+    const float old = off > 0 ? *scale_at : 0.f;
     // Largest |x| of the run, as bits: for finite numbers these order alike.
     uint32_t top = 0, bad = 0;
-    const T* xr = x + t0 * x_token;
-#pragma unroll 4
-    for (int i = sub; i < n; i += kRows) {
-      const uint4 w = *reinterpret_cast<const uint4*>(xr + i * x_token);
-      const uint32_t a = finite_only<T>(w.x, bad), b = finite_only<T>(w.y, bad);
-      const uint32_t c = finite_only<T>(w.z, bad), d = finite_only<T>(w.w, bad);
-      top = __vmaxu2(top, __vmaxu2(__vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu),
-                                   __vmaxu2(c & 0x7fff7fffu, d & 0x7fff7fffu)));
+#pragma unroll
+    for (int i = 0; i < kIters; ++i) {
+      w[i].x = finite_only<T>(w[i].x, bad);
+      w[i].y = finite_only<T>(w[i].y, bad);
+      w[i].z = finite_only<T>(w[i].z, bad);
+      w[i].w = finite_only<T>(w[i].w, bad);
+      top = __vmaxu2(top, __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu),
+                                   __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu)));
     }
     top = max(top & 0xffffu, top >> 16);
 #pragma unroll
     for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
-    const bool any_bad = __any_sync(~0u, bad != 0);
+    bool any_bad = __any_sync(~0u, bad != 0);
+    if constexpr (WHOLE) {
+      if ((lane & 15) == 0) tops[is_v][warp] = top;
+      if (lane == 0) bads[warp] = any_bad;
+      __syncthreads();  // (every thread has read the old scale, too)
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        top = max(top, tops[is_v][i]);
+        any_bad |= bads[i] != 0;
+      }
+    } else {
+      __syncwarp();
+    }
 
     const float want = power_of_two(exponent_for<CODE>(Bits<T>::to_float(top)));
     const bool dead = off > 0 && old != old;  // a NaN scale stays until the block is begun anew
     const float now = (off > 0 && old > want) ? old : want;
     const bool grew = off > 0 && !dead && now > old;
-    __syncwarp();  // every lane has read the old scale
-    if ((lane & 15) == 0) *scale_at = ((any_bad && !is_v) || dead) ? __int_as_float(0x7fffffff) : now;
+    if ((lane & 15) == 0 && (!WHOLE || warp == 0))
+      *scale_at = ((any_bad && !is_v) || dead) ? __int_as_float(0x7fffffff) : now;
 
     // Dividing by `now`: by its reciprocal where that is exact.
     const bool pow2 = (__float_as_int(now) & 0x7fffff) == 0;
@@ -170,50 +170,98 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams 
 
     if (grew) {  // codes in front of the run, to the new scale
       const float r = old / now;
-      for (int i = sub; i < off; i += kRows) {
-        uint2* at = reinterpret_cast<uint2*>(rows + static_cast<long long>(i) * D + 8 * part);
+      for (int i = row; i < off; i += kStep) {
+        uint2* at = reinterpret_cast<uint2*>(rows + static_cast<long long>(i) * D);
         uint2 c = *at;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&c);
+        uint32_t* u = reinterpret_cast<uint32_t*>(&c);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float2 a = half2_to_float2(Code<CODE>::half2_lo(w[j]));
-          const float2 b = half2_to_float2(Code<CODE>::half2_hi(w[j]));
-          w[j] = Code<CODE>::encode2(a.x * r, a.y * r) | (Code<CODE>::encode2(b.x * r, b.y * r) << 16);
+          const float2 a = half2_to_float2(Code<CODE>::half2_lo(u[j]));
+          const float2 b = half2_to_float2(Code<CODE>::half2_hi(u[j]));
+          u[j] = Code<CODE>::encode2(a.x * r, a.y * r) | (Code<CODE>::encode2(b.x * r, b.y * r) << 16);
         }
         *at = c;
       }
     }
-#pragma unroll 4
-    for (int i = sub; i < n; i += kRows) {
-      uint4 w = *reinterpret_cast<const uint4*>(xr + i * x_token);
-      uint32_t* u = reinterpret_cast<uint32_t*>(&w);
-      uint2 c;
-      uint32_t e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = Bits<T>::to_float2(finite_only<T>(u[j], bad));
-        e[j] = Code<CODE>::encode2(scaled(f.x), scaled(f.y));
+    for (int i = 0; i < kIters; ++i) {
+      if (row + i * kStep < n) {
+        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        uint32_t e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = Bits<T>::to_float2(u[j]);
+          e[j] = Code<CODE>::encode2(scaled(f.x), scaled(f.y));
+        }
+        *reinterpret_cast<uint2*>(rows + static_cast<long long>(off + row + i * kStep) * D) =
+            make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
       }
-      c.x = e[0] | (e[1] << 16);
-      c.y = e[2] | (e[3] << 16);
-      *reinterpret_cast<uint2*>(rows + static_cast<long long>(off + i) * D + 8 * part) = c;
     }
-    t0 += n;
+    if constexpr (WHOLE) __syncthreads();  // tops and bads may be written again
+  };
+
+  auto slot_at = [&](long long t) {
+    const int s = p.slots[t];
+    return s >= 0 && s < p.num_slots ? s : -1;
+  };
+
+  int short_runs = 0;
+  for (long long base = begin; base < end; base += 32) {
+    // Tokens base .. base + 31, one a lane: which begin a run (they have a slot
+    // into which the token before does not lead), and which go on with one.
+    const long long t = base + lane;
+    const int mine = t < p.tokens ? slot_at(t) : -1;
+    const bool goes_on = mine >= 0 && (mine & (bs - 1)) > 0 && t > 0 && slot_at(t - 1) == mine - 1;
+    const unsigned follow = __ballot_sync(~0u, goes_on);
+    unsigned starts = __ballot_sync(~0u, mine >= 0 && !goes_on && t < end);
+    while (starts != 0) {
+      const int s = __ffs(starts) - 1;
+      starts &= starts - 1;
+      const int slot = __shfl_sync(~0u, mine, s);
+      // Tokens that go on behind it, beyond these 32 too.
+      const unsigned rest = s == 31 ? 0u : ~(follow >> (s + 1));
+      int n = 1 + (s == 31 ? 0 : min(__ffs(rest) - 1, 31 - s));
+      if (s + n == 32) {
+        const int most = static_cast<int>(
+            min(static_cast<long long>(bs - (slot & (bs - 1))), p.tokens - (base + s)));
+        while (n < most) {
+          const int i = n + lane;
+          const unsigned next =
+              __ballot_sync(~0u, i < most && p.slots[base + s + i] == slot + i);
+          n += next == ~0u ? 32 : __ffs(~next) - 1;
+          if (next != ~0u) break;
+        }
+      }
+      if (n > kShort)
+        run(std::true_type{}, base + s, n, slot);
+      else if (short_runs++ % kWarps == warp)
+        run(std::false_type{}, base + s, n, slot);
+    }
   }
+}
+
+template <typename T, int CODE, int D, int ITERS>
+int launch_iters(const AppendParams& p, cudaStream_t st) {
+  const dim3 grid((static_cast<unsigned>(p.tokens) + p.chunk - 1) / p.chunk,
+                  static_cast<unsigned>(p.heads));
+  append_kernel<T, CODE, D, ITERS><<<grid, 32 * kWarps, 0, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
 }
 
 template <typename T, int CODE, int D>
 int launch(const AppendParams& p0, cudaStream_t st) {
   AppendParams p = p0;
-  // One token a warp up to some 16 warps an SM; beyond that a block's worth,
-  // since most tokens then follow others into their block.
-  const long long warps = static_cast<long long>(p.tokens) * p.heads;
-  p.chunk = warps <= 148 * 16 ? 1 : 1 << p.shift;
-  const long long groups = (static_cast<long long>(p.tokens) + p.chunk - 1) / p.chunk;
-  const dim3 grid(static_cast<unsigned>((groups + kWarps - 1) / kWarps),
-                  static_cast<unsigned>(p.heads));
-  append_kernel<T, CODE, D><<<grid, 32 * kWarps, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
+  // Tokens a CTA looks at: as many as leave some eight CTAs an SM, between one
+  // (few tokens: all begin runs) and a block's worth (prompts: one run each).
+  const long long per_cta = static_cast<long long>(p.tokens) * p.heads / (148 * 8);
+  p.chunk = 1;
+  while (2 * p.chunk <= per_cta && p.chunk < (1 << p.shift)) p.chunk *= 2;
+  // Rounds that a CTA needs for a whole block, held in registers.
+  constexpr int kStep = kWarps * 16 / (D / 8);
+  const int rounds = ((1 << p.shift) + kStep - 1) / kStep;
+  if (rounds <= 4) return launch_iters<T, CODE, D, 4>(p, st);
+  if (rounds <= 8) return launch_iters<T, CODE, D, 8>(p, st);
+  return launch_iters<T, CODE, D, 16>(p, st);
 }
 
 template <typename T, int CODE>

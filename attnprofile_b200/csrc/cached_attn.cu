@@ -56,7 +56,7 @@ extern "C" int attn_cached(const void* q, long long q_token_stride, long long q_
   p.num_blocks = num_blocks;
   p.shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
   const long long capacity = static_cast<long long>(width) * block_size;
-  p.capacity = capacity > INT_MAX - 1024 ? INT_MAX - 1024 : static_cast<int>(capacity);
+  p.capacity = capacity > INT_MAX - 4096 ? INT_MAX - 4096 : static_cast<int>(capacity);
   p.causal = causal != 0;
   p.scale_log2 = static_cast<float>(
       (scale > 0.f ? static_cast<double>(scale) : 1.0 / std::sqrt(static_cast<double>(D))) *

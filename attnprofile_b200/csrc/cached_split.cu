@@ -4,20 +4,28 @@
 //
 // Work.  A unit is 8 NT query rows (token x head of the group) of one request
 // and kv head, over chunks of 256 keys; all units' chunks, in order, are cut
-// into equal ranges, one a CTA, whatever the requests' lengths.  A range may
+// into equal ranges, one a CTA, whatever the requests' lengths (a unit counts
+// as one chunk more than it has, for what it costs to begin).  A range may
 // hold parts of two units and any number of whole ones; whole units are
 // written at once, parts go to the workspace as (max, sum, O) and a second
 // kernel joins them in the order of the keys, so results do not depend on which
 // CTA came first.  The ranges are found by every CTA from the lengths alone.
 //
-// Inside a CTA four warps take 64 keys of a chunk each.  S^T = K Q^T and
-// O^T = V^T P^T run on m16n8k16 MMAs with the keys (then the head dimension)
-// on the 16 side and 8 query rows on the other, so that the 1 to 8 rows of a
-// decode step waste nothing; tcgen05's smallest tile of 64 to 128 rows would be
-// almost empty, and its operands would have to go through shared memory in 16
-// bits.  Codes go from global memory straight into registers: which key or
-// which head dimension a lane holds is free in a contraction as long as both
-// operands agree, so lanes take 16 bytes of a row and convert them in place.
+// Inside a CTA one warp fetches and four compute.  The fetching warp walks
+// through the CTA's range, over the ends of units, and keeps a ring of steps
+// full: per step 64 or 128 keys' codes of K and V by TMA, 16 keys at a time,
+// under the 128-byte swizzle, and their blocks' scales by cp.async.  HBM needs
+// 6.5 TB/s times some 1.2 us on its way, 53 KB an SM; two CTAs' rings hold 192.
+// (Codes read straight into registers by the computing warps: 4.0 TB/s on 64
+// requests of 5 to 8191 tokens; a ring for each warp that ran empty at each
+// unit's end: 4.7; this form: see the table of results.)
+// Each computing warp takes 16 or 32 keys of a step.  S^T = K Q^T and O^T =
+// V^T P^T run on m16n8k16 MMAs with the keys (then the head dimension) on the 16
+// side and 8 query rows on the other, so that the 1 to 8 rows of a decode step
+// waste nothing; tcgen05's smallest tile of 64 to 128 rows would be almost
+// empty.  Which key or which head dimension a lane holds is free in a
+// contraction as long as both operands agree, so lanes take 16 bytes of a row
+// and convert them in place.
 // K's scale multiplies the scores in f32; V's scale multiplies each block's
 // sum of p v in f32, so no scale is rounded.  P is rounded to f16, by at most
 // 2^-11 of itself as an f16 result is (a bf16 result by 2^-8): it is held as
@@ -26,17 +34,19 @@
 // power of two per row, which loses nothing above 2^-38 of the row's largest.
 #include <climits>
 
+#include "attn_host.cuh"
 #include "cached_attn.cuh"
-#include "ptx.cuh"
 
 namespace attnprof {
+unsigned long long current_timeout_ns();
+
 namespace cache {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kWarps = 4;                    // that compute
+constexpr int kThreads = 256;                // two warpgroups: computing, fetching (one warp of it)
 constexpr int kChunk = 256;                  // keys
-constexpr int kWarpKeys = kChunk / kWarps;   // keys of a chunk that a warp takes
+constexpr int kOver = 1;                     // chunks that beginning a unit counts for
 constexpr float kLift = 15.f;                // P is held as 2^kLift p
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -64,20 +74,20 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 16 or 8 bytes of codes (a lane's share of one row).
+// 16 or 8 bytes of codes (a lane's share of one row) from shared memory.
 template <int WORDS>
 struct Words {
   uint32_t w[WORDS];
 };
 template <int WORDS>
-__device__ __forceinline__ void load_codes(Words<WORDS>& d, const uint8_t* p) {
-  if constexpr (WORDS == 4) {
-    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
-    d.w[0] = v.x; d.w[1] = v.y; d.w[2] = v.z; d.w[3] = v.w;
-  } else {
-    const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
-    d.w[0] = v.x; d.w[1] = v.y;
-  }
+__device__ __forceinline__ void load_codes(Words<WORDS>& d, uint32_t a) {
+  if constexpr (WORDS == 4)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(d.w[0]), "=r"(d.w[1]), "=r"(d.w[2]), "=r"(d.w[3])
+                 : "r"(a)
+                 : "memory");
+  else
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(d.w[0]), "=r"(d.w[1]) : "r"(a) : "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -85,6 +95,10 @@ __device__ __forceinline__ void load_codes(Words<WORDS>& d, const uint8_t* p) {
 // ---------------------------------------------------------------------------
 struct Shape {
   int units, chunks;  // of one request: its units, and the chunks of each
+  __device__ __forceinline__ int weight() const { return chunks + kOver; }
+  __device__ __forceinline__ long long work() const {
+    return static_cast<long long>(units) * weight();
+  }
 };
 
 template <int NT>
@@ -97,19 +111,18 @@ __device__ __forceinline__ Shape shape_of(const CachedParams& p, const Request& 
 
 struct Place {
   int request;
-  long long before;  // chunks of all requests in front of it
+  long long before;  // work of all requests in front of it
 };
 
-// Sum of all requests' chunks; a place in them is looked up afterwards: each
+// Sum of all requests' work; a place in it is looked up afterwards: each
 // thread keeps the sum of its share of the requests.
 template <int NT>
-__device__ __forceinline__ long long count_chunks(const CachedParams& p, long long* part) {
+__device__ __forceinline__ long long count_work(const CachedParams& p, long long* part) {
   const int each = (p.batch + blockDim.x - 1) / blockDim.x;
   const int first = static_cast<int>(threadIdx.x) * each;
   long long sum = 0;
   for (int r = first; r < min(first + each, p.batch); ++r) {
-    const Shape s = shape_of<NT>(p, request_at(p, r));
-    sum += static_cast<long long>(s.units) * s.chunks;
+    sum += shape_of<NT>(p, request_at(p, r)).work();
   }
   // Inclusive prefix over the threads.
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -128,7 +141,7 @@ __device__ __forceinline__ long long count_chunks(const CachedParams& p, long lo
   return part[blockDim.x - 1];
 }
 
-// The request that holds chunk `at` (at < the total); by one thread.
+// The request that holds place `at` (below the total); by one thread.
 template <int NT>
 __device__ __forceinline__ Place find_place(const CachedParams& p, const long long* part,
                                             long long at) {
@@ -140,21 +153,65 @@ __device__ __forceinline__ Place find_place(const CachedParams& p, const long lo
   const int each = (p.batch + blockDim.x - 1) / blockDim.x;
   Place pl{hi * each, hi > 0 ? part[hi - 1] : 0};
   while (true) {
-    const Shape s = shape_of<NT>(p, request_at(p, pl.request));
-    const long long w = static_cast<long long>(s.units) * s.chunks;
+    const long long w = shape_of<NT>(p, request_at(p, pl.request)).work();
     if (pl.before + w > at || pl.request + 1 >= p.batch) return pl;
     pl.before += w;
     ++pl.request;
   }
 }
 
-__device__ __forceinline__ long long chunks_each(long long total) {
+__device__ __forceinline__ long long work_each(long long total) {
   return (total + gridDim.x - 1) / gridDim.x;
 }
 
-// Where a part of CTA `cta` lies in the workspace: slot 1 for the part that
-// begins its unit, slot 0 for one that begins inside it.  [rows][D] f32 of O
-// for all slots, then (max, sum) per row.
+// x / y for 0 <= x, 0 < y; most work counts fit 32 bits.
+__device__ __forceinline__ int quotient(long long x, int y) {
+  return (x >> 32) != 0 ? static_cast<int>(x / y)
+                        : static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y));
+}
+
+// Chunks [c0, c1) of one unit.
+struct Part {
+  Request rq;
+  int request, kvh, row0, c0, c1, chunks;
+};
+
+// A CTA's range, part by part.
+template <int NT>
+struct Cursor {
+  long long at, stop;
+  Place pl;
+  __device__ __forceinline__ bool next(const CachedParams& p, Part& x) {
+    while (at < stop && pl.request < p.batch) {
+      x.rq = request_at(p, pl.request);
+      const Shape sh = shape_of<NT>(p, x.rq);
+      if (at >= pl.before + sh.work()) {
+        pl.before += sh.work();
+        ++pl.request;
+        continue;
+      }
+      const int w = sh.weight();
+      const int unit = quotient(at - pl.before, w);
+      const int off = static_cast<int>(at - pl.before - static_cast<long long>(unit) * w);
+      const int end = static_cast<int>(min(static_cast<long long>(w), off + (stop - at)));
+      at += end - off;
+      x.c0 = max(0, off - kOver);
+      x.c1 = max(0, end - kOver);
+      if (x.c0 == x.c1) continue;
+      const int tiles = sh.units / p.kv_heads;
+      x.request = pl.request;
+      x.chunks = sh.chunks;
+      x.kvh = unit / tiles;
+      x.row0 = (unit - x.kvh * tiles) * 8 * NT;
+      return true;
+    }
+    return false;
+  }
+};
+
+// Parts in the workspace: [rows][D] f32 of O for all slots, then (max, sum)
+// per row.  CTA c has slot 2 c + 1 for the part that begins its unit and slot
+// 2 c for one that begins inside it (it has at most one of each).
 template <int NT, int D>
 struct Parts {
   static constexpr int kRows = 8 * NT;
@@ -167,7 +224,7 @@ struct Parts {
 };
 
 // ---------------------------------------------------------------------------
-// One warp's share of a part: the online softmax over its keys.
+// The kernel.
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ float to_float(T x);
@@ -186,55 +243,161 @@ __device__ __forceinline__ uint32_t pack_out<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+constexpr int kStageBytes = 32768;  // a step's codes of K, then of V
+
+template <int D, int NT>
+struct Smem {
+  static constexpr int kGroup = 16 * D;                          // bytes of 16 keys
+  static constexpr int kGroups = kStageBytes / 2 / kGroup;       // of a step: 8 or 16
+  static constexpr int kStages = NT >= 4 ? 2 : 3;
+  static constexpr int kOffHop = kStages * kStageBytes;          // a warp's sums on their way
+  static constexpr int kHop = 32 * NT * (D / 4 + 4) * 4;
+  static constexpr int kOffQ = kOffHop + kHop;                   // Q operands (NT = 4)
+  static constexpr int kOffScale = kOffQ + (NT >= 4 ? NT * (D / 16) * 32 * 8 : 0);
+  static constexpr int kOffBar = kOffScale + kStages * 2 * kGroups * 4;
+  static constexpr int kBytes = kOffBar + 16 * kStages + 1024;   // + alignment
+  static_assert(kThreads * 8 <= kHop, "the prefix sums use the hop's place first");
+  static_assert(2 * (kBytes + 2048) <= 228 * 1024, "two CTAs an SM");
+};
+
+struct SplitParams : CachedParams {
+  int* status;
+  unsigned long long timeout_ns;
+};
+
+// Named barriers: sums handed from warp h + 1 to warp h, the last reader done,
+// Q operands in shared memory.
+constexpr int kBarHop = 1, kBarRead = 4, kBarQ = 5;
+
+__device__ __forceinline__ void named_bar_arrive(uint32_t id, uint32_t nthreads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
+// The fetching warp.  Lane i holds the block of group i of 32 (-1: no keys
+// there, or no block of the pool) and fetches that group's codes and scales.
+template <int D, int NT>
+__device__ void fetch_role(const CUtensorMap* map_k, const CUtensorMap* map_v,
+                           const SplitParams& p, Cursor<NT> cursor, uint32_t sbase,
+                           const WaitCtx& w) {
+  using S = Smem<D, NT>;
+  constexpr int kPerBatch = 32 / S::kGroups;  // steps whose blocks the lanes hold
+  const int lane = threadIdx.x & 31;
+  const int mine = lane % S::kGroups;         // group of a step
+  const uint32_t full = sbase + S::kOffBar, empty = full + 8 * S::kStages;
+  int put = 0, sent = 0;
+  uint32_t parity = 1;  // of the place's emptying; at first all are empty
+  Part x;
+  bool ok = true;
+  while (ok && cursor.next(p, x)) {
+    const int* table = p.tables + x.request * p.table_stride;
+    const int key_end = min(x.c1 * kChunk, x.rq.kv);
+    auto block_at = [&](int key) {
+      if (key < key_end) {
+        const int b = table[key >> p.shift];
+        if (b >= 0 && b < p.num_blocks) return b;
+      }
+      return -1;
+    };
+    const int begin = x.c0 * kChunk + 16 * lane;
+    int id = block_at(begin), id_next = block_at(begin + 512);
+    for (int key0 = x.c0 * kChunk; key0 < key_end && ok; key0 += 512) {
+#pragma unroll
+      for (int s = 0; s < kPerBatch; ++s) {
+        if (key0 + s * 16 * S::kGroups >= key_end) break;
+        ok = __all_sync(~0u, wait_bar(empty + 8 * put, parity, w, kSiteKvEmpty));
+        if (!ok) break;
+        const bool turn = lane / S::kGroups == s;
+        const bool there = turn && id >= 0;
+        const int n = __popc(__ballot_sync(~0u, there));
+        const uint32_t bar = full + 8 * put;
+        if (lane == 0) ptx::mbar_arrive_expect_tx(bar, n * 2 * S::kGroup);
+        __syncwarp();
+        const uint32_t scale_at = sbase + S::kOffScale + (put * 2 * S::kGroups + mine) * 4;
+        if (there) {
+          const int off = (key0 + 16 * lane) & ((1 << p.shift) - 1);
+          const int piece = id * p.kv_heads + x.kvh;
+          const uint32_t at = sbase + put * kStageBytes + mine * S::kGroup;
+          ptx::tma_load_3d(at, map_k, bar, 0, D == 128 ? off : off / 2, piece);
+          ptx::tma_load_3d(at + kStageBytes / 2, map_v, bar, 0, D == 128 ? off : off / 2, piece);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scale_at),
+                       "l"(p.ks + piece)
+                       : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scale_at + 4 * S::kGroups),
+                       "l"(p.vs + piece)
+                       : "memory");
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar)
+                       : "memory");
+        } else if (turn) {  // a negative scale: nothing here
+          ptx::st_shared_f32(scale_at, -1.f);
+          ptx::st_shared_f32(scale_at + 4 * S::kGroups, 0.f);
+          ptx::mbar_arrive(bar);
+        }
+        ++sent;
+        if (++put == S::kStages) {
+          put = 0;
+          parity ^= 1;
+        }
+      }
+      id = id_next;
+      id_next = block_at(key0 + 1024 + 16 * lane);
+    }
+  }
+  // After a wait that ran out (the host reads of it in the status word): copies
+  // on their way end before the shared memory that they go to does.
+  if (*w.abort) {
+    for (int i = max(0, sent - S::kStages); i < sent; ++i) {
+      const unsigned long long t0 = ptx::globaltimer_ns();
+      while (!ptx::mbar_try_wait(full + 8 * (i % S::kStages), (i / S::kStages) & 1) &&
+             ptx::globaltimer_ns() - t0 < p.timeout_ns) {
+      }
+    }
+  }
+}
+
 template <typename T, int CODE, int D, int NT>
-__global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
-  constexpr int kRows = 8 * NT;
+__device__ void compute_role(const SplitParams& p, Cursor<NT> cursor, uint32_t sbase,
+                             uint8_t* smem, const WaitCtx& w) {
+  using S = Smem<D, NT>;
   constexpr int KSTEPS = D / 16;               // MMAs along the head dimension
   constexpr int MT = D / 16;                   // 16-row tiles of O^T
   constexpr int VW = D / 32;                   // words of a V row that a lane holds (D / 8 bytes)
   constexpr int KP = D / 64;                   // 16-byte pieces of a K row that a lane holds
   constexpr bool kQShared = NT >= 4;           // Q operands from shared memory, to save registers
-  constexpr int KT = NT >= 4 ? 1 : 2;          // 16-key tiles of one step
-  constexpr int kStep = 16 * KT;
-
-  __shared__ long long part_sum[kThreads];
-  __shared__ Place place;
-  __shared__ float row_m[kWarps][kRows], row_l[kWarps][kRows];
-  extern __shared__ float smem[];              // [kWarps][kRows][D + 4] f32, then Q operands
-  constexpr int kPitch = D + 4;
-  uint2* q_sh = reinterpret_cast<uint2*>(smem + kWarps * kRows * kPitch);
-
+  constexpr int KT = S::kGroups / kWarps;      // 16-key tiles of a warp's step: 2 or 4
+  constexpr int kStep = 16 * S::kGroups;       // keys of a step
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
+  const uint32_t full = sbase + S::kOffBar, empty = full + 8 * S::kStages;
+  uint2* q_sh = reinterpret_cast<uint2*>(smem + S::kOffQ);
+  float* hop = reinterpret_cast<float*>(smem + S::kOffHop) + lane;
 
-  const long long total = count_chunks<NT>(p, part_sum);
-  const long long each = chunks_each(total);
-  long long at = each * blockIdx.x;
-  const long long stop = min(at + each, total);
-  asm volatile("griddepcontrol.launch_dependents;");
-  if (at >= stop) return;
-  if (threadIdx.x == 0) place = find_place<NT>(p, part_sum, at);
-  __syncthreads();
-  Place pl = place;
-
-  while (at < stop) {
-    const Request rq = request_at(p, pl.request);
-    const Shape sh = shape_of<NT>(p, rq);
-    const long long work = static_cast<long long>(sh.units) * sh.chunks;
-    if (at >= pl.before + work) {
-      pl.before += work;
-      if (++pl.request >= p.batch) return;
-      continue;
+  // Where the lane's pieces lie in a group's 16 rows (D = 64: 8 rows of two
+  // keys) under the 128-byte swizzle: 16-byte piece c of row r at c ^ (r % 8).
+  uint32_t k_at[2][KP], v_at[4];
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int pc = 0; pc < KP; ++pc) {
+      const int key = g + 8 * r;
+      k_at[r][pc] = D == 128 ? key * 128 + (((4 * pc + t) ^ (key & 7)) << 4)
+                             : (key >> 1) * 128 + ((((key & 1) * 4 + t) ^ (key >> 1)) << 4);
     }
-    const long long in = at - pl.before;
-    const int unit = static_cast<int>(in / sh.chunks);
-    const int c0 = static_cast<int>(in - static_cast<long long>(unit) * sh.chunks);
-    const int c1 = static_cast<int>(min(static_cast<long long>(sh.chunks), c0 + (stop - at)));
-    const int tiles = sh.units / p.kv_heads;
-    const int kvh = unit / tiles;
-    const int row0 = (unit - kvh * tiles) * kRows;  // of the request's rows of this kv head
-    const int rows_in = rq.n * p.group;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int key = 2 * t + (r & 1) + 8 * (r >> 1);
+    v_at[r] = D == 128 ? key * 128 + ((g ^ (key & 7)) << 4)
+                       : (key >> 1) * 128 + ((((key & 1) * 4 + (g >> 1)) ^ (key >> 1)) << 4) +
+                             8 * (g & 1);
+  }
 
+  int take = 0;
+  uint32_t parity = 0;
+  bool ok = true, first = true;
+  Part x;
+  while (cursor.next(p, x)) {
+    const Request& rq = x.rq;
+    const int rows_in = rq.n * p.group;
+    if constexpr (kQShared) ptx::named_bar_sync(kBarQ, 32 * kWarps);  // the last ones are used up
     // Q operands: lane (g, t) holds row 8 nt + g, the head dimensions that its
     // K bytes belong to.
     uint32_t qb[kQShared ? 1 : NT][kQShared ? 1 : KSTEPS][2];
@@ -243,11 +406,11 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
     int least = INT_MAX;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = row0 + 8 * nt + g;
+      const int row = x.row0 + 8 * nt + g;
       const bool live = row < rows_in;
       const int tok = live ? row / p.group : 0;
       const T* qr = static_cast<const T*>(p.q) + (rq.start + tok) * p.q_token +
-                    (kvh * p.group + (live ? row - tok * p.group : 0)) * p.q_head;
+                    (x.kvh * p.group + (live ? row - tok * p.group : 0)) * p.q_head;
       float f = 1.f;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         uint32_t top = 0;
@@ -292,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         row_f[nt][j] = __shfl_sync(~0u, mine, (2 * t + j) * 4);
-        const int r = row0 + 8 * nt + 2 * t + j;
+        const int r = x.row0 + 8 * nt + 2 * t + j;
         // (rows behind the last one: zeros that see everything)
         limit[nt][j] = r < rows_in && p.causal ? rq.kv - rq.n + r / p.group + 1 : rq.kv;
         limit[nt][j] = min(limit[nt][j], rq.kv);
@@ -300,7 +463,7 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
       }
     }
     least = __reduce_min_sync(~0u, least);
-    if constexpr (kQShared) __syncthreads();
+    if constexpr (kQShared) ptx::named_bar_sync(kBarQ, 32 * kWarps);
 
     float o[NT][MT][4];
     float m[NT][2], l[NT][2];
@@ -314,94 +477,36 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
       l[nt][0] = l[nt][1] = 0.f;
     }
 
-    // This warp's steps: kWarpKeys / kStep of them in each chunk.
-    const int* table = p.tables + pl.request * p.table_stride;
-    constexpr int kPerChunk = kWarpKeys / kStep;
-    const int steps = (c1 - c0) * kPerChunk;
-    auto key_of = [&](int s) {
-      return (c0 + s / kPerChunk) * kChunk + warp * kWarpKeys + (s % kPerChunk) * kStep;
-    };
-    // Block of each 16-key tile of step s (-1: no keys there, or not a block).
-    auto blocks_of = [&](int s, int (&id)[KT]) {
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        const int key = key_of(s) + 16 * k;
-        id[k] = -1;
-        if (s < steps && key < rq.kv) {
-          const int b = table[key >> p.shift];
-          if (b >= 0 && b < p.num_blocks) id[k] = b;
-        }
-      }
-    };
-    Words<4> kw[KT][2][KP];   // [tile][row g, row g + 8][piece]
-    Words<VW> vw[KT][4];      // [tile][keys 2t, 2t + 1, 2t + 8, 2t + 9]
-    float ksc[KT], vsc[KT];
-    auto tile_at = [&](int s, int k, int id) {
-      const int off = (key_of(s) + 16 * k) & ((1 << p.shift) - 1);
-      return ((((static_cast<long long>(id) * p.kv_heads + kvh) << p.shift) + off)) * D;
-    };
-    // Codes are read also behind the request's last token, within its block;
-    // what lies there does not count (masked; V codes are zeroed).
-    auto load_k = [&](int s, const int (&id)[KT]) {
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        if (id[k] >= 0) {
-          const uint8_t* b = p.kc + tile_at(s, k, id[k]);
-          ksc[k] = p.ks[static_cast<long long>(id[k]) * p.kv_heads + kvh];
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int pc = 0; pc < KP; ++pc)
-              load_codes(kw[k][r][pc], b + (g + 8 * r) * D + 64 * pc + 16 * t);
-        } else {
-          ksc[k] = 0.f;
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int pc = 0; pc < KP; ++pc)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) kw[k][r][pc].w[i] = 0u;
-        }
-      }
-    };
-    auto load_v = [&](int s, const int (&id)[KT]) {
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        if (id[k] >= 0) {
-          const uint8_t* b = p.vc + tile_at(s, k, id[k]);
-          vsc[k] = p.vs[static_cast<long long>(id[k]) * p.kv_heads + kvh];
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            load_codes(vw[k][r], b + (2 * t + (r & 1) + 8 * (r >> 1)) * D + 4 * VW * g);
-        } else {
-          vsc[k] = 0.f;
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int i = 0; i < VW; ++i) vw[k][r].w[i] = 0u;
-        }
-      }
-    };
-
-    int id[KT], id_next[KT];
-    blocks_of(0, id);
-    load_k(0, id);
-    load_v(0, id);
-    blocks_of(1, id_next);
-
-    for (int s = 0; s < steps; ++s) {
-      const int key0 = key_of(s);
+    const int key_end = min(x.c1 * kChunk, rq.kv);
+    for (int key_s = x.c0 * kChunk; key_s < key_end; key_s += kStep) {
+      const int key0 = key_s + 16 * KT * warp;
+      const uint32_t from = sbase + take * kStageBytes + warp * KT * S::kGroup;
+      const float* scale = reinterpret_cast<const float*>(smem + S::kOffScale) +
+                           take * 2 * S::kGroups + warp * KT;
+      // (After a wait that ran out this goes on without waiting, so that all
+      // warps meet at their barriers; the status word tells the host.)
+      if (ok) ok = __all_sync(~0u, wait_bar(full + 8 * take, parity, w, kSiteKvFull));
       // S^T = K Q^T
       float sc[NT][KT][4];
+      float kscale[KT], vsc[KT];
+      bool held[KT];
 #pragma unroll
       for (int k = 0; k < KT; ++k) {
+        kscale[k] = scale[k];
+        vsc[k] = scale[S::kGroups + k];
+        held[k] = !(kscale[k] < 0.f);
+        Words<4> kw[2][KP];  // [row g, row g + 8][piece]
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int pc = 0; pc < KP; ++pc) load_codes(kw[r][pc], from + k * S::kGroup + k_at[r][pc]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) sc[nt][k][i] = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ++ks) {
-          const uint32_t w0 = kw[k][0][ks / 4].w[ks % 4], w1 = kw[k][1][ks / 4].w[ks % 4];
+          const uint32_t w0 = kw[0][ks / 4].w[ks % 4], w1 = kw[1][ks / 4].w[ks % 4];
           const uint32_t a[4] = {Code<CODE>::half2_lo(w0), Code<CODE>::half2_lo(w1),
                                  Code<CODE>::half2_hi(w0), Code<CODE>::half2_hi(w1)};
 #pragma unroll
@@ -415,17 +520,9 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
           }
         }
       }
-      float kscale[KT];
-      bool held[KT];
-#pragma unroll
-      for (int k = 0; k < KT; ++k) {
-        kscale[k] = ksc[k];
-        held[k] = id[k] >= 0;
-      }
-      load_k(s + 1, id_next);
 
       // Scores in log2 units, masked; the running maximum.
-      const bool whole = key0 + kStep <= least;
+      const bool whole = key0 + 16 * KT <= least;
       bool moved = false;
       float alpha[NT][2];
 #pragma unroll
@@ -481,19 +578,30 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
           pb[nt][k][0] = transpose_8x8(pack_half2(sc[nt][k][0], sc[nt][k][1]));
           pb[nt][k][1] = transpose_8x8(pack_half2(sc[nt][k][2], sc[nt][k][3]));
         }
-      // Codes behind the last token may be any bits, NaN among them.
-      if (key0 + kStep > rq.kv) {
+      // V: [tile][keys 2t, 2t + 1, 2t + 8, 2t + 9].  What lies behind the last
+      // token, or where nothing was fetched, may be any bits, NaN among them.
+      Words<VW> vw[KT][4];
+      const bool tail = key0 + 16 * KT > rq.kv;
 #pragma unroll
-        for (int k = 0; k < KT; ++k)
+      for (int k = 0; k < KT; ++k)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (key0 + 16 * k + 2 * t + (r & 1) + 8 * (r >> 1) >= rq.kv)
+        for (int r = 0; r < 4; ++r) {
+          load_codes(vw[k][r], from + kStageBytes / 2 + k * S::kGroup + v_at[r]);
+          if (!held[k] ||
+              (tail && key0 + 16 * k + 2 * t + (r & 1) + 8 * (r >> 1) >= rq.kv)) {
 #pragma unroll
-              for (int i = 0; i < VW; ++i) vw[k][r].w[i] = 0u;
+            for (int i = 0; i < VW; ++i) vw[k][r].w[i] = 0u;
+          }
+        }
+      __syncwarp();  // every lane has its codes: the place may be filled again
+      if (lane == 0) ptx::mbar_arrive(empty + 8 * take);
+      if (++take == S::kStages) {
+        take = 0;
+        parity ^= 1;
       }
-      // O^T += scale (V^T P^T), the scale once a block: tiles of one block add up first.
-      // (Their scale is the first one's: the second may have no token.)
-      const bool joint = KT == 2 && p.shift > 4;
+      // O^T += scale (V^T P^T), the scale once a block: tiles of one block add
+      // up first (their scale is the first one's: others may have no token).
+      const int joint = p.shift > 5 ? KT : p.shift > 4 ? 2 : 1;
 #pragma unroll
       for (int mp = 0; mp < MT / 2; ++mp) {
         float acc[2][NT][4];
@@ -503,6 +611,7 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[h][nt][i] = 0.f;
+        float f = 0.f;
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
           const uint32_t x0 = byte_perm(vw[k][0].w[mp], vw[k][1].w[mp], 0x5140);
@@ -518,8 +627,8 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
             mma_16816(acc[0][nt], a0, pb[nt][k][0], pb[nt][k][1]);
             mma_16816(acc[1][nt], a1, pb[nt][k][0], pb[nt][k][1]);
           }
-          if (!joint || k == KT - 1) {
-            const float f = joint ? vsc[0] : vsc[k];
+          if ((k & (joint - 1)) == 0) f = vsc[k];
+          if (((k + 1) & (joint - 1)) == 0) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -532,71 +641,133 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const CachedParams p) {
           }
         }
       }
-      load_v(s + 1, id_next);
-#pragma unroll
-      for (int k = 0; k < KT; ++k) id[k] = id_next[k];
-      blocks_of(s + 2, id_next);
     }
 
-    // The four warps' results together.
+    // The four warps' sums together, from warp 3 to warp 0, lane by lane (the
+    // same lane of each warp holds the same rows and head dimensions).
+    if (warp == kWarps - 1) {
+      if (!first) ptx::named_bar_sync(kBarRead, 64);  // by warp 0, in the unit before
+    } else {
+      ptx::named_bar_sync(kBarHop + warp, 64);
+      float* from = hop;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float mine[2], other[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j, from += 64) {
+          const float m2 = from[0], l2 = from[32];
+          const float now = fmaxf(m[nt][j], m2), base = now == -INFINITY ? 0.f : now;
+          mine[j] = ptx::ex2_approx(m[nt][j] - base);
+          other[j] = ptx::ex2_approx(m2 - base);
+          m[nt][j] = now;
+          l[nt][j] = l[nt][j] * mine[j] + l2 * other[j];
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i, from += 32)
+            o[nt][mt][i] = o[nt][mt][i] * mine[i & 1] + *from * other[i & 1];
+      }
+    }
+    first = false;
+    if (warp > 0) {
+      float* to = hop;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j, to += 64) {
+          to[0] = m[nt][j];
+          to[32] = l[nt][j];
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i, to += 32) *to = o[nt][mt][i];
+      }
+      named_bar_arrive(kBarHop + warp - 1, 64);
+      continue;
+    }
+    named_bar_arrive(kBarRead, 64);
+    const bool all_keys = x.c0 == 0 && x.c1 == x.chunks;
+    const long long slot = 2ll * blockIdx.x + (x.c0 == 0 ? 1 : 0);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float s = l[nt][j];
-        s += __shfl_xor_sync(~0u, s, 4);
-        s += __shfl_xor_sync(~0u, s, 8);
-        s += __shfl_xor_sync(~0u, s, 16);
-        if (g == 0) {
-          row_m[warp][8 * nt + 2 * t + j] = m[nt][j];
-          row_l[warp][8 * nt + 2 * t + j] = s;
-        }
-        float* dst = smem + (warp * kRows + 8 * nt + 2 * t + j) * kPitch + 4 * VW * g;
-#pragma unroll
-        for (int mt = 0; mt < MT; mt += 2)
-          *reinterpret_cast<float4*>(dst + 2 * mt) =
-              make_float4(o[nt][mt][j], o[nt][mt][2 + j], o[nt][mt + 1][j], o[nt][mt + 1][2 + j]);
-      }
-    __syncthreads();
-    const bool all_keys = c0 == 0 && c1 == sh.chunks;
-    const long long slot = 2ll * blockIdx.x + (c0 == 0 ? 1 : 0);
-    for (int i = threadIdx.x; i < kRows * (D / 4); i += kThreads) {
-      const int r = i / (D / 4), d = 4 * (i % (D / 4));
-      float top = row_m[0][r];
-#pragma unroll
-      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, row_m[w][r]);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f;
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = ptx::ex2_approx(row_m[w][r] - base);
-        const float4 y = *reinterpret_cast<const float4*>(smem + (w * kRows + r) * kPitch + d);
-        sum = fmaf(row_l[w][r], f, sum);
-        x.x = fmaf(y.x, f, x.x);
-        x.y = fmaf(y.y, f, x.y);
-        x.z = fmaf(y.z, f, x.z);
-        x.w = fmaf(y.w, f, x.w);
-      }
-      if (all_keys) {
-        const int row = row0 + r;
-        if (row < rows_in) {
-          const float n = top == -INFINITY ? 0.f : 1.f / sum;
+        float sum = l[nt][j];
+        sum += __shfl_xor_sync(~0u, sum, 4);
+        sum += __shfl_xor_sync(~0u, sum, 8);
+        sum += __shfl_xor_sync(~0u, sum, 16);
+        const int r = 8 * nt + 2 * t + j, row = x.row0 + r;
+        if (row >= rows_in) continue;
+        if (all_keys) {
+          const float n = m[nt][j] == -INFINITY && sum == sum ? 0.f : 1.f / sum;
           const int tok = row / p.group;
-          T* dst = static_cast<T*>(p.out) + (rq.start + tok) * p.o_token +
-                   (kvh * p.group + row - tok * p.group) * p.o_head + d;
-          *reinterpret_cast<uint2*>(dst) =
-              make_uint2(pack_out<T>(x.x * n, x.y * n), pack_out<T>(x.z * n, x.w * n));
+          uint4* dst = reinterpret_cast<uint4*>(
+              static_cast<T*>(p.out) + (rq.start + tok) * p.o_token +
+              (x.kvh * p.group + row - tok * p.group) * p.o_head + 4 * VW * g);
+#pragma unroll
+          for (int mt = 0; mt < MT; mt += 4)
+            dst[mt / 4] = make_uint4(pack_out<T>(o[nt][mt][j] * n, o[nt][mt][2 + j] * n),
+                                     pack_out<T>(o[nt][mt + 1][j] * n, o[nt][mt + 1][2 + j] * n),
+                                     pack_out<T>(o[nt][mt + 2][j] * n, o[nt][mt + 2][2 + j] * n),
+                                     pack_out<T>(o[nt][mt + 3][j] * n, o[nt][mt + 3][2 + j] * n));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(Parts<NT, D>::o(p.ws, slot) + r * D + 4 * VW * g);
+#pragma unroll
+          for (int mt = 0; mt < MT; mt += 2)
+            dst[mt / 2] = make_float4(o[nt][mt][j], o[nt][mt][2 + j], o[nt][mt + 1][j],
+                                      o[nt][mt + 1][2 + j]);
+          if (g == 0)
+            Parts<NT, D>::ml(p.ws, 2ll * gridDim.x, slot)[r] = make_float2(m[nt][j], sum);
         }
-      } else {
-        *reinterpret_cast<float4*>(Parts<NT, D>::o(p.ws, slot) + r * D + d) = x;
-        if (d == 0)
-          Parts<NT, D>::ml(p.ws, 2ll * gridDim.x, slot)[r] = make_float2(top, sum);
       }
-    }
-    __syncthreads();
-    at += c1 - c0;
   }
+  if (warp == kWarps - 1 && !first) ptx::named_bar_sync(kBarRead, 64);
+}
+
+template <typename T, int CODE, int D, int NT>
+__global__ void __launch_bounds__(kThreads, 2)
+split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+             const SplitParams p) {
+#if defined(__CUDA_ARCH_FEAT_SM100_ALL)
+  using S = Smem<D, NT>;
+  __shared__ Place place;
+  __shared__ int abort_flag;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (sbase - raw);
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      ptx::mbar_init(sbase + S::kOffBar + 8 * i, S::kGroups + 1);
+      ptx::mbar_init(sbase + S::kOffBar + 8 * (S::kStages + i), kWarps);
+    }
+    abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  long long* part_sum = reinterpret_cast<long long*>(smem + S::kOffHop);
+  const long long total = count_work<NT>(p, part_sum);
+  const long long each = work_each(total);
+  Cursor<NT> cursor;
+  cursor.at = each * blockIdx.x;
+  cursor.stop = min(cursor.at + each, total);
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (cursor.at >= cursor.stop) return;
+  if (threadIdx.x == 0) place = find_place<NT>(p, part_sum, cursor.at);
+  __syncthreads();
+  cursor.pl = place;
+  const WaitCtx w{&abort_flag, p.status, p.timeout_ns};
+  // Registers: 128 x (216 + 40) = 256 x 128.
+  if (warp < kWarps) {
+    ptx::setmaxnreg_inc<216>();
+    compute_role<T, CODE, D, NT>(p, cursor, sbase, smem, w);
+  } else {
+    ptx::setmaxnreg_dec<40>();
+    if (warp == kWarps) fetch_role<D, NT>(&map_k, &map_v, p, cursor, sbase, w);
+  }
+#endif
 }
 
 // Joins the parts of the units that were cut.  CTA c > 0 looks at the cut in
@@ -609,8 +780,8 @@ __global__ void __launch_bounds__(256) join_kernel(const CachedParams p) {
   __shared__ long long part_sum[256];
   __shared__ Place place;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long total = count_chunks<NT>(p, part_sum);
-  const long long each = chunks_each(total);
+  const long long total = count_work<NT>(p, part_sum);
+  const long long each = work_each(total);
   const long long cut = each * (blockIdx.x + 1ll);
   if (threadIdx.x == 0 && cut < total) place = find_place<NT>(p, part_sum, cut);
   __syncthreads();
@@ -621,11 +792,11 @@ __global__ void __launch_bounds__(256) join_kernel(const CachedParams p) {
   const Place pl = place;
   const Request rq = request_at(p, pl.request);
   const Shape sh = shape_of<NT>(p, rq);
-  const long long in = cut - pl.before;
-  const int unit = static_cast<int>(in / sh.chunks);
-  const long long begin = pl.before + static_cast<long long>(unit) * sh.chunks;
-  const long long end = begin + sh.chunks;
-  if (begin == cut || begin < cut - each) return;  // not cut here, or not for the first time
+  const int unit = quotient(cut - pl.before, sh.weight());
+  const long long begin = pl.before + static_cast<long long>(unit) * sh.weight();
+  const long long end = begin + sh.weight();
+  // Only if chunks lie in front of this cut, and none in front of the last one.
+  if (cut <= begin + kOver || cut - each > begin + kOver) return;
   const int tiles = sh.units / p.kv_heads;
   const int kvh = unit / tiles;
   const int row0 = (unit - kvh * tiles) * kRows;
@@ -663,7 +834,7 @@ __global__ void __launch_bounds__(256) join_kernel(const CachedParams p) {
         x[1] = fmaf(y.y, f, x[1]);
       }
     }
-    const float n = top == -INFINITY ? 0.f : 1.f / sum;
+    const float n = top == -INFINITY && sum == sum ? 0.f : 1.f / sum;
     const int row = row0 + r, tok = row / p.group;
     T* dst = static_cast<T*>(p.out) + (rq.start + tok) * p.o_token +
              (kvh * p.group + row - tok * p.group) * p.o_head + lane * (D / 32);
@@ -686,10 +857,7 @@ int row_tiles(int group, int max_new) {
   return want <= 8 ? 1 : want <= 16 ? 2 : 4;
 }
 
-template <int D, int NT>
-constexpr size_t smem_bytes() {
-  return sizeof(float) * kWarps * 8 * NT * (D + 4) + (NT >= 4 ? NT * (D / 16) * 32 * 8 : 0);
-}
+constexpr int kMostCtasPerSm = 2;  // by shared memory and registers; bounds the workspace
 
 template <typename T, int CODE, int D, int NT>
 int resident_ctas(int* ctas) {
@@ -698,7 +866,7 @@ int resident_ctas(int* ctas) {
   if (cudaGetDevice(&dev) != cudaSuccess) return ATTN_ERR_CUDA;
   int n = dev < 64 ? *static_cast<volatile int*>(&known[dev]) : 0;
   if (n == 0) {
-    constexpr int smem = static_cast<int>(smem_bytes<D, NT>());
+    constexpr int smem = Smem<D, NT>::kBytes;
     auto kern = split_kernel<T, CODE, D, NT>;
     int sms = 0, occ = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
@@ -707,19 +875,46 @@ int resident_ctas(int* ctas) {
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kThreads, smem) != cudaSuccess)
       return ATTN_ERR_CUDA;
     if (occ < 1) return ATTN_ERR_RESOURCE;
-    n = sms * occ;
+    n = sms * (occ < kMostCtasPerSm ? occ : kMostCtasPerSm);
     if (dev < 64) *static_cast<volatile int*>(&known[dev]) = n;
   }
   *ctas = n;
   return ATTN_OK;
 }
 
-constexpr int kMostCtasPerSm = 8;  // bounds the workspace (registers allow fewer)
-
 size_t part_bytes(int D, int nt) { return sizeof(float) * 8 * nt * (D + 2) * 2; }
 
+// The codes of a pool as [num_blocks * kv_heads][bytes of a block / 128][128
+// bytes], fetched 16 keys at a time with the 128-byte swizzle.
+template <int D>
+int codes_map(CUtensorMap* m, const void* codes, const CachedParams& p) {
+  const EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr) return ATTN_ERR_CUDA;
+  const long long pieces = static_cast<long long>(p.num_blocks) * p.kv_heads;
+  if (pieces > INT_MAX) return ATTN_ERR_INVALID_ARG;  // (a coordinate)
+  const cuuint64_t block = static_cast<cuuint64_t>(D) << p.shift;
+  const cuuint64_t dims[3] = {128, block / 128, static_cast<cuuint64_t>(pieces)};
+  const cuuint64_t strides[2] = {128, block};
+  const cuuint32_t box[3] = {128, 16 * D / 128, 1};
+  const cuuint32_t one[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, one,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? ATTN_OK
+             : ATTN_ERR_TENSOR_MAP;
+}
+
 template <typename T, int CODE, int D, int NT>
-int launch(CachedParams p, int max_new, void* ws, unsigned long long ws_bytes, cudaStream_t st) {
+int launch(const CachedParams& cp, int max_new, void* ws, unsigned long long ws_bytes,
+           cudaStream_t st) {
+  SplitParams p;
+  static_cast<CachedParams&>(p) = cp;
+  p.status = device_status_ptr();
+  if (p.status == nullptr) return ATTN_ERR_CUDA;
+  p.timeout_ns = current_timeout_ns();
+  CUtensorMap map_k, map_v;
+  if (const int e = codes_map<D>(&map_k, p.kc, p)) return e;
+  if (const int e = codes_map<D>(&map_v, p.vc, p)) return e;
   int ctas = 0;
   const int rc = resident_ctas<T, CODE, D, NT>(&ctas);
   if (rc != ATTN_OK) return rc;
@@ -731,7 +926,7 @@ int launch(CachedParams p, int max_new, void* ws, unsigned long long ws_bytes, c
   if (most < ctas) ctas = static_cast<int>(most);
   if (ws_bytes < part_bytes(D, NT) * ctas) return ATTN_ERR_SCRATCH_LIMIT;
   p.ws = static_cast<float*>(ws);
-  split_kernel<T, CODE, D, NT><<<ctas, kThreads, smem_bytes<D, NT>(), st>>>(p);
+  split_kernel<T, CODE, D, NT><<<ctas, kThreads, Smem<D, NT>::kBytes, st>>>(map_k, map_v, p);
   if (cudaGetLastError() != cudaSuccess) return ATTN_ERR_CUDA;
   if (chunks == 1 || ctas == 1) return ATTN_OK;  // no unit can be cut
   // The joining kernel starts while the first still runs (its search of the
@@ -745,7 +940,7 @@ int launch(CachedParams p, int max_new, void* ws, unsigned long long ws_bytes, c
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, p) == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, static_cast<const CachedParams&>(p)) == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
 }
 
 template <typename T, int CODE, int D>
