@@ -1,6 +1,8 @@
 // Attention over the paged 8-bit cache: what its kernels share.
 #pragma once
 
+#include <cuda.h>
+
 #include "cache.cuh"
 
 namespace attnprof {
@@ -33,6 +35,7 @@ __device__ __forceinline__ Request request_at(const CachedParams& p, int r) {
   return Request{a, max(b - a, 0), min(max(p.kv_lens[r], 0), p.capacity)};
 }
 
+int codes_map(CUtensorMap* m, const void* codes, const CachedParams& p, int D);
 int launch_split(const CachedParams& p, int D, int dtype, int code, int max_new, void* ws,
                  unsigned long long ws_bytes, cudaStream_t st);
 int launch_tiled(const CachedParams& p, int D, int dtype, int code, cudaStream_t st);

@@ -884,26 +884,6 @@ int resident_ctas(int* ctas) {
 
 size_t part_bytes(int D, int nt) { return sizeof(float) * 8 * nt * (D + 2) * 2; }
 
-// The codes of a pool as [num_blocks * kv_heads][bytes of a block / 128][128
-// bytes], fetched 16 keys at a time with the 128-byte swizzle.
-template <int D>
-int codes_map(CUtensorMap* m, const void* codes, const CachedParams& p) {
-  const EncodeTiledFn enc = encode_tiled_fn();
-  if (enc == nullptr) return ATTN_ERR_CUDA;
-  const long long pieces = static_cast<long long>(p.num_blocks) * p.kv_heads;
-  if (pieces > INT_MAX) return ATTN_ERR_INVALID_ARG;  // (a coordinate)
-  const cuuint64_t block = static_cast<cuuint64_t>(D) << p.shift;
-  const cuuint64_t dims[3] = {128, block / 128, static_cast<cuuint64_t>(pieces)};
-  const cuuint64_t strides[2] = {128, block};
-  const cuuint32_t box[3] = {128, 16 * D / 128, 1};
-  const cuuint32_t one[3] = {1, 1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, one,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-             ? ATTN_OK
-             : ATTN_ERR_TENSOR_MAP;
-}
-
 template <typename T, int CODE, int D, int NT>
 int launch(const CachedParams& cp, int max_new, void* ws, unsigned long long ws_bytes,
            cudaStream_t st) {
@@ -913,8 +893,8 @@ int launch(const CachedParams& cp, int max_new, void* ws, unsigned long long ws_
   if (p.status == nullptr) return ATTN_ERR_CUDA;
   p.timeout_ns = current_timeout_ns();
   CUtensorMap map_k, map_v;
-  if (const int e = codes_map<D>(&map_k, p.kc, p)) return e;
-  if (const int e = codes_map<D>(&map_v, p.vc, p)) return e;
+  if (const int e = codes_map(&map_k, p.kc, p, D)) return e;
+  if (const int e = codes_map(&map_v, p.vc, p, D)) return e;
   int ctas = 0;
   const int rc = resident_ctas<T, CODE, D, NT>(&ctas);
   if (rc != ATTN_OK) return rc;
@@ -965,6 +945,25 @@ int launch_code(const CachedParams& p, int D, int code, int n, void* ws, unsigne
 }
 
 }  // namespace
+
+// The codes of a pool as [num_blocks * kv_heads][bytes of a block / 128][128
+// bytes], fetched 16 keys at a time with the 128-byte swizzle.
+int codes_map(CUtensorMap* m, const void* codes, const CachedParams& p, int D) {
+  const EncodeTiledFn enc = encode_tiled_fn();
+  if (enc == nullptr) return ATTN_ERR_CUDA;
+  const long long pieces = static_cast<long long>(p.num_blocks) * p.kv_heads;
+  if (pieces > INT_MAX) return ATTN_ERR_INVALID_ARG;  // (a coordinate)
+  const cuuint64_t block = static_cast<cuuint64_t>(D) << p.shift;
+  const cuuint64_t dims[3] = {128, block / 128, static_cast<cuuint64_t>(pieces)};
+  const cuuint64_t strides[2] = {128, block};
+  const cuuint32_t box[3] = {128, static_cast<cuuint32_t>(16 * D / 128), 1};
+  const cuuint32_t one[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, one,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? ATTN_OK
+             : ATTN_ERR_TENSOR_MAP;
+}
 
 int launch_split(const CachedParams& p, int D, int dtype, int code, int max_new, void* ws,
                  unsigned long long ws_bytes, cudaStream_t st) {

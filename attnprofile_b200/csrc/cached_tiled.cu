@@ -6,10 +6,12 @@
 // share every key and value) of one request and kv head: two tiles of 128 rows
 // whose softmax steps take turns, as in the dense kernel of this library.  Per
 // 128 keys:
-//   * a warpgroup reads the codes (through L2: the row tiles of a head follow
-//     each other), turns them into f16 and writes them into a ring of shared
+//   * one warp fetches codes by TMA and scales by cp.async (through L2: the row
+//     tiles of a head follow each other);
+//   * a warpgroup turns them into f16 and writes them into a ring of shared
 //     memory tiles in the tensor cores' 128-byte swizzle: 8 bits to 16 once for
-//     256 rows.  The codes of the next tile are on their way meanwhile.
+//     256 rows.  (Codes read by that warpgroup itself into registers: 1295 us
+//     where this form takes @@ on 3 chunks of 2048 tokens, 32 heads of 128.)
 //   * one thread issues tcgen05.mma: S = Q K^T and O += P V, sums in tensor
 //     memory, P read from there too (it overwrites S);
 //   * a warpgroup per tile runs the online softmax, a thread a row, and moves O
@@ -38,7 +40,8 @@ constexpr int kBM = 128;                 // rows of a tile
 constexpr int kBN = 128;                 // keys of a step
 constexpr int kUnit = 2 * kBM;           // rows of a CTA
 constexpr int kThreads = 512;            // 2 softmax warpgroups, 1 converting, 1 with the issuer
-constexpr int kScaleRing = 8;            // steps whose K scales are kept (see convert_role)
+constexpr int kScaleRing = 8;            // steps whose K scales are kept: the fetching warp is at
+                                         // most 6 steps in front of the softmax
 constexpr float kMove = 8.f;             // growth of the maximum (log2) that moves O
 constexpr float kLift = 7.f;             // P is held as 2^kLift p
 
@@ -46,11 +49,16 @@ template <int D>
 struct Tile {
   static constexpr int kBytes = kBN * D * 2;        // one tile in 16 bits
   static constexpr int kBlock = kBN * 128;          // its 64-column blocks
-  static constexpr int kSlots = D == 128 ? 5 : 8;   // of the ring
+  static constexpr int kSlots = D == 128 ? 4 : 6;   // of the ring of tiles in 16 bits
+  static constexpr int kCodes = kBN * D;            // one tile in 8 bits
+  static constexpr int kGroup = 16 * D;             // 16 keys of it
+  static constexpr int kStages = D == 128 ? 2 : 4;  // of the ring of tiles in 8 bits
   static constexpr int kOffKv = 2 * kBytes;
-  static constexpr int kOffScale = kOffKv + kSlots * kBytes;        // [kScaleRing][12] f32
-  static constexpr int kOffBar = kOffScale + kScaleRing * 12 * 4;
-  static constexpr int kBars = 2 * kSlots + 2 + 2 + 4 + 2 + 1;
+  static constexpr int kOffCodes = kOffKv + kSlots * kBytes;
+  static constexpr int kOffScale = kOffCodes + kStages * kCodes;    // [kScaleRing][12] of K
+  static constexpr int kOffVScale = kOffScale + kScaleRing * 12 * 4;  // [kStages][8]
+  static constexpr int kOffBar = kOffVScale + kStages * 8 * 4;
+  static constexpr int kBars = 2 * kSlots + 2 * kStages + 2 + 2 + 4 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;
   static constexpr int kSmem = kOffMisc + 32 + 1024;                // + alignment
   static_assert(kSmem <= 232448, "shared memory");
@@ -61,7 +69,9 @@ template <int D>
 struct Bar {
   static constexpr int kFull = 0;
   static constexpr int kEmpty = Tile<D>::kSlots;
-  static constexpr int kQ = 2 * Tile<D>::kSlots;
+  static constexpr int kCodesFull = 2 * Tile<D>::kSlots;
+  static constexpr int kCodesEmpty = kCodesFull + Tile<D>::kStages;
+  static constexpr int kQ = kCodesEmpty + Tile<D>::kStages;
   static constexpr int kS = kQ + 2;
   static constexpr int kP = kS + 2;       // [tile][part]
   static constexpr int kO = kP + 4;
@@ -156,7 +166,83 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) {
 }
 
 // ---------------------------------------------------------------------------
-// Converting warpgroup: items K_0, V_0, K_1, V_1, ... through the ring.
+// Fetching warp: items K_0, V_0, K_1, V_1, ... in 8 bits.  Lane g < 8 fetches
+// keys 16 g .. 16 g + 15 of each.
+// ---------------------------------------------------------------------------
+template <int D>
+__device__ void fetch_role(const CUtensorMap* map_k, const CUtensorMap* map_v,
+                           const TiledParams& p, const Unit& u, uint32_t sbase,
+                           const WaitCtx& w) {
+  using T = Tile<D>;
+  auto bar = [&](int i) { return sbase + T::kOffBar + 8u * i; };
+  const int lane = threadIdx.x & 31;
+  const int* table = p.tables + u.request * p.table_stride;
+  auto id_of = [&](int j) {
+    const int key = j * kBN + 16 * lane;
+    if (lane < 8 && key < u.kv_end) {
+      const int id = table[key >> p.shift];
+      if (id >= 0 && id < p.num_blocks) return id;
+    }
+    return -1;
+  };
+  int sent = 0;
+  auto fetch = [&](bool is_v, int j, int id) {
+    const int stage = sent % T::kStages;
+    if (!__all_sync(~0u, wait_bar(bar(Bar<D>::kCodesEmpty + stage), ((sent / T::kStages) & 1) ^ 1, w,
+                                  kSiteKvEmpty)))
+      return false;
+    const uint32_t full = bar(Bar<D>::kCodesFull + stage);
+    const int n = __popc(__ballot_sync(~0u, id >= 0));
+    // Where the group's scale goes: K's to the softmax, V's to the conversion.
+    const uint32_t scale_at =
+        sbase + (is_v ? T::kOffVScale + 4 * (8 * stage + lane)
+                      : T::kOffScale + 4 * (12 * (j % kScaleRing) + lane));
+    if (!is_v) {  // groups whose block is none, bit by bit
+      const unsigned holes =
+          __ballot_sync(~0u, lane < 8 && id < 0 && j * kBN + 16 * lane < u.kv_end);
+      if (lane == 0)
+        ptx::st_shared_f32(sbase + T::kOffScale + 4 * (12 * (j % kScaleRing) + 8),
+                           __uint_as_float(holes));
+    }
+    if (lane == 0) ptx::mbar_arrive_expect_tx(full, n * T::kGroup);
+    __syncwarp();
+    if (id >= 0) {
+      const int off = (j * kBN + 16 * lane) & ((1 << p.shift) - 1);
+      const int piece = id * p.kv_heads + u.kvh;
+      ptx::tma_load_3d(sbase + T::kOffCodes + stage * T::kCodes + lane * T::kGroup,
+                       is_v ? map_v : map_k, full, 0, D == 128 ? off : off / 2, piece);
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scale_at),
+                   "l"((is_v ? p.vs : p.ks) + piece)
+                   : "memory");
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full) : "memory");
+    } else if (lane < 8) {
+      ptx::st_shared_f32(scale_at, 0.f);
+      ptx::mbar_arrive(full);
+    }
+    ++sent;
+    return true;
+  };
+  int id = id_of(0), next = id_of(1);
+  for (int j = 0; j < u.steps; ++j) {
+    const int after = id_of(j + 2);
+    if (!fetch(false, j, id) || !fetch(true, j, id)) break;
+    id = next;
+    next = after;
+  }
+  // After a wait that ran out: copies on their way end before the shared
+  // memory that they go to does.
+  if (*w.abort) {
+    for (int i = max(0, sent - T::kStages); i < sent; ++i) {
+      const unsigned long long t0 = ptx::globaltimer_ns();
+      while (!ptx::mbar_try_wait(bar(Bar<D>::kCodesFull + i % T::kStages), (i / T::kStages) & 1) &&
+             ptx::globaltimer_ns() - t0 < p.timeout_ns) {
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Converting warpgroup: 8 bits to 16, item by item.
 // ---------------------------------------------------------------------------
 template <int CODE, int D>
 __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase, uint8_t* sgen,
@@ -166,16 +252,16 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
   constexpr float kVLift = CODE == ATTN_CODE_E4M3 ? 128.f : 256.f;
   auto bar = [&](int i) { return sbase + T::kOffBar + 8u * i; };
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 3;
-  const int* table = p.tables + u.request * p.table_stride;
   float* misc = reinterpret_cast<float*>(sgen + T::kOffMisc);
-  auto valid = [&](int id) { return id >= 0 && id < p.num_blocks; };
 
   // The largest V scale in sight.
   float ref = 0.f;
+  const int* table = p.tables + u.request * p.table_stride;
   const int blocks = (u.kv_end + (1 << p.shift) - 1) >> p.shift;
   for (int b = 32 * warp + lane; b < blocks; b += 128) {
     const int id = table[b];
-    if (valid(id)) ref = fmaxf(ref, p.vs[static_cast<long long>(id) * p.kv_heads + u.kvh]);
+    if (id >= 0 && id < p.num_blocks)
+      ref = fmaxf(ref, p.vs[static_cast<long long>(id) * p.kv_heads + u.kvh]);
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) ref = fmaxf(ref, __shfl_xor_sync(~0u, ref, d));
@@ -186,109 +272,91 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
   if (warp == 0 && lane == 0) misc[2] = ref / kVLift;  // what O is multiplied by
   const float to_v = kVLift / ref;
 
-  // Lane g < 8 holds what concerns keys 16 g .. 16 g + 15 of a step.
-  auto ids_of = [&](int j) {
-    const int key = j * kBN + 16 * lane;
-    if (j < u.steps && lane < 8 && key < u.rq.kv) {
-      const int id = table[key >> p.shift];
-      if (valid(id)) return id;
-    }
-    return -1;
-  };
-  // A thread's piece `it` of a tile: row and 16-byte piece of that row, so that
-  // global reads cover whole rows and, in the 16-bit tile, the 8 lanes of
-  // one shared memory pass hit 8 different 16-byte banks.
-  auto row_of = [&](int it) {
-    return D == 128 ? 16 * it + 4 * warp + 2 * (lane >> 4) + ((lane >> 2) & 1)
-                    : 32 * it + 8 * warp + (lane >> 2);
-  };
+  // A thread's piece `it` of a tile: a row and 16 codes of it, so that the 8
+  // lanes of one pass through shared memory meet 8 different 16-byte banks both
+  // in the 8-bit tile (16 keys after 16 keys, 128-byte rows) and in the 16-bit
+  // one (64-column blocks of 128-byte rows).
+  const int row0 = D == 128 ? 4 * warp + 2 * (lane >> 4) + ((lane >> 2) & 1) : 8 * warp + (lane >> 2);
   const int piece = D == 128 ? (lane & 3) + 4 * (((lane >> 2) ^ (lane >> 3)) & 1) : lane & 3;
+  constexpr int kRowStep = D == 128 ? 16 : 32;   // rows from one piece to the next
+  const int line = D == 128 ? row0 : row0 >> 1;  // 128-byte line of codes
+  const int at8 = D == 128 ? piece : (row0 & 1) * 4 + piece;
+  const uint32_t codes_at = sbase + T::kOffCodes + line * 128 + ((at8 ^ (line & 7)) << 4);
+  const int k16 = (2 * piece) & 7;
+  const uint32_t tile_at = sbase + T::kOffKv + (piece >> 2) * T::kBlock + row0 * 128;
+  const uint32_t at_lo = (k16 ^ (row0 & 7)) << 4, at_hi = ((k16 + 1) ^ (row0 & 7)) << 4;
   auto group_of = [&](int it) { return D == 128 ? it : 2 * it + (warp >> 1); };
-
-  uint4 c[kIters];
-  auto load = [&](int it, int j, bool is_v, int ids) {
-    const int id = __shfl_sync(~0u, ids, group_of(it));
-    const int row = row_of(it), key = j * kBN + row;
-    c[it] = make_uint4(0, 0, 0, 0);
-    // (keys behind the last token may be any bits: masked in the scores, and
-    // zero among the values, where 0 * NaN would reach a sum)
-    if (id >= 0 && (!is_v || key < u.rq.kv)) {
-      const long long at =
-          (((static_cast<long long>(id) * p.kv_heads + u.kvh) << p.shift) +
-           (key & ((1 << p.shift) - 1))) * D + 16 * piece;
-      c[it] = __ldg(reinterpret_cast<const uint4*>((is_v ? p.vc : p.kc) + at));
-    }
-  };
-
-  int ids = ids_of(0), ids_next = ids_of(1);
-  float ks = 0.f, vs = 0.f;  // of this lane's group, for the step being converted
-  auto scales_of = [&](int id) {
-    const long long at = static_cast<long long>(id) * p.kv_heads + u.kvh;
-    ks = id >= 0 ? p.ks[at] * p.scale_log2 : -1.f;  // -1: not a block of the pool
-    vs = id >= 0 ? p.vs[at] * to_v : 0.f;
-  };
-  scales_of(ids);
-#pragma unroll
-  for (int it = 0; it < kIters; ++it) load(it, 0, false, ids);
 
   for (int t = 0; t < 2 * u.steps; ++t) {
     const bool is_v = (t & 1) != 0;
     const int j = t >> 1;
-    const int slot = t % T::kSlots;
-    const bool ok = wait_bar(bar(Bar<D>::kEmpty + slot), ((t / T::kSlots) & 1) ^ 1, w, kSiteKvEmpty);
+    const int stage = t % T::kStages, slot = t % T::kSlots;
+    bool ok = wait_bar(bar(Bar<D>::kCodesFull + stage), (t / T::kStages) & 1, w, kSiteKvFull);
     if (!__all_sync(~0u, ok)) return;
-    const uint32_t tile = sbase + T::kOffKv + slot * T::kBytes;
-    if (!is_v && warp == 0) {
-      // K scales of the step.  The place's last reader was the softmax of step
-      // j - kScaleRing; this slot came free after P V of a later step.
-      float* dst = reinterpret_cast<float*>(sgen + T::kOffScale) + (j % kScaleRing) * 12;
-      const bool hole = lane < 8 && ks == -1.f && j * kBN + 16 * lane < u.rq.kv;
-      const unsigned holes = __ballot_sync(~0u, hole);
-      if (lane < 8) dst[lane] = ks;
-      if (lane == 8) dst[8] = __uint_as_float(holes);
+    uint32_t c[kIters][4];
+#pragma unroll
+    for (int it = 0; it < kIters; ++it)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(c[it][0]), "=r"(c[it][1]), "=r"(c[it][2]), "=r"(c[it][3])
+                   : "r"(codes_at + stage * T::kCodes + it * kRowStep * D)
+                   : "memory");
+    float vs[kIters];
+    if (is_v) {
+      const float* scale = reinterpret_cast<const float*>(sgen + T::kOffVScale) + 8 * stage;
+#pragma unroll
+      for (int it = 0; it < kIters; ++it) vs[it] = scale[group_of(it)] * to_v;
+      // What lies behind the last token, or where nothing was fetched, may be
+      // any bits: 0 * NaN would reach a sum.  (Among the keys it is masked.)
+      if (j * kBN + kBN > u.rq.kv) {
+#pragma unroll
+        for (int it = 0; it < kIters; ++it)
+          if (j * kBN + row0 + it * kRowStep >= u.rq.kv) c[it][0] = c[it][1] = c[it][2] = c[it][3] = 0u;
+      }
+#pragma unroll
+      for (int it = 0; it < kIters; ++it)
+        if (vs[it] == 0.f) c[it][0] = c[it][1] = c[it][2] = c[it][3] = 0u;
     }
-    // The next item's codes replace this one's as they are used up.
-    const bool more = t + 1 < 2 * u.steps;
-    const int ids_load = is_v ? ids_next : ids;
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar(Bar<D>::kCodesEmpty + stage));
+    ok = wait_bar(bar(Bar<D>::kEmpty + slot), ((t / T::kSlots) & 1) ^ 1, w, kSiteKvEmpty);
+    if (!__all_sync(~0u, ok)) return;
+    const uint32_t tile = tile_at + slot * T::kBytes;
 #pragma unroll
     for (int it = 0; it < kIters; ++it) {
       uint32_t h[8];
-      const uint32_t word[4] = {c[it].x, c[it].y, c[it].z, c[it].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        h[2 * i] = Code<CODE>::half2_lo(word[i]);
-        h[2 * i + 1] = Code<CODE>::half2_hi(word[i]);
+        h[2 * i] = Code<CODE>::half2_lo(c[it][i]);
+        h[2 * i + 1] = Code<CODE>::half2_hi(c[it][i]);
       }
       if (is_v) {
-        const float f = __shfl_sync(~0u, vs, group_of(it));
-        if ((__float_as_int(f) & 0x7fffff) == 0) {  // a power of two (or 0)
-          const __half2 f2 = __float2half2_rn(f);
+        if ((__float_as_int(vs[it]) & 0x7fffff) == 0) {  // a power of two (or 0)
+          const __half2 f2 = __float2half2_rn(vs[it]);
 #pragma unroll
           for (int i = 0; i < 8; ++i) h[i] = mul_half2(h[i], f2);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float2 x = half2_to_float2(h[i]);
-            h[i] = half2_of(x.x * f, x.y * f);
+            h[i] = half2_of(x.x * vs[it], x.y * vs[it]);
           }
         }
       }
-      if (more) load(it, (t + 1) >> 1, !is_v, ids_load);
-      const int row = row_of(it);
-      const uint32_t base = tile + (piece >> 2) * T::kBlock + row * 128;
-      const int k16 = (2 * piece) & 7;
-      st_shared_v4(base + (((k16) ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
-      st_shared_v4(base + (((k16 + 1) ^ (row & 7)) << 4), h[4], h[5], h[6], h[7]);
+      const uint32_t base = tile + it * kRowStep * 128;
+      st_shared_v4(base + at_lo, h[0], h[1], h[2], h[3]);
+      st_shared_v4(base + at_hi, h[4], h[5], h[6], h[7]);
     }
     ptx::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(bar(Bar<D>::kFull + slot));
-    if (is_v) {
-      ids = ids_next;
-      scales_of(ids);
-      ids_next = ids_of(j + 2);
-    }
   }
+}
+
+__device__ __forceinline__ uint64_t descriptor(uint32_t lo) {
+  constexpr uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "n"(hi));
+  return d;
 }
 
 // ---------------------------------------------------------------------------
@@ -302,31 +370,34 @@ __device__ void mma_role(const Unit& u, uint32_t tmem, uint32_t sbase, const Wai
   constexpr uint32_t kIdescPV = ptx::idesc_f16(kBM, D, false, true);
   const int tiles = u.rows_in - u.row0 > kBM ? 2 : 1;
   const int n = u.steps;
-  uint64_t qd[2];
-  for (int i = 0; i < 2; ++i) qd[i] = ptx::smem_desc_sw128(sbase + i * T::kBytes, 16, 1024);
-  const uint64_t kd0 = ptx::smem_desc_sw128(sbase + T::kOffKv, 16, 1024);
-  const uint64_t vd0 = ptx::smem_desc_sw128(sbase + T::kOffKv, T::kBlock, 1024);
-  auto slot_off = [](int t) { return static_cast<uint32_t>((t % T::kSlots) * T::kBytes) >> 4; };
+  // Shared memory descriptors: their upper word is the same for all operands
+  // (SBO 1024, version 1, 128-byte swizzle), the lower one has the address >> 4
+  // and, from bit 16, LBO >> 4 (64-column blocks of V).  Only lower words are
+  // kept: with 64-bit ones this thread's registers overflowed into local memory.
   auto ring_wait = [&](int t) {
     const bool ok = wait_bar(bar(Bar<D>::kFull + t % T::kSlots), (t / T::kSlots) & 1, w, kSiteKvFull);
     if (ok) ptx::tc_fence_after();
     return ok;
   };
+  const uint32_t q_lo = (sbase >> 4) | (1u << 16);
+  const uint32_t kv_lo = (sbase + T::kOffKv) >> 4;
   auto issue_s = [&](int i, int t) {
-    const uint64_t kd = ptx::desc_add(kd0, slot_off(t));
+    const uint32_t q = q_lo + i * (T::kBytes >> 4);
+    const uint32_t k = kv_lo + (t % T::kSlots) * (T::kBytes >> 4) + (1u << 16);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       const uint32_t off = static_cast<uint32_t>((kk >> 2) * T::kBlock + (kk & 3) * 32) >> 4;
-      ptx::mma_ss(tmem + i * kBN, ptx::desc_add(qd[i], off), ptx::desc_add(kd, off), kIdescS,
+      ptx::mma_ss(tmem + i * kBN, descriptor(q + off), descriptor(k + off), kIdescS,
                   kk > 0 ? 1u : 0u);
     }
   };
   auto issue_pv = [&](int i, int j, int t, int k0, int k1) {
-    const uint64_t vd = ptx::desc_add(vd0, slot_off(t));
+    const uint32_t v =
+        kv_lo + (t % T::kSlots) * (T::kBytes >> 4) + (static_cast<uint32_t>(T::kBlock >> 4) << 16);
 #pragma unroll
     for (int kk = k0; kk < k1; ++kk)
       ptx::mma_ts(tmem + 2 * kBN + i * D, tmem + i * kBN + kk * 8,
-                  ptx::desc_add(vd, static_cast<uint32_t>(kk * 2048) >> 4), kIdescPV,
+                  descriptor(v + (static_cast<uint32_t>(kk * 2048) >> 4)), kIdescPV,
                   (j > 0 || kk > 0) ? 1u : 0u);
   };
 
@@ -426,6 +497,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
 
   const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * wi) << 16);
   const uint32_t s_col = i * kBN, o_col = 2 * kBN + i * D;
+  const float to_log2 = row_f * p.scale_log2;
   float m = -INFINITY, l = 0.f;  // maximum in log2 units, sum of 2^kLift p
   bool ok = true;
   for (int j = 0; j < u.steps && tile_there; ++j) {
@@ -446,15 +518,17 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
       for (int c = 0; c < kBN; ++c)
         if (c >= lim || ((holes >> (c / 16)) & 1u)) s[c] = __float_as_uint(-INFINITY);
     }
-    // Factor of group g's scores.  That of a group which the row does not see
-    // may be anything (NaN): 1 keeps -inf there.  The least factor keeps
+    // Factors of the groups' scores.  That of a group which the row does not
+    // see may be anything (NaN): 1 keeps -inf there.  The least factor keeps
     // -inf too, where ks * row_f may reach 0 (f16 products are below 2^32, so
     // scores that small are 0 either way); NaN stays.
-    auto factor = [&](int g) {
-      float f = ks[g] * row_f;
+    float factor[kBN / 16];
+#pragma unroll
+    for (int g = 0; g < kBN / 16; ++g) {
+      float f = ks[g] * to_log2;
       if (f < 0x1p-90f) f = 0x1p-90f;
-      return (16 * g >= lim || ((holes >> g) & 1u)) ? 1.f : f;
-    };
+      factor[g] = (16 * g >= lim || ((holes >> g) & 1u)) ? 1.f : f;
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int g = 0; g < kBN / 16; ++g) {
@@ -465,7 +539,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
                           __uint_as_float(s[16 * g + 3 * k + 2]));
       const float b = ptx::fmax3(a[0], a[1], a[2]);
       const float d = ptx::fmax3(a[3], a[4], __uint_as_float(s[16 * g + 15]));
-      top = fmaxf(top, fmaxf(b, d) * factor(g));
+      top = fmaxf(top, fmaxf(b, d) * factor[g]);
     }
     float alpha = 1.f;
     bool move = false;
@@ -498,7 +572,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int c0 = 32 * c + 2 * e;
-        const float f = factor(c0 / 16);
+        const float f = factor[c0 / 16];
         const uint64_t x2 = ptx::f2_fma(
             ptx::f2_pack(__uint_as_float(s[c0]), __uint_as_float(s[c0 + 1])), ptx::f2_pack(f, f),
             neg2);
@@ -561,7 +635,9 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
 }
 
 template <typename TQ, int CODE, int D>
-__global__ void __launch_bounds__(kThreads, 1) tiled_kernel(const TiledParams p) {
+__global__ void __launch_bounds__(kThreads, 1)
+tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+             const TiledParams p) {
 #if defined(__CUDA_ARCH_FEAT_SM100_ALL)
   using T = Tile<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -579,6 +655,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiled_kernel(const TiledParams p)
     for (int s = 0; s < T::kSlots; ++s) {
       ptx::mbar_init(bar(Bar<D>::kFull + s), 4);
       ptx::mbar_init(bar(Bar<D>::kEmpty + s), 1);
+    }
+    for (int s = 0; s < T::kStages; ++s) {
+      ptx::mbar_init(bar(Bar<D>::kCodesFull + s), 8 + 1);
+      ptx::mbar_init(bar(Bar<D>::kCodesEmpty + s), 4);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(bar(Bar<D>::kQ + i), kBM);
@@ -601,16 +681,17 @@ __global__ void __launch_bounds__(kThreads, 1) tiled_kernel(const TiledParams p)
   const uint32_t tmem = *tmem_slot;
   const WaitCtx w{abort_flag, p.status, p.timeout_ns};
 
-  // Registers of the four warpgroups: 128 x (2 * 184 + 96 + 48) = 512 * 128.
+  // Registers of the four warpgroups: 128 x (2 * 176 + 88 + 72) = 512 * 128.
   if (warp < 8) {
-    ptx::setmaxnreg_inc<184>();
+    ptx::setmaxnreg_inc<176>();
     softmax_role<TQ, D>(p, u, warp >> 2, tmem, sbase, sgen, w);
   } else if (warp < 12) {
-    ptx::setmaxnreg_dec<96>();
+    ptx::setmaxnreg_dec<88>();
     convert_role<CODE, D>(p, u, sbase, sgen, w);
   } else {
-    ptx::setmaxnreg_dec<48>();
+    ptx::setmaxnreg_dec<72>();
     if (warp == 12 && lane == 0) mma_role<D>(u, tmem, sbase, w);
+    if (warp == 13) fetch_role<D>(&map_k, &map_v, p, u, sbase, w);
     __syncwarp();
   }
   ptx::tc_fence_before();
@@ -625,6 +706,9 @@ __global__ void __launch_bounds__(kThreads, 1) tiled_kernel(const TiledParams p)
 template <typename TQ, int CODE, int D>
 int launch(const TiledParams& p, cudaStream_t st) {
   auto kern = tiled_kernel<TQ, CODE, D>;
+  CUtensorMap map_k, map_v;
+  if (const int e = codes_map(&map_k, p.kc, p, D)) return e;
+  if (const int e = codes_map(&map_v, p.vc, p, D)) return e;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<D>::kSmem) !=
       cudaSuccess)
     return ATTN_ERR_RESOURCE;
@@ -632,7 +716,7 @@ int launch(const TiledParams& p, cudaStream_t st) {
   const long long units =
       p.kv_heads * (static_cast<long long>(p.tokens) * p.group / kUnit + p.batch);
   if (units > INT_MAX) return ATTN_ERR_INVALID_ARG;
-  kern<<<static_cast<unsigned>(units), kThreads, Tile<D>::kSmem, st>>>(p);
+  kern<<<static_cast<unsigned>(units), kThreads, Tile<D>::kSmem, st>>>(map_k, map_v, p);
   return cudaGetLastError() == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
 }
 
