@@ -99,45 +99,50 @@ __device__ __forceinline__ int row_limit(const CachedParams& p, const Request& r
   return min(max(last, 0), rq.kv);
 }
 
-// The unit of this CTA.  Units are taken from the last to the first, and
-// within a request the heads of a row tile follow each other: causal rows
-// that see most keys begin first, and neighbours share keys in L2.
-__device__ bool find_unit(const CachedParams& p, Unit& u) {
-  __shared__ long long warp_sum[kThreads / 32];
+// The unit of this CTA.  The requests with most keys come first and, in each,
+// the last rows (causal: those that see most), so that the last CTAs to start
+// are short; the heads of a row tile follow each other, so that neighbours share
+// keys in L2.  (More requests than threads, each with a long prompt: in their
+// own order.)  `scratch`: 12 bytes a thread.
+__device__ bool find_unit(const CachedParams& p, Unit& u, uint8_t* scratch) {
+  long long* units = reinterpret_cast<long long*>(scratch);
+  int* keys = reinterpret_cast<int*>(units + kThreads);
   __shared__ long long where[2];
   const int each = (p.batch + kThreads - 1) / kThreads;
-  const int first = static_cast<int>(threadIdx.x) * each;
-  long long sum = 0;
-  for (int r = first; r < min(first + each, p.batch); ++r) sum += units_of(p, request_at(p, r));
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long in = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long a = __shfl_up_sync(~0u, in, d);
-    if (lane >= d) in += a;
+  const int me = static_cast<int>(threadIdx.x);
+  const int first = me * each, last = min(first + each, p.batch);
+  long long mine = 0;
+  int kv = 0;
+  for (int r = first; r < last; ++r) {
+    const Request rq = request_at(p, r);
+    mine += units_of(p, rq);
+    kv = rq.kv;
   }
-  if (lane == 31) warp_sum[warp] = in;
+  units[me] = mine;
+  keys[me] = kv;
+  if (me == 0) where[0] = -1;
   __syncthreads();
-  long long before = 0, total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
-  }
-  const long long mine = before + in - sum;  // units in front of this thread's requests
-  const long long at = total - 1 - static_cast<long long>(blockIdx.x);
-  if (at < 0) return false;
-  if (at >= mine && at < mine + sum) {
-    long long b = mine;
-    int r = first;
-    for (;; ++r) {
-      const long long n = units_of(p, request_at(p, r));
-      if (at < b + n || r + 1 >= min(first + each, p.batch)) break;
-      b += n;
+  const long long at = blockIdx.x;
+  if (mine > 0) {
+    long long before = 0;
+    const int threads = min(kThreads, p.batch);
+    for (int i = 0; i < threads; ++i) {
+      const bool earlier = each == 1 ? keys[i] > kv || (keys[i] == kv && i < me) : i < me;
+      if (earlier) before += units[i];
     }
-    where[0] = r;
-    where[1] = at - b;
+    if (at >= before && at < before + mine) {
+      int r = first;
+      for (; r + 1 < last; ++r) {
+        const long long n = units_of(p, request_at(p, r));
+        if (at < before + n) break;
+        before += n;
+      }
+      where[0] = r;
+      where[1] = units_of(p, request_at(p, r)) - 1 - (at - before);
+    }
   }
   __syncthreads();
+  if (where[0] < 0) return false;
   u.request = static_cast<int>(where[0]);
   u.rq = request_at(p, u.request);
   const int in_request = static_cast<int>(where[1]);
@@ -646,7 +651,7 @@ tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
   uint8_t* sgen = smem_raw + (sbase - raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Unit u;
-  if (!find_unit(p, u)) return;
+  if (!find_unit(p, u, sgen)) return;
 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + T::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + T::kOffMisc + 4);
