@@ -13,7 +13,11 @@
 //     256 rows.  (Codes read by that warpgroup itself into registers: 1295 us
 //     where this form takes @@ on 3 chunks of 2048 tokens, 32 heads of 128.)
 //   * one thread issues tcgen05.mma: S = Q K^T and O += P V, sums in tensor
-//     memory, P read from there too (it overwrites S);
+//     memory, P read from there too.  At D = 128 its 512 columns hold S and O of
+//     both tiles and P overwrites S.  At D = 64 P has columns of its own, a
+//     tile's next S is computed during its softmax step, and each tile has a
+//     thread of its own, since one thread would hold one tile's S back until it
+//     has P of the other (@@D64@@);
 //   * a warpgroup per tile runs the online softmax, a thread a row, and moves O
 //     to a new maximum only when that grew by more than 2^8.
 //
@@ -40,8 +44,7 @@ constexpr int kBM = 128;                 // rows of a tile
 constexpr int kBN = 128;                 // keys of a step
 constexpr int kUnit = 2 * kBM;           // rows of a CTA
 constexpr int kThreads = 512;            // 2 softmax warpgroups, 1 converting, 1 with the issuer
-constexpr int kScaleRing = 8;            // steps whose K scales are kept: the fetching warp is at
-                                         // most 6 steps in front of the softmax
+constexpr int kScaleRing = 8;            // steps whose K scales are kept (see fetch_role)
 constexpr float kMove = 8.f;             // growth of the maximum (log2) that moves O
 constexpr float kLift = 7.f;             // P is held as 2^kLift p
 
@@ -53,12 +56,18 @@ struct Tile {
   static constexpr int kCodes = kBN * D;            // one tile in 8 bits
   static constexpr int kGroup = 16 * D;             // 16 keys of it
   static constexpr int kStages = D == 128 ? 2 : 4;  // of the ring of tiles in 8 bits
+  // Tensor memory columns.
+  static constexpr bool kOwnP = D == 64;            // P beside S, not over it
+  static constexpr int kTile = kOwnP ? kBN + kBN / 2 : kBN;  // S (and P) of a tile
+  static constexpr int kPCol = kOwnP ? kBN : 0;     // P from S
+  static constexpr int kOCol = 2 * kTile;           // then O of both tiles
+  static_assert(kOCol + 2 * D <= 512, "tensor memory");
   static constexpr int kOffKv = 2 * kBytes;
   static constexpr int kOffCodes = kOffKv + kSlots * kBytes;
   static constexpr int kOffScale = kOffCodes + kStages * kCodes;    // [kScaleRing][12] of K
   static constexpr int kOffVScale = kOffScale + kScaleRing * 12 * 4;  // [kStages][8]
   static constexpr int kOffBar = kOffVScale + kStages * 8 * 4;
-  static constexpr int kBars = 2 * kSlots + 2 * kStages + 2 + 2 + 4 + 2 + 1;
+  static constexpr int kBars = 2 * kSlots + 2 * kStages + 2 + 2 + 2 + 4 + 2 + 2 + 2;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;
   static constexpr int kSmem = kOffMisc + 32 + 1024;                // + alignment
   static_assert(kSmem <= 232448, "shared memory");
@@ -73,9 +82,11 @@ struct Bar {
   static constexpr int kCodesEmpty = kCodesFull + Tile<D>::kStages;
   static constexpr int kQ = kCodesEmpty + Tile<D>::kStages;
   static constexpr int kS = kQ + 2;
-  static constexpr int kP = kS + 2;       // [tile][part]
-  static constexpr int kO = kP + 4;
-  static constexpr int kDrain = kO + 2;
+  static constexpr int kSRead = kS + 2;   // S is in registers (kOwnP)
+  static constexpr int kP = kSRead + 2;   // [tile][part]
+  static constexpr int kPV = kP + 4;      // a step's P V has ended (kOwnP)
+  static constexpr int kO = kPV + 2;
+  static constexpr int kDrain = kO + 2;   // [issuer]
 };
 
 struct Unit {
@@ -172,7 +183,10 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) {
 
 // ---------------------------------------------------------------------------
 // Fetching warp: items K_0, V_0, K_1, V_1, ... in 8 bits.  Lane g < 8 fetches
-// keys 16 g .. 16 g + 15 of each.
+// keys 16 g .. 16 g + 15 of each.  Its K scales go straight to the softmax: the
+// place of step j is written again for step j + 8, which waits (through both
+// rings, 10 items at most) until S of step j + 3 has ended, and that was issued
+// after the softmax had read S, and then the scales, of step j + 1 at least.
 // ---------------------------------------------------------------------------
 template <int D>
 __device__ void fetch_role(const CUtensorMap* map_k, const CUtensorMap* map_v,
@@ -365,25 +379,25 @@ __device__ __forceinline__ uint64_t descriptor(uint32_t lo) {
 }
 
 // ---------------------------------------------------------------------------
-// The issuer: one thread, both tiles' MMAs in turn.
+// Issuers.  kOwnP: one thread a tile (`me` = 0, 1), else one for both.
 // ---------------------------------------------------------------------------
 template <int D>
-__device__ void mma_role(const Unit& u, uint32_t tmem, uint32_t sbase, const WaitCtx& w) {
+__device__ void mma_role(const Unit& u, int me, uint32_t tmem, uint32_t sbase, const WaitCtx& w) {
   using T = Tile<D>;
   auto bar = [&](int i) { return sbase + T::kOffBar + 8u * i; };
   constexpr uint32_t kIdescS = ptx::idesc_f16(kBM, kBN, false, false);
   constexpr uint32_t kIdescPV = ptx::idesc_f16(kBM, D, false, true);
   const int tiles = u.rows_in - u.row0 > kBM ? 2 : 1;
   const int n = u.steps;
-  // Shared memory descriptors: their upper word is the same for all operands
-  // (SBO 1024, version 1, 128-byte swizzle), the lower one has the address >> 4
-  // and, from bit 16, LBO >> 4 (64-column blocks of V).  Only lower words are
-  // kept: with 64-bit ones this thread's registers overflowed into local memory.
   auto ring_wait = [&](int t) {
     const bool ok = wait_bar(bar(Bar<D>::kFull + t % T::kSlots), (t / T::kSlots) & 1, w, kSiteKvFull);
     if (ok) ptx::tc_fence_after();
     return ok;
   };
+  // Shared memory descriptors: their upper word is the same for all operands
+  // (SBO 1024, version 1, 128-byte swizzle), the lower one has the address >> 4
+  // and, from bit 16, LBO >> 4 (64-column blocks of V).  Only lower words are
+  // kept: with 64-bit ones this thread's registers overflowed into local memory.
   const uint32_t q_lo = (sbase >> 4) | (1u << 16);
   const uint32_t kv_lo = (sbase + T::kOffKv) >> 4;
   auto issue_s = [&](int i, int t) {
@@ -392,54 +406,74 @@ __device__ void mma_role(const Unit& u, uint32_t tmem, uint32_t sbase, const Wai
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       const uint32_t off = static_cast<uint32_t>((kk >> 2) * T::kBlock + (kk & 3) * 32) >> 4;
-      ptx::mma_ss(tmem + i * kBN, descriptor(q + off), descriptor(k + off), kIdescS,
+      ptx::mma_ss(tmem + i * T::kTile, descriptor(q + off), descriptor(k + off), kIdescS,
                   kk > 0 ? 1u : 0u);
     }
+    ptx::mma_commit(bar(Bar<D>::kS + i));
   };
   auto issue_pv = [&](int i, int j, int t, int k0, int k1) {
     const uint32_t v =
         kv_lo + (t % T::kSlots) * (T::kBytes >> 4) + (static_cast<uint32_t>(T::kBlock >> 4) << 16);
 #pragma unroll
     for (int kk = k0; kk < k1; ++kk)
-      ptx::mma_ts(tmem + 2 * kBN + i * D, tmem + i * kBN + kk * 8,
+      ptx::mma_ts(tmem + T::kOCol + i * D, tmem + i * T::kTile + T::kPCol + kk * 8,
                   descriptor(v + (static_cast<uint32_t>(kk * 2048) >> 4)), kIdescPV,
                   (j > 0 || kk > 0) ? 1u : 0u);
   };
+  auto p_wait = [&](int i, int part, int j) {
+    const bool ok = wait_bar(bar(Bar<D>::kP + 2 * i + part), j & 1, w, kSitePReady);
+    if (ok) ptx::tc_fence_after();
+    return ok;
+  };
 
-  bool ok = n > 0 && ring_wait(0);
-  for (int i = 0; i < tiles && ok; ++i) {
+  const int i0 = T::kOwnP ? me : 0, i1 = T::kOwnP ? min(me + 1, tiles) : tiles;
+  bool ok = n > 0 && i0 < i1 && ring_wait(0);
+  for (int i = i0; i < i1 && ok; ++i) {
     if (!(ok = wait_bar(bar(Bar<D>::kQ + i), 0, w, kSiteQ))) break;
     ptx::tc_fence_after();
     issue_s(i, 0);
-    ptx::mma_commit(bar(Bar<D>::kS + i));
   }
   if (ok) ptx::mma_commit(bar(Bar<D>::kEmpty));
   for (int j = 0; j < n && ok; ++j) {
     const int tv = 2 * j + 1, tk = 2 * j + 2;
-    if (!(ok = ring_wait(tv))) break;
-    for (int i = 0; i < tiles && ok; ++i) {
-      if (!(ok = wait_bar(bar(Bar<D>::kP + 2 * i), j & 1, w, kSitePReady))) break;
-      ptx::tc_fence_after();
-      issue_pv(i, j, tv, 0, 6);
-      if (i == 0 && j + 1 < n && !(ok = ring_wait(tk))) break;
-      if (!(ok = wait_bar(bar(Bar<D>::kP + 2 * i + 1), j & 1, w, kSitePReady))) break;
-      ptx::tc_fence_after();
-      issue_pv(i, j, tv, 6, 8);
+    if constexpr (T::kOwnP) {
+      const int i = i0;
       if (j + 1 < n) {
+        if (!(ok = wait_bar(bar(Bar<D>::kSRead + i), j & 1, w, kSiteSFull))) break;
+        if (!(ok = ring_wait(tk))) break;
+        ptx::tc_fence_after();
         issue_s(i, tk);
-        ptx::mma_commit(bar(Bar<D>::kS + i));  // covers this step's P V too
-      } else {
-        ptx::mma_commit(bar(Bar<D>::kO + i));
+        ptx::mma_commit(bar(Bar<D>::kEmpty + tk % T::kSlots));
       }
+      if (!(ok = ring_wait(tv))) break;
+      if (!(ok = p_wait(i, 0, j))) break;
+      issue_pv(i, j, tv, 0, 6);
+      if (!(ok = p_wait(i, 1, j))) break;
+      issue_pv(i, j, tv, 6, 8);
+      ptx::mma_commit(bar(Bar<D>::kPV + i));
+      ptx::mma_commit(bar(Bar<D>::kEmpty + tv % T::kSlots));
+    } else {
+      if (!(ok = ring_wait(tv))) break;
+      for (int i = 0; i < tiles && ok; ++i) {
+        if (!(ok = p_wait(i, 0, j))) break;
+        issue_pv(i, j, tv, 0, 6);
+        if (i == 0 && j + 1 < n && !(ok = ring_wait(tk))) break;
+        if (!(ok = p_wait(i, 1, j))) break;
+        issue_pv(i, j, tv, 6, 8);
+        if (j + 1 < n)
+          issue_s(i, tk);  // its commit covers this step's P V too
+        else
+          ptx::mma_commit(bar(Bar<D>::kO + i));
+      }
+      if (!ok) break;
+      ptx::mma_commit(bar(Bar<D>::kEmpty + tv % T::kSlots));
+      if (j + 1 < n) ptx::mma_commit(bar(Bar<D>::kEmpty + tk % T::kSlots));
     }
-    if (!ok) break;
-    ptx::mma_commit(bar(Bar<D>::kEmpty + tv % T::kSlots));
-    if (j + 1 < n) ptx::mma_commit(bar(Bar<D>::kEmpty + tk % T::kSlots));
   }
   // Every MMA issued here has ended before tensor memory is freed.
-  ptx::mma_commit(bar(Bar<D>::kDrain));
+  ptx::mma_commit(bar(Bar<D>::kDrain + me));
   const unsigned long long t0 = ptx::globaltimer_ns();
-  while (!ptx::mbar_try_wait(bar(Bar<D>::kDrain), 0)) {
+  while (!ptx::mbar_try_wait(bar(Bar<D>::kDrain + me), 0)) {
     if (ptx::globaltimer_ns() - t0 > w.timeout_ns) {
       if (w.status) atomicCAS(w.status, 0, kDeviceTimeoutBase + kSiteDrain);
       break;
@@ -501,7 +535,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
   }
 
   const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * wi) << 16);
-  const uint32_t s_col = i * kBN, o_col = 2 * kBN + i * D;
+  const uint32_t s_col = i * T::kTile, p_col = s_col + T::kPCol, o_col = T::kOCol + i * D;
   const float to_log2 = row_f * p.scale_log2;
   float m = -INFINITY, l = 0.f;  // maximum in log2 units, sum of 2^kLift p
   bool ok = true;
@@ -518,6 +552,11 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     const int lim = limit - j * kBN;  // columns below it are seen
     ptx::tmem_wait_ld();
     ptx::reg_fence(s);
+    if constexpr (T::kOwnP) {  // the next S may come
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(bar(Bar<D>::kSRead + i));
+    }
     if (__any_sync(~0u, lim < kBN) || holes != 0) {
 #pragma unroll
       for (int c = 0; c < kBN; ++c)
@@ -555,8 +594,13 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
       m = top;
       move = true;
     }
+    if (T::kOwnP && j > 0) {  // P's columns are free, O has the sum so far
+      ok = __all_sync(~0u, wait_bar(bar(Bar<D>::kPV + i), (j - 1) & 1, w, kSiteODone));
+      if (!ok) break;
+      ptx::tc_fence_after();
+    }
     if (__any_sync(~0u, move)) {
-      // O holds the sum through the step before (S was issued behind its P V).
+      // (P over S: S was issued behind the last step's P V, so that has ended.)
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -587,7 +631,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
         part[e & 1] = ptx::f2_add(part[e & 1], ptx::f2_pack(p0, p1));
         pk[e] = half2_of(p0, p1);
       }
-      ptx::tmem_st16(lane_base + s_col + 16 * c, pk);
+      ptx::tmem_st16(lane_base + p_col + 16 * c, pk);
       if (c == 2) {  // P V of 96 keys may begin
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
@@ -608,7 +652,10 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
   if (!tile_there || !ok) return;
   float f = 0.f;
   if (u.steps > 0) {
-    if (!__all_sync(~0u, wait_bar(bar(Bar<D>::kO + i), 0, w, kSiteODone))) return;
+    const bool done = T::kOwnP
+                          ? wait_bar(bar(Bar<D>::kPV + i), (u.steps - 1) & 1, w, kSiteODone)
+                          : wait_bar(bar(Bar<D>::kO + i), 0, w, kSiteODone);
+    if (!__all_sync(~0u, done)) return;
     ptx::tc_fence_after();
     if (m != -INFINITY || l != l)
       f = reinterpret_cast<const float*>(sgen + T::kOffMisc)[2] / l;
@@ -659,7 +706,8 @@ tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     auto bar = [&](int i) { return sbase + T::kOffBar + 8u * i; };
     for (int s = 0; s < T::kSlots; ++s) {
       ptx::mbar_init(bar(Bar<D>::kFull + s), 4);
-      ptx::mbar_init(bar(Bar<D>::kEmpty + s), 1);
+      ptx::mbar_init(bar(Bar<D>::kEmpty + s),
+                     T::kOwnP && u.rows_in - u.row0 > kBM ? 2 : 1);  // issuers
     }
     for (int s = 0; s < T::kStages; ++s) {
       ptx::mbar_init(bar(Bar<D>::kCodesFull + s), 8 + 1);
@@ -671,8 +719,10 @@ tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
       ptx::mbar_init(bar(Bar<D>::kP + 2 * i), 4);
       ptx::mbar_init(bar(Bar<D>::kP + 2 * i + 1), 4);
       ptx::mbar_init(bar(Bar<D>::kO + i), 1);
+      ptx::mbar_init(bar(Bar<D>::kSRead + i), 4);
+      ptx::mbar_init(bar(Bar<D>::kPV + i), 1);
+      ptx::mbar_init(bar(Bar<D>::kDrain + i), 1);
     }
-    ptx::mbar_init(bar(Bar<D>::kDrain), 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
@@ -686,16 +736,17 @@ tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
   const uint32_t tmem = *tmem_slot;
   const WaitCtx w{abort_flag, p.status, p.timeout_ns};
 
-  // Registers of the four warpgroups: 128 x (2 * 176 + 88 + 72) = 512 * 128.
+  // Registers of the four warpgroups: 128 x (2 * 184 + 80 + 64) = 512 * 128.
   if (warp < 8) {
-    ptx::setmaxnreg_inc<176>();
+    ptx::setmaxnreg_inc<184>();
     softmax_role<TQ, D>(p, u, warp >> 2, tmem, sbase, sgen, w);
   } else if (warp < 12) {
-    ptx::setmaxnreg_dec<88>();
+    ptx::setmaxnreg_dec<80>();
     convert_role<CODE, D>(p, u, sbase, sgen, w);
   } else {
-    ptx::setmaxnreg_dec<72>();
-    if (warp == 12 && lane == 0) mma_role<D>(u, tmem, sbase, w);
+    ptx::setmaxnreg_dec<64>();
+    if ((warp == 12 || (T::kOwnP && warp == 14)) && lane == 0)
+      mma_role<D>(u, warp == 12 ? 0 : 1, tmem, sbase, w);
     if (warp == 13) fetch_role<D>(&map_k, &map_v, p, u, sbase, w);
     __syncwarp();
   }
