@@ -547,9 +547,24 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
 #pragma unroll
     for (int c = 0; c < kBN / 32; ++c)
       ptx::tmem_ld32(lane_base + s_col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-    const float* ks = reinterpret_cast<const float*>(sgen + T::kOffScale) + (j % kScaleRing) * 12;
-    const uint32_t holes = __float_as_uint(ks[8]);
     const int lim = limit - j * kBN;  // columns below it are seen
+    // Factors of the groups' scores, and the groups whose block is none.
+    float factor[kBN / 16];
+    uint32_t holes;
+    {
+      const uint32_t at = sbase + T::kOffScale + 48 * (j % kScaleRing);
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(factor[0]), "=f"(factor[1]), "=f"(factor[2]), "=f"(factor[3])
+                   : "r"(at)
+                   : "memory");
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(factor[4]), "=f"(factor[5]), "=f"(factor[6]), "=f"(factor[7])
+                   : "r"(at + 16)
+                   : "memory");
+      holes = __float_as_uint(ptx::ld_shared_f32(at + 32));
+    }
+#pragma unroll
+    for (int g = 0; g < kBN / 16; ++g) factor[g] *= to_log2;
     ptx::tmem_wait_ld();
     ptx::reg_fence(s);
     if constexpr (T::kOwnP) {  // the next S may come
@@ -561,17 +576,15 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
 #pragma unroll
       for (int c = 0; c < kBN; ++c)
         if (c >= lim || ((holes >> (c / 16)) & 1u)) s[c] = __float_as_uint(-INFINITY);
-    }
-    // Factors of the groups' scores.  That of a group which the row does not
-    // see may be anything (NaN): 1 keeps -inf there.  The least factor keeps
-    // -inf too, where ks * row_f may reach 0 (f16 products are below 2^32, so
-    // scores that small are 0 either way); NaN stays.
-    float factor[kBN / 16];
+      // The factor of a group which the row does not see may be anything (NaN):
+      // 1 keeps -inf there.  The least factor keeps -inf too, where the product
+      // above may reach 0 (f16 products are below 2^32, so scores that small
+      // are 0 either way); NaN stays.
 #pragma unroll
-    for (int g = 0; g < kBN / 16; ++g) {
-      float f = ks[g] * to_log2;
-      if (f < 0x1p-90f) f = 0x1p-90f;
-      factor[g] = (16 * g >= lim || ((holes >> g) & 1u)) ? 1.f : f;
+      for (int g = 0; g < kBN / 16; ++g) {
+        if (factor[g] < 0x1p-90f) factor[g] = 0x1p-90f;
+        if (16 * g >= lim || ((holes >> g) & 1u)) factor[g] = 1.f;
+      }
     }
     float top = -INFINITY;
 #pragma unroll
@@ -594,13 +607,18 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
       m = top;
       move = true;
     }
-    if (T::kOwnP && j > 0) {  // P's columns are free, O has the sum so far
-      ok = __all_sync(~0u, wait_bar(bar(Bar<D>::kPV + i), (j - 1) & 1, w, kSiteODone));
-      if (!ok) break;
-      ptx::tc_fence_after();
-    }
+    // The last step's P V has ended: O has the sum so far, P's columns are free.
+    // (P over S: S was issued behind that P V, so its commit said so.)
+    bool waited = !T::kOwnP || j == 0;
+    auto pv_wait = [&]() {
+      if (!waited) {
+        ok = __all_sync(~0u, wait_bar(bar(Bar<D>::kPV + i), (j - 1) & 1, w, kSiteODone));
+        ptx::tc_fence_after();
+        waited = true;
+      }
+    };
     if (__any_sync(~0u, move)) {
-      // (P over S: S was issued behind the last step's P V, so that has ended.)
+      pv_wait();
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -631,6 +649,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
         part[e & 1] = ptx::f2_add(part[e & 1], ptx::f2_pack(p0, p1));
         pk[e] = half2_of(p0, p1);
       }
+      if (c == 0) pv_wait();
       ptx::tmem_st16(lane_base + p_col + 16 * c, pk);
       if (c == 2) {  // P V of 96 keys may begin
         ptx::tmem_wait_st();
