@@ -67,11 +67,13 @@ struct Code<ATTN_CODE_E4M3> {
         : "r"(w));
     return r;
   }
-  // Two numbers rounded to the nearest code (ties to even), a in the low byte.
-  static __device__ __forceinline__ uint32_t encode2(float a, float b) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
-    return r;
+  // Four numbers in the codes' range, times f, rounded to the nearest code
+  // (ties to even), x in the lowest byte.
+  static __device__ __forceinline__ uint32_t encode4(float x, float y, float z, float w, float f) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y * f), "f"(x * f));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(w * f), "f"(z * f));
+    return lo | (static_cast<uint32_t>(hi) << 16);
   }
 };
 
@@ -88,10 +90,19 @@ struct Code<ATTN_CODE_INT8> {
   }
   static __device__ __forceinline__ uint32_t half2_lo(uint32_t w) { return biased(w, 0x4140); }
   static __device__ __forceinline__ uint32_t half2_hi(uint32_t w) { return biased(w, 0x4342); }
-  static __device__ __forceinline__ uint32_t encode2(float a, float b) {
-    const int i = max(-127, min(127, __float2int_rn(a)));
-    const int j = max(-127, min(127, __float2int_rn(b)));
-    return (static_cast<uint32_t>(i) & 0xffu) | ((static_cast<uint32_t>(j) & 0xffu) << 8);
+  // Added to 1.5 * 2^23 a number is rounded to a whole one (ties to even), whose
+  // low 8 bits are the sum's: one FMA a number, and no conversion.
+  static __device__ __forceinline__ uint32_t encode4(float x, float y, float z, float w, float f) {
+    constexpr float kWhole = 12582912.f;
+    uint32_t lo, hi, r;
+    asm("prmt.b32 %0, %1, %2, 0x0040;"
+        : "=r"(lo)
+        : "r"(__float_as_uint(fmaf(x, f, kWhole))), "r"(__float_as_uint(fmaf(y, f, kWhole))));
+    asm("prmt.b32 %0, %1, %2, 0x0040;"
+        : "=r"(hi)
+        : "r"(__float_as_uint(fmaf(z, f, kWhole))), "r"(__float_as_uint(fmaf(w, f, kWhole))));
+    asm("prmt.b32 %0, %1, %2, 0x5410;" : "=r"(r) : "r"(lo), "r"(hi));
+    return r;
   }
 };
 

@@ -65,13 +65,10 @@ struct Bits<__nv_bfloat16> {
   static __device__ __forceinline__ float to_float(uint32_t b) { return __uint_as_float(b << 16); }
 };
 
-// Both halves of each word: those that are not finite become 0; `bad` gathers
-// whether there were any.
+// Both halves of a word: those that are not finite become 0.
 template <typename T>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w, uint32_t& bad) {
-  const uint32_t m = __vcmpgeu2(w & 0x7fff7fffu, Bits<T>::kInf * 0x10001u);
-  bad |= m;
-  return w & ~m;
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  return w & ~__vcmpgeu2(w & 0x7fff7fffu, Bits<T>::kInf * 0x10001u);
 }
 
 // The least e >= kLeastExponent with a <= C * 2^e (a >= 0, finite).
@@ -128,21 +125,31 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams 
         w[i] = __ldcs(reinterpret_cast<const uint4*>(x + (t0 + row + i * kStep) * x_token));
     }
     const float old = off > 0 ? *scale_at : 0.f;
-    // Largest |x| of the run, as bits: for finite numbers these order alike.
-    uint32_t top = 0, bad = 0;
+    // Largest |x| of the run, as bits: for finite numbers these order alike,
+    // and the others are above them.
+    auto largest = [&]() {
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < kIters; ++i) {
-      w[i].x = finite_only<T>(w[i].x, bad);
-      w[i].y = finite_only<T>(w[i].y, bad);
-      w[i].z = finite_only<T>(w[i].z, bad);
-      w[i].w = finite_only<T>(w[i].w, bad);
-      top = __vmaxu2(top, __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu),
-                                   __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu)));
+      for (int i = 0; i < kIters; ++i)
+        top = __vmaxu2(top, __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu),
+                                     __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu)));
+      top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
+      return top;
+    };
+    uint32_t top = largest();
+    bool any_bad = __any_sync(~0u, top >= Bits<T>::kInf);
+    if (any_bad) {
+#pragma unroll
+      for (int i = 0; i < kIters; ++i) {
+        w[i].x = finite_only<T>(w[i].x);
+        w[i].y = finite_only<T>(w[i].y);
+        w[i].z = finite_only<T>(w[i].z);
+        w[i].w = finite_only<T>(w[i].w);
+      }
+      top = largest();
     }
-    top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-    for (int d = 8; d > 0; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
-    bool any_bad = __any_sync(~0u, bad != 0);
     if constexpr (WHOLE) {
       if ((lane & 15) == 0) tops[is_v][warp] = top;
       if (lane == 0) bads[warp] = any_bad;
@@ -163,11 +170,6 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams 
     if ((lane & 15) == 0 && (!WHOLE || warp == 0))
       *scale_at = ((any_bad && !is_v) || dead) ? __int_as_float(0x7fffffff) : now;
 
-    // Dividing by `now`: by its reciprocal where that is exact.
-    const bool pow2 = (__float_as_int(now) & 0x7fffff) == 0;
-    const float inv = pow2 ? 1.f / now : 0.f;
-    auto scaled = [&](float f) { return pow2 ? f * inv : f / now; };
-
     if (grew) {  // codes in front of the run, to the new scale
       const float r = old / now;
       for (int i = row; i < off; i += kStep) {
@@ -178,23 +180,38 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams 
         for (int j = 0; j < 2; ++j) {
           const float2 a = half2_to_float2(Code<CODE>::half2_lo(u[j]));
           const float2 b = half2_to_float2(Code<CODE>::half2_hi(u[j]));
-          u[j] = Code<CODE>::encode2(a.x * r, a.y * r) | (Code<CODE>::encode2(b.x * r, b.y * r) << 16);
+          u[j] = Code<CODE>::encode4(a.x, a.y, b.x, b.y, r);
         }
         *at = c;
       }
     }
+    if ((__float_as_int(now) & 0x7fffff) == 0) {  // a power of two: its reciprocal is exact
+      const float inv = 1.f / now;
 #pragma unroll
-    for (int i = 0; i < kIters; ++i) {
-      if (row + i * kStep < n) {
-        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-        uint32_t e[4];
+      for (int i = 0; i < kIters; ++i) {
+        if (row + i * kStep < n) {
+          const float2 a = Bits<T>::to_float2(w[i].x), b = Bits<T>::to_float2(w[i].y);
+          const float2 c = Bits<T>::to_float2(w[i].z), d = Bits<T>::to_float2(w[i].w);
+          *reinterpret_cast<uint2*>(rows + static_cast<long long>(off + row + i * kStep) * D) =
+              make_uint2(Code<CODE>::encode4(a.x, a.y, b.x, b.y, inv),
+                         Code<CODE>::encode4(c.x, c.y, d.x, d.y, inv));
+        }
+      }
+    } else {  // a scale that the caller brought
+#pragma unroll 1
+      for (int i = row; i < n; i += kStep) {
+        uint4 v = *reinterpret_cast<const uint4*>(x + (t0 + i) * x_token);
+        uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+        float f[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 f = Bits<T>::to_float2(u[j]);
-          e[j] = Code<CODE>::encode2(scaled(f.x), scaled(f.y));
+          const float2 a = Bits<T>::to_float2(finite_only<T>(u[j]));
+          f[2 * j] = a.x / now;
+          f[2 * j + 1] = a.y / now;
         }
-        *reinterpret_cast<uint2*>(rows + static_cast<long long>(off + row + i * kStep) * D) =
-            make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+        *reinterpret_cast<uint2*>(rows + static_cast<long long>(off + i) * D) =
+            make_uint2(Code<CODE>::encode4(f[0], f[1], f[2], f[3], 1.f),
+                       Code<CODE>::encode4(f[4], f[5], f[6], f[7], 1.f));
       }
     }
     if constexpr (WHOLE) __syncthreads();  // tops and bads may be written again
