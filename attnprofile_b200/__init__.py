@@ -27,6 +27,7 @@ __all__ = [
 ERR = {
     "OK": 0, "INVALID_ARG": -1, "UNSUPPORTED": -2, "MISALIGNED": -3, "CUDA": -4,
     "TENSOR_MAP": -5, "DEVICE_TIMEOUT": -6, "RESOURCE": -7, "SHARD": -8, "SCRATCH_LIMIT": -9,
+    "WORKSPACE": -10,
 }
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
@@ -84,15 +85,10 @@ def lib() -> ctypes.CDLL:
                                          ctypes.POINTER(ctypes.c_double)]
         L.attn_plan_split.argtypes = [ll, i, ll, i, ctypes.POINTER(i), llp, llp]
         L.attn_query_split.argtypes = [i, i, i, i, i, i, i, ctypes.POINTER(i), llp, llp, u64p]
-        f, ull = ctypes.c_float, ctypes.c_ulonglong
-        L.attn_block_tables.argtypes = [vp, vp, i, vp, i, ll, vp, vp, i, i, vp, vp, vp, i, vp, vp,
-                                        vp]
-        L.attn_block_trim.argtypes = [vp, vp, i, vp, i, ll, vp, vp, i, i, vp, vp, vp, vp]
-        L.attn_cache_append.argtypes = [vp, ll, ll, vp, ll, ll, vp, i, i, i, i, vp, vp, vp, vp, i,
-                                        i, i, vp]
-        L.attn_cached.argtypes = [vp, ll, ll, vp, ll, ll, i, i, i, i, i, vp, vp, vp, vp, i, i, i,
-                                  vp, i, ll, vp, vp, i, i, i, f, vp, ull, vp]
-        L.attn_cached_workspace.argtypes = [i, i, i, i, ctypes.POINTER(ull)]
+        # Arguments of the cache's entry points: one packed struct each.
+        for name in ("attn_block_tables", "attn_block_trim", "attn_cache_append", "attn_cached"):
+            getattr(L, name).argtypes = [ctypes.c_char_p, vp]
+        L.attn_cached_workspace.argtypes = [i, i, i, i, u64p]
         for name in ("attn_fwd", "attn_fwd_padded", "attn_fwd_profiled", "attn_fwd_sharded",
                      "attn_shard_range", "attn_get_status", "attn_query_config",
                      "attn_profile_layout", "attn_debug_fault", "attn_version",

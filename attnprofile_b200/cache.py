@@ -14,6 +14,7 @@ device), never synchronises, and can be captured into a CUDA graph.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -47,6 +48,13 @@ def _stream(device, stream) -> int:
     if stream.device != device:
         raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
     return stream.cuda_stream
+
+
+# The argument structs of include/attnprof.h, field by field in their order.
+_TABLES = struct.Struct("@10Qq5i").pack
+_TRIM = struct.Struct("@8Qq4i").pack
+_APPEND = struct.Struct("@7Q4q7i").pack
+_CACHED = struct.Struct("@11Q5q12if").pack
 
 
 def _call(name, device, *args):
@@ -201,14 +209,14 @@ def block_tables(pool: BlockPool, lens, new_lens, tables, tokens: int, *, plan=N
     if free_left is None:
         free_left = pool.free_count
     t, width, stride = _table(tables, device, batch)
-    _call("attn_block_tables", device, _ints("lens", lens, device, batch),
-          _ints("new_lens", new_lens, device, batch), batch, t, width, stride,
-          pool.free.data_ptr(), pool.free_count.data_ptr(), pool.num_blocks, pool.block_size,
-          _ints("plan.kv_lens", plan.kv_lens, device, batch),
-          _ints("plan.starts", plan.starts, device, batch + 1),
-          _ints("plan.slots", plan.slots, device, tokens), tokens,
-          _ints("free_left", free_left, device, 1), _ints("plan.status", plan.status, device, 1),
-          s)
+    _call("attn_block_tables", device, _TABLES(
+        _ints("lens", lens, device, batch), _ints("new_lens", new_lens, device, batch), t,
+        pool.free.data_ptr(), pool.free_count.data_ptr(),
+        _ints("plan.kv_lens", plan.kv_lens, device, batch),
+        _ints("plan.starts", plan.starts, device, batch + 1),
+        _ints("plan.slots", plan.slots, device, tokens), _ints("free_left", free_left, device, 1),
+        _ints("plan.status", plan.status, device, 1), stride, batch, width, pool.num_blocks,
+        pool.block_size, tokens), s)
     return plan
 
 
@@ -227,11 +235,12 @@ def block_trim(pool: BlockPool, lens, keep, tables, *, lens_left=None, free_left
     if status is None:
         status = _empty(1, torch.int32, device, stream)
     t, width, stride = _table(tables, device, batch)
-    _call("attn_block_trim", device, _ints("lens", lens, device, batch),
-          _ints("keep", keep, device, batch), batch, t, width, stride, pool.free.data_ptr(),
-          pool.free_count.data_ptr(), pool.num_blocks, pool.block_size,
-          _ints("lens_left", lens_left, device, batch), _ints("free_left", free_left, device, 1),
-          _ints("status", status, device, 1), s)
+    _call("attn_block_trim", device, _TRIM(
+        _ints("lens", lens, device, batch), _ints("keep", keep, device, batch), t,
+        pool.free.data_ptr(), pool.free_count.data_ptr(),
+        _ints("lens_left", lens_left, device, batch), _ints("free_left", free_left, device, 1),
+        _ints("status", status, device, 1), stride, batch, width, pool.num_blocks,
+        pool.block_size), s)
     return status
 
 
@@ -268,9 +277,10 @@ def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
     if v_kind != kind or v_shape != shape:
         raise ValueError("k and v must share one shape and dtype")
     tokens = shape[0]
-    _call("attn_cache_append", device, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token,
-          v_head, _ints("slots", slots, device, tokens), tokens, heads, dim, kind, *cache.ptrs,
-          cache.code, cache.num_blocks, cache.block_size, _stream(device, stream))
+    _call("attn_cache_append", device, _APPEND(
+        k.data_ptr(), v.data_ptr(), _ints("slots", slots, device, tokens), *cache.ptrs, k_token,
+        k_head, v_token, v_head, tokens, heads, dim, kind, cache.code, cache.num_blocks,
+        cache.block_size), _stream(device, stream))
 
 
 def _workspace(device, heads, kv_heads, dim, max_new) -> int:
@@ -329,10 +339,11 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
         if workspace.device != device:
             raise ValueError(f"workspace must be on {device}")
         need = workspace.numel()
-    _call("attn_cached", device, q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head,
-          tokens, heads, kv_heads, dim, kind, *cache.ptrs, cache.code, cache.num_blocks,
-          cache.block_size, t, width, stride, lens_ptr, starts_ptr, batch, max_new,
-          1 if causal else 0, scale, workspace.data_ptr(), need, s)
+    _call("attn_cached", device, _CACHED(
+        q.data_ptr(), out.data_ptr(), *cache.ptrs, t, lens_ptr, starts_ptr, workspace.data_ptr(),
+        need, q_token, q_head, o_token, o_head, stride, tokens, heads, kv_heads, dim, kind,
+        cache.code, cache.num_blocks, cache.block_size, width, batch, max_new,
+        1 if causal else 0, scale), s)
     return out
 
 

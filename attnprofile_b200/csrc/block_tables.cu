@@ -83,11 +83,9 @@ __device__ __forceinline__ void end_of_reading(int ctas) {
     __syncthreads();
 }
 
-struct TablesParams {
-  const int *lens, *new_lens, *free_blocks, *free_count;
-  int *tables, *kv_lens, *starts, *slots, *free_left, *status;
-  long long table_stride;
-  int batch, width, tokens, num_blocks, shift;
+struct TablesParams : attn_block_tables_args {
+  TablesParams(const attn_block_tables_args& a, int s) : attn_block_tables_args(a), shift(s) {}
+  int shift;  // of block_size
 };
 
 __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) {
@@ -201,11 +199,9 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
   }
 }
 
-struct TrimParams {
-  const int *lens, *keep, *tables, *free_count;
-  int *free_blocks, *lens_left, *free_left, *status;
-  long long table_stride;
-  int batch, width, num_blocks, shift;
+struct TrimParams : attn_block_trim_args {
+  TrimParams(const attn_block_trim_args& a, int s) : attn_block_trim_args(a), shift(s) {}
+  int shift;
 };
 
 __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
@@ -292,12 +288,6 @@ int launch_cluster(void (*kern)(P), const P& p, int ctas, size_t smem, cudaStrea
   return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
 }
 
-int shift_of(int block_size) {
-  int s = 0;
-  while ((1 << s) < block_size) ++s;
-  return s;
-}
-
 int check_batch(int batch, int width, long long table_stride, int num_blocks, int block_size) {
   if (!block_size_ok(block_size)) return ATTN_ERR_UNSUPPORTED;
   if (batch < 0 || width < 0 || table_stride < width || num_blocks <= 0)
@@ -313,36 +303,32 @@ int check_batch(int batch, int width, long long table_stride, int num_blocks, in
 
 using namespace attnprof::cache;
 
-extern "C" int attn_block_tables(const int* lens, const int* new_lens, int batch, int* tables,
-                                 int width, long long table_stride, const int* free_blocks,
-                                 const int* free_count, int num_blocks, int block_size,
-                                 int* kv_lens, int* starts, int* slots, int tokens,
-                                 int* free_left, int* status, void* stream) {
-  const int rc = check_batch(batch, width, table_stride, num_blocks, block_size);
+extern "C" int attn_block_tables(const attn_block_tables_args* args, void* stream) {
+  if (!args) return ATTN_ERR_INVALID_ARG;
+  const attn_block_tables_args& a = *args;
+  const int rc = check_batch(a.batch, a.width, a.table_stride, a.num_blocks, a.block_size);
   if (rc != ATTN_OK) return rc;
-  if (tokens < 0) return ATTN_ERR_INVALID_ARG;
-  if (!free_blocks || !free_count || !starts || !free_left || !status) return ATTN_ERR_INVALID_ARG;
-  if (batch > 0 && (!lens || !new_lens || !kv_lens)) return ATTN_ERR_INVALID_ARG;
-  if ((batch > 0 && width > 0 && !tables) || (tokens > 0 && !slots)) return ATTN_ERR_INVALID_ARG;
-  TablesParams p{lens,    new_lens, free_blocks, free_count,   tables, kv_lens, starts,     slots,
-                 free_left, status, table_stride, batch,       width,  tokens,  num_blocks, shift_of(block_size)};
-  return launch_cluster(tables_kernel, p, ctas_for(tokens), 3ull * sizeof(int) * batch,
+  if (a.tokens < 0) return ATTN_ERR_INVALID_ARG;
+  if (!a.free_blocks || !a.free_count || !a.starts || !a.free_left || !a.status)
+    return ATTN_ERR_INVALID_ARG;
+  if (a.batch > 0 && (!a.lens || !a.new_lens || !a.kv_lens)) return ATTN_ERR_INVALID_ARG;
+  if ((a.batch > 0 && a.width > 0 && !a.tables) || (a.tokens > 0 && !a.slots))
+    return ATTN_ERR_INVALID_ARG;
+  const TablesParams p{a, shift_of(a.block_size)};
+  return launch_cluster(tables_kernel, p, ctas_for(a.tokens), 3ull * sizeof(int) * a.batch,
                         static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int attn_block_trim(const int* lens, const int* keep, int batch, const int* tables,
-                               int width, long long table_stride, int* free_blocks,
-                               const int* free_count, int num_blocks, int block_size,
-                               int* lens_left, int* free_left, int* status, void* stream) {
-  const int rc = check_batch(batch, width, table_stride, num_blocks, block_size);
+extern "C" int attn_block_trim(const attn_block_trim_args* args, void* stream) {
+  if (!args) return ATTN_ERR_INVALID_ARG;
+  const attn_block_trim_args& a = *args;
+  const int rc = check_batch(a.batch, a.width, a.table_stride, a.num_blocks, a.block_size);
   if (rc != ATTN_OK) return rc;
-  if (!free_blocks || !free_count || !free_left || !status) return ATTN_ERR_INVALID_ARG;
-  if (batch > 0 && (!lens || !keep || !lens_left)) return ATTN_ERR_INVALID_ARG;
-  if (batch > 0 && width > 0 && !tables) return ATTN_ERR_INVALID_ARG;
-  TrimParams p{lens,      keep,   tables,       free_count, free_blocks, lens_left,
-               free_left, status, table_stride, batch,      width,       num_blocks,
-               shift_of(block_size)};
-  const long long most = static_cast<long long>(batch) * width;
-  return launch_cluster(trim_kernel, p, ctas_for(most < num_blocks ? most : num_blocks),
-                        2ull * sizeof(int) * batch, static_cast<cudaStream_t>(stream));
+  if (!a.free_blocks || !a.free_count || !a.free_left || !a.status) return ATTN_ERR_INVALID_ARG;
+  if (a.batch > 0 && (!a.lens || !a.keep || !a.lens_left)) return ATTN_ERR_INVALID_ARG;
+  if (a.batch > 0 && a.width > 0 && !a.tables) return ATTN_ERR_INVALID_ARG;
+  const TrimParams p{a, shift_of(a.block_size)};
+  const long long most = static_cast<long long>(a.batch) * a.width;
+  return launch_cluster(trim_kernel, p, ctas_for(most < a.num_blocks ? most : a.num_blocks),
+                        2ull * sizeof(int) * a.batch, static_cast<cudaStream_t>(stream));
 }

@@ -27,6 +27,9 @@ constexpr int kLeastExponent = -100;  // of a block's power-of-two scale
 inline bool code_ok(int code) { return code == ATTN_CODE_E4M3 || code == ATTN_CODE_INT8; }
 inline bool dtype_ok(int dtype) { return dtype == ATTN_DTYPE_F16 || dtype == ATTN_DTYPE_BF16; }
 inline bool block_size_ok(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs == 128; }
+inline int shift_of(int block_size) {
+  return block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
+}
 inline bool aligned(const void* p, unsigned n) {
   return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
 }

@@ -298,38 +298,37 @@ int launch_code(const AppendParams& p, int D, int code, cudaStream_t st) {
 
 using namespace attnprof::cache;
 
-extern "C" int attn_cache_append(const void* k, long long k_token_stride, long long k_head_stride,
-                                 const void* v, long long v_token_stride, long long v_head_stride,
-                                 const int* slots, int tokens, int kv_heads, int D, int dtype,
-                                 void* k_codes, void* v_codes, float* k_scale, float* v_scale,
-                                 int code, int num_blocks, int block_size, void* stream) {
-  const int rc = check_pool(num_blocks, kv_heads, block_size, D, code);
+extern "C" int attn_cache_append(const attn_cache_append_args* args, void* stream) {
+  if (!args) return ATTN_ERR_INVALID_ARG;
+  const attn_cache_append_args& a = *args;
+  const int rc = check_pool(a.num_blocks, a.kv_heads, a.block_size, a.D, a.code);
   if (rc != ATTN_OK) return rc;
-  if (!dtype_ok(dtype)) return ATTN_ERR_UNSUPPORTED;
-  if (tokens < 0 || kv_heads > 65535) return ATTN_ERR_INVALID_ARG;
-  if (tokens == 0) return ATTN_OK;
-  if (!k || !v || !slots || !k_codes || !v_codes || !k_scale || !v_scale)
+  if (!dtype_ok(a.dtype)) return ATTN_ERR_UNSUPPORTED;
+  if (a.tokens < 0 || a.kv_heads > 65535) return ATTN_ERR_INVALID_ARG;
+  if (a.tokens == 0) return ATTN_OK;
+  if (!a.k || !a.v || !a.slots || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale)
     return ATTN_ERR_INVALID_ARG;
-  if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_codes, 16) || !aligned(v_codes, 16) ||
-      ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7) != 0)
+  if (!aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.k_codes, 16) ||
+      !aligned(a.v_codes, 16) ||
+      ((a.k_token_stride | a.k_head_stride | a.v_token_stride | a.v_head_stride) & 7) != 0)
     return ATTN_ERR_MISALIGNED;
   AppendParams p{};
-  p.k = k;
-  p.v = v;
-  p.slots = slots;
-  p.kc = static_cast<uint8_t*>(k_codes);
-  p.vc = static_cast<uint8_t*>(v_codes);
-  p.ks = k_scale;
-  p.vs = v_scale;
-  p.k_token = k_token_stride;
-  p.k_head = k_head_stride;
-  p.v_token = v_token_stride;
-  p.v_head = v_head_stride;
-  p.tokens = tokens;
-  p.heads = kv_heads;
-  p.num_slots = num_blocks * block_size;
-  p.shift = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
+  p.k = a.k;
+  p.v = a.v;
+  p.slots = a.slots;
+  p.kc = static_cast<uint8_t*>(a.k_codes);
+  p.vc = static_cast<uint8_t*>(a.v_codes);
+  p.ks = a.k_scale;
+  p.vs = a.v_scale;
+  p.k_token = a.k_token_stride;
+  p.k_head = a.k_head_stride;
+  p.v_token = a.v_token_stride;
+  p.v_head = a.v_head_stride;
+  p.tokens = a.tokens;
+  p.heads = a.kv_heads;
+  p.num_slots = a.num_blocks * a.block_size;
+  p.shift = shift_of(a.block_size);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == ATTN_DTYPE_F16 ? launch_code<__half>(p, D, code, st)
-                                 : launch_code<__nv_bfloat16>(p, D, code, st);
+  return a.dtype == ATTN_DTYPE_F16 ? launch_code<__half>(p, a.D, a.code, st)
+                                   : launch_code<__nv_bfloat16>(p, a.D, a.code, st);
 }

@@ -16,6 +16,7 @@ struct CachedParams {
   const int *tables, *kv_lens, *starts;
   long long q_token, q_head, o_token, o_head, table_stride;
   int tokens, heads, kv_heads, group, batch, num_blocks, shift, capacity, causal;
+  int whole;  // split kernel: no unit is cut
   float scale_log2;  // score scale * log2(e)
   // Requests of more than `rows_most` query rows a kv head (tokens * group)
   // belong to the other kernel: the split one takes those up to it, the tiled

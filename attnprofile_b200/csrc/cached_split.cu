@@ -32,6 +32,7 @@
 // 2^15 p, in [0, 2^15], so that also weights down to 2^-29 of the largest keep
 // all their bits.  Maximum, sum and O are f32.  bf16 queries become f16 times a
 // power of two per row, which loses nothing above 2^-38 of the row's largest.
+#include <atomic>
 #include <climits>
 
 #include "attn_host.cuh"
@@ -47,6 +48,11 @@ constexpr int kWarps = 4;                    // that compute
 constexpr int kThreads = 256;                // two warpgroups: computing, fetching (one warp of it)
 constexpr int kChunk = 256;                  // keys
 constexpr int kOver = 1;                     // chunks that beginning a unit counts for
+// Requests of up to this many chunks are not cut: a second kernel would cost
+// more than the keys that it lets other SMs read.  (32 heads over 8, D = 128, in
+// graphs: 16 requests of 500 tokens 8.4 us whole, 12.3 cut; 64 of them 17.9 and
+// 21.3; 200 46.5 and 46.6.  Of 1000 tokens, 1 request 11.1 and 9.7, 200 74 and 65.)
+constexpr int kWholeChunks = 2;
 constexpr float kLift = 15.f;                // P is held as 2^kLift p
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -94,19 +100,19 @@ __device__ __forceinline__ void load_codes(Words<WORDS>& d, uint32_t a) {
 // The cut of all work into ranges.
 // ---------------------------------------------------------------------------
 struct Shape {
-  int units, chunks;  // of one request: its units, and the chunks of each
-  __device__ __forceinline__ int weight() const { return chunks + kOver; }
+  int units, chunks, weight;  // of one request: its units, and the chunks and weight of each
   __device__ __forceinline__ long long work() const {
-    return static_cast<long long>(units) * weight();
+    return static_cast<long long>(units) * weight;
   }
 };
 
 template <int NT>
 __device__ __forceinline__ Shape shape_of(const CachedParams& p, const Request& r) {
   const long long rows = static_cast<long long>(r.n) * p.group;
-  if (rows == 0 || rows > p.rows_most) return Shape{0, 1};
-  return Shape{p.kv_heads * static_cast<int>((rows + 8 * NT - 1) / (8 * NT)),
-               max(1, (r.kv + kChunk - 1) / kChunk)};
+  if (rows == 0 || rows > p.rows_most) return Shape{0, 1, 1};
+  const int chunks = max(1, (r.kv + kChunk - 1) / kChunk);
+  return Shape{p.kv_heads * static_cast<int>((rows + 8 * NT - 1) / (8 * NT)), chunks,
+               p.whole ? 1 : chunks + kOver};
 }
 
 struct Place {
@@ -160,6 +166,31 @@ __device__ __forceinline__ Place find_place(const CachedParams& p, const long lo
   }
 }
 
+// The same for at most 32 requests, by every warp for itself: lane r has
+// request r, the sum of all work up to and with it, and its shape.
+struct Lanes {
+  long long upto;
+  Shape sh;
+};
+template <int NT>
+__device__ __forceinline__ Lanes count_lanes(const CachedParams& p, long long* total) {
+  const int lane = threadIdx.x & 31;
+  Lanes x{0, Shape{0, 1, 1}};
+  if (lane < p.batch) x.sh = shape_of<NT>(p, request_at(p, lane));
+  x.upto = x.sh.work();
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long a = __shfl_up_sync(~0u, x.upto, d);
+    if (lane >= d) x.upto += a;
+  }
+  *total = __shfl_sync(~0u, x.upto, 31);
+  return x;
+}
+__device__ __forceinline__ Place place_in(const Lanes& x, long long at) {
+  const int r = __ffs(__ballot_sync(~0u, x.upto > at)) - 1;
+  return Place{r, __shfl_sync(~0u, x.upto - x.sh.work(), r)};
+}
+
 __device__ __forceinline__ long long work_each(long long total) {
   return (total + gridDim.x - 1) / gridDim.x;
 }
@@ -190,13 +221,13 @@ struct Cursor {
         ++pl.request;
         continue;
       }
-      const int w = sh.weight();
+      const int w = sh.weight;
       const int unit = quotient(at - pl.before, w);
       const int off = static_cast<int>(at - pl.before - static_cast<long long>(unit) * w);
       const int end = static_cast<int>(min(static_cast<long long>(w), off + (stop - at)));
       at += end - off;
-      x.c0 = max(0, off - kOver);
-      x.c1 = max(0, end - kOver);
+      x.c0 = p.whole ? 0 : max(0, off - kOver);
+      x.c1 = p.whole ? sh.chunks : max(0, end - kOver);
       if (x.c0 == x.c1) continue;
       const int tiles = sh.units / p.kv_heads;
       x.request = pl.request;
@@ -226,13 +257,6 @@ struct Parts {
 // ---------------------------------------------------------------------------
 // The kernel.
 // ---------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ float to_float(T x);
-template <>
-__device__ __forceinline__ float to_float<__half>(__half x) { return __half2float(x); }
-template <>
-__device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack_out(float a, float b);
 template <>
@@ -441,8 +465,11 @@ __device__ void compute_role(const SplitParams& p, Cursor<NT> cursor, uint32_t s
           if constexpr (std::is_same<T, __half>::value) {
             b = *reinterpret_cast<const uint2*>(qr + d);
           } else {
-            b.x = pack_half2(to_float(qr[d]) * inv, to_float(qr[d + 1]) * inv);
-            b.y = pack_half2(to_float(qr[d + 2]) * inv, to_float(qr[d + 3]) * inv);
+            const uint2 v = *reinterpret_cast<const uint2*>(qr + d);
+            b.x = pack_half2(__uint_as_float(v.x << 16) * inv,
+                             __uint_as_float(v.x & 0xffff0000u) * inv);
+            b.y = pack_half2(__uint_as_float(v.y << 16) * inv,
+                             __uint_as_float(v.y & 0xffff0000u) * inv);
           }
         }
         if constexpr (kQShared) {
@@ -747,17 +774,28 @@ split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  long long* part_sum = reinterpret_cast<long long*>(smem + S::kOffHop);
-  const long long total = count_work<NT>(p, part_sum);
-  const long long each = work_each(total);
-  Cursor<NT> cursor;
-  cursor.at = each * blockIdx.x;
-  cursor.stop = min(cursor.at + each, total);
   asm volatile("griddepcontrol.launch_dependents;");
-  if (cursor.at >= cursor.stop) return;
-  if (threadIdx.x == 0) place = find_place<NT>(p, part_sum, cursor.at);
-  __syncthreads();
-  cursor.pl = place;
+  Cursor<NT> cursor;
+  long long total;
+  if (p.batch <= 32) {
+    const Lanes lanes = count_lanes<NT>(p, &total);
+    const long long each = work_each(total);
+    cursor.at = each * blockIdx.x;
+    cursor.stop = min(cursor.at + each, total);
+    if (cursor.at >= cursor.stop) return;
+    cursor.pl = place_in(lanes, cursor.at);
+    __syncthreads();  // the barriers are there
+  } else {
+    long long* part_sum = reinterpret_cast<long long*>(smem + S::kOffHop);
+    total = count_work<NT>(p, part_sum);
+    const long long each = work_each(total);
+    cursor.at = each * blockIdx.x;
+    cursor.stop = min(cursor.at + each, total);
+    if (cursor.at >= cursor.stop) return;
+    if (threadIdx.x == 0) place = find_place<NT>(p, part_sum, cursor.at);
+    __syncthreads();
+    cursor.pl = place;
+  }
   const WaitCtx w{&abort_flag, p.status, p.timeout_ns};
   // Registers: 128 x (216 + 40) = 256 x 128.
   if (warp < kWarps) {
@@ -792,9 +830,9 @@ __global__ void __launch_bounds__(256) join_kernel(const CachedParams p) {
   const Place pl = place;
   const Request rq = request_at(p, pl.request);
   const Shape sh = shape_of<NT>(p, rq);
-  const int unit = quotient(cut - pl.before, sh.weight());
-  const long long begin = pl.before + static_cast<long long>(unit) * sh.weight();
-  const long long end = begin + sh.weight();
+  const int unit = quotient(cut - pl.before, sh.weight);
+  const long long begin = pl.before + static_cast<long long>(unit) * sh.weight;
+  const long long end = begin + sh.weight;
   // Only if chunks lie in front of this cut, and none in front of the last one.
   if (cut <= begin + kOver || cut - each > begin + kOver) return;
   const int tiles = sh.units / p.kv_heads;
@@ -846,6 +884,89 @@ __global__ void __launch_bounds__(256) join_kernel(const CachedParams p) {
   }
 }
 
+// The same where units are few (at most kFewUnits of at most 32 requests) and
+// so have many parts each: a CTA per unit and row, its warps share the parts.
+constexpr int kFewUnits = 64;
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) join_few_kernel(const CachedParams p, int ctas) {
+  __shared__ float top_of[8], sum_of[8];
+  __shared__ float x_of[8][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long total;
+  const Lanes lanes = count_lanes<NT>(p, &total);
+  const long long each = (total + ctas - 1) / ctas;
+  // The request that holds this unit.
+  int upto = lanes.sh.units;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int a = __shfl_up_sync(~0u, upto, d);
+    if (lane >= d) upto += a;
+  }
+  const int r = __ffs(__ballot_sync(~0u, upto > static_cast<int>(blockIdx.x))) - 1;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (r < 0) return;
+  const int units = __shfl_sync(~0u, lanes.sh.units, r), weight = __shfl_sync(~0u, lanes.sh.weight, r);
+  const int unit = static_cast<int>(blockIdx.x) - (__shfl_sync(~0u, upto, r) - units);
+  const long long begin = __shfl_sync(~0u, lanes.upto, r) -
+                          static_cast<long long>(units - unit) * weight;
+  const long long end = begin + weight;
+  // Ranges with chunks of the unit: the one that its first chunk lies in, to the last.
+  const int c0 = static_cast<int>((begin + kOver) / each), c1 = static_cast<int>((end - 1) / each);
+  if (c0 == c1) return;  // not cut
+  const Request rq = request_at(p, r);
+  const int tiles = units / p.kv_heads;
+  const int kvh = unit / tiles;
+  const int row_in = blockIdx.y, row = (unit - kvh * tiles) * 8 * NT + row_in;
+  if (row >= rq.n * p.group) return;
+  const long long slots = 2ll * ctas;
+  auto slot_of = [&](int c) { return 2ll * c + (c == c0 ? 1 : 0); };
+
+  constexpr int kPer = D / 32;
+  float top = -INFINITY, sum = 0.f, x[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) x[j] = 0.f;
+  for (int c = c0 + warp; c <= c1; c += 8) {
+    const float2 ml = Parts<NT, D>::ml(p.ws, slots, slot_of(c))[row_in];
+    const float* o = Parts<NT, D>::o(p.ws, slot_of(c)) + row_in * D + lane * kPer;
+    float y[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) y[j] = o[j];
+    const float now = fmaxf(top, ml.x), base = now == -INFINITY ? 0.f : now;
+    const float a = ptx::ex2_approx(top - base), b = ptx::ex2_approx(ml.x - base);
+    top = now;
+    sum = sum * a + ml.y * b;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[j] = x[j] * a + y[j] * b;
+  }
+  if (lane == 0) {
+    top_of[warp] = top;
+    sum_of[warp] = sum;
+  }
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) x_of[warp][lane * kPer + j] = x[j];
+  __syncthreads();
+  const int d = 2 * threadIdx.x;  // two head dimensions a thread
+  if (d >= D) return;
+  top = top_of[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, top_of[i]);
+  const float base = top == -INFINITY ? 0.f : top;
+  sum = 0.f;
+  float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float f = ptx::ex2_approx(top_of[i] - base);
+    sum = fmaf(sum_of[i], f, sum);
+    x0 = fmaf(x_of[i][d], f, x0);
+    x1 = fmaf(x_of[i][d + 1], f, x1);
+  }
+  const float n = top == -INFINITY && sum == sum ? 0.f : 1.f / sum;
+  const int tok = row / p.group;
+  T* dst = static_cast<T*>(p.out) + (rq.start + tok) * p.o_token +
+           (kvh * p.group + row - tok * p.group) * p.o_head + d;
+  *reinterpret_cast<uint32_t*>(dst) = pack_out<T>(x0 * n, x1 * n);
+}
+
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
@@ -861,10 +982,10 @@ constexpr int kMostCtasPerSm = 2;  // by shared memory and registers; bounds the
 
 template <typename T, int CODE, int D, int NT>
 int resident_ctas(int* ctas) {
-  static int known[64];  // per device; the same value whoever writes it
+  static std::atomic<int> known[64];  // per device, 0 until it is set up
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return ATTN_ERR_CUDA;
-  int n = dev < 64 ? *static_cast<volatile int*>(&known[dev]) : 0;
+  int n = dev < 64 ? known[dev].load(std::memory_order_acquire) : 0;
   if (n == 0) {
     constexpr int smem = Smem<D, NT>::kBytes;
     auto kern = split_kernel<T, CODE, D, NT>;
@@ -876,7 +997,7 @@ int resident_ctas(int* ctas) {
       return ATTN_ERR_CUDA;
     if (occ < 1) return ATTN_ERR_RESOURCE;
     n = sms * (occ < kMostCtasPerSm ? occ : kMostCtasPerSm);
-    if (dev < 64) *static_cast<volatile int*>(&known[dev]) = n;
+    if (dev < 64) known[dev].store(n, std::memory_order_release);
   }
   *ctas = n;
   return ATTN_OK;
@@ -898,29 +1019,34 @@ int launch(const CachedParams& cp, int max_new, void* ws, unsigned long long ws_
   int ctas = 0;
   const int rc = resident_ctas<T, CODE, D, NT>(&ctas);
   if (rc != ATTN_OK) return rc;
-  // No more ranges than there can be chunks.
   const long long rows = static_cast<long long>(p.group) * max_new;
-  const long long tiles = (rows + 8 * NT - 1) / (8 * NT);
-  const long long chunks = p.capacity <= kChunk ? 1 : (p.capacity + kChunk - 1) / kChunk;
-  const double most = static_cast<double>(p.batch) * p.kv_heads * tiles * chunks;
+  const double units = static_cast<double>(p.batch) * p.kv_heads * ((rows + 8 * NT - 1) / (8 * NT));
+  const int chunks = p.capacity <= kChunk ? 1 : (p.capacity + kChunk - 1) / kChunk;
+  p.whole = chunks <= kWholeChunks;
+  // No more ranges than there can be chunks.
+  const double most = units * (p.whole ? 1 : chunks);
   if (most < ctas) ctas = static_cast<int>(most);
-  if (ws_bytes < part_bytes(D, NT) * ctas) return ATTN_ERR_SCRATCH_LIMIT;
+  if (ws_bytes < part_bytes(D, NT) * ctas) return ATTN_ERR_WORKSPACE;
   p.ws = static_cast<float*>(ws);
   split_kernel<T, CODE, D, NT><<<ctas, kThreads, Smem<D, NT>::kBytes, st>>>(map_k, map_v, p);
   if (cudaGetLastError() != cudaSuccess) return ATTN_ERR_CUDA;
-  if (chunks == 1 || ctas == 1) return ATTN_OK;  // no unit can be cut
+  if (p.whole || ctas == 1) return ATTN_OK;
   // The joining kernel starts while the first still runs (its search of the
   // cuts overlaps) and waits for it before it reads the parts.
+  const bool few = p.batch <= 32 && units <= kFewUnits;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.gridDim = few ? dim3(static_cast<unsigned>(units), 8 * NT) : dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, static_cast<const CachedParams&>(p)) == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
+  const CachedParams& base = p;
+  const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, join_few_kernel<T, D, NT>, base, ctas)
+                            : cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, base);
+  return e == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
 }
 
 template <typename T, int CODE, int D>

@@ -31,6 +31,8 @@
 // f16 once.  P is rounded to f16 as in the split kernel, held as 2^7 p with p
 // up to 2^8 between two moves of the maximum.  bf16 queries become f16 times
 // a power of two per row.
+#include <atomic>
+
 #include "attn_kernel.cuh"
 #include "cached_attn.cuh"
 
@@ -785,9 +787,16 @@ int launch(const TiledParams& p, cudaStream_t st) {
   CUtensorMap map_k, map_v;
   if (const int e = codes_map(&map_k, p.kc, p, D)) return e;
   if (const int e = codes_map(&map_v, p.vc, p, D)) return e;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<D>::kSmem) !=
-      cudaSuccess)
-    return ATTN_ERR_RESOURCE;
+  // Once per device (setting it again does no harm).
+  static std::atomic<bool> set_up[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return ATTN_ERR_CUDA;
+  if (dev >= 64 || !set_up[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Tile<D>::kSmem) != cudaSuccess)
+      return ATTN_ERR_RESOURCE;
+    if (dev < 64) set_up[dev].store(true, std::memory_order_release);
+  }
   // Each request's rows end in at most one tile that is not full.
   const long long units =
       p.kv_heads * (static_cast<long long>(p.tokens) * p.group / kUnit + p.batch);

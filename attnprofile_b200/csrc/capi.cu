@@ -290,6 +290,7 @@ const char* attn_error_string(int code) {
     case ATTN_ERR_SCRATCH_LIMIT:
       return "problem needs more scratch than the fixed no-allocation buffer holds "
              "(ATTN_NOALLOC_SCRATCH_BYTES); use attn_fwd";
+    case ATTN_ERR_WORKSPACE: return "workspace smaller than attn_cached_workspace() says";
     default: return "unknown error";
   }
 }

@@ -40,6 +40,7 @@ extern "C" {
 #define ATTN_ERR_RESOURCE -7       /* shared memory / TMEM request over the limit   */
 #define ATTN_ERR_SHARD -8          /* multi-GPU partition error                     */
 #define ATTN_ERR_SCRATCH_LIMIT -9  /* attn_fwd_noalloc: scratch over its fixed size  */
+#define ATTN_ERR_WORKSPACE -10     /* attn_cached: workspace too small               */
 
 /*
  * attn_fwd -- one attention forward over contiguous [B, H, S, D] tensors.
@@ -290,10 +291,15 @@ int attn_fwd_noalloc(const void* Q, const void* K, const void* V, void* O, int B
  * overlap.  Asynchronous; needs no scratch, so it can be captured and replayed.
  * batch at most ATTN_BLOCKS_MAX_BATCH.
  */
-int attn_block_tables(const int* lens, const int* new_lens, int batch, int* tables, int width,
-                      long long table_stride, const int* free_blocks, const int* free_count,
-                      int num_blocks, int block_size, int* kv_lens, int* starts, int* slots,
-                      int tokens, int* free_left, int* status, void* stream);
+typedef struct {
+  const int *lens, *new_lens;
+  int* tables;
+  const int *free_blocks, *free_count;
+  int *kv_lens, *starts, *slots, *free_left, *status;
+  long long table_stride;
+  int batch, width, num_blocks, block_size, tokens;
+} attn_block_tables_args;
+int attn_block_tables(const attn_block_tables_args* args, void* stream);
 
 /*
  * attn_block_trim -- requests give blocks back: request r keeps its first
@@ -305,10 +311,15 @@ int attn_block_tables(const int* lens, const int* new_lens, int batch, int* tabl
  * entries, which mean nothing behind lens_left.  A block that several requests
  * share must be given back by one of them only.
  */
-int attn_block_trim(const int* lens, const int* keep, int batch, const int* tables, int width,
-                    long long table_stride, int* free_blocks, const int* free_count,
-                    int num_blocks, int block_size, int* lens_left, int* free_left, int* status,
-                    void* stream);
+typedef struct {
+  const int *lens, *keep, *tables;
+  int* free_blocks;
+  const int* free_count;
+  int *lens_left, *free_left, *status;
+  long long table_stride;
+  int batch, width, num_blocks, block_size;
+} attn_block_trim_args;
+int attn_block_trim(const attn_block_trim_args* args, void* stream);
 
 /*
  * attn_cache_append -- k and v of `tokens` new tokens ([tokens, kv_heads, D],
@@ -325,11 +336,15 @@ int attn_block_trim(const int* lens, const int* keep, int batch, const int* tabl
  * The tokens of one block must follow each other in the call with ascending
  * slots, as attn_block_tables gives them; a block must not appear twice.
  */
-int attn_cache_append(const void* k, long long k_token_stride, long long k_head_stride,
-                      const void* v, long long v_token_stride, long long v_head_stride,
-                      const int* slots, int tokens, int kv_heads, int D, int dtype, void* k_codes,
-                      void* v_codes, float* k_scale, float* v_scale, int code, int num_blocks,
-                      int block_size, void* stream);
+typedef struct {
+  const void *k, *v;
+  const int* slots;
+  void *k_codes, *v_codes;
+  float *k_scale, *v_scale;
+  long long k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int tokens, kv_heads, D, dtype, code, num_blocks, block_size;
+} attn_cache_append_args;
+int attn_cache_append(const attn_cache_append_args* args, void* stream);
 
 /*
  * attn_cached -- attention of each request's newest tokens over its cache.
@@ -347,13 +362,20 @@ int attn_cache_append(const void* k, long long k_token_stride, long long k_head_
  * workspace: 16-byte aligned, attn_cached_workspace(...) bytes, needs no
  * initial value; calls that may overlap need one each.  Asynchronous.
  */
-int attn_cached(const void* q, long long q_token_stride, long long q_head_stride, void* out,
-                long long out_token_stride, long long out_head_stride, int tokens, int heads,
-                int kv_heads, int D, int dtype, const void* k_codes, const void* v_codes,
-                const float* k_scale, const float* v_scale, int code, int num_blocks,
-                int block_size, const int* tables, int width, long long table_stride,
-                const int* kv_lens, const int* starts, int batch, int max_new, int causal,
-                float scale, void* workspace, unsigned long long workspace_bytes, void* stream);
+typedef struct {
+  const void* q;
+  void* out;
+  const void *k_codes, *v_codes;
+  const float *k_scale, *v_scale;
+  const int *tables, *kv_lens, *starts;
+  void* workspace;
+  unsigned long long workspace_bytes;
+  long long q_token_stride, q_head_stride, out_token_stride, out_head_stride, table_stride;
+  int tokens, heads, kv_heads, D, dtype, code, num_blocks, block_size, width, batch, max_new,
+      causal;
+  float scale;
+} attn_cached_args;
+int attn_cached(const attn_cached_args* args, void* stream);
 
 /* Workspace bytes of attn_cached on the current device, whatever the lengths. */
 int attn_cached_workspace(int heads, int kv_heads, int D, int max_new,

@@ -6,18 +6,20 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+from attnprofile_b200 import cache  # noqa: E402
+
 P = 4096  # an address that is aligned and never read
 
 
-def call(engine, name, order, good, **change):
-    a = {**good, **change}
+def call(engine, name, pack, good, **change):
     assert set(change) <= set(good)
-    return getattr(engine.lib(), name)(*[a[k] for k in order])
+    a = {**good, **change}
+    return getattr(engine.lib(), name)(pack(*[0 if v is None else v for v in a.values()]), None)
 
 
-TABLES = dict(lens=P, new_lens=P, batch=4, tables=P, width=8, table_stride=8, free=P,
-              free_count=P, num_blocks=64, block_size=16, kv_lens=P, starts=P, slots=P, tokens=9,
-              free_left=P, status=P, stream=None)
+TABLES = dict(lens=P, new_lens=P, tables=P, free=P, free_count=P, kv_lens=P, starts=P, slots=P,
+              free_left=P, status=P, table_stride=8, batch=4, width=8, num_blocks=64,
+              block_size=16, tokens=9)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -30,11 +32,11 @@ TABLES = dict(lens=P, new_lens=P, batch=4, tables=P, width=8, table_stride=8, fr
                                            "kv_lens", "starts", "slots", "free_left", "status")],
 ])
 def test_block_tables_refusals(engine, change, code):
-    assert call(engine, "attn_block_tables", TABLES, TABLES, **change) == engine.ERR[code]
+    assert call(engine, "attn_block_tables", cache._TABLES, TABLES, **change) == engine.ERR[code]
 
 
-TRIM = dict(lens=P, keep=P, batch=4, tables=P, width=8, table_stride=8, free=P, free_count=P,
-            num_blocks=64, block_size=16, lens_left=P, free_left=P, status=P, stream=None)
+TRIM = dict(lens=P, keep=P, tables=P, free=P, free_count=P, lens_left=P, free_left=P, status=P,
+            table_stride=8, batch=4, width=8, num_blocks=64, block_size=16)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -45,12 +47,12 @@ TRIM = dict(lens=P, keep=P, batch=4, tables=P, width=8, table_stride=8, free=P, 
                                            "lens_left", "free_left", "status")],
 ])
 def test_block_trim_refusals(engine, change, code):
-    assert call(engine, "attn_block_trim", TRIM, TRIM, **change) == engine.ERR[code]
+    assert call(engine, "attn_block_trim", cache._TRIM, TRIM, **change) == engine.ERR[code]
 
 
-APPEND = dict(k=P, k_token=256, k_head=128, v=P, v_token=256, v_head=128, slots=P, tokens=5,
-              kv_heads=2, D=128, dtype=0, k_codes=P, v_codes=P, k_scale=P, v_scale=P, code=0,
-              num_blocks=64, block_size=16, stream=None)
+APPEND = dict(k=P, v=P, slots=P, k_codes=P, v_codes=P, k_scale=P, v_scale=P, k_token=256,
+              k_head=128, v_token=256, v_head=128, tokens=5, kv_heads=2, D=128, dtype=0, code=0,
+              num_blocks=64, block_size=16)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -64,18 +66,17 @@ APPEND = dict(k=P, k_token=256, k_head=128, v=P, v_token=256, v_head=128, slots=
                                            "v_scale")],
 ])
 def test_cache_append_refusals(engine, change, code):
-    assert call(engine, "attn_cache_append", APPEND, APPEND, **change) == engine.ERR[code]
+    assert call(engine, "attn_cache_append", cache._APPEND, APPEND, **change) == engine.ERR[code]
 
 
 def test_cache_append_of_nothing(engine):
-    assert call(engine, "attn_cache_append", APPEND, APPEND, tokens=0, k=None) == 0
+    assert call(engine, "attn_cache_append", cache._APPEND, APPEND, tokens=0, k=None) == 0
 
 
-ATTN = dict(q=P, q_token=512, q_head=128, out=P, o_token=512, o_head=128, tokens=3, heads=4,
-            kv_heads=2, D=128, dtype=1, k_codes=P, v_codes=P, k_scale=P, v_scale=P, code=1,
-            num_blocks=64, block_size=32, tables=P, width=8, table_stride=8, kv_lens=P, starts=P,
-            batch=3, max_new=1, causal=1, scale=0.0, workspace=P, workspace_bytes=1 << 30,
-            stream=None)
+ATTN = dict(q=P, out=P, k_codes=P, v_codes=P, k_scale=P, v_scale=P, tables=P, kv_lens=P, starts=P,
+            workspace=P, workspace_bytes=1 << 30, q_token=512, q_head=128, o_token=512, o_head=128,
+            table_stride=8, tokens=3, heads=4, kv_heads=2, D=128, dtype=1, code=1, num_blocks=64,
+            block_size=32, width=8, batch=3, max_new=1, causal=1, scale=0.0)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -92,12 +93,12 @@ ATTN = dict(q=P, q_token=512, q_head=128, out=P, o_token=512, o_head=128, tokens
                                            "tables", "kv_lens", "starts", "workspace")],
 ])
 def test_attn_cached_refusals(engine, change, code):
-    assert call(engine, "attn_cached", ATTN, ATTN, **change) == engine.ERR[code]
+    assert call(engine, "attn_cached", cache._CACHED, ATTN, **change) == engine.ERR[code]
 
 
 @pytest.mark.parametrize("change", [{"tokens": 0}, {"batch": 0}, {"max_new": 0}])
 def test_attn_cached_of_nothing(engine, change):
-    assert call(engine, "attn_cached", ATTN, ATTN, q=None, **change) == 0
+    assert call(engine, "attn_cached", cache._CACHED, ATTN, q=None, **change) == 0
 
 
 @pytest.mark.parametrize("args,code", [((4, 3, 64, 1), "INVALID_ARG"), ((4, 0, 64, 1), "INVALID_ARG"),
@@ -106,6 +107,11 @@ def test_workspace_refusals(engine, args, code):
     out = ctypes.c_ulonglong()
     assert engine.lib().attn_cached_workspace(*args, ctypes.byref(out)) == engine.ERR[code]
     assert engine.lib().attn_cached_workspace(4, 2, 64, 1, None) == engine.ERR["INVALID_ARG"]
+
+
+def test_no_arguments_at_all(engine):
+    for name in ("attn_block_tables", "attn_block_trim", "attn_cache_append", "attn_cached"):
+        assert getattr(engine.lib(), name)(None, None) == engine.ERR["INVALID_ARG"]
 
 
 def test_python_face_refuses_cpu_tensors_and_shapes(engine):
