@@ -120,6 +120,13 @@ struct Place {
   long long before;  // work of all requests in front of it
 };
 
+// x / y for 0 <= x, 0 < y, the quotient in 32 bits; nearly all work counts fit 32
+// bits, and a 64-bit division is long.
+__device__ __forceinline__ int quotient(long long x, long long y) {
+  return ((x | y) >> 32) != 0 ? static_cast<int>(x / y)
+                              : static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y));
+}
+
 // Sum of all requests' work; a place in it is looked up afterwards: each
 // thread keeps the sum of its share of the requests.
 template <int NT>
@@ -166,18 +173,19 @@ __device__ __forceinline__ Place find_place(const CachedParams& p, const long lo
   }
 }
 
-// The same for at most 32 requests, by every warp for itself: lane r has
-// request r, the sum of all work up to and with it, and its shape.
+// The same for up to kLaneRequests requests, by every warp for itself and so
+// without a barrier: a lane has up to four requests in a row.
+constexpr int kLaneRequests = 128;
 struct Lanes {
-  long long upto;
-  Shape sh;
+  long long work, upto;  // of the lane's requests; of all up to and with them
 };
 template <int NT>
 __device__ __forceinline__ Lanes count_lanes(const CachedParams& p, long long* total) {
-  const int lane = threadIdx.x & 31;
-  Lanes x{0, Shape{0, 1, 1}};
-  if (lane < p.batch) x.sh = shape_of<NT>(p, request_at(p, lane));
-  x.upto = x.sh.work();
+  const int lane = threadIdx.x & 31, each = (p.batch + 31) / 32;
+  Lanes x{0, 0};
+  for (int r = lane * each; r < min(lane * each + each, p.batch); ++r)
+    x.work += shape_of<NT>(p, request_at(p, r)).work();
+  x.upto = x.work;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const long long a = __shfl_up_sync(~0u, x.upto, d);
@@ -186,20 +194,23 @@ __device__ __forceinline__ Lanes count_lanes(const CachedParams& p, long long* t
   *total = __shfl_sync(~0u, x.upto, 31);
   return x;
 }
-__device__ __forceinline__ Place place_in(const Lanes& x, long long at) {
-  const int r = __ffs(__ballot_sync(~0u, x.upto > at)) - 1;
-  return Place{r, __shfl_sync(~0u, x.upto - x.sh.work(), r)};
+template <int NT>
+__device__ __forceinline__ Place place_in(const CachedParams& p, const Lanes& x, long long at) {
+  const int each = (p.batch + 31) / 32;
+  const int lane = __ffs(__ballot_sync(~0u, x.upto > at)) - 1;
+  Place pl{lane * each, __shfl_sync(~0u, x.upto - x.work, lane)};
+  for (; pl.request + 1 < min(lane * each + each, p.batch); ++pl.request) {
+    const long long w = shape_of<NT>(p, request_at(p, pl.request)).work();
+    if (pl.before + w > at) break;
+    pl.before += w;
+  }
+  return pl;
 }
 
-__device__ __forceinline__ long long work_each(long long total) {
-  return (total + gridDim.x - 1) / gridDim.x;
+__device__ __forceinline__ long long work_each(long long total, int ctas) {
+  return quotient(total + ctas - 1, ctas);
 }
 
-// x / y for 0 <= x, 0 < y; most work counts fit 32 bits.
-__device__ __forceinline__ int quotient(long long x, int y) {
-  return (x >> 32) != 0 ? static_cast<int>(x / y)
-                        : static_cast<int>(static_cast<uint32_t>(x) / static_cast<uint32_t>(y));
-}
 
 // Chunks [c0, c1) of one unit.
 struct Part {
@@ -777,18 +788,18 @@ split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
   asm volatile("griddepcontrol.launch_dependents;");
   Cursor<NT> cursor;
   long long total;
-  if (p.batch <= 32) {
+  if (p.batch <= kLaneRequests) {
     const Lanes lanes = count_lanes<NT>(p, &total);
-    const long long each = work_each(total);
+    const long long each = work_each(total, gridDim.x);
     cursor.at = each * blockIdx.x;
     cursor.stop = min(cursor.at + each, total);
     if (cursor.at >= cursor.stop) return;
-    cursor.pl = place_in(lanes, cursor.at);
+    cursor.pl = place_in<NT>(p, lanes, cursor.at);
     __syncthreads();  // the barriers are there
   } else {
     long long* part_sum = reinterpret_cast<long long*>(smem + S::kOffHop);
     total = count_work<NT>(p, part_sum);
-    const long long each = work_each(total);
+    const long long each = work_each(total, gridDim.x);
     cursor.at = each * blockIdx.x;
     cursor.stop = min(cursor.at + each, total);
     if (cursor.at >= cursor.stop) return;
@@ -808,6 +819,28 @@ split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #endif
 }
 
+// Parts of one row joined one after the other: a lane has N head dimensions.
+template <int N>
+struct Sums {
+  float top = -INFINITY, sum = 0.f, x[N] = {};
+  __device__ __forceinline__ void add(float2 ml, const float* o) {
+    float y[N];
+    if constexpr (N == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(o);
+      y[0] = v.x; y[1] = v.y; y[2] = v.z; y[3] = v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(o);
+      y[0] = v.x; y[1] = v.y;
+    }
+    const float now = fmaxf(top, ml.x), base = now == -INFINITY ? 0.f : now;
+    const float a = ptx::ex2_approx(top - base), b = ptx::ex2_approx(ml.x - base);
+    top = now;
+    sum = sum * a + ml.y * b;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = x[j] * a + y[j] * b;
+  }
+};
+
 // Joins the parts of the units that were cut.  CTA c > 0 looks at the cut in
 // front of range c and, if that is the first cut in its unit, joins the unit:
 // the part that ends range c - 1, then those that begin ranges c, c + 1, ...
@@ -818,16 +851,25 @@ __global__ void __launch_bounds__(256) join_kernel(const CachedParams p) {
   __shared__ long long part_sum[256];
   __shared__ Place place;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long total = count_work<NT>(p, part_sum);
-  const long long each = work_each(total);
-  const long long cut = each * (blockIdx.x + 1ll);
-  if (threadIdx.x == 0 && cut < total) place = find_place<NT>(p, part_sum, cut);
-  __syncthreads();
+  long long total, each, cut;
+  Place pl{0, 0};
+  if (p.batch <= kLaneRequests) {
+    const Lanes lanes = count_lanes<NT>(p, &total);
+    each = work_each(total, gridDim.x);
+    cut = each * (blockIdx.x + 1ll);
+    if (cut < total) pl = place_in<NT>(p, lanes, cut);
+  } else {
+    total = count_work<NT>(p, part_sum);
+    each = work_each(total, gridDim.x);
+    cut = each * (blockIdx.x + 1ll);
+    if (threadIdx.x == 0 && cut < total) place = find_place<NT>(p, part_sum, cut);
+    __syncthreads();
+    pl = place;
+  }
   // By every CTA, those without work too: this kernel may not end before the
   // one in front of it.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (cut >= total) return;
-  const Place pl = place;
   const Request rq = request_at(p, pl.request);
   const Shape sh = shape_of<NT>(p, rq);
   const int unit = quotient(cut - pl.before, sh.weight);
@@ -839,48 +881,26 @@ __global__ void __launch_bounds__(256) join_kernel(const CachedParams p) {
   const int kvh = unit / tiles;
   const int row0 = (unit - kvh * tiles) * kRows;
   const int rows_in = rq.n * p.group;
-  const int parts = static_cast<int>((end - cut + each - 1) / each) + 1;
+  const int parts = quotient(end - cut + each - 1, each) + 1;
   const long long slots = 2ll * gridDim.x;
 
   auto slot_of = [&](int i) { return i == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + i); };
+  constexpr int kPer = D / 32;
   for (int r = warp; r < kRows && row0 + r < rows_in; r += 8) {
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32)
-      top = fmaxf(top, Parts<NT, D>::ml(p.ws, slots, slot_of(i))[r].x);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    float x[D / 32];
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) x[j] = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float2 ml = Parts<NT, D>::ml(p.ws, slots, slot_of(i))[r];
-      const float f = ptx::ex2_approx(ml.x - base);
-      const float* o = Parts<NT, D>::o(p.ws, slot_of(i)) + r * D + lane * (D / 32);
-      sum = fmaf(ml.y, f, sum);
-      if constexpr (D == 128) {
-        const float4 y = *reinterpret_cast<const float4*>(o);
-        x[0] = fmaf(y.x, f, x[0]);
-        x[1] = fmaf(y.y, f, x[1]);
-        x[2] = fmaf(y.z, f, x[2]);
-        x[3] = fmaf(y.w, f, x[3]);
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(o);
-        x[0] = fmaf(y.x, f, x[0]);
-        x[1] = fmaf(y.y, f, x[1]);
-      }
-    }
-    const float n = top == -INFINITY && sum == sum ? 0.f : 1.f / sum;
+    Sums<kPer> s;
+#pragma unroll 2
+    for (int i = 0; i < parts; ++i)
+      s.add(Parts<NT, D>::ml(p.ws, slots, slot_of(i))[r],
+            Parts<NT, D>::o(p.ws, slot_of(i)) + r * D + lane * kPer);
+    const float n = s.top == -INFINITY && s.sum == s.sum ? 0.f : 1.f / s.sum;
     const int row = row0 + r, tok = row / p.group;
     T* dst = static_cast<T*>(p.out) + (rq.start + tok) * p.o_token +
-             (kvh * p.group + row - tok * p.group) * p.o_head + lane * (D / 32);
+             (kvh * p.group + row - tok * p.group) * p.o_head + lane * kPer;
     if constexpr (D == 128)
       *reinterpret_cast<uint2*>(dst) =
-          make_uint2(pack_out<T>(x[0] * n, x[1] * n), pack_out<T>(x[2] * n, x[3] * n));
+          make_uint2(pack_out<T>(s.x[0] * n, s.x[1] * n), pack_out<T>(s.x[2] * n, s.x[3] * n));
     else
-      *reinterpret_cast<uint32_t*>(dst) = pack_out<T>(x[0] * n, x[1] * n);
+      *reinterpret_cast<uint32_t*>(dst) = pack_out<T>(s.x[0] * n, s.x[1] * n);
   }
 }
 
@@ -892,11 +912,14 @@ __global__ void __launch_bounds__(256) join_few_kernel(const CachedParams p, int
   __shared__ float top_of[8], sum_of[8];
   __shared__ float x_of[8][D];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // Lane r has request r.
+  Shape sh{0, 1, 1};
+  if (lane < p.batch) sh = shape_of<NT>(p, request_at(p, lane));
   long long total;
   const Lanes lanes = count_lanes<NT>(p, &total);
-  const long long each = (total + ctas - 1) / ctas;
+  const long long each = work_each(total, ctas);
   // The request that holds this unit.
-  int upto = lanes.sh.units;
+  int upto = sh.units;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const int a = __shfl_up_sync(~0u, upto, d);
@@ -905,13 +928,13 @@ __global__ void __launch_bounds__(256) join_few_kernel(const CachedParams p, int
   const int r = __ffs(__ballot_sync(~0u, upto > static_cast<int>(blockIdx.x))) - 1;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (r < 0) return;
-  const int units = __shfl_sync(~0u, lanes.sh.units, r), weight = __shfl_sync(~0u, lanes.sh.weight, r);
+  const int units = __shfl_sync(~0u, sh.units, r), weight = __shfl_sync(~0u, sh.weight, r);
   const int unit = static_cast<int>(blockIdx.x) - (__shfl_sync(~0u, upto, r) - units);
   const long long begin = __shfl_sync(~0u, lanes.upto, r) -
                           static_cast<long long>(units - unit) * weight;
   const long long end = begin + weight;
   // Ranges with chunks of the unit: the one that its first chunk lies in, to the last.
-  const int c0 = static_cast<int>((begin + kOver) / each), c1 = static_cast<int>((end - 1) / each);
+  const int c0 = quotient(begin + kOver, each), c1 = quotient(end - 1, each);
   if (c0 == c1) return;  // not cut
   const Request rq = request_at(p, r);
   const int tiles = units / p.kv_heads;
@@ -922,37 +945,25 @@ __global__ void __launch_bounds__(256) join_few_kernel(const CachedParams p, int
   auto slot_of = [&](int c) { return 2ll * c + (c == c0 ? 1 : 0); };
 
   constexpr int kPer = D / 32;
-  float top = -INFINITY, sum = 0.f, x[kPer];
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) x[j] = 0.f;
-  for (int c = c0 + warp; c <= c1; c += 8) {
-    const float2 ml = Parts<NT, D>::ml(p.ws, slots, slot_of(c))[row_in];
-    const float* o = Parts<NT, D>::o(p.ws, slot_of(c)) + row_in * D + lane * kPer;
-    float y[kPer];
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) y[j] = o[j];
-    const float now = fmaxf(top, ml.x), base = now == -INFINITY ? 0.f : now;
-    const float a = ptx::ex2_approx(top - base), b = ptx::ex2_approx(ml.x - base);
-    top = now;
-    sum = sum * a + ml.y * b;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) x[j] = x[j] * a + y[j] * b;
-  }
+  Sums<kPer> s;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += 8)
+    s.add(Parts<NT, D>::ml(p.ws, slots, slot_of(c))[row_in],
+          Parts<NT, D>::o(p.ws, slot_of(c)) + row_in * D + lane * kPer);
   if (lane == 0) {
-    top_of[warp] = top;
-    sum_of[warp] = sum;
+    top_of[warp] = s.top;
+    sum_of[warp] = s.sum;
   }
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) x_of[warp][lane * kPer + j] = x[j];
+  for (int j = 0; j < kPer; ++j) x_of[warp][lane * kPer + j] = s.x[j];
   __syncthreads();
   const int d = 2 * threadIdx.x;  // two head dimensions a thread
   if (d >= D) return;
-  top = top_of[0];
+  float top = top_of[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) top = fmaxf(top, top_of[i]);
   const float base = top == -INFINITY ? 0.f : top;
-  sum = 0.f;
-  float x0 = 0.f, x1 = 0.f;
+  float sum = 0.f, x0 = 0.f, x1 = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float f = ptx::ex2_approx(top_of[i] - base);
