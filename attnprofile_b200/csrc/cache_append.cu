@@ -18,9 +18,9 @@
 // a sum; a NaN among the values would instead spread to masked rows as 0 * NaN.
 //
 // Tokens that follow each other into one block (a run) share its scale, so the
-// unit of work is one run and one head.  A CTA of eight warps looks at `chunk`
+// unit of work is one run and one head.  A CTA of 2 to 8 warps looks at `chunk`
 // consecutive tokens of one head and takes the runs that begin there: a short
-// run (single tokens, drafts) by one warp, so that eight go at once, a longer
+// run (single tokens, drafts) by one warp, so that several go at once, a longer
 // one by the whole CTA, which holds it in registers between finding its largest
 // number and rounding it: every number is read once, with all loads on their
 // way at the same time.  Half of each warp works on K and half on V, so that
@@ -33,7 +33,6 @@ namespace attnprof {
 namespace cache {
 namespace {
 
-constexpr int kWarps = 8;
 
 struct AppendParams {
   const void *k, *v;
@@ -83,7 +82,7 @@ __device__ __forceinline__ int exponent_for(float a) {
   return max(e, kLeastExponent);
 }
 
-template <typename T, int CODE, int D, int ITERS>
+template <typename T, int CODE, int D, int kWarps, int ITERS>
 __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams p) {
   constexpr int kLanes = D / 8;              // lanes on one token's row: 16 bytes each
   constexpr int kRows = 16 / kLanes;         // tokens a half warp takes at once
@@ -257,11 +256,11 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams 
   }
 }
 
-template <typename T, int CODE, int D, int ITERS>
-int launch_iters(const AppendParams& p, cudaStream_t st) {
+template <typename T, int CODE, int D, int WARPS, int ITERS>
+int launch_rounds(const AppendParams& p, cudaStream_t st) {
   const dim3 grid((static_cast<unsigned>(p.tokens) + p.chunk - 1) / p.chunk,
                   static_cast<unsigned>(p.heads));
-  append_kernel<T, CODE, D, ITERS><<<grid, 32 * kWarps, 0, st>>>(p);
+  append_kernel<T, CODE, D, WARPS, ITERS><<<grid, 32 * WARPS, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
 }
 
@@ -273,12 +272,18 @@ int launch(const AppendParams& p0, cudaStream_t st) {
   const long long per_cta = static_cast<long long>(p.tokens) * p.heads / (148 * 8);
   p.chunk = 1;
   while (2 * p.chunk <= per_cta && p.chunk < (1 << p.shift)) p.chunk *= 2;
-  // Rounds that a CTA needs for a whole block, held in registers.
-  constexpr int kStep = kWarps * 16 / (D / 8);
-  const int rounds = ((1 << p.shift) + kStep - 1) / kStep;
-  if (rounds <= 4) return launch_iters<T, CODE, D, 4>(p, st);
-  if (rounds <= 8) return launch_iters<T, CODE, D, 8>(p, st);
-  return launch_iters<T, CODE, D, 16>(p, st);
+  // Rounds of one warp for a whole block; the CTA's warps share them and hold
+  // theirs in registers.  On 15,000 tokens of 8 heads of 128: blocks of 16
+  // tokens 19.3 us with 2 warps, 21.9 with 4, 37 with 8; of 64 24.4 us with 4,
+  // 25.8 with 8, 34 with 16; of 128 28.6 with 8, 32 with 4.
+  constexpr int kTokens = 16 / (D / 8);
+  switch ((1 << p.shift) / kTokens) {
+    case 8: return launch_rounds<T, CODE, D, 2, 4>(p, st);
+    case 16: return launch_rounds<T, CODE, D, 2, 8>(p, st);
+    case 32: return launch_rounds<T, CODE, D, 4, 8>(p, st);
+    case 64: return launch_rounds<T, CODE, D, 4, 16>(p, st);
+    default: return launch_rounds<T, CODE, D, 8, 16>(p, st);
+  }
 }
 
 template <typename T, int CODE>
