@@ -29,8 +29,8 @@
 // K's scale multiplies the scores in f32; V's scale multiplies each block's
 // sum of p v in f32, so no scale is rounded.  P is rounded to f16, by at most
 // 2^-11 of itself as an f16 result is (a bf16 result by 2^-8): it is held as
-// 2^15 p, in [0, 2^15], so that also weights down to 2^-29 of the largest keep
-// all their bits.  Maximum, sum and O are f32.  bf16 queries become f16 times a
+// 2^7 p (p up to 2^8 between two moves of the maximum), so that also weights down
+// to 2^-21 of the largest keep all their bits.  Maximum, sum and O are f32.  bf16 queries become f16 times a
 // power of two per row, which loses nothing above 2^-38 of the row's largest.
 #include <atomic>
 #include <climits>
@@ -53,7 +53,8 @@ constexpr int kOver = 1;                     // chunks that beginning a unit cou
 // graphs: 16 requests of 500 tokens 8.4 us whole, 12.3 cut; 64 of them 17.9 and
 // 21.3; 200 46.5 and 46.6.  Of 1000 tokens, 1 request 11.1 and 9.7, 200 74 and 65.)
 constexpr int kWholeChunks = 2;
-constexpr float kLift = 15.f;                // P is held as 2^kLift p
+constexpr float kMove = 8.f;                 // growth of the maximum (log2) that moves it
+constexpr float kLift = 7.f;                 // P is held as 2^kLift p
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                           uint32_t b1) {
@@ -533,6 +534,7 @@ __device__ void compute_role(const SplitParams& p, Cursor<NT> cursor, uint32_t s
         kscale[k] = scale[k];
         vsc[k] = scale[S::kGroups + k];
         held[k] = !(kscale[k] < 0.f);
+        if (!held[k]) kscale[k] = 1.f;  // (of scores that will be -inf)
         Words<4> kw[2][KP];  // [row g, row g + 8][piece]
 #pragma unroll
         for (int r = 0; r < 2; ++r)
@@ -559,53 +561,77 @@ __device__ void compute_role(const SplitParams& p, Cursor<NT> cursor, uint32_t s
         }
       }
 
-      // Scores in log2 units, masked; the running maximum.
-      const bool whole = key0 + 16 * KT <= least;
-      bool moved = false;
-      float alpha[NT][2];
+      // Masks, where not every key is there for every row.
+      bool clean = key0 + 16 * KT <= least;
+#pragma unroll
+      for (int k = 0; k < KT; ++k) clean &= held[k];
+      if (!clean) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!held[k] || key0 + 16 * k + 8 * (i >> 1) + g >= limit[nt][i & 1])
+                sc[nt][k][i] = -INFINITY;
+      }
+      // The maximum moves only when a score exceeds it by 2^kMove (as the first
+      // ones do): then, and only then, the lanes of a row agree on it and the
+      // sums are rescaled.
+      float top[NT][2];
+      bool move = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float top = -INFINITY;
+          float x = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+            x = fmaxf(x, fmaxf(sc[nt][k][j], sc[nt][k][2 + j]) * (kscale[k] * row_f[nt][j]));
+          top[nt][j] = x;
+          move |= x > m[nt][j] + kMove;
+        }
+      if (__any_sync(~0u, move)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float x = top[nt][j];
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+            const float now = fmaxf(m[nt][j], x);
+            const float alpha = now == -INFINITY ? 1.f : ptx::ex2_approx(m[nt][j] - now);
+            m[nt][j] = now;
+            l[nt][j] *= alpha;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              o[nt][mt][j] *= alpha;
+              o[nt][mt][2 + j] *= alpha;
+            }
+          }
+      }
+      // P.  (A masked score is -inf; times a factor that is NaN or 0 it is not.)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float neg = m[nt][j] == -INFINITY ? 0.f : kLift - m[nt][j];
+          float sum = 0.f;
 #pragma unroll
           for (int k = 0; k < KT; ++k) {
             const float f = kscale[k] * row_f[nt][j];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float x = sc[nt][k][2 * h + j] * f;
-              if (!held[k] || (!whole && key0 + 16 * k + 8 * h + g >= limit[nt][j])) x = -INFINITY;
-              sc[nt][k][2 * h + j] = x;
-              top = fmaxf(top, x);
-            }
-          }
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-          const float now = fmaxf(m[nt][j], top);
-          const float base = now == -INFINITY ? 0.f : now - kLift;
-          alpha[nt][j] = ptx::ex2_approx(m[nt][j] - kLift - base);
-          moved |= now != m[nt][j];
-          m[nt][j] = now;
-          float sum = 0.f;
-#pragma unroll
-          for (int k = 0; k < KT; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float e = ptx::ex2_approx(sc[nt][k][2 * h + j] - base);
+              const float x = sc[nt][k][2 * h + j];
+              float e = ptx::ex2_approx(fmaf(x, f, neg));
+              if (!clean && x == -INFINITY) e = 0.f;
               sc[nt][k][2 * h + j] = e;
               sum += e;
             }
-          l[nt][j] = l[nt][j] * alpha[nt][j] + sum;
+          }
+          l[nt][j] += sum;
         }
-      if (__any_sync(~0u, moved)) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[nt][mt][i] *= alpha[nt][i & 1];
-      }
 
       // P^T as the second operand: keys move from lanes' rows to their columns.
       uint32_t pb[NT][KT][2];
@@ -616,21 +642,25 @@ __device__ void compute_role(const SplitParams& p, Cursor<NT> cursor, uint32_t s
           pb[nt][k][0] = transpose_8x8(pack_half2(sc[nt][k][0], sc[nt][k][1]));
           pb[nt][k][1] = transpose_8x8(pack_half2(sc[nt][k][2], sc[nt][k][3]));
         }
-      // V: [tile][keys 2t, 2t + 1, 2t + 8, 2t + 9].  What lies behind the last
-      // token, or where nothing was fetched, may be any bits, NaN among them.
+      // V: [tile][keys 2t, 2t + 1, 2t + 8, 2t + 9].
       Words<VW> vw[KT][4];
-      const bool tail = key0 + 16 * KT > rq.kv;
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < 4; ++r)
           load_codes(vw[k][r], from + kStageBytes / 2 + k * S::kGroup + v_at[r]);
-          if (!held[k] ||
-              (tail && key0 + 16 * k + 2 * t + (r & 1) + 8 * (r >> 1) >= rq.kv)) {
+      if (!clean) {
+        // What lies behind the last token, or where nothing was fetched, may be
+        // any bits: 0 * NaN would reach a sum.
 #pragma unroll
-            for (int i = 0; i < VW; ++i) vw[k][r].w[i] = 0u;
-          }
-        }
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!held[k] || key0 + 16 * k + 2 * t + (r & 1) + 8 * (r >> 1) >= rq.kv) {
+#pragma unroll
+              for (int i = 0; i < VW; ++i) vw[k][r].w[i] = 0u;
+            }
+      }
       __syncwarp();  // every lane has its codes: the place may be filled again
       if (lane == 0) ptx::mbar_arrive(empty + 8 * take);
       if (++take == S::kStages) {
