@@ -450,19 +450,19 @@ __device__ void mma_role(const Unit& u, int me, uint32_t tmem, uint32_t sbase, c
       }
       if (!(ok = ring_wait(tv))) break;
       if (!(ok = p_wait(i, 0, j))) break;
-      issue_pv(i, j, tv, 0, 6);
+      issue_pv(i, j, tv, 0, 4);
       if (!(ok = p_wait(i, 1, j))) break;
-      issue_pv(i, j, tv, 6, 8);
+      issue_pv(i, j, tv, 4, 8);
       ptx::mma_commit(bar(Bar<D>::kPV + i));
       ptx::mma_commit(bar(Bar<D>::kEmpty + tv % T::kSlots));
     } else {
       if (!(ok = ring_wait(tv))) break;
       for (int i = 0; i < tiles && ok; ++i) {
         if (!(ok = p_wait(i, 0, j))) break;
-        issue_pv(i, j, tv, 0, 6);
+        issue_pv(i, j, tv, 0, 4);
         if (i == 0 && j + 1 < n && !(ok = ring_wait(tk))) break;
         if (!(ok = p_wait(i, 1, j))) break;
-        issue_pv(i, j, tv, 6, 8);
+        issue_pv(i, j, tv, 4, 8);
         if (j + 1 < n)
           issue_s(i, tk);  // its commit covers this step's P V too
         else
@@ -654,7 +654,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
       }
       if (c == 0) pv_wait();
       ptx::tmem_st16(lane_base + p_col + 16 * c, pk);
-      if (c == 2) {  // P V of 96 keys may begin
+      if (c == 1) {  // P V of 64 keys may begin
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
         __syncwarp();
