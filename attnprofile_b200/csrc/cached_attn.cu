@@ -6,8 +6,13 @@
 using namespace attnprof::cache;
 
 namespace {
-constexpr long long kSplitRows = 64;
-}
+// Rows of one request and kv head up to which the split kernel is used, above
+// it the tiled one.  Measured in graphs, both ways (8 kv heads, e4m3; split |
+// tiled, us): D = 64, 32 rows: 8 requests of 4000 tokens 32 | 41, 2 of 30,000
+// 34 | 55; 48 rows: 44 | 39, 69 | 55.  D = 128, 16 rows: 24 | 44, 36 | 69; 24
+// rows: 47 | 45, 67 | 69, 64 requests of 1000 tokens 102 | 90.
+constexpr long long split_rows(int D) { return D == 64 ? 32 : 16; }
+}  // namespace
 
 extern "C" int attn_cached(const attn_cached_args* args, void* stream) {
   if (!args) return ATTN_ERR_INVALID_ARG;
@@ -58,18 +63,17 @@ extern "C" int attn_cached(const attn_cached_args* args, void* stream) {
   p.scale_log2 = static_cast<float>(
       (a.scale > 0.f ? static_cast<double>(a.scale) : 1.0 / std::sqrt(static_cast<double>(a.D))) *
       1.4426950408889634);
-  // Rows of one request and kv head: up to kSplitRows the keys' bytes are what
-  // counts and the split kernel reads them with every SM; above, the tiled one.
-  // A batch may hold both kinds (the lengths are on the GPU): then both run,
+  // A batch may hold requests for both kernels (the lengths are on the GPU): then both run,
   // each on its own requests.  A single request, or none that can be long,
   // needs one launch.
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (most <= kSplitRows) {
+  if (most <= split_rows(a.D)) {
     p.rows_most = LLONG_MAX;
   } else {
-    p.rows_most = a.batch == 1 ? 0 : kSplitRows;
-    const int rt = launch_tiled(p, a.D, a.dtype, a.code, st);
-    if (rt != ATTN_OK || a.batch == 1) return rt;
+    const bool tiled_only = a.batch == 1 || group > split_rows(a.D);
+    p.rows_most = tiled_only ? 0 : split_rows(a.D);
+    const int rt = launch_tiled(p, a.D, a.dtype, a.code, a.workspace, a.workspace_bytes, st);
+    if (rt != ATTN_OK || tiled_only) return rt;
   }
   return launch_split(p, a.D, a.dtype, a.code, a.max_new, a.workspace, a.workspace_bytes, st);
 }
@@ -79,5 +83,12 @@ extern "C" int attn_cached_workspace(int heads, int kv_heads, int D, int max_new
   if (!bytes || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || max_new < 0)
     return ATTN_ERR_INVALID_ARG;
   if (D != 64 && D != 128) return ATTN_ERR_UNSUPPORTED;
-  return split_workspace(heads / kv_heads, D, max_new > 0 ? max_new : 1, bytes);
+  const int group = heads / kv_heads;
+  int rc = split_workspace(group, D, max_new > 0 ? max_new : 1, bytes);
+  if (rc == ATTN_OK && static_cast<long long>(max_new) * group > split_rows(D)) {
+    unsigned long long tiled = 0;
+    rc = tiled_workspace(D, &tiled);
+    if (rc == ATTN_OK && tiled > *bytes) *bytes = tiled;
+  }
+  return rc;
 }

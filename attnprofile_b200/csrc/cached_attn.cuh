@@ -39,7 +39,9 @@ __device__ __forceinline__ Request request_at(const CachedParams& p, int r) {
 int codes_map(CUtensorMap* m, const void* codes, const CachedParams& p, int D);
 int launch_split(const CachedParams& p, int D, int dtype, int code, int max_new, void* ws,
                  unsigned long long ws_bytes, cudaStream_t st);
-int launch_tiled(const CachedParams& p, int D, int dtype, int code, cudaStream_t st);
+int launch_tiled(const CachedParams& p, int D, int dtype, int code, void* ws,
+                 unsigned long long ws_bytes, cudaStream_t st);
+int tiled_workspace(int D, unsigned long long* bytes);
 int split_workspace(int group, int D, int max_new, unsigned long long* bytes);
 
 }  // namespace cache

@@ -1011,12 +1011,12 @@ __global__ void __launch_bounds__(256) join_few_kernel(const CachedParams p, int
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// Rows of 8 that a unit holds: as many as the longest request's rows need, up
-// to 32; where longer requests go to the tiled kernel, what single tokens need.
-int row_tiles(int group, int max_new) {
+// Rows of 8 that a unit holds: as many as the longest request's rows need;
+// where longer requests go to the tiled kernel, what single tokens need.
+int row_tiles(int group, int D, int max_new) {
   const long long rows = static_cast<long long>(group) * max_new;
-  const long long want = rows <= 32 ? rows : group;
-  return want <= 8 ? 1 : want <= 16 ? 2 : 4;
+  const long long want = rows <= (D == 64 ? 32 : 16) ? rows : group;
+  return want <= 8 ? 1 : want <= 16 || D == 128 ? 2 : 4;
 }
 
 constexpr int kMostCtasPerSm = 2;  // by shared memory and registers; bounds the workspace
@@ -1092,10 +1092,12 @@ int launch(const CachedParams& cp, int max_new, void* ws, unsigned long long ws_
 
 template <typename T, int CODE, int D>
 int launch_nt(const CachedParams& p, int max_new, void* ws, unsigned long long b, cudaStream_t st) {
-  switch (row_tiles(p.group, max_new)) {
+  switch (row_tiles(p.group, D, max_new)) {
     case 1: return launch<T, CODE, D, 1>(p, max_new, ws, b, st);
     case 2: return launch<T, CODE, D, 2>(p, max_new, ws, b, st);
-    default: return launch<T, CODE, D, 4>(p, max_new, ws, b, st);
+    default:
+      if constexpr (D == 64) return launch<T, CODE, D, 4>(p, max_new, ws, b, st);
+      return ATTN_ERR_UNSUPPORTED;  // (not reached: D = 128 has at most 16 rows here)
   }
 }
 
@@ -1143,7 +1145,7 @@ int split_workspace(int group, int D, int max_new, unsigned long long* bytes) {
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return ATTN_ERR_CUDA;
-  *bytes = part_bytes(D, row_tiles(group, max_new)) * sms * kMostCtasPerSm;
+  *bytes = part_bytes(D, row_tiles(group, D, max_new)) * sms * kMostCtasPerSm;
   return ATTN_OK;
 }
 

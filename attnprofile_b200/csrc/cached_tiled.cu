@@ -92,14 +92,32 @@ struct Bar {
   static constexpr int kDrain = kO + 2;   // [issuer]
 };
 
+// 256 rows of one request and kv head, over steps [step0, step0 + steps) of
+// kBN keys: all that they see, or one of `parts` ranges of it.
 struct Unit {
   Request rq;
-  int request, kvh, row0, rows_in, steps, kv_end;
+  int request, kvh, row0, rows_in, step0, steps, kv_end;  // kv_end: of this range
+  int index;                                              // among all units
+  // At most 128 rows: both tiles are these rows, tile i over steps i, i + 2, ...
+  bool dual;
 };
 
 struct TiledParams : CachedParams {
   int* status;
   unsigned long long timeout_ns;
+  int parts;  // CTAs of a unit; above 1 they leave (max, sum, O) in the workspace
+};
+
+// Part `part` of a unit in the workspace, `slots` of them in all: [256][D] f32
+// of O, then (max, sum) per row.
+template <int D>
+struct TilePart {
+  static __device__ __forceinline__ float* o(float* ws, long long slot, int row) {
+    return ws + (slot * kUnit + row) * D;
+  }
+  static __device__ __forceinline__ float2* ml(float* ws, long long slots, long long slot, int row) {
+    return reinterpret_cast<float2*>(ws + slots * kUnit * D) + slot * kUnit + row;
+  }
 };
 
 __device__ __forceinline__ long long units_of(const CachedParams& p, const Request& r) {
@@ -113,17 +131,17 @@ __device__ __forceinline__ int row_limit(const CachedParams& p, const Request& r
   return min(max(last, 0), rq.kv);
 }
 
-// The unit of this CTA.  The requests with most keys come first and, in each,
+// Unit number `at`.  The requests with most keys come first and, in each,
 // the last rows (causal: those that see most), so that the last CTAs to start
 // are short; the heads of a row tile follow each other, so that neighbours share
 // keys in L2.  (More requests than threads, each with a long prompt: in their
 // own order.)  `scratch`: 12 bytes a thread.
-__device__ bool find_unit(const CachedParams& p, Unit& u, uint8_t* scratch) {
+__device__ bool find_unit(const CachedParams& p, long long at, Unit& u, uint8_t* scratch) {
   long long* units = reinterpret_cast<long long*>(scratch);
   int* keys = reinterpret_cast<int*>(units + kThreads);
   __shared__ long long where[2];
   const int each = (p.batch + kThreads - 1) / kThreads;
-  const int me = static_cast<int>(threadIdx.x);
+  const int me = static_cast<int>(threadIdx.x);  // of at least kThreads threads
   const int first = me * each, last = min(first + each, p.batch);
   long long mine = 0;
   int kv = 0;
@@ -136,7 +154,6 @@ __device__ bool find_unit(const CachedParams& p, Unit& u, uint8_t* scratch) {
   keys[me] = kv;
   if (me == 0) where[0] = -1;
   __syncthreads();
-  const long long at = blockIdx.x;
   if (mine > 0) {
     long long before = 0;
     const int threads = min(kThreads, p.batch);
@@ -164,8 +181,20 @@ __device__ bool find_unit(const CachedParams& p, Unit& u, uint8_t* scratch) {
   u.row0 = in_request / p.kv_heads * kUnit;
   u.rows_in = u.rq.n * p.group;
   u.kv_end = row_limit(p, u.rq, min(u.row0 + kUnit, u.rows_in) - 1);
+  u.step0 = 0;
   u.steps = (u.kv_end + kBN - 1) / kBN;
+  u.index = static_cast<int>(at);
+  u.dual = u.rows_in - u.row0 <= kBM && u.steps > 1;
   return true;
+}
+
+// Range `part` of `parts` of it.
+__device__ __forceinline__ void take_part(Unit& u, int part, int parts) {
+  const int each = (u.steps + parts - 1) / parts;
+  u.step0 = min(part * each, u.steps);
+  u.steps = min(each, u.steps - u.step0);
+  u.kv_end = min(u.kv_end, (u.step0 + u.steps) * kBN);
+  u.dual = u.dual && u.steps > 1;
 }
 
 __device__ __forceinline__ void st_shared_v4(uint32_t a, uint32_t x, uint32_t y, uint32_t z,
@@ -200,7 +229,7 @@ __device__ void fetch_role(const CUtensorMap* map_k, const CUtensorMap* map_v,
   const int lane = threadIdx.x & 31;
   const int* table = p.tables + u.request * p.table_stride;
   auto id_of = [&](int j) {
-    const int key = j * kBN + 16 * lane;
+    const int key = (u.step0 + j) * kBN + 16 * lane;
     if (lane < 8 && key < u.kv_end) {
       const int id = table[key >> p.shift];
       if (id >= 0 && id < p.num_blocks) return id;
@@ -221,7 +250,7 @@ __device__ void fetch_role(const CUtensorMap* map_k, const CUtensorMap* map_v,
                       : T::kOffScale + 4 * (12 * (j % kScaleRing) + lane));
     if (!is_v) {  // groups whose block is none, bit by bit
       const unsigned holes =
-          __ballot_sync(~0u, lane < 8 && id < 0 && j * kBN + 16 * lane < u.kv_end);
+          __ballot_sync(~0u, lane < 8 && id < 0 && (u.step0 + j) * kBN + 16 * lane < u.kv_end);
       if (lane == 0)
         ptx::st_shared_f32(sbase + T::kOffScale + 4 * (12 * (j % kScaleRing) + 8),
                            __uint_as_float(holes));
@@ -229,7 +258,7 @@ __device__ void fetch_role(const CUtensorMap* map_k, const CUtensorMap* map_v,
     if (lane == 0) ptx::mbar_arrive_expect_tx(full, n * T::kGroup);
     __syncwarp();
     if (id >= 0) {
-      const int off = (j * kBN + 16 * lane) & ((1 << p.shift) - 1);
+      const int off = ((u.step0 + j) * kBN + 16 * lane) & ((1 << p.shift) - 1);
       const int piece = id * p.kv_heads + u.kvh;
       ptx::tma_load_3d(sbase + T::kOffCodes + stage * T::kCodes + lane * T::kGroup,
                        is_v ? map_v : map_k, full, 0, D == 128 ? off : off / 2, piece);
@@ -280,7 +309,7 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
   float ref = 0.f;
   const int* table = p.tables + u.request * p.table_stride;
   const int blocks = (u.kv_end + (1 << p.shift) - 1) >> p.shift;
-  for (int b = 32 * warp + lane; b < blocks; b += 128) {
+  for (int b = ((u.step0 * kBN) >> p.shift) + 32 * warp + lane; b < blocks; b += 128) {
     const int id = table[b];
     if (id >= 0 && id < p.num_blocks)
       ref = fmaxf(ref, p.vs[static_cast<long long>(id) * p.kv_heads + u.kvh]);
@@ -329,10 +358,11 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
       for (int it = 0; it < kIters; ++it) vs[it] = scale[group_of(it)] * to_v;
       // What lies behind the last token, or where nothing was fetched, may be
       // any bits: 0 * NaN would reach a sum.  (Among the keys it is masked.)
-      if (j * kBN + kBN > u.rq.kv) {
+      const int key0 = (u.step0 + j) * kBN;
+      if (key0 + kBN > u.rq.kv) {
 #pragma unroll
         for (int it = 0; it < kIters; ++it)
-          if (j * kBN + row0 + it * kRowStep >= u.rq.kv) c[it][0] = c[it][1] = c[it][2] = c[it][3] = 0u;
+          if (key0 + row0 + it * kRowStep >= u.rq.kv) c[it][0] = c[it][1] = c[it][2] = c[it][3] = 0u;
       }
 #pragma unroll
       for (int it = 0; it < kIters; ++it)
@@ -430,47 +460,85 @@ __device__ void mma_role(const Unit& u, int me, uint32_t tmem, uint32_t sbase, c
   };
 
   const int i0 = T::kOwnP ? me : 0, i1 = T::kOwnP ? min(me + 1, tiles) : tiles;
-  bool ok = n > 0 && i0 < i1 && ring_wait(0);
-  for (int i = i0; i < i1 && ok; ++i) {
-    if (!(ok = wait_bar(bar(Bar<D>::kQ + i), 0, w, kSiteQ))) break;
+  bool ok = true;
+  auto first_s = [&](int i, int t) {
+    ok = ring_wait(t) && wait_bar(bar(Bar<D>::kQ + i), 0, w, kSiteQ);
+    if (!ok) return;
     ptx::tc_fence_after();
-    issue_s(i, 0);
-  }
-  if (ok) ptx::mma_commit(bar(Bar<D>::kEmpty));
-  for (int j = 0; j < n && ok; ++j) {
-    const int tv = 2 * j + 1, tk = 2 * j + 2;
-    if constexpr (T::kOwnP) {
-      const int i = i0;
-      if (j + 1 < n) {
-        if (!(ok = wait_bar(bar(Bar<D>::kSRead + i), j & 1, w, kSiteSFull))) break;
+    issue_s(i, t);
+  };
+  if (u.dual) {
+    // Both tiles' steps in turn (kOwnP: one tile's); S of a tile's next step
+    // goes behind P V of the present one, or as soon as S has been read.
+    const int by = T::kOwnP ? 2 : 1, from = T::kOwnP ? me : 0;
+    for (int j = from; j < 2 && ok; j += by) {
+      first_s(j, 2 * j);
+      if (ok) ptx::mma_commit(bar(Bar<D>::kEmpty + (2 * j) % T::kSlots));
+    }
+    for (int j = from; j < n && ok; j += by) {
+      const int i = j & 1, c = j >> 1, tv = 2 * j + 1, tk = 2 * j + 4;
+      const bool more = j + 2 < n;
+      if (T::kOwnP && more) {
+        if (!(ok = wait_bar(bar(Bar<D>::kSRead + i), c & 1, w, kSiteSFull))) break;
         if (!(ok = ring_wait(tk))) break;
         ptx::tc_fence_after();
         issue_s(i, tk);
         ptx::mma_commit(bar(Bar<D>::kEmpty + tk % T::kSlots));
       }
       if (!(ok = ring_wait(tv))) break;
-      if (!(ok = p_wait(i, 0, j))) break;
-      issue_pv(i, j, tv, 0, 4);
-      if (!(ok = p_wait(i, 1, j))) break;
-      issue_pv(i, j, tv, 4, 8);
-      ptx::mma_commit(bar(Bar<D>::kPV + i));
+      if (!(ok = p_wait(i, 0, c))) break;
+      issue_pv(i, c, tv, 0, 4);
+      if (!T::kOwnP && more && !(ok = ring_wait(tk))) break;
+      if (!(ok = p_wait(i, 1, c))) break;
+      issue_pv(i, c, tv, 4, 8);
+      if (T::kOwnP) {
+        ptx::mma_commit(bar(Bar<D>::kPV + i));
+      } else if (more) {
+        issue_s(i, tk);
+        ptx::mma_commit(bar(Bar<D>::kEmpty + tk % T::kSlots));
+      } else {
+        ptx::mma_commit(bar(Bar<D>::kO + i));
+      }
       ptx::mma_commit(bar(Bar<D>::kEmpty + tv % T::kSlots));
-    } else {
-      if (!(ok = ring_wait(tv))) break;
-      for (int i = 0; i < tiles && ok; ++i) {
+    }
+  } else if (n > 0 && i0 < i1) {
+    for (int i = i0; i < i1 && ok; ++i) first_s(i, 0);
+    if (ok) ptx::mma_commit(bar(Bar<D>::kEmpty));
+    for (int j = 0; j < n && ok; ++j) {
+      const int tv = 2 * j + 1, tk = 2 * j + 2;
+      if constexpr (T::kOwnP) {
+        const int i = i0;
+        if (j + 1 < n) {
+          if (!(ok = wait_bar(bar(Bar<D>::kSRead + i), j & 1, w, kSiteSFull))) break;
+          if (!(ok = ring_wait(tk))) break;
+          ptx::tc_fence_after();
+          issue_s(i, tk);
+          ptx::mma_commit(bar(Bar<D>::kEmpty + tk % T::kSlots));
+        }
+        if (!(ok = ring_wait(tv))) break;
         if (!(ok = p_wait(i, 0, j))) break;
         issue_pv(i, j, tv, 0, 4);
-        if (i == 0 && j + 1 < n && !(ok = ring_wait(tk))) break;
         if (!(ok = p_wait(i, 1, j))) break;
         issue_pv(i, j, tv, 4, 8);
-        if (j + 1 < n)
-          issue_s(i, tk);  // its commit covers this step's P V too
-        else
-          ptx::mma_commit(bar(Bar<D>::kO + i));
+        ptx::mma_commit(bar(Bar<D>::kPV + i));
+        ptx::mma_commit(bar(Bar<D>::kEmpty + tv % T::kSlots));
+      } else {
+        if (!(ok = ring_wait(tv))) break;
+        for (int i = 0; i < tiles && ok; ++i) {
+          if (!(ok = p_wait(i, 0, j))) break;
+          issue_pv(i, j, tv, 0, 4);
+          if (i == 0 && j + 1 < n && !(ok = ring_wait(tk))) break;
+          if (!(ok = p_wait(i, 1, j))) break;
+          issue_pv(i, j, tv, 4, 8);
+          if (j + 1 < n)
+            issue_s(i, tk);  // its commit covers this step's P V too
+          else
+            ptx::mma_commit(bar(Bar<D>::kO + i));
+        }
+        if (!ok) break;
+        ptx::mma_commit(bar(Bar<D>::kEmpty + tv % T::kSlots));
+        if (j + 1 < n) ptx::mma_commit(bar(Bar<D>::kEmpty + tk % T::kSlots));
       }
-      if (!ok) break;
-      ptx::mma_commit(bar(Bar<D>::kEmpty + tv % T::kSlots));
-      if (j + 1 < n) ptx::mma_commit(bar(Bar<D>::kEmpty + tk % T::kSlots));
     }
   }
   // Every MMA issued here has ended before tensor memory is freed.
@@ -494,12 +562,13 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
   auto bar = [&](int b) { return sbase + T::kOffBar + 8u * b; };
   const int lane = threadIdx.x & 31, wi = (threadIdx.x >> 5) & 3;
   const int r = 32 * wi + lane;                 // row of the tile, lane of tensor memory
-  const int row = u.row0 + i * kBM + r;
+  const int row = u.row0 + (u.dual ? 0 : i * kBM) + r;
   const bool live = row < u.rows_in;
   const int tok = live ? row / p.group : 0;
   const int head = u.kvh * p.group + (live ? row - tok * p.group : 0);
-  const int limit = live ? row_limit(p, u.rq, row) : 0;
-  const bool tile_there = u.row0 + i * kBM < u.rows_in;
+  // (rows behind the last one: zeros that see everything, so that they mask nothing)
+  const int limit = live ? row_limit(p, u.rq, row) : INT_MAX;
+  const bool tile_there = u.dual || u.row0 + i * kBM < u.rows_in;
 
   // Q: this row to shared memory, in f16.
   float row_f = 1.f;
@@ -542,15 +611,18 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
   const float to_log2 = row_f * p.scale_log2;
   float m = -INFINITY, l = 0.f;  // maximum in log2 units, sum of 2^kLift p
   bool ok = true;
-  for (int j = 0; j < u.steps && tile_there; ++j) {
-    ok = __all_sync(~0u, wait_bar(bar(Bar<D>::kS + i), j & 1, w, kSiteSFull));
+  // c counts this tile's steps, j all of them.
+  const int by = u.dual ? 2 : 1;
+  int c = 0;
+  for (int j = u.dual ? i : 0; j < u.steps && tile_there; j += by, ++c) {
+    ok = __all_sync(~0u, wait_bar(bar(Bar<D>::kS + i), c & 1, w, kSiteSFull));
     if (!ok) break;
     ptx::tc_fence_after();
     uint32_t s[kBN];
 #pragma unroll
-    for (int c = 0; c < kBN / 32; ++c)
-      ptx::tmem_ld32(lane_base + s_col + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-    const int lim = limit - j * kBN;  // columns below it are seen
+    for (int b = 0; b < kBN / 32; ++b)
+      ptx::tmem_ld32(lane_base + s_col + 32 * b, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * b]));
+    const int lim = min(limit, u.kv_end) - (u.step0 + j) * kBN;  // columns below it are seen
     // Factors of the groups' scores, and the groups whose block is none.
     float factor[kBN / 16];
     uint32_t holes;
@@ -577,8 +649,8 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     }
     if (__any_sync(~0u, lim < kBN) || holes != 0) {
 #pragma unroll
-      for (int c = 0; c < kBN; ++c)
-        if (c >= lim || ((holes >> (c / 16)) & 1u)) s[c] = __float_as_uint(-INFINITY);
+      for (int k = 0; k < kBN; ++k)
+        if (k >= lim || ((holes >> (k / 16)) & 1u)) s[k] = __float_as_uint(-INFINITY);
       // The factor of a group which the row does not see may be anything (NaN):
       // 1 keeps -inf there.  The least factor keeps -inf too, where the product
       // above may reach 0 (f16 products are below 2^32, so scores that small
@@ -603,7 +675,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     }
     float alpha = 1.f;
     bool move = false;
-    if (j == 0) {
+    if (c == 0) {
       m = top;
     } else if (top - m > kMove) {
       alpha = ptx::ex2_approx(m - top);
@@ -612,10 +684,10 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     }
     // The last step's P V has ended: O has the sum so far, P's columns are free.
     // (P over S: S was issued behind that P V, so its commit said so.)
-    bool waited = !T::kOwnP || j == 0;
+    bool waited = !T::kOwnP || c == 0;
     auto pv_wait = [&]() {
       if (!waited) {
-        ok = __all_sync(~0u, wait_bar(bar(Bar<D>::kPV + i), (j - 1) & 1, w, kSiteODone));
+        ok = __all_sync(~0u, wait_bar(bar(Bar<D>::kPV + i), (c - 1) & 1, w, kSiteODone));
         ptx::tc_fence_after();
         waited = true;
       }
@@ -623,25 +695,25 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     if (__any_sync(~0u, move)) {
       pv_wait();
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int b = 0; b < D / 32; ++b) {
         uint32_t o[32];
-        ptx::tmem_ld32(lane_base + o_col + 32 * c, o);
+        ptx::tmem_ld32(lane_base + o_col + 32 * b, o);
         ptx::tmem_wait_ld();
         ptx::reg_fence(o);
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-        ptx::tmem_st32(lane_base + o_col + 32 * c, o);
+        ptx::tmem_st32(lane_base + o_col + 32 * b, o);
       }
     }
     const float neg = m == -INFINITY ? 0.f : kLift - m;
     const uint64_t neg2 = ptx::f2_pack(neg, neg);
     uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
-    for (int c = 0; c < kBN / 32; ++c) {
+    for (int b = 0; b < kBN / 32; ++b) {
       uint32_t pk[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int c0 = 32 * c + 2 * e;
+        const int c0 = 32 * b + 2 * e;
         const float f = factor[c0 / 16];
         const uint64_t x2 = ptx::f2_fma(
             ptx::f2_pack(__uint_as_float(s[c0]), __uint_as_float(s[c0 + 1])), ptx::f2_pack(f, f),
@@ -652,9 +724,9 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
         part[e & 1] = ptx::f2_add(part[e & 1], ptx::f2_pack(p0, p1));
         pk[e] = half2_of(p0, p1);
       }
-      if (c == 0) pv_wait();
-      ptx::tmem_st16(lane_base + p_col + 16 * c, pk);
-      if (c == 1) {  // P V of 64 keys may begin
+      if (b == 0) pv_wait();
+      ptx::tmem_st16(lane_base + p_col + 16 * b, pk);
+      if (b == 1) {  // P V of 64 keys may begin
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
         __syncwarp();
@@ -671,41 +743,141 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     l = l * alpha + ((sa + sb) + (sc + sd));
   }
 
-  if (!tile_there || !ok) return;
+  if (!tile_there) return;
   float f = 0.f;
   if (u.steps > 0) {
-    const bool done = T::kOwnP
-                          ? wait_bar(bar(Bar<D>::kPV + i), (u.steps - 1) & 1, w, kSiteODone)
-                          : wait_bar(bar(Bar<D>::kO + i), 0, w, kSiteODone);
-    if (!__all_sync(~0u, done)) return;
-    ptx::tc_fence_after();
-    if (m != -INFINITY || l != l)
-      f = reinterpret_cast<const float*>(sgen + T::kOffMisc)[2] / l;
+    if (ok) {
+      const bool done = T::kOwnP ? wait_bar(bar(Bar<D>::kPV + i), (c - 1) & 1, w, kSiteODone)
+                                 : wait_bar(bar(Bar<D>::kO + i), 0, w, kSiteODone);
+      ok = __all_sync(~0u, done);
+      ptx::tc_fence_after();
+    }
+    f = reinterpret_cast<const float*>(sgen + T::kOffMisc)[2];
+  }
+  // Two tiles of the same rows: tile 1 hands its sums over in the rings' place,
+  // once both have no MMA left that reads there; tile 0 adds them to its own.
+  float other = 0.f;
+  float4* hand = reinterpret_cast<float4*>(const_cast<uint8_t*>(sgen) + T::kOffKv) + r;
+  if (u.dual) {
+    float2* hand_ml = reinterpret_cast<float2*>(hand - r + kBM * (D / 4)) + r;
+    ptx::named_bar_sync(2, 2 * kBM);
+    if (i == 1) {
+#pragma unroll 1
+      for (int b = 0; b < D / 32; ++b) {
+        uint32_t o[32];
+        ptx::tmem_ld32(lane_base + o_col + 32 * b, o);
+        ptx::tmem_wait_ld();
+        ptx::reg_fence(o);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          hand[(8 * b + k) * kBM] =
+              make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                          __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+      }
+      *hand_ml = make_float2(m, l);
+    }
+    ptx::named_bar_sync(2, 2 * kBM);
+    if (i == 1) return;
+    const float2 ml = *hand_ml;
+    const float now = fmaxf(m, ml.x), base = now == -INFINITY ? 0.f : now;
+    const float mine = ptx::ex2_approx(m - base);
+    other = ptx::ex2_approx(ml.x - base) * f;
+    f *= mine;
+    l = l * mine + ml.y * ptx::ex2_approx(ml.x - base);
+    m = now;
+  }
+  if (!ok) return;
+  if (p.parts == 1 && u.steps > 0) {
+    const float n = m == -INFINITY && l == l ? 0.f : 1.f / l;
+    f *= n;
+    other *= n;
   }
   TQ* out = static_cast<TQ*>(p.out) + (u.rq.start + tok) * p.o_token + head * p.o_head;
+  const long long slots = gridDim.x, slot = blockIdx.x;
+  float* o_part = TilePart<D>::o(p.ws, slot, i * kBM + r);
+  if (p.parts > 1 && live)
+    *TilePart<D>::ml(p.ws, slots, slot, i * kBM + r) = make_float2(m, u.steps > 0 ? l : 0.f);
 #pragma unroll 1
-  for (int c = 0; c < D / 32; ++c) {
+  for (int b = 0; b < D / 32; ++b) {
     uint32_t o[32];
     if (u.steps > 0) {
-      ptx::tmem_ld32(lane_base + o_col + 32 * c, o);
+      ptx::tmem_ld32(lane_base + o_col + 32 * b, o);
       ptx::tmem_wait_ld();
       ptx::reg_fence(o);
     } else {
 #pragma unroll
       for (int e = 0; e < 32; ++e) o[e] = 0u;
     }
-    if (live) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t y[4];
+    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+    if (u.dual) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          y[e] = pack2<TQ>(__uint_as_float(o[8 * k + 2 * e]) * f,
-                           __uint_as_float(o[8 * k + 2 * e + 1]) * f);
-        *reinterpret_cast<uint4*>(out + 32 * c + 8 * k) = make_uint4(y[0], y[1], y[2], y[3]);
+      for (int k = 0; k < 8; ++k) {
+        const float4 y = hand[(8 * b + k) * kBM];
+        o[4 * k] = __float_as_uint(fmaf(y.x, other, __uint_as_float(o[4 * k])));
+        o[4 * k + 1] = __float_as_uint(fmaf(y.y, other, __uint_as_float(o[4 * k + 1])));
+        o[4 * k + 2] = __float_as_uint(fmaf(y.z, other, __uint_as_float(o[4 * k + 2])));
+        o[4 * k + 3] = __float_as_uint(fmaf(y.w, other, __uint_as_float(o[4 * k + 3])));
       }
     }
+    if (!live) continue;
+    if (p.parts > 1) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        *reinterpret_cast<float4*>(o_part + 32 * b + 4 * k) = make_float4(
+            __uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+            __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+      continue;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[e] = pack2<TQ>(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
+      *reinterpret_cast<uint4*>(out + 32 * b + 8 * k) = make_uint4(y[0], y[1], y[2], y[3]);
+    }
   }
+}
+
+// Joins the parts of unit blockIdx.x, rows 16 blockIdx.y .. + 15: a warp a row.
+template <typename TQ, int D>
+__global__ void __launch_bounds__(kThreads) join_kernel(const TiledParams p) {
+  __shared__ __align__(16) uint8_t scratch[12 * kThreads];
+  Unit u;
+  const bool there = find_unit(p, blockIdx.x, u, scratch);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!there) return;
+  const int lane = threadIdx.x & 31, r = 16 * blockIdx.y + (threadIdx.x >> 5);
+  const int row = u.row0 + r;
+  if (row >= u.rows_in) return;
+  const long long slots = static_cast<long long>(gridDim.x) * p.parts;
+  constexpr int kPer = D / 32;
+  float top = -INFINITY, sum = 0.f, x[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) x[e] = 0.f;
+#pragma unroll 4
+  for (int part = 0; part < p.parts; ++part) {
+    const long long slot = static_cast<long long>(u.index) * p.parts + part;
+    const float2 ml = *TilePart<D>::ml(p.ws, slots, slot, r);
+    const float* o = TilePart<D>::o(p.ws, slot, r) + lane * kPer;
+    float y[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) y[e] = o[e];
+    const float now = fmaxf(top, ml.x), base = now == -INFINITY ? 0.f : now;
+    const float a = ptx::ex2_approx(top - base), b = ptx::ex2_approx(ml.x - base);
+    top = now;
+    sum = sum * a + ml.y * b;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = x[e] * a + y[e] * b;
+  }
+  const float n = top == -INFINITY && sum == sum ? 0.f : 1.f / sum;
+  const int tok = row / p.group;
+  TQ* out = static_cast<TQ*>(p.out) + (u.rq.start + tok) * p.o_token +
+            (u.kvh * p.group + row - tok * p.group) * p.o_head + lane * kPer;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2)
+    *reinterpret_cast<uint32_t*>(out + e) = pack2<TQ>(x[e] * n, x[e + 1] * n);
 }
 
 template <typename TQ, int CODE, int D>
@@ -720,7 +892,9 @@ tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
   uint8_t* sgen = smem_raw + (sbase - raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Unit u;
-  if (!find_unit(p, u, sgen)) return;
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (!find_unit(p, blockIdx.x / p.parts, u, sgen)) return;
+  if (p.parts > 1) take_part(u, blockIdx.x % p.parts, p.parts);
 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + T::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + T::kOffMisc + 4);
@@ -729,7 +903,7 @@ tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     for (int s = 0; s < T::kSlots; ++s) {
       ptx::mbar_init(bar(Bar<D>::kFull + s), 4);
       ptx::mbar_init(bar(Bar<D>::kEmpty + s),
-                     T::kOwnP && u.rows_in - u.row0 > kBM ? 2 : 1);  // issuers
+                     T::kOwnP && u.rows_in - u.row0 > kBM ? 2 : 1);  // issuers that read it
     }
     for (int s = 0; s < T::kStages; ++s) {
       ptx::mbar_init(bar(Bar<D>::kCodesFull + s), 8 + 1);
@@ -782,7 +956,7 @@ tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 }
 
 template <typename TQ, int CODE, int D>
-int launch(const TiledParams& p, cudaStream_t st) {
+int launch(const TiledParams& p, long long units, cudaStream_t st) {
   auto kern = tiled_kernel<TQ, CODE, D>;
   CUtensorMap map_k, map_v;
   if (const int e = codes_map(&map_k, p.kc, p, D)) return e;
@@ -797,35 +971,81 @@ int launch(const TiledParams& p, cudaStream_t st) {
       return ATTN_ERR_RESOURCE;
     if (dev < 64) set_up[dev].store(true, std::memory_order_release);
   }
-  // Each request's rows end in at most one tile that is not full.
-  const long long units =
-      p.kv_heads * (static_cast<long long>(p.tokens) * p.group / kUnit + p.batch);
-  if (units > INT_MAX) return ATTN_ERR_INVALID_ARG;
-  kern<<<static_cast<unsigned>(units), kThreads, Tile<D>::kSmem, st>>>(map_k, map_v, p);
-  return cudaGetLastError() == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
+  kern<<<static_cast<unsigned>(units * p.parts), kThreads, Tile<D>::kSmem, st>>>(map_k, map_v, p);
+  if (cudaGetLastError() != cudaSuccess) return ATTN_ERR_CUDA;
+  if (p.parts == 1) return ATTN_OK;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units), kUnit / 16);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<TQ, D>, p) == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
 }
 
 template <typename TQ, int CODE>
-int launch_d(const TiledParams& p, int D, cudaStream_t st) {
-  return D == 64 ? launch<TQ, CODE, 64>(p, st) : launch<TQ, CODE, 128>(p, st);
+int launch_d(const TiledParams& p, int D, long long units, cudaStream_t st) {
+  return D == 64 ? launch<TQ, CODE, 64>(p, units, st) : launch<TQ, CODE, 128>(p, units, st);
 }
 
 template <typename TQ>
-int launch_code(const TiledParams& p, int D, int code, cudaStream_t st) {
-  return code == ATTN_CODE_E4M3 ? launch_d<TQ, ATTN_CODE_E4M3>(p, D, st)
-                                : launch_d<TQ, ATTN_CODE_INT8>(p, D, st);
+int launch_code(const TiledParams& p, int D, int code, long long units, cudaStream_t st) {
+  return code == ATTN_CODE_E4M3 ? launch_d<TQ, ATTN_CODE_E4M3>(p, D, units, st)
+                                : launch_d<TQ, ATTN_CODE_INT8>(p, D, units, st);
+}
+
+// Steps that a range of keys has at least, where the table allows for more.
+constexpr int kLeastSteps = 8;
+
+size_t part_bytes(int D) { return sizeof(float) * kUnit * (D + 2); }
+
+int sm_count(int* sms) {
+  static std::atomic<int> known[64];  // per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return ATTN_ERR_CUDA;
+  int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return ATTN_ERR_CUDA;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  *sms = n;
+  return ATTN_OK;
 }
 
 }  // namespace
 
-int launch_tiled(const CachedParams& q, int D, int dtype, int code, cudaStream_t st) {
+int launch_tiled(const CachedParams& q, int D, int dtype, int code, void* ws,
+                 unsigned long long ws_bytes, cudaStream_t st) {
   TiledParams p;
   static_cast<CachedParams&>(p) = q;
   p.status = device_status_ptr();
   if (p.status == nullptr) return ATTN_ERR_CUDA;
   p.timeout_ns = current_timeout_ns();
-  return dtype == ATTN_DTYPE_F16 ? launch_code<__half>(p, D, code, st)
-                                 : launch_code<__nv_bfloat16>(p, D, code, st);
+  // Each request's rows end in at most one unit that is not full.
+  const long long rows = static_cast<long long>(p.tokens) * p.group;
+  const long long units =
+      p.kv_heads * (p.batch == 1 ? (rows + kUnit - 1) / kUnit : rows / kUnit + p.batch);
+  if (units > INT_MAX) return ATTN_ERR_INVALID_ARG;
+  // Fewer units than SMs: their keys are cut so that every SM has some, but
+  // into no more ranges than leave each kLeastSteps steps.
+  int sms = 0;
+  if (const int e = sm_count(&sms)) return e;
+  const int most = (p.capacity + kLeastSteps * kBN - 1) / (kLeastSteps * kBN);
+  p.parts = static_cast<int>(units > 0 && units < sms ? sms / units : 1);
+  if (p.parts > most) p.parts = most > 1 ? most : 1;
+  if (p.parts > 1 && ws_bytes < part_bytes(D) * units * p.parts) return ATTN_ERR_WORKSPACE;
+  p.ws = static_cast<float*>(ws);
+  return dtype == ATTN_DTYPE_F16 ? launch_code<__half>(p, D, code, units, st)
+                                 : launch_code<__nv_bfloat16>(p, D, code, units, st);
+}
+
+int tiled_workspace(int D, unsigned long long* bytes) {
+  int sms = 0;
+  if (const int e = sm_count(&sms)) return e;
+  *bytes = part_bytes(D) * sms;
+  return ATTN_OK;
 }
 
 }  // namespace cache
