@@ -59,6 +59,9 @@ struct Tile {
   static constexpr int kCodes = kBN * D;            // one tile in 8 bits
   static constexpr int kGroup = 16 * D;             // 16 keys of it
   static constexpr int kStages = D == 128 ? 2 : 4;  // of the ring of tiles in 8 bits
+  // Units of 128 rows read each key for fewer rows, and more often from HBM: at
+  // D = 128 the second Q tile's place, which they do not need, makes two more.
+  static constexpr int kDualStages = 4;
   // Tensor memory columns.
   static constexpr bool kOwnP = D == 64;            // P beside S, not over it
   static constexpr int kTile = kOwnP ? kBN + kBN / 2 : kBN;  // S (and P) of a tile
@@ -68,12 +71,17 @@ struct Tile {
   static constexpr int kOffKv = 2 * kBytes;
   static constexpr int kOffCodes = kOffKv + kSlots * kBytes;
   static constexpr int kOffScale = kOffCodes + kStages * kCodes;    // [kScaleRing][12] of K
-  static constexpr int kOffVScale = kOffScale + kScaleRing * 12 * 4;  // [kStages][8]
-  static constexpr int kOffBar = kOffVScale + kStages * 8 * 4;
-  static constexpr int kBars = 2 * kSlots + 2 * kStages + 2 + 2 + 2 + 4 + 2 + 2 + 2;
+  static constexpr int kOffVScale = kOffScale + kScaleRing * 12 * 4;  // [kDualStages][8]
+  static constexpr int kOffBar = kOffVScale + kDualStages * 8 * 4;
+  static constexpr int kBars = 2 * kSlots + 2 * kDualStages + 2 + 2 + 2 + 4 + 2 + 2 + 2;
   static constexpr int kOffMisc = kOffBar + 8 * kBars;
   static constexpr int kSmem = kOffMisc + 32 + 1024;                // + alignment
   static_assert(kSmem <= 232448, "shared memory");
+  static_assert(kStages == kDualStages || 2 * kCodes == kBytes, "two more in a Q tile's place");
+  // Where stage s lies.
+  static __device__ __forceinline__ uint32_t codes_at(int s) {
+    return s < kStages ? kOffCodes + s * kCodes : kBytes + (s - kStages) * kCodes;
+  }
 };
 
 // Barriers.
@@ -82,8 +90,8 @@ struct Bar {
   static constexpr int kFull = 0;
   static constexpr int kEmpty = Tile<D>::kSlots;
   static constexpr int kCodesFull = 2 * Tile<D>::kSlots;
-  static constexpr int kCodesEmpty = kCodesFull + Tile<D>::kStages;
-  static constexpr int kQ = kCodesEmpty + Tile<D>::kStages;
+  static constexpr int kCodesEmpty = kCodesFull + Tile<D>::kDualStages;
+  static constexpr int kQ = kCodesEmpty + Tile<D>::kDualStages;
   static constexpr int kS = kQ + 2;
   static constexpr int kSRead = kS + 2;   // S is in registers (kOwnP)
   static constexpr int kP = kSRead + 2;   // [tile][part]
@@ -236,10 +244,11 @@ __device__ void fetch_role(const CUtensorMap* map_k, const CUtensorMap* map_v,
     }
     return -1;
   };
+  const int stages = u.dual ? T::kDualStages : T::kStages, shift = stages == 4 ? 2 : 1;
   int sent = 0;
   auto fetch = [&](bool is_v, int j, int id) {
-    const int stage = sent % T::kStages;
-    if (!__all_sync(~0u, wait_bar(bar(Bar<D>::kCodesEmpty + stage), ((sent / T::kStages) & 1) ^ 1, w,
+    const int stage = sent & (stages - 1);
+    if (!__all_sync(~0u, wait_bar(bar(Bar<D>::kCodesEmpty + stage), ((sent >> shift) & 1) ^ 1, w,
                                   kSiteKvEmpty)))
       return false;
     const uint32_t full = bar(Bar<D>::kCodesFull + stage);
@@ -260,7 +269,7 @@ __device__ void fetch_role(const CUtensorMap* map_k, const CUtensorMap* map_v,
     if (id >= 0) {
       const int off = ((u.step0 + j) * kBN + 16 * lane) & ((1 << p.shift) - 1);
       const int piece = id * p.kv_heads + u.kvh;
-      ptx::tma_load_3d(sbase + T::kOffCodes + stage * T::kCodes + lane * T::kGroup,
+      ptx::tma_load_3d(sbase + T::codes_at(stage) + lane * T::kGroup,
                        is_v ? map_v : map_k, full, 0, D == 128 ? off : off / 2, piece);
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scale_at),
                    "l"((is_v ? p.vs : p.ks) + piece)
@@ -283,9 +292,9 @@ __device__ void fetch_role(const CUtensorMap* map_k, const CUtensorMap* map_v,
   // After a wait that ran out: copies on their way end before the shared
   // memory that they go to does.
   if (*w.abort) {
-    for (int i = max(0, sent - T::kStages); i < sent; ++i) {
+    for (int i = max(0, sent - stages); i < sent; ++i) {
       const unsigned long long t0 = ptx::globaltimer_ns();
-      while (!ptx::mbar_try_wait(bar(Bar<D>::kCodesFull + i % T::kStages), (i / T::kStages) & 1) &&
+      while (!ptx::mbar_try_wait(bar(Bar<D>::kCodesFull + (i & (stages - 1))), (i >> shift) & 1) &&
              ptx::globaltimer_ns() - t0 < p.timeout_ns) {
       }
     }
@@ -332,24 +341,25 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
   constexpr int kRowStep = D == 128 ? 16 : 32;   // rows from one piece to the next
   const int line = D == 128 ? row0 : row0 >> 1;  // 128-byte line of codes
   const int at8 = D == 128 ? piece : (row0 & 1) * 4 + piece;
-  const uint32_t codes_at = sbase + T::kOffCodes + line * 128 + ((at8 ^ (line & 7)) << 4);
+  const uint32_t codes_at = sbase + line * 128 + ((at8 ^ (line & 7)) << 4);
   const int k16 = (2 * piece) & 7;
   const uint32_t tile_at = sbase + T::kOffKv + (piece >> 2) * T::kBlock + row0 * 128;
   const uint32_t at_lo = (k16 ^ (row0 & 7)) << 4, at_hi = ((k16 + 1) ^ (row0 & 7)) << 4;
   auto group_of = [&](int it) { return D == 128 ? it : 2 * it + (warp >> 1); };
 
+  const int stages = u.dual ? T::kDualStages : T::kStages, shift = stages == 4 ? 2 : 1;
   for (int t = 0; t < 2 * u.steps; ++t) {
     const bool is_v = (t & 1) != 0;
     const int j = t >> 1;
-    const int stage = t % T::kStages, slot = t % T::kSlots;
-    bool ok = wait_bar(bar(Bar<D>::kCodesFull + stage), (t / T::kStages) & 1, w, kSiteKvFull);
+    const int stage = t & (stages - 1), slot = t % T::kSlots;
+    bool ok = wait_bar(bar(Bar<D>::kCodesFull + stage), (t >> shift) & 1, w, kSiteKvFull);
     if (!__all_sync(~0u, ok)) return;
     uint32_t c[kIters][4];
 #pragma unroll
     for (int it = 0; it < kIters; ++it)
       asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(c[it][0]), "=r"(c[it][1]), "=r"(c[it][2]), "=r"(c[it][3])
-                   : "r"(codes_at + stage * T::kCodes + it * kRowStep * D)
+                   : "r"(codes_at + T::codes_at(stage) + it * kRowStep * D)
                    : "memory");
     float vs[kIters];
     if (is_v) {
@@ -434,7 +444,7 @@ __device__ void mma_role(const Unit& u, int me, uint32_t tmem, uint32_t sbase, c
   const uint32_t q_lo = (sbase >> 4) | (1u << 16);
   const uint32_t kv_lo = (sbase + T::kOffKv) >> 4;
   auto issue_s = [&](int i, int t) {
-    const uint32_t q = q_lo + i * (T::kBytes >> 4);
+    const uint32_t q = q_lo + (u.dual ? 0 : i) * (T::kBytes >> 4);
     const uint32_t k = kv_lo + (t % T::kSlots) * (T::kBytes >> 4) + (1u << 16);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
@@ -462,7 +472,7 @@ __device__ void mma_role(const Unit& u, int me, uint32_t tmem, uint32_t sbase, c
   const int i0 = T::kOwnP ? me : 0, i1 = T::kOwnP ? min(me + 1, tiles) : tiles;
   bool ok = true;
   auto first_s = [&](int i, int t) {
-    ok = ring_wait(t) && wait_bar(bar(Bar<D>::kQ + i), 0, w, kSiteQ);
+    ok = ring_wait(t) && wait_bar(bar(Bar<D>::kQ + (u.dual ? 0 : i)), 0, w, kSiteQ);
     if (!ok) return;
     ptx::tc_fence_after();
     issue_s(i, t);
@@ -567,10 +577,11 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
   const int tok = live ? row / p.group : 0;
   const int head = u.kvh * p.group + (live ? row - tok * p.group : 0);
   // (rows behind the last one: zeros that see everything, so that they mask nothing)
-  const int limit = live ? row_limit(p, u.rq, row) : INT_MAX;
+  const int limit =
+      (live ? min(row_limit(p, u.rq, row), u.kv_end) : u.kv_end) - u.step0 * kBN;
   const bool tile_there = u.dual || u.row0 + i * kBM < u.rows_in;
 
-  // Q: this row to shared memory, in f16.
+  // Q: this row to shared memory, in f16 (two tiles of the same rows share it).
   float row_f = 1.f;
   if (tile_there && u.steps > 0) {
     const TQ* q = static_cast<const TQ*>(p.q) + (u.rq.start + tok) * p.q_token + head * p.q_head;
@@ -588,22 +599,24 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
       const int e = static_cast<int>(top >> 7) - 127;
       if (top > 0 && e < 128) row_f = power_of_two(min(max(e - 14, -112), 112));
     }
-    const float inv = 1.f / row_f;
-    const uint32_t base = sbase + i * T::kBytes + r * 128;
+    if (!u.dual || i == 0) {
+      const float inv = 1.f / row_f;
+      const uint32_t base = sbase + i * T::kBytes + r * 128;
 #pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
-      if constexpr (std::is_same<TQ, __nv_bfloat16>::value) {
-        uint32_t* y = reinterpret_cast<uint32_t*>(&x);
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
+        if constexpr (std::is_same<TQ, __nv_bfloat16>::value) {
+          uint32_t* y = reinterpret_cast<uint32_t*>(&x);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          y[k] = half2_of(__uint_as_float(y[k] << 16) * inv,
-                          __uint_as_float(y[k] & 0xffff0000u) * inv);
+          for (int k = 0; k < 4; ++k)
+            y[k] = half2_of(__uint_as_float(y[k] << 16) * inv,
+                            __uint_as_float(y[k] & 0xffff0000u) * inv);
+        }
+        st_shared_v4(base + (c >> 3) * T::kBlock + (((c & 7) ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
       }
-      st_shared_v4(base + (c >> 3) * T::kBlock + (((c & 7) ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive(bar(Bar<D>::kQ + i));
     }
-    ptx::fence_proxy_async_smem();
-    ptx::mbar_arrive(bar(Bar<D>::kQ + i));
   }
 
   const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * wi) << 16);
@@ -622,7 +635,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
 #pragma unroll
     for (int b = 0; b < kBN / 32; ++b)
       ptx::tmem_ld32(lane_base + s_col + 32 * b, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * b]));
-    const int lim = min(limit, u.kv_end) - (u.step0 + j) * kBN;  // columns below it are seen
+    const int lim = limit - j * kBN;  // columns below it are seen
     // Factors of the groups' scores, and the groups whose block is none.
     float factor[kBN / 16];
     uint32_t holes;
@@ -905,7 +918,7 @@ tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
       ptx::mbar_init(bar(Bar<D>::kEmpty + s),
                      T::kOwnP && u.rows_in - u.row0 > kBM ? 2 : 1);  // issuers that read it
     }
-    for (int s = 0; s < T::kStages; ++s) {
+    for (int s = 0; s < T::kDualStages; ++s) {
       ptx::mbar_init(bar(Bar<D>::kCodesFull + s), 8 + 1);
       ptx::mbar_init(bar(Bar<D>::kCodesEmpty + s), 4);
     }
