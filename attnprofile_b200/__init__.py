@@ -21,7 +21,7 @@ __all__ = [
     "shard_range", "set_split", "set_schedule", "plan_split", "plan_schedule", "query_split",
     "set_correction",
     "PagedCache", "BlockPool", "BlockPlan", "CacheBatch", "block_tables", "block_trim",
-    "cache_append", "attn_cached",
+    "cache_append", "attn_cached", "cached_workspace",
 ]
 
 ERR = {
@@ -88,7 +88,7 @@ def lib() -> ctypes.CDLL:
         # Arguments of the cache's entry points: one packed struct each.
         for name in ("attn_block_tables", "attn_block_trim", "attn_cache_append", "attn_cached"):
             getattr(L, name).argtypes = [ctypes.c_char_p, vp]
-        L.attn_cached_workspace.argtypes = [i, i, i, i, u64p]
+        L.attn_cached_workspace.argtypes = [i, i, i, i, i, i, u64p]
         for name in ("attn_fwd", "attn_fwd_padded", "attn_fwd_profiled", "attn_fwd_sharded",
                      "attn_shard_range", "attn_get_status", "attn_query_config",
                      "attn_profile_layout", "attn_debug_fault", "attn_version",
@@ -295,7 +295,7 @@ def shard_range(units: int, n_dev: int, g: int) -> tuple[int, int]:
 
 
 _CACHE_NAMES = ("PagedCache", "BlockPool", "BlockPlan", "CacheBatch", "block_tables", "block_trim",
-                "cache_append", "attn_cached")
+                "cache_append", "attn_cached", "cached_workspace")
 
 
 def __getattr__(name):

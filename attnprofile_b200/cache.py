@@ -21,7 +21,7 @@ import torch
 from . import _check, lib
 
 __all__ = ["PagedCache", "BlockPool", "BlockPlan", "CacheBatch", "block_tables", "block_trim",
-           "cache_append", "attn_cached", "BLOCK_SIZES", "BLOCKS", "MAX_BATCH"]
+           "cache_append", "attn_cached", "cached_workspace", "BLOCK_SIZES", "BLOCKS", "MAX_BATCH"]
 
 BLOCK_SIZES = (16, 32, 64, 128)
 #: Values of the status word that block_tables and block_trim write.
@@ -283,14 +283,24 @@ def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
         cache.block_size), _stream(device, stream))
 
 
-def _workspace(device, heads, kv_heads, dim, max_new) -> int:
-    key = (device.index, heads, kv_heads, dim, max_new)
+def _workspace(device, heads, kv_heads, dim, max_new, block_size, width) -> int:
+    key = (device.index, heads, kv_heads, dim, max_new, block_size, width)
     n = _workspace_bytes.get(key)
     if n is None:
+        if len(_workspace_bytes) > 4096:
+            _workspace_bytes.clear()
         out = ctypes.c_ulonglong()
-        _call("attn_cached_workspace", device, heads, kv_heads, dim, max_new, ctypes.byref(out))
+        _call("attn_cached_workspace", device, heads, kv_heads, dim, max_new, block_size, width,
+              ctypes.byref(out))
         n = _workspace_bytes[key] = out.value
     return n
+
+
+def cached_workspace(cache: PagedCache, heads: int, max_new: int, width: int) -> int:
+    """Bytes of workspace that attn_cached needs with `heads` query heads and
+    tables of `width` entries, whatever the lengths (0: none)."""
+    return _workspace(cache.device, heads, cache.kv_heads, cache.dim, max_new, cache.block_size,
+                      width)
 
 
 def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
@@ -305,8 +315,9 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     or all of them; a row that sees none becomes 0.  max_new: the most rows of
     any request.  scale: of the scores, 1 / sqrt(D) by default.  Rows of `out`
     behind starts[-1] are left as they were (with out=None: undefined).
-    workspace: a uint8 tensor to use instead of a new one per call; calls that
-    may overlap on the GPU need one each."""
+    workspace: a uint8 tensor to use instead of a new one per call, of
+    cached_workspace(...) bytes; calls that may overlap on the GPU need one
+    each."""
     device, kv_heads, dim = cache.device, cache.kv_heads, cache.dim
     kind, shape, (q_token, q_head, _) = _rows("q", q, device, 0, dim)
     tokens, heads, _ = shape
@@ -331,8 +342,9 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
         if o_kind != kind or o_shape != shape:
             raise ValueError("out must have the shape and dtype of q")
     if workspace is None:
-        need = _workspace(device, heads, kv_heads, dim, max_new)
-        workspace = _empty(need, torch.uint8, device, stream)
+        need = _workspace(device, heads, kv_heads, dim, max_new, cache.block_size, width)
+        if need:
+            workspace = _empty(need, torch.uint8, device, stream)
     else:
         if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
             raise TypeError("workspace must be a contiguous uint8 tensor")
@@ -340,8 +352,8 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
             raise ValueError(f"workspace must be on {device}")
         need = workspace.numel()
     _call("attn_cached", device, _CACHED(
-        q.data_ptr(), out.data_ptr(), *cache.ptrs, t, lens_ptr, starts_ptr, workspace.data_ptr(),
-        need, q_token, q_head, o_token, o_head, stride, tokens, heads, kv_heads, dim, kind,
+        q.data_ptr(), out.data_ptr(), *cache.ptrs, t, lens_ptr, starts_ptr,
+        workspace.data_ptr() if need else 0, need, q_token, q_head, o_token, o_head, stride, tokens, heads, kv_heads, dim, kind,
         cache.code, cache.num_blocks, cache.block_size, width, batch, max_new,
         1 if causal else 0, scale), s)
     return out

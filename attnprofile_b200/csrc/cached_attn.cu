@@ -6,6 +6,11 @@
 using namespace attnprof::cache;
 
 namespace {
+int capacity_of(int width, int block_size) {
+  const long long n = static_cast<long long>(width) * block_size;
+  return n > INT_MAX - 4096 ? INT_MAX - 4096 : static_cast<int>(n);
+}
+
 // Rows of one request and kv head up to which the split kernel is used, above
 // it the tiled one.  Measured in graphs, both ways (8 kv heads, e4m3; split |
 // tiled, us): D = 64, 32 rows: 8 requests of 4000 tokens 32 | 41, 2 of 30,000
@@ -26,7 +31,7 @@ extern "C" int attn_cached(const attn_cached_args* args, void* stream) {
     return ATTN_ERR_INVALID_ARG;
   if (a.tokens == 0 || a.batch == 0 || a.max_new == 0) return ATTN_OK;
   if (!a.q || !a.out || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.kv_lens ||
-      !a.starts || !a.workspace || (a.width > 0 && !a.tables))
+      !a.starts || (a.width > 0 && !a.tables))
     return ATTN_ERR_INVALID_ARG;
   if (!aligned(a.q, 16) || !aligned(a.out, 16) || !aligned(a.k_codes, 16) ||
       !aligned(a.v_codes, 16) || !aligned(a.workspace, 16) ||
@@ -57,8 +62,7 @@ extern "C" int attn_cached(const attn_cached_args* args, void* stream) {
   p.batch = a.batch;
   p.num_blocks = a.num_blocks;
   p.shift = shift_of(a.block_size);
-  const long long capacity = static_cast<long long>(a.width) * a.block_size;
-  p.capacity = capacity > INT_MAX - 4096 ? INT_MAX - 4096 : static_cast<int>(capacity);
+  p.capacity = capacity_of(a.width, a.block_size);
   p.causal = a.causal != 0;
   p.scale_log2 = static_cast<float>(
       (a.scale > 0.f ? static_cast<double>(a.scale) : 1.0 / std::sqrt(static_cast<double>(a.D))) *
@@ -78,16 +82,17 @@ extern "C" int attn_cached(const attn_cached_args* args, void* stream) {
   return launch_split(p, a.D, a.dtype, a.code, a.max_new, a.workspace, a.workspace_bytes, st);
 }
 
-extern "C" int attn_cached_workspace(int heads, int kv_heads, int D, int max_new,
-                                     unsigned long long* bytes) {
-  if (!bytes || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || max_new < 0)
+extern "C" int attn_cached_workspace(int heads, int kv_heads, int D, int max_new, int block_size,
+                                     int width, unsigned long long* bytes) {
+  if (!bytes || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || max_new < 0 || width < 0)
     return ATTN_ERR_INVALID_ARG;
-  if (D != 64 && D != 128) return ATTN_ERR_UNSUPPORTED;
-  const int group = heads / kv_heads;
-  int rc = split_workspace(group, D, max_new > 0 ? max_new : 1, bytes);
-  if (rc == ATTN_OK && static_cast<long long>(max_new) * group > split_rows(D)) {
+  if ((D != 64 && D != 128) || !block_size_ok(block_size)) return ATTN_ERR_UNSUPPORTED;
+  const int group = heads / kv_heads, capacity = capacity_of(width, block_size);
+  const int rows = max_new > 0 ? max_new : 1;
+  int rc = split_workspace(group, D, rows, capacity, bytes);
+  if (rc == ATTN_OK && static_cast<long long>(rows) * group > split_rows(D)) {
     unsigned long long tiled = 0;
-    rc = tiled_workspace(D, &tiled);
+    rc = tiled_workspace(D, capacity, &tiled);
     if (rc == ATTN_OK && tiled > *bytes) *bytes = tiled;
   }
   return rc;

@@ -41,8 +41,8 @@ int launch_split(const CachedParams& p, int D, int dtype, int code, int max_new,
                  unsigned long long ws_bytes, cudaStream_t st);
 int launch_tiled(const CachedParams& p, int D, int dtype, int code, void* ws,
                  unsigned long long ws_bytes, cudaStream_t st);
-int tiled_workspace(int D, unsigned long long* bytes);
-int split_workspace(int group, int D, int max_new, unsigned long long* bytes);
+int tiled_workspace(int D, int capacity, unsigned long long* bytes);
+int split_workspace(int group, int D, int max_new, int capacity, unsigned long long* bytes);
 
 }  // namespace cache
 }  // namespace attnprof

@@ -1063,11 +1063,12 @@ int launch(const CachedParams& cp, int max_new, void* ws, unsigned long long ws_
   const long long rows = static_cast<long long>(p.group) * max_new;
   const double units = static_cast<double>(p.batch) * p.kv_heads * ((rows + 8 * NT - 1) / (8 * NT));
   const int chunks = p.capacity <= kChunk ? 1 : (p.capacity + kChunk - 1) / kChunk;
-  p.whole = chunks <= kWholeChunks;
+  p.whole = p.capacity <= kWholeChunks * kChunk;
   // No more ranges than there can be chunks.
   const double most = units * (p.whole ? 1 : chunks);
   if (most < ctas) ctas = static_cast<int>(most);
-  if (ws_bytes < part_bytes(D, NT) * ctas) return ATTN_ERR_WORKSPACE;
+  if (!p.whole && (ws == nullptr || ws_bytes < part_bytes(D, NT) * ctas))
+    return ATTN_ERR_WORKSPACE;
   p.ws = static_cast<float*>(ws);
   split_kernel<T, CODE, D, NT><<<ctas, kThreads, Smem<D, NT>::kBytes, st>>>(map_k, map_v, p);
   if (cudaGetLastError() != cudaSuccess) return ATTN_ERR_CUDA;
@@ -1140,7 +1141,9 @@ int launch_split(const CachedParams& p, int D, int dtype, int code, int max_new,
                                  : launch_code<__nv_bfloat16>(p, D, code, max_new, ws, ws_bytes, st);
 }
 
-int split_workspace(int group, int D, int max_new, unsigned long long* bytes) {
+int split_workspace(int group, int D, int max_new, int capacity, unsigned long long* bytes) {
+  *bytes = 0;
+  if (capacity <= kWholeChunks * kChunk) return ATTN_OK;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)

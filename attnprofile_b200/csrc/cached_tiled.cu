@@ -1013,6 +1013,11 @@ int launch_code(const TiledParams& p, int D, int code, long long units, cudaStre
 // Steps that a range of keys has at least, where the table allows for more.
 constexpr int kLeastSteps = 8;
 
+int most_parts(int capacity) {
+  const int n = (capacity + kLeastSteps * kBN - 1) / (kLeastSteps * kBN);
+  return n > 1 ? n : 1;
+}
+
 size_t part_bytes(int D) { return sizeof(float) * kUnit * (D + 2); }
 
 int sm_count(int* sms) {
@@ -1045,16 +1050,19 @@ int launch_tiled(const CachedParams& q, int D, int dtype, int code, void* ws,
   // into no more ranges than leave each kLeastSteps steps.
   int sms = 0;
   if (const int e = sm_count(&sms)) return e;
-  const int most = (p.capacity + kLeastSteps * kBN - 1) / (kLeastSteps * kBN);
+  const int most = most_parts(p.capacity);
   p.parts = static_cast<int>(units > 0 && units < sms ? sms / units : 1);
-  if (p.parts > most) p.parts = most > 1 ? most : 1;
-  if (p.parts > 1 && ws_bytes < part_bytes(D) * units * p.parts) return ATTN_ERR_WORKSPACE;
+  if (p.parts > most) p.parts = most;
+  if (p.parts > 1 && (ws == nullptr || ws_bytes < part_bytes(D) * units * p.parts))
+    return ATTN_ERR_WORKSPACE;
   p.ws = static_cast<float*>(ws);
   return dtype == ATTN_DTYPE_F16 ? launch_code<__half>(p, D, code, units, st)
                                  : launch_code<__nv_bfloat16>(p, D, code, units, st);
 }
 
-int tiled_workspace(int D, unsigned long long* bytes) {
+int tiled_workspace(int D, int capacity, unsigned long long* bytes) {
+  *bytes = 0;
+  if (most_parts(capacity) == 1) return ATTN_OK;
   int sms = 0;
   if (const int e = sm_count(&sms)) return e;
   *bytes = part_bytes(D) * sms;

@@ -359,8 +359,9 @@ int attn_cache_append(const attn_cache_append_args* args, void* stream);
  * hold no token is never used, whatever it is.  kv_lens is taken as at most
  * width * block_size, starts as within [0, tokens]; a table entry that is no
  * block of the pool is left out.
- * workspace: 16-byte aligned, attn_cached_workspace(...) bytes, needs no
- * initial value; calls that may overlap need one each.  Asynchronous.
+ * workspace: 16-byte aligned, attn_cached_workspace(...) bytes (NULL where
+ * that is 0), needs no initial value; calls that may overlap need one each.
+ * Asynchronous.
  */
 typedef struct {
   const void* q;
@@ -377,8 +378,10 @@ typedef struct {
 } attn_cached_args;
 int attn_cached(const attn_cached_args* args, void* stream);
 
-/* Workspace bytes of attn_cached on the current device, whatever the lengths. */
-int attn_cached_workspace(int heads, int kv_heads, int D, int max_new,
+/* Workspace bytes of attn_cached on the current device for tables of `width`
+ * entries, whatever the lengths and the number of requests: 0 where no request
+ * can be long enough to be cut. */
+int attn_cached_workspace(int heads, int kv_heads, int D, int max_new, int block_size, int width,
                           unsigned long long* bytes);
 
 /* Human-readable text for a return code.  Never NULL. */

@@ -90,7 +90,7 @@ ATTN = dict(q=P, out=P, k_codes=P, v_codes=P, k_scale=P, v_scale=P, tables=P, kv
     ({"q": P + 8}, "MISALIGNED"), ({"out": P + 2}, "MISALIGNED"), ({"q_token": 516}, "MISALIGNED"),
     ({"o_head": 132}, "MISALIGNED"), ({"workspace": P + 4}, "MISALIGNED"),
     *[({k: None}, "INVALID_ARG") for k in ("q", "out", "k_codes", "v_codes", "k_scale", "v_scale",
-                                           "tables", "kv_lens", "starts", "workspace")],
+                                           "tables", "kv_lens", "starts")],
 ])
 def test_attn_cached_refusals(engine, change, code):
     assert call(engine, "attn_cached", cache._CACHED, ATTN, **change) == engine.ERR[code]
@@ -101,12 +101,21 @@ def test_attn_cached_of_nothing(engine, change):
     assert call(engine, "attn_cached", cache._CACHED, ATTN, q=None, **change) == 0
 
 
-@pytest.mark.parametrize("args,code", [((4, 3, 64, 1), "INVALID_ARG"), ((4, 0, 64, 1), "INVALID_ARG"),
-                                       ((4, 2, 80, 1), "UNSUPPORTED"), ((4, 2, 64, -1), "INVALID_ARG")])
+@pytest.mark.parametrize("args,code", [
+    ((4, 3, 64, 1, 16, 9), "INVALID_ARG"), ((4, 0, 64, 1, 16, 9), "INVALID_ARG"),
+    ((4, 2, 80, 1, 16, 9), "UNSUPPORTED"), ((4, 2, 64, -1, 16, 9), "INVALID_ARG"),
+    ((4, 2, 64, 1, 24, 9), "UNSUPPORTED"), ((4, 2, 64, 1, 16, -1), "INVALID_ARG"),
+])
 def test_workspace_refusals(engine, args, code):
     out = ctypes.c_ulonglong()
     assert engine.lib().attn_cached_workspace(*args, ctypes.byref(out)) == engine.ERR[code]
-    assert engine.lib().attn_cached_workspace(4, 2, 64, 1, None) == engine.ERR["INVALID_ARG"]
+    assert engine.lib().attn_cached_workspace(4, 2, 64, 1, 16, 9, None) == engine.ERR["INVALID_ARG"]
+
+
+def test_short_requests_need_no_workspace(engine):
+    out = ctypes.c_ulonglong(7)
+    assert engine.lib().attn_cached_workspace(4, 2, 64, 1, 16, 32, ctypes.byref(out)) == 0
+    assert out.value == 0
 
 
 def test_no_arguments_at_all(engine):
