@@ -40,6 +40,7 @@
 
 namespace attnprof {
 unsigned long long current_timeout_ns();
+int current_fault_mode();
 
 namespace cache {
 namespace {
@@ -299,6 +300,7 @@ struct Smem {
 struct SplitParams : CachedParams {
   int* status;
   unsigned long long timeout_ns;
+  int fault_mode;  // 1: nothing is fetched (test of the bounded waits)
 };
 
 // Named barriers: sums handed from warp h + 1 to warp h, the last reader done,
@@ -844,7 +846,8 @@ split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     compute_role<T, CODE, D, NT>(p, cursor, sbase, smem, w);
   } else {
     ptx::setmaxnreg_dec<40>();
-    if (warp == kWarps) fetch_role<D, NT>(&map_k, &map_v, p, cursor, sbase, w);
+    if (warp == kWarps && p.fault_mode == 0)
+      fetch_role<D, NT>(&map_k, &map_v, p, cursor, sbase, w);
   }
 #endif
 }
@@ -1054,6 +1057,7 @@ int launch(const CachedParams& cp, int max_new, void* ws, unsigned long long ws_
   p.status = device_status_ptr();
   if (p.status == nullptr) return ATTN_ERR_CUDA;
   p.timeout_ns = current_timeout_ns();
+  p.fault_mode = current_fault_mode();
   CUtensorMap map_k, map_v;
   if (const int e = codes_map(&map_k, p.kc, p, D)) return e;
   if (const int e = codes_map(&map_v, p.vc, p, D)) return e;

@@ -39,6 +39,7 @@
 namespace attnprof {
 int* device_status_ptr();
 unsigned long long current_timeout_ns();
+int current_fault_mode();
 
 namespace cache {
 namespace {
@@ -113,6 +114,7 @@ struct Unit {
 struct TiledParams : CachedParams {
   int* status;
   unsigned long long timeout_ns;
+  int fault_mode;  // 1: nothing is fetched (test of the bounded waits)
   int parts;  // CTAs of a unit; above 1 they leave (max, sum, O) in the workspace
 };
 
@@ -956,7 +958,7 @@ tiled_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     ptx::setmaxnreg_dec<64>();
     if ((warp == 12 || (T::kOwnP && warp == 14)) && lane == 0)
       mma_role<D>(u, warp == 12 ? 0 : 1, tmem, sbase, w);
-    if (warp == 13) fetch_role<D>(&map_k, &map_v, p, u, sbase, w);
+    if (warp == 13 && p.fault_mode == 0) fetch_role<D>(&map_k, &map_v, p, u, sbase, w);
     __syncwarp();
   }
   ptx::tc_fence_before();
@@ -1041,6 +1043,7 @@ int launch_tiled(const CachedParams& q, int D, int dtype, int code, void* ws,
   p.status = device_status_ptr();
   if (p.status == nullptr) return ATTN_ERR_CUDA;
   p.timeout_ns = current_timeout_ns();
+  p.fault_mode = current_fault_mode();
   // Each request's rows end in at most one unit that is not full.
   const long long rows = static_cast<long long>(p.tokens) * p.group;
   const long long units =

@@ -104,6 +104,9 @@ int current_split_mode() { return g_split_mode.load(); }
 // The bounded-wait limit that attn_set_timeout_ns last stored.
 unsigned long long current_timeout_ns() { return g_timeout_ns.load(); }
 
+// What attn_debug_fault last stored.
+int current_fault_mode() { return g_fault_mode.load(); }
+
 // Launch with a caller-provided workspace and per-call tensor maps (no
 // device or host allocation, never the stream-ordered pool: a plan that
 // needs more than ws_bytes returns ATTN_ERR_SCRATCH_LIMIT); split_mode as

@@ -361,7 +361,8 @@ int attn_cache_append(const attn_cache_append_args* args, void* stream);
  * block of the pool is left out.
  * workspace: 16-byte aligned, attn_cached_workspace(...) bytes (NULL where
  * that is 0), needs no initial value; calls that may overlap need one each.
- * Asynchronous.
+ * Asynchronous; like attn_fwd's, its waits are bounded (attn_set_timeout_ns)
+ * and one that runs out is reported by attn_get_status.
  */
 typedef struct {
   const void* q;
@@ -392,6 +393,7 @@ const char* attn_error_string(int code);
  * launches' producer warp load Q but never K/V, so every consumer's bounded
  * wait expires and the kernel returns with ATTN_ERR_DEVICE_TIMEOUT in the
  * status word (no fault, no trap, no hang).  mode 0 restores normal runs.
+ * attn_cached likewise fetches no keys and values in mode 1.
  */
 int attn_debug_fault(int mode);
 

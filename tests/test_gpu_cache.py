@@ -367,6 +367,45 @@ def test_attn_cached_long_keys(ap):
     attend_case(ap, torch.bfloat16, INT8, 64, 16, 8, 2, [9000], [2], seed=4)
 
 
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("dim,heads,kv_heads,kv_lens,new", [
+    (128, 4, 2, [5000], [40]), (64, 4, 2, [5000, 700], [40, 33]), (128, 1, 1, [4100], [257]),
+    (64, 3, 1, [3000, 2900], [170, 1]), (128, 8, 1, [2500], [16]), (64, 2, 2, [1030], [129]),
+    (128, 32, 1, [3000, 20], [1, 1]), (64, 71, 1, [2100], [1]),
+])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attn_cached_few_rows_and_many_keys(ap, kind, code, dim, heads, kv_heads, kv_lens, new,
+                                            causal):
+    """More rows than the split kernel takes and fewer units than SMs: the
+    keys of a unit are cut, and units of up to 128 rows use both tiles."""
+    attend_case(ap, kind, code, dim, 16, heads, kv_heads, kv_lens, new, causal, seed=heads)
+
+
+@pytest.mark.parametrize("batch,longest", [(33, 1500), (129, 900), (200, 1500), (700, 300)])
+def test_attn_cached_many_requests(ap, batch, longest):
+    """One token each: more requests than the lanes of a warp hold, than the
+    threads of a CTA, units cut between ranges and short ones whole."""
+    rng = random.Random(batch)
+    kv = [rng.choice([1, rng.randint(1, longest)]) for _ in range(batch)]
+    attend_case(ap, torch.float16, E4M3, 64, 32, 4, 2, kv, [1] * batch, seed=batch)
+
+
+def test_attn_cached_more_prompts_than_threads(ap):
+    rng = random.Random(3)
+    new = [rng.choice([1, 33, 40]) for _ in range(600)]
+    attend_case(ap, torch.bfloat16, INT8, 64, 16, 1, 1, [n + rng.randint(0, 60) for n in new], new,
+                seed=4)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attn_cached_single_tokens_beside_prompts(ap, dim, code):
+    """Both kernels in one call, each on its own requests."""
+    attend_case(ap, torch.float16, code, dim, 32, 6, 2, [1500, 130, 1, 0, 600, 77, 300],
+                [1, 130, 1, 2, 4, 40, 300], seed=12)
+
+
 @pytest.mark.parametrize("new", [[3, 0, 0, 1], [40, 0, 90, 1]])
 def test_attn_cached_rows_without_keys(ap, new):
     """No cache, fewer tokens than rows, requests without rows, padding."""
@@ -470,13 +509,12 @@ def test_attn_cached_marks_only_rows_that_see_a_bad_block(ap, new):
     def bad(q, cache, host, tables):
         cache.k_scale[tables[0][(300 - 1) // 16], 0] = math.nan
         host[2][tables[0][(300 - 1) // 16], 0] = math.nan
-        if new > 1:  # a block that the first rows do not see
-            return
-    out = attend_case(ap, torch.float16, E4M3, 128, 16, 4, 2, [300, 40], [new, 1], seed=7,
-                      prepare=bad) if new == 1 else None
     if new == 1:
+        out = attend_case(ap, torch.float16, E4M3, 128, 16, 4, 2, [300, 40], [new, 1], seed=7,
+                          prepare=bad)
         assert torch.isnan(out[0, :2]).all() and not torch.isnan(out[0, 2:]).any()
         return
+    # a block that the first rows do not see
     cache, host = make_cache(ap, 20, 1, 16, 128, E4M3, 4)
     cache.k_scale[19] = math.nan  # tokens 288 .. 299
     table = ints([[(i + 1) % 20 for i in range(19)]])
@@ -591,6 +629,46 @@ def test_captured_and_replayed_with_other_lengths(ap, new):
         want, tol = ref.attend_ref(q.cpu(), *host, batch.tables.tolist(), lens, starts, True)
         n = sum(add)
         assert torch.all((out[:n].double().cpu() - want[:n]).abs() <= tol[:n])
+
+
+def test_waits_that_run_out_are_reported(ap):
+    """Nothing is fetched: the bounded waits expire, the status word says so,
+    and the next call is right again."""
+    cache, host = make_cache(ap, 30, 1, 16, 64, E4M3, 4)
+    table, lens = ints([list(range(30))]), ints([470])
+    assert ap.get_status(0)[0] == 0
+    for new in (1, 40, 200):  # the split kernel; the tiled one with one and two tiles of rows
+        q = torch.randn(new, 1, 64, device="cuda").half()
+        want = ap.attn_cached(q, cache, table, lens, ints([0, new]), max_new=new)
+        ap.set_timeout_ns(50_000_000)
+        ap.debug_fault(1)
+        try:
+            ap.attn_cached(q, cache, table, lens, ints([0, new]), max_new=new)
+            rc, site = ap.get_status(0, reset=True)
+        finally:
+            ap.debug_fault(0)
+            ap.set_timeout_ns(2_000_000_000)
+        assert rc == ap.ERR["DEVICE_TIMEOUT"] and site != 0
+        got = ap.attn_cached(q, cache, table, lens, ints([0, new]), max_new=new)
+        assert ap.get_status(0)[0] == 0
+        assert torch.equal(got, want)
+
+
+def test_a_workspace_given_and_one_too_small(ap):
+    cache, _ = make_cache(ap, 100, 1, 16, 64, E4M3, 4)
+    table, lens = ints([list(range(100))]), ints([1600])
+    for new in (1, 40):
+        q = torch.randn(new, 1, 64, device="cuda").half()
+        starts = ints([0, new])
+        want = ap.attn_cached(q, cache, table, lens, starts, max_new=new)
+        need = ap.cached_workspace(cache, 1, new, 100)
+        ws = torch.full((need,), 0xff, dtype=torch.uint8, device="cuda")  # any contents
+        got = ap.attn_cached(q, cache, table, lens, starts, max_new=new, workspace=ws)
+        assert torch.equal(got, want)
+        with pytest.raises(ap.AttnError) as e:
+            ap.attn_cached(q, cache, table, lens, starts, max_new=new, workspace=ws[:16])
+        assert e.value.code == ap.ERR["WORKSPACE"]
+    assert ap.cached_workspace(cache, 1, 1, 4) == 0
 
 
 def test_two_graphs_at_once(ap):
