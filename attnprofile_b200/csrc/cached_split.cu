@@ -18,7 +18,7 @@
 // 6.5 TB/s times some 1.2 us on its way, 53 KB an SM; two CTAs' rings hold 192.
 // (Codes read straight into registers by the computing warps: 4.0 TB/s on 64
 // requests of 5 to 8191 tokens; a ring for each warp that ran empty at each
-// unit's end: 4.7; this form: see the table of results.)
+// unit's end: 4.7; this form: 5.9, 91 us, 4.8 of them the joining kernel.)
 // Each computing warp takes 16 or 32 keys of a step.  S^T = K Q^T and O^T =
 // V^T P^T run on m16n8k16 MMAs with the keys (then the head dimension) on the 16
 // side and 8 query rows on the other, so that the 1 to 8 rows of a decode step
