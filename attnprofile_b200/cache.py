@@ -245,7 +245,8 @@ def block_trim(pool: BlockPool, lens, keep, tables, *, lens_left=None, free_left
 
 
 def _rows(name, x, device, heads, dim):
-    """Checks a [tokens, heads, D] tensor; its dtype code, shape and strides."""
+    """Checks a [tokens, heads, D] tensor; its dtype code, shape, and the strides
+    of tokens and heads (0 where there is one only, whose stride means nothing)."""
     kind = _DTYPES.get(x.dtype)
     if kind is None:
         raise TypeError(f"unsupported dtype {x.dtype} of {name} (float16 or bfloat16)")
@@ -257,7 +258,7 @@ def _rows(name, x, device, heads, dim):
     strides = x.stride()
     if strides[2] != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    return kind, shape, strides
+    return kind, shape, strides[0] if shape[0] > 1 else 0, strides[1] if shape[1] > 1 else 0
 
 
 def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
@@ -272,8 +273,8 @@ def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
     and no block appears twice."""
     device = cache.device
     heads, dim = cache.kv_heads, cache.dim
-    kind, shape, (k_token, k_head, _) = _rows("k", k, device, heads, dim)
-    v_kind, v_shape, (v_token, v_head, _) = _rows("v", v, device, heads, dim)
+    kind, shape, k_token, k_head = _rows("k", k, device, heads, dim)
+    v_kind, v_shape, v_token, v_head = _rows("v", v, device, heads, dim)
     if v_kind != kind or v_shape != shape:
         raise ValueError("k and v must share one shape and dtype")
     tokens = shape[0]
@@ -314,12 +315,13 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     already).  Row i of n sees the first kv_lens[r] - n + i + 1 tokens (causal)
     or all of them; a row that sees none becomes 0.  max_new: the most rows of
     any request.  scale: of the scores, 1 / sqrt(D) by default.  Rows of `out`
-    behind starts[-1] are left as they were (with out=None: undefined).
+    behind starts[-1] are left as they were (with out=None: undefined); out
+    must not overlap q.
     workspace: a uint8 tensor to use instead of a new one per call, of
     cached_workspace(...) bytes; calls that may overlap on the GPU need one
     each."""
     device, kv_heads, dim = cache.device, cache.kv_heads, cache.dim
-    kind, shape, (q_token, q_head, _) = _rows("q", q, device, 0, dim)
+    kind, shape, q_token, q_head = _rows("q", q, device, 0, dim)
     tokens, heads, _ = shape
     if heads == 0 or heads % kv_heads:
         raise ValueError(f"{heads} heads are not a multiple of the cache's {kv_heads}")
@@ -338,7 +340,7 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
         out = _empty(shape, q.dtype, device, stream)
         o_token, o_head = heads * dim, dim
     else:
-        o_kind, o_shape, (o_token, o_head, _) = _rows("out", out, device, heads, dim)
+        o_kind, o_shape, o_token, o_head = _rows("out", out, device, heads, dim)
         if o_kind != kind or o_shape != shape:
             raise ValueError("out must have the shape and dtype of q")
     if workspace is None:
@@ -365,34 +367,42 @@ class CacheBatch:
 
     A step is advance() once, then attend() for each layer:
 
-        batch = CacheBatch(BlockPool.full(num_blocks, 32), rows=64, max_len=8192)
+        batch = CacheBatch(BlockPool.full(num_blocks, 32), rows=64, max_len=8192,
+                           max_tokens=4096)
         cache = [PagedCache.empty(num_blocks, 8, 128) for _ in layers]
         batch.advance(new_lens, tokens=q.shape[0])
         for each layer: o = batch.attend(cache[i], q, k, v, max_new=1)
         batch.trim(keep)        # ended requests: 0, refused drafts: fewer
 
     q, k, v hold the new tokens of all requests, request after request;
-    padding may follow the last one.  Nothing waits for the GPU: `status` holds
-    the last advance()'s word (BLOCKS) there.  Where it is not OK the step has
-    no tokens: nothing is appended, and attend() leaves its output alone."""
+    padding may follow the last one.  max_tokens: the most rows of any step.
+    Nothing waits for the GPU: `status` holds the last advance()'s word (BLOCKS)
+    there.  Where it is not OK the step has no tokens: nothing is appended, and
+    attend() leaves its output alone.  All arrays are made here and stay where
+    they are, so steps can be captured into CUDA graphs (after one step outside);
+    the steps of one batch follow each other on the GPU."""
 
-    def __init__(self, pool: BlockPool, rows: int, max_len: int):
+    def __init__(self, pool: BlockPool, rows: int, max_len: int, max_tokens: int):
         device, bs = pool.device, pool.block_size
-        if rows <= 0 or max_len <= 0:
-            raise ValueError("rows and max_len must be positive")
+        if rows <= 0 or max_len <= 0 or max_tokens <= 0:
+            raise ValueError("rows, max_len and max_tokens must be positive")
+        if rows > MAX_BATCH:
+            raise ValueError(f"at most {MAX_BATCH} rows")
         self.pool = pool
         self.lens = torch.zeros(rows, dtype=torch.int32, device=device)
         self.tables = torch.full((rows, -(-max_len // bs)), -1, dtype=torch.int32, device=device)
         self.starts = torch.zeros(rows + 1, dtype=torch.int32, device=device)
+        self.slots = torch.full((max_tokens,), -1, dtype=torch.int32, device=device)
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.trim_status = torch.zeros(1, dtype=torch.int32, device=device)
         self.plan = None
 
     def advance(self, new_lens, tokens: int, *, stream=None) -> BlockPlan:
         """new_lens[r] tokens more for request r, in a slot map of `tokens`."""
+        if not 0 <= tokens <= self.slots.shape[0]:
+            raise ValueError(f"tokens must be at most max_tokens = {self.slots.shape[0]}")
         if self.plan is None or self.plan.slots.shape[0] != tokens:
-            slots = _empty(tokens, torch.int32, self.pool.device, stream)
-            self.plan = BlockPlan(self.lens, self.starts, slots, self.status)
+            self.plan = BlockPlan(self.lens, self.starts, self.slots[:tokens], self.status)
         return block_tables(self.pool, self.lens, new_lens, self.tables, tokens, plan=self.plan,
                             stream=stream)
 

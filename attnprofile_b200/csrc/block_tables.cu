@@ -15,6 +15,8 @@
 // barrier ends the reading, and then all threads of the cluster write.  The
 // barrier makes in-place calls (kv_lens = lens, free_left = free_count) safe
 // without any scratch memory, atomics or order between CTAs.
+#include <initializer_list>
+
 #include "cache.cuh"
 #include "ptx.cuh"
 
@@ -314,6 +316,12 @@ extern "C" int attn_block_tables(const attn_block_tables_args* args, void* strea
   if (a.batch > 0 && (!a.lens || !a.new_lens || !a.kv_lens)) return ATTN_ERR_INVALID_ARG;
   if ((a.batch > 0 && a.width > 0 && !a.tables) || (a.tokens > 0 && !a.slots))
     return ATTN_ERR_INVALID_ARG;
+  for (const void* x : {static_cast<const void*>(a.lens), static_cast<const void*>(a.new_lens),
+                        static_cast<const void*>(a.tables), static_cast<const void*>(a.free_blocks),
+                        static_cast<const void*>(a.free_count), static_cast<const void*>(a.kv_lens),
+                        static_cast<const void*>(a.starts), static_cast<const void*>(a.slots),
+                        static_cast<const void*>(a.free_left), static_cast<const void*>(a.status)})
+    if (!aligned(x, 4)) return ATTN_ERR_MISALIGNED;
   const TablesParams p{a, shift_of(a.block_size)};
   return launch_cluster(tables_kernel, p, ctas_for(a.tokens), 3ull * sizeof(int) * a.batch,
                         static_cast<cudaStream_t>(stream));
@@ -327,6 +335,12 @@ extern "C" int attn_block_trim(const attn_block_trim_args* args, void* stream) {
   if (!a.free_blocks || !a.free_count || !a.free_left || !a.status) return ATTN_ERR_INVALID_ARG;
   if (a.batch > 0 && (!a.lens || !a.keep || !a.lens_left)) return ATTN_ERR_INVALID_ARG;
   if (a.batch > 0 && a.width > 0 && !a.tables) return ATTN_ERR_INVALID_ARG;
+  for (const void* x : {static_cast<const void*>(a.lens), static_cast<const void*>(a.keep),
+                        static_cast<const void*>(a.tables), static_cast<const void*>(a.free_blocks),
+                        static_cast<const void*>(a.free_count),
+                        static_cast<const void*>(a.lens_left),
+                        static_cast<const void*>(a.free_left), static_cast<const void*>(a.status)})
+    if (!aligned(x, 4)) return ATTN_ERR_MISALIGNED;
   const TrimParams p{a, shift_of(a.block_size)};
   const long long most = static_cast<long long>(a.batch) * a.width;
   return launch_cluster(trim_kernel, p, ctas_for(most < a.num_blocks ? most : a.num_blocks),

@@ -314,7 +314,8 @@ extern "C" int attn_cache_append(const attn_cache_append_args* args, void* strea
   if (!a.k || !a.v || !a.slots || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale)
     return ATTN_ERR_INVALID_ARG;
   if (!aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.k_codes, 16) ||
-      !aligned(a.v_codes, 16) ||
+      !aligned(a.v_codes, 16) || !aligned(a.k_scale, 4) || !aligned(a.v_scale, 4) ||
+      !aligned(a.slots, 4) ||
       ((a.k_token_stride | a.k_head_stride | a.v_token_stride | a.v_head_stride) & 7) != 0)
     return ATTN_ERR_MISALIGNED;
   AppendParams p{};

@@ -33,8 +33,14 @@ extern "C" int attn_cached(const attn_cached_args* args, void* stream) {
   if (!a.q || !a.out || !a.k_codes || !a.v_codes || !a.k_scale || !a.v_scale || !a.kv_lens ||
       !a.starts || (a.width > 0 && !a.tables))
     return ATTN_ERR_INVALID_ARG;
+  // Rows that would be written over each other, or read after they were written.
+  if ((a.tokens > 1 && a.out_token_stride == 0) || (a.heads > 1 && a.out_head_stride == 0) ||
+      a.q == a.out)
+    return ATTN_ERR_INVALID_ARG;
   if (!aligned(a.q, 16) || !aligned(a.out, 16) || !aligned(a.k_codes, 16) ||
-      !aligned(a.v_codes, 16) || !aligned(a.workspace, 16) ||
+      !aligned(a.v_codes, 16) || !aligned(a.workspace, 16) || !aligned(a.k_scale, 4) ||
+      !aligned(a.v_scale, 4) || !aligned(a.tables, 4) || !aligned(a.kv_lens, 4) ||
+      !aligned(a.starts, 4) ||
       ((a.q_token_stride | a.q_head_stride | a.out_token_stride | a.out_head_stride) & 7) != 0)
     return ATTN_ERR_MISALIGNED;
   const int group = a.heads / a.kv_heads;
@@ -60,6 +66,7 @@ extern "C" int attn_cached(const attn_cached_args* args, void* stream) {
   p.kv_heads = a.kv_heads;
   p.group = group;
   p.batch = a.batch;
+  p.max_new = a.max_new;
   p.num_blocks = a.num_blocks;
   p.shift = shift_of(a.block_size);
   p.capacity = capacity_of(a.width, a.block_size);

@@ -16,7 +16,8 @@ struct CachedParams {
   const int *tables, *kv_lens, *starts;
   long long q_token, q_head, o_token, o_head, table_stride;
   int tokens, heads, kv_heads, group, batch, num_blocks, shift, capacity, causal;
-  int whole;  // split kernel: no unit is cut
+  int whole;    // split kernel: no unit is cut
+  int max_new;  // rows of a request at most
   float scale_log2;  // score scale * log2(e)
   // Requests of more than `rows_most` query rows a kv head (tokens * group)
   // belong to the other kernel: the split one takes those up to it, the tiled
@@ -33,7 +34,7 @@ struct Request {
 __device__ __forceinline__ Request request_at(const CachedParams& p, int r) {
   const int a = min(max(p.starts[r], 0), p.tokens);
   const int b = min(max(p.starts[r + 1], 0), p.tokens);
-  return Request{a, max(b - a, 0), min(max(p.kv_lens[r], 0), p.capacity)};
+  return Request{a, min(max(b - a, 0), p.max_new), min(max(p.kv_lens[r], 0), p.capacity)};
 }
 
 int codes_map(CUtensorMap* m, const void* codes, const CachedParams& p, int D);

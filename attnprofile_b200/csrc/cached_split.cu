@@ -13,13 +13,13 @@
 //
 // Inside a CTA one warp fetches and four compute.  The fetching warp walks
 // through the CTA's range, over the ends of units, and keeps a ring of steps
-// full: per step 64 or 128 keys' codes of K and V by TMA, 16 keys at a time,
+// full: per step 128 (D = 128) or 256 keys' codes of K and V by TMA, 16 keys at a time,
 // under the 128-byte swizzle, and their blocks' scales by cp.async.  HBM needs
 // 6.5 TB/s times some 1.2 us on its way, 53 KB an SM; two CTAs' rings hold 192.
 // (Codes read straight into registers by the computing warps: 4.0 TB/s on 64
 // requests of 5 to 8191 tokens; a ring for each warp that ran empty at each
 // unit's end: 4.7; this form: 5.9, 91 us, 4.8 of them the joining kernel.)
-// Each computing warp takes 16 or 32 keys of a step.  S^T = K Q^T and O^T =
+// Each computing warp takes 32 or 64 keys of a step.  S^T = K Q^T and O^T =
 // V^T P^T run on m16n8k16 MMAs with the keys (then the head dimension) on the 16
 // side and 8 query rows on the other, so that the 1 to 8 rows of a decode step
 // waste nothing; tcgen05's smallest tile of 64 to 128 rows would be almost
@@ -30,8 +30,9 @@
 // sum of p v in f32, so no scale is rounded.  P is rounded to f16, by at most
 // 2^-11 of itself as an f16 result is (a bf16 result by 2^-8): it is held as
 // 2^7 p (p up to 2^8 between two moves of the maximum), so that also weights down
-// to 2^-21 of the largest keep all their bits.  Maximum, sum and O are f32.  bf16 queries become f16 times a
-// power of two per row, which loses nothing above 2^-38 of the row's largest.
+// to 2^-21 of the largest keep all their bits.  Maximum, sum and O are f32.
+// bf16 queries become f16 times a power of two per row, which loses nothing
+// above 2^-38 of the row's largest.
 #include <atomic>
 #include <climits>
 
@@ -467,7 +468,7 @@ __device__ void compute_role(const SplitParams& p, Cursor<NT> cursor, uint32_t s
         // The row's largest |q| to [2^14, 2^15); rows that are zero or not
         // finite as they are.
         const int e = static_cast<int>(top >> 7) - 127;
-        if (top > 0 && e < 128) f = power_of_two(min(max(e - 14, -112), 112));
+        if (top > 0 && e < 128) f = power_of_two(max(e - 14, -112));
       }
       const float inv = 1.f / f;  // a power of two
       const float mine = f * p.scale_log2;

@@ -599,7 +599,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
       }
       top = max(top & 0xffffu, top >> 16);
       const int e = static_cast<int>(top >> 7) - 127;
-      if (top > 0 && e < 128) row_f = power_of_two(min(max(e - 14, -112), 112));
+      if (top > 0 && e < 128) row_f = power_of_two(max(e - 14, -112));
     }
     if (!u.dual || i == 0) {
       const float inv = 1.f / row_f;

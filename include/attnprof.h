@@ -335,6 +335,7 @@ int attn_block_trim(const attn_block_trim_args* args, void* stream);
  * others, until the block is written from its first slot again.
  * The tokens of one block must follow each other in the call with ascending
  * slots, as attn_block_tables gives them; a block must not appear twice.
+ * Asynchronous; needs no scratch.
  */
 typedef struct {
   const void *k, *v;
@@ -354,15 +355,17 @@ int attn_cache_append(const attn_cache_append_args* args, void* stream);
  * kv head h / (heads / kv_heads).  With causal != 0, row i of n sees the first
  * kv_lens[r] - n + i + 1 tokens, else all kv_lens[r].  scale multiplies the
  * scores (0: 1 / sqrt(D)).  A row that sees no token becomes 0.  Rows behind
- * starts[batch] are left as they were.  Scales must be positive; V scales and
- * the codes of tokens held must be finite numbers.  What lies in slots that
+ * starts[batch] are left as they were; rows of a request beyond max_new are
+ * not computed.  out must not overlap q.  Scales must be positive; V scales and
+ * the codes of tokens held must be finite numbers, |v| below 2^100.  What lies in slots that
  * hold no token is never used, whatever it is.  kv_lens is taken as at most
  * width * block_size, starts as within [0, tokens]; a table entry that is no
  * block of the pool is left out.
  * workspace: 16-byte aligned, attn_cached_workspace(...) bytes (NULL where
  * that is 0), needs no initial value; calls that may overlap need one each.
  * Asynchronous; like attn_fwd's, its waits are bounded (attn_set_timeout_ns)
- * and one that runs out is reported by attn_get_status.
+ * and one that runs out is reported by attn_get_status.  The first call on a
+ * device looks up that status word: make one before a stream capture.
  */
 typedef struct {
   const void* q;

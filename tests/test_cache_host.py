@@ -9,6 +9,7 @@ torch = pytest.importorskip("torch")
 from attnprofile_b200 import cache  # noqa: E402
 
 P = 4096  # an address that is aligned and never read
+R = 8192  # another
 
 
 def call(engine, name, pack, good, **change):
@@ -27,7 +28,7 @@ TABLES = dict(lens=P, new_lens=P, tables=P, free=P, free_count=P, kv_lens=P, sta
     ({"batch": 16385}, "UNSUPPORTED"), ({"batch": -1}, "INVALID_ARG"),
     ({"width": -1}, "INVALID_ARG"), ({"table_stride": 7}, "INVALID_ARG"),
     ({"num_blocks": 0}, "INVALID_ARG"), ({"num_blocks": 2 ** 27}, "INVALID_ARG"),
-    ({"tokens": -1}, "INVALID_ARG"),
+    ({"tokens": -1}, "INVALID_ARG"), ({"slots": P + 1}, "MISALIGNED"),
     *[({k: None}, "INVALID_ARG") for k in ("lens", "new_lens", "tables", "free", "free_count",
                                            "kv_lens", "starts", "slots", "free_left", "status")],
 ])
@@ -42,7 +43,7 @@ TRIM = dict(lens=P, keep=P, tables=P, free=P, free_count=P, lens_left=P, free_le
 @pytest.mark.parametrize("change,code", [
     ({"block_size": 24}, "UNSUPPORTED"), ({"batch": 16385}, "UNSUPPORTED"),
     ({"batch": -2}, "INVALID_ARG"), ({"table_stride": 3}, "INVALID_ARG"),
-    ({"num_blocks": -1}, "INVALID_ARG"),
+    ({"num_blocks": -1}, "INVALID_ARG"), ({"keep": P + 3}, "MISALIGNED"),
     *[({k: None}, "INVALID_ARG") for k in ("lens", "keep", "tables", "free", "free_count",
                                            "lens_left", "free_left", "status")],
 ])
@@ -60,7 +61,7 @@ APPEND = dict(k=P, v=P, slots=P, k_codes=P, v_codes=P, k_scale=P, v_scale=P, k_t
     ({"block_size": 256}, "UNSUPPORTED"), ({"tokens": -1}, "INVALID_ARG"),
     ({"kv_heads": 0}, "INVALID_ARG"), ({"kv_heads": 65536}, "INVALID_ARG"),
     ({"num_blocks": 2 ** 27}, "INVALID_ARG"), ({"k": P + 8}, "MISALIGNED"),
-    ({"v": P + 2}, "MISALIGNED"), ({"k_codes": P + 8}, "MISALIGNED"),
+    ({"v": P + 2}, "MISALIGNED"), ({"slots": P + 2}, "MISALIGNED"), ({"k_codes": P + 8}, "MISALIGNED"),
     ({"k_token": 260}, "MISALIGNED"), ({"v_head": 4}, "MISALIGNED"),
     *[({k: None}, "INVALID_ARG") for k in ("k", "v", "slots", "k_codes", "v_codes", "k_scale",
                                            "v_scale")],
@@ -73,7 +74,7 @@ def test_cache_append_of_nothing(engine):
     assert call(engine, "attn_cache_append", cache._APPEND, APPEND, tokens=0, k=None) == 0
 
 
-ATTN = dict(q=P, out=P, k_codes=P, v_codes=P, k_scale=P, v_scale=P, tables=P, kv_lens=P, starts=P,
+ATTN = dict(q=P, out=R, k_codes=P, v_codes=P, k_scale=P, v_scale=P, tables=P, kv_lens=P, starts=P,
             workspace=P, workspace_bytes=1 << 30, q_token=512, q_head=128, o_token=512, o_head=128,
             table_stride=8, tokens=3, heads=4, kv_heads=2, D=128, dtype=1, code=1, num_blocks=64,
             block_size=32, width=8, batch=3, max_new=1, causal=1, scale=0.0)
@@ -87,6 +88,8 @@ ATTN = dict(q=P, out=P, k_codes=P, v_codes=P, k_scale=P, v_scale=P, tables=P, kv
     ({"max_new": -1}, "INVALID_ARG"), ({"max_new": 2 ** 31 - 1}, "INVALID_ARG"),
     ({"table_stride": 7}, "INVALID_ARG"), ({"scale": -1.0}, "INVALID_ARG"),
     ({"scale": float("nan")}, "INVALID_ARG"), ({"scale": float("inf")}, "INVALID_ARG"),
+    ({"out": P}, "INVALID_ARG"), ({"o_token": 0}, "INVALID_ARG"), ({"o_head": 0}, "INVALID_ARG"),
+    ({"starts": P + 2}, "MISALIGNED"), ({"v_scale": P + 1}, "MISALIGNED"),
     ({"q": P + 8}, "MISALIGNED"), ({"out": P + 2}, "MISALIGNED"), ({"q_token": 516}, "MISALIGNED"),
     ({"o_head": 132}, "MISALIGNED"), ({"workspace": P + 4}, "MISALIGNED"),
     *[({k: None}, "INVALID_ARG") for k in ("q", "out", "k_codes", "v_codes", "k_scale", "v_scale",

@@ -77,6 +77,25 @@ def test_block_tables(ap, batch, longest, most_new, bs, pad, in_place):
     assert run_tables(ap, *state, bs, tokens, in_place) == ref.tables_ref(*state, bs, tokens)
 
 
+def test_block_tables_and_trim_of_the_largest_batch(ap):
+    rng = random.Random(2)
+    state = batch_state(rng, 16384, 30, 3, 16)
+    tokens = sum(state[1])
+    got = run_tables(ap, *state, 16, tokens, True)
+    assert got == ref.tables_ref(*state, 16, tokens)
+    lens, tables, free, count = got[1], got[0], state[3], got[4]
+    keep = [rng.choice([0, n, n - 1 if n else 0]) for n in lens]
+    pool = ap.BlockPool(ints(free), ints([count]), 16)
+    lens_t = ints(lens)
+    status = ap.block_trim(pool, lens_t, ints(keep), ints(tables))
+    assert (pool.free.tolist(), lens_t.tolist(), pool.free_count.item(), status.item()) \
+        == ref.trim_ref(lens, keep, tables, free, count, 16)
+    with pytest.raises(ap.AttnError):
+        ap.block_tables(pool, torch.zeros(16385, dtype=torch.int32, device="cuda"),
+                        torch.zeros(16385, dtype=torch.int32, device="cuda"),
+                        torch.zeros(16385, 1, dtype=torch.int32, device="cuda"), 4)
+
+
 def test_block_tables_of_no_requests_and_of_no_tokens(ap):
     for batch in (0, 4):
         lens, new = [16 * i for i in range(batch)], [0] * batch
@@ -543,6 +562,33 @@ def test_attn_cached_strides_and_scale(ap, new):
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("new", [1, 70])
+def test_attn_cached_one_token_or_head_of_any_stride(ap, new):
+    """The stride of a dimension of size one means nothing."""
+    cache, host = make_cache(ap, 6, 1, 16, 64, E4M3, 4)
+    table, lens, starts = ints([[0, 1, 2, 3, 4, 5]]), ints([90]), ints([0, new])
+    base = torch.randn(new * 64 + 70, device="cuda").half()
+    q = base.as_strided((new, 1, 64), (64, 7, 1))
+    out = torch.empty(new * 64, device="cuda").half().as_strided((new, 1, 64), (64, 13, 1))
+    ap.attn_cached(q, cache, table, lens, starts, max_new=new, out=out)
+    want = ap.attn_cached(q.contiguous(), cache, table, lens, starts, max_new=new)
+    assert torch.equal(out, want)
+    with pytest.raises(ap.AttnError):  # rows written over each other
+        ap.attn_cached(q, cache, table, lens, starts, max_new=new, out=q)
+
+
+@pytest.mark.parametrize("new", [3, 50])
+def test_attn_cached_takes_no_more_rows_than_max_new(ap, new):
+    cache, host = make_cache(ap, 40, 1, 16, 64, E4M3, 4)
+    q = torch.randn(new + 200, 2, 64, device="cuda").half()
+    out = torch.full_like(q, 3.0)
+    ap.attn_cached(q, cache, ints([list(range(40))]), ints([640]), ints([0, new + 200]),
+                   max_new=new, causal=False, out=out)
+    want = ap.attn_cached(q[:new], cache, ints([list(range(40))]), ints([640]), ints([0, new]),
+                          max_new=new, causal=False)
+    assert torch.equal(out[:new], want) and torch.all(out[new:] == 3)
+
+
 @pytest.mark.parametrize("new", [1, 4, 100])
 def test_attn_cached_gives_the_same_bits_again(ap, new):
     outs = [attend_case(ap, torch.float16, E4M3, 128, 32, 8, 2, [3000, 100, 777], [new, 1, new],
@@ -593,7 +639,8 @@ def test_captured_and_replayed_with_other_lengths(ap, new):
     """A graph of a whole step follows the lengths that it finds."""
     bs, heads, dim = 16, 2, 64
     cache = ap.PagedCache.empty(80, heads, dim, block_size=bs)
-    batch = ap.CacheBatch(ap.BlockPool.full(80, bs), rows=3, max_len=600)
+    batch = ap.CacheBatch(ap.BlockPool.full(80, bs), rows=3, max_len=600,
+                          max_tokens=2 * new + 1)
     new_lens = ints([new, 0, 1])
     tokens = 2 * new + 1
     qkv = torch.zeros(tokens, 8, dim, device="cuda").half()
@@ -705,7 +752,8 @@ def test_steps_of_a_server(ap, code):
     plain 64-bit ones."""
     bs, heads, kv_heads, dim, rows, blocks = 16, 4, 2, 64, 4, 30
     cache = ap.PagedCache.empty(blocks, kv_heads, dim, block_size=bs, dtype=code)
-    batch = ap.CacheBatch(ap.BlockPool.full(blocks, bs), rows=rows, max_len=300)
+    batch = ap.CacheBatch(ap.BlockPool.full(blocks, bs), rows=rows, max_len=300,
+                          max_tokens=400)
     state = [x.cpu() for x in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
     want_kv = [x.double() for x in state]
     lens, tables = [0] * rows, [[-1] * 19 for _ in range(rows)]
