@@ -364,10 +364,14 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
                    : "r"(codes_at + T::codes_at(stage) + it * kRowStep * D)
                    : "memory");
     float vs[kIters];
+    bool pow2 = true;  // all factors are powers of two, or 0
     if (is_v) {
       const float* scale = reinterpret_cast<const float*>(sgen + T::kOffVScale) + 8 * stage;
 #pragma unroll
-      for (int it = 0; it < kIters; ++it) vs[it] = scale[group_of(it)] * to_v;
+      for (int it = 0; it < kIters; ++it) {
+        vs[it] = scale[group_of(it)] * to_v;
+        pow2 &= (__float_as_int(vs[it]) & 0x7fffff) == 0;
+      }
       // What lies behind the last token, or where nothing was fetched, may be
       // any bits: 0 * NaN would reach a sum.  (Among the keys it is masked.)
       const int key0 = (u.step0 + j) * kBN;
@@ -385,30 +389,47 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
     ok = wait_bar(bar(Bar<D>::kEmpty + slot), ((t / T::kSlots) & 1) ^ 1, w, kSiteKvEmpty);
     if (!__all_sync(~0u, ok)) return;
     const uint32_t tile = tile_at + slot * T::kBytes;
-#pragma unroll
-    for (int it = 0; it < kIters; ++it) {
-      uint32_t h[8];
+    auto store = [&](int it, const uint32_t (&h)[8]) {
+      const uint32_t base = tile + it * kRowStep * 128;
+      st_shared_v4(base + at_lo, h[0], h[1], h[2], h[3]);
+      st_shared_v4(base + at_hi, h[4], h[5], h[6], h[7]);
+    };
+    auto convert = [&](int it, uint32_t (&h)[8]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         h[2 * i] = Code<CODE>::half2_lo(c[it][i]);
         h[2 * i + 1] = Code<CODE>::half2_hi(c[it][i]);
       }
-      if (is_v) {
-        if ((__float_as_int(vs[it]) & 0x7fffff) == 0) {  // a power of two (or 0)
-          const __half2 f2 = __float2half2_rn(vs[it]);
+    };
+    if (!is_v) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = mul_half2(h[i], f2);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 x = half2_to_float2(h[i]);
-            h[i] = half2_of(x.x * vs[it], x.y * vs[it]);
-          }
-        }
+      for (int it = 0; it < kIters; ++it) {
+        uint32_t h[8];
+        convert(it, h);
+        store(it, h);
       }
-      const uint32_t base = tile + it * kRowStep * 128;
-      st_shared_v4(base + at_lo, h[0], h[1], h[2], h[3]);
-      st_shared_v4(base + at_hi, h[4], h[5], h[6], h[7]);
+    } else if (__builtin_expect(pow2, 1)) {
+#pragma unroll
+      for (int it = 0; it < kIters; ++it) {
+        uint32_t h[8];
+        convert(it, h);
+        const __half2 f2 = __float2half2_rn(vs[it]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = mul_half2(h[i], f2);
+        store(it, h);
+      }
+    } else {  // scales that the caller brought: one rounding to f16
+#pragma unroll
+      for (int it = 0; it < kIters; ++it) {
+        uint32_t h[8];
+        convert(it, h);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 x = half2_to_float2(h[i]);
+          h[i] = half2_of(x.x * vs[it], x.y * vs[it]);
+        }
+        store(it, h);
+      }
     }
     ptx::fence_proxy_async_smem();
     __syncwarp();
@@ -567,69 +588,141 @@ __device__ void mma_role(const Unit& u, int me, uint32_t tmem, uint32_t sbase, c
 // ---------------------------------------------------------------------------
 // Softmax warpgroup of tile i: a thread a row.
 // ---------------------------------------------------------------------------
+struct Row {
+  int r, lane, warp;  // row of the tile (lane of tensor memory), in its warp
+  int row, tok, head; // of the request's rows of this kv head; token and query head
+  bool live;
+};
+// A thread's row.  The thread's number is read anew each time, so that what
+// only the beginning and the end need takes no registers in the steps between
+// (kept, it cost the steps 9 % at D = 128).
+__device__ __forceinline__ Row row_of(const CachedParams& p, const Unit& u, int i) {
+  int tid;
+  asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid));
+  Row x;
+  x.lane = tid & 31;
+  x.warp = (tid >> 5) & 3;
+  x.r = tid & (kBM - 1);
+  x.row = u.row0 + (u.dual ? 0 : i * kBM) + x.r;
+  x.live = x.row < u.rows_in;
+  x.tok = x.live ? x.row / p.group : 0;
+  x.head = u.kvh * p.group + (x.live ? x.row - x.tok * p.group : 0);
+  return x;
+}
+
+template <typename TQ, int D>
+__device__ __forceinline__ float load_q(const TiledParams& p, const Unit& u, int i, uint32_t sbase) {
+  using T = Tile<D>;
+  auto bar = [&](int b) { return sbase + T::kOffBar + 8u * b; };
+  const Row x_of = row_of(p, u, i);
+  const int lane = x_of.lane, wi = x_of.warp;
+  const bool live = x_of.live;
+  // Q to shared memory, in f16 (two tiles of the same rows share it).  A warp
+  // takes its 32 rows kAtOnce at a time, 16 bytes a lane: rows of a head lie far
+  // apart, and threads that read their own rows took up to 15,000 cycles.
+  constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kRounds = 32 / kAtOnce;
+  const int sub = lane / kLanes, piece = lane % kLanes;
+  const uint32_t tile = sbase + i * T::kBytes;
+  const uint32_t row_at = tile + (piece >> 3) * T::kBlock + (32 * wi + sub) * 128;
+  const TQ* q = static_cast<const TQ*>(p.q) + (u.rq.start + x_of.tok) * p.q_token +
+                x_of.head * p.q_head;
+  if (!u.dual || i == 0) {
+#pragma unroll 1
+    for (int it0 = 0; it0 < kRounds; it0 += 8) {
+      uint4 x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int from = kAtOnce * (it0 + k) + sub;
+        const auto at = __shfl_sync(~0u, reinterpret_cast<unsigned long long>(q), from);
+        x[k] = __shfl_sync(~0u, live, from) ? __ldg(reinterpret_cast<const uint4*>(at) + piece)
+                                            : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int at = kAtOnce * (it0 + k) + sub;  // row of the warp's 32
+        st_shared_v4(row_at + (it0 + k) * kAtOnce * 128 + (((piece & 7) ^ (at & 7)) << 4), x[k].x,
+                     x[k].y, x[k].z, x[k].w);
+      }
+    }
+    __syncwarp();
+  }
+  float row_f = 1.f;
+  if constexpr (std::is_same<TQ, __nv_bfloat16>::value) {
+    // bf16: each thread turns its own row, there, into f16 times a power of two.
+    const int r = x_of.r;
+    auto chunk_at = [&](int c) {
+      return tile + (c >> 3) * T::kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    };
+    uint32_t y[D / 8][4], top = 0;
+    if (!u.dual || i == 0) {
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(y[c][0]), "=r"(y[c][1]), "=r"(y[c][2]), "=r"(y[c][3])
+                     : "r"(chunk_at(c))
+                     : "memory");
+    } else {  // (the other tile has it there; only the power is wanted)
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 v = live ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
+        y[c][0] = v.x;
+        y[c][1] = v.y;
+        y[c][2] = v.z;
+        y[c][3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c)
+      top = __vmaxu2(top, __vmaxu2(__vmaxu2(y[c][0] & 0x7fff7fffu, y[c][1] & 0x7fff7fffu),
+                                   __vmaxu2(y[c][2] & 0x7fff7fffu, y[c][3] & 0x7fff7fffu)));
+    top = max(top & 0xffffu, top >> 16);
+    const int e = static_cast<int>(top >> 7) - 127;
+    const int shift = top > 0 && e < 128 ? max(e - 14, -112) : 0;
+    row_f = power_of_two(shift);
+    const float inv = power_of_two(-shift);
+    if (!u.dual || i == 0) {
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          h[k] = half2_of(__uint_as_float(y[c][k] << 16) * inv,
+                          __uint_as_float(y[c][k] & 0xffff0000u) * inv);
+        st_shared_v4(chunk_at(c), h[0], h[1], h[2], h[3]);
+      }
+    }
+  }
+  if (!u.dual || i == 0) {
+    ptx::fence_proxy_async_smem();
+    ptx::mbar_arrive(bar(Bar<D>::kQ + i));
+  }
+  return row_f;
+}
+
 template <typename TQ, int D>
 __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_t tmem,
                              uint32_t sbase, const uint8_t* sgen, const WaitCtx& w) {
   using T = Tile<D>;
   auto bar = [&](int b) { return sbase + T::kOffBar + 8u * b; };
   const int lane = threadIdx.x & 31, wi = (threadIdx.x >> 5) & 3;
-  const int r = 32 * wi + lane;                 // row of the tile, lane of tensor memory
-  const int row = u.row0 + (u.dual ? 0 : i * kBM) + r;
-  const bool live = row < u.rows_in;
-  const int tok = live ? row / p.group : 0;
-  const int head = u.kvh * p.group + (live ? row - tok * p.group : 0);
-  // (rows behind the last one: zeros that see everything, so that they mask nothing)
-  const int limit =
-      (live ? min(row_limit(p, u.rq, row), u.kv_end) : u.kv_end) - u.step0 * kBN;
   const bool tile_there = u.dual || u.row0 + i * kBM < u.rows_in;
-
-  // Q: this row to shared memory, in f16 (two tiles of the same rows share it).
-  float row_f = 1.f;
-  if (tile_there && u.steps > 0) {
-    const TQ* q = static_cast<const TQ*>(p.q) + (u.rq.start + tok) * p.q_token + head * p.q_head;
-    if constexpr (std::is_same<TQ, __nv_bfloat16>::value) {
-      uint32_t top = 0;
-      if (live) {
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(q) + c);
-          top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
-                                       __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
-        }
-      }
-      top = max(top & 0xffffu, top >> 16);
-      const int e = static_cast<int>(top >> 7) - 127;
-      if (top > 0 && e < 128) row_f = power_of_two(max(e - 14, -112));
-    }
-    if (!u.dual || i == 0) {
-      const float inv = 1.f / row_f;
-      const uint32_t base = sbase + i * T::kBytes + r * 128;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
-        if constexpr (std::is_same<TQ, __nv_bfloat16>::value) {
-          uint32_t* y = reinterpret_cast<uint32_t*>(&x);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            y[k] = half2_of(__uint_as_float(y[k] << 16) * inv,
-                            __uint_as_float(y[k] & 0xffff0000u) * inv);
-        }
-        st_shared_v4(base + (c >> 3) * T::kBlock + (((c & 7) ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
-      }
-      ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(bar(Bar<D>::kQ + i));
-    }
+  if (!tile_there) return;
+  float to_log2 = p.scale_log2;
+  if (u.steps > 0) to_log2 *= load_q<TQ, D>(p, u, i, sbase);
+  int limit;  // keys of this range that the row sees
+  {
+    // (rows behind the last one: zeros that see everything, so that they mask nothing)
+    const Row x = row_of(p, u, i);
+    limit = (x.live ? min(row_limit(p, u.rq, x.row), u.kv_end) : u.kv_end) - u.step0 * kBN;
   }
-
   const uint32_t lane_base = tmem + (static_cast<uint32_t>(32 * wi) << 16);
   const uint32_t s_col = i * T::kTile, p_col = s_col + T::kPCol, o_col = T::kOCol + i * D;
-  const float to_log2 = row_f * p.scale_log2;
   float m = -INFINITY, l = 0.f;  // maximum in log2 units, sum of 2^kLift p
   bool ok = true;
   // c counts this tile's steps, j all of them.
   const int by = u.dual ? 2 : 1;
   int c = 0;
-  for (int j = u.dual ? i : 0; j < u.steps && tile_there; j += by, ++c) {
+  for (int j = u.dual ? i : 0; j < u.steps; j += by, ++c) {
     ok = __all_sync(~0u, wait_bar(bar(Bar<D>::kS + i), c & 1, w, kSiteSFull));
     if (!ok) break;
     ptx::tc_fence_after();
@@ -758,7 +851,6 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     l = l * alpha + ((sa + sb) + (sc + sd));
   }
 
-  if (!tile_there) return;
   float f = 0.f;
   if (u.steps > 0) {
     if (ok) {
@@ -771,6 +863,9 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
   }
   // Two tiles of the same rows: tile 1 hands its sums over in the rings' place,
   // once both have no MMA left that reads there; tile 0 adds them to its own.
+  const Row x_of = row_of(p, u, i);
+  const int r = x_of.r;
+  const bool live = x_of.live;
   float other = 0.f;
   float4* hand = reinterpret_cast<float4*>(const_cast<uint8_t*>(sgen) + T::kOffKv) + r;
   if (u.dual) {
@@ -807,7 +902,8 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     f *= n;
     other *= n;
   }
-  TQ* out = static_cast<TQ*>(p.out) + (u.rq.start + tok) * p.o_token + head * p.o_head;
+  TQ* out = static_cast<TQ*>(p.out) + (u.rq.start + x_of.tok) * p.o_token +
+            x_of.head * p.o_head;
   const long long slots = gridDim.x, slot = blockIdx.x;
   float* o_part = TilePart<D>::o(p.ws, slot, i * kBM + r);
   if (p.parts > 1 && live)
@@ -835,8 +931,8 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
         o[4 * k + 3] = __float_as_uint(fmaf(y.w, other, __uint_as_float(o[4 * k + 3])));
       }
     }
-    if (!live) continue;
     if (p.parts > 1) {
+      if (!live) continue;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         *reinterpret_cast<float4*>(o_part + 32 * b + 4 * k) = make_float4(
@@ -844,14 +940,35 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
             __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
       continue;
     }
+    // Through the place of this tile's Q, which no MMA reads any more.
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       uint32_t y[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         y[e] = pack2<TQ>(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
-      *reinterpret_cast<uint4*>(out + 32 * b + 8 * k) = make_uint4(y[0], y[1], y[2], y[3]);
+      const int chunk = 4 * b + k;
+      st_shared_v4(sbase + i * T::kBytes + (chunk >> 3) * T::kBlock + r * 128 +
+                       (((chunk & 7) ^ (r & 7)) << 4),
+                   y[0], y[1], y[2], y[3]);
     }
+  }
+  if (p.parts > 1) return;
+  constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kRounds = 32 / kAtOnce;
+  const int sub = x_of.lane / kLanes, piece = x_of.lane % kLanes;
+  const uint32_t row_at =
+      sbase + i * T::kBytes + (piece >> 3) * T::kBlock + (32 * x_of.warp + sub) * 128;
+  __syncwarp();
+#pragma unroll 4
+  for (int it = 0; it < kRounds; ++it) {
+    const int at = kAtOnce * it + sub;
+    const auto dst = __shfl_sync(~0u, reinterpret_cast<unsigned long long>(out), at);
+    uint4 y;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                 : "r"(row_at + it * kAtOnce * 128 + (((piece & 7) ^ (at & 7)) << 4))
+                 : "memory");
+    if (__shfl_sync(~0u, live, at)) reinterpret_cast<uint4*>(dst)[piece] = y;
   }
 }
 
