@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
   int* first = sm + p.batch;            // [batch] rank of its first new block
   int* len = sm + 2 * p.batch;          // [batch] tokens held before
   __shared__ Counts warp_sum[kThreads / 32];
+  begin_behind();
   const int ctas = static_cast<int>(gridDim.x);
   const int mask = (1 << p.shift) - 1;
 
@@ -211,6 +212,7 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
   int* first = sm;              // [batch] rank of the first block given back
   int* left = sm + p.batch;     // [batch] tokens kept
   __shared__ Counts warp_sum[kThreads / 32];
+  begin_behind();
   const int ctas = static_cast<int>(gridDim.x);
   const int mask = (1 << p.shift) - 1;
 
@@ -275,19 +277,10 @@ int launch_cluster(void (*kern)(P), const P& p, int ctas, size_t smem, cudaStrea
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return ATTN_ERR_RESOURCE;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
+  return launch_behind(kern, dim3(static_cast<unsigned>(ctas)), kThreads, smem, ctas, st, p) ==
+                 cudaSuccess
+             ? ATTN_OK
+             : ATTN_ERR_CUDA;
 }
 
 int check_batch(int batch, int width, long long table_stride, int num_blocks, int block_size) {

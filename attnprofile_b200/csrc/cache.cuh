@@ -119,5 +119,35 @@ __device__ __forceinline__ float power_of_two(int e) {
 }
 #endif  // __CUDACC__
 
+// A launch whose blocks may start while the kernel in front of it in the stream
+// ends: every block of `kern` runs begin_behind() before it touches memory.
+// cluster: blocks of one, or 0.
+template <typename... P, typename... A>
+inline cudaError_t launch_behind(void (*kern)(P...), dim3 grid, int threads, size_t smem,
+                                 int cluster, cudaStream_t st, const A&... args) {
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// Waits for the end of the kernel in front, whose writes are then seen; the
+// next one's blocks may start as soon as all blocks of this one are here.
+__device__ __forceinline__ void begin_behind() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 }  // namespace cache
 }  // namespace attnprof

@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const AppendParams 
   constexpr int kShort = 2 * kRows;          // tokens of a run that one warp takes
   __shared__ uint32_t tops[2][kWarps];
   __shared__ uint32_t bads[kWarps];
+  begin_behind();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool is_v = lane >= 16;
   const int sub = (lane & 15) / kLanes;      // which of the kRows tokens
@@ -260,8 +261,10 @@ template <typename T, int CODE, int D, int WARPS, int ITERS>
 int launch_rounds(const AppendParams& p, cudaStream_t st) {
   const dim3 grid((static_cast<unsigned>(p.tokens) + p.chunk - 1) / p.chunk,
                   static_cast<unsigned>(p.heads));
-  append_kernel<T, CODE, D, WARPS, ITERS><<<grid, 32 * WARPS, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
+  return launch_behind(append_kernel<T, CODE, D, WARPS, ITERS>, grid, 32 * WARPS, 0, 0, st, p) ==
+                 cudaSuccess
+             ? ATTN_OK
+             : ATTN_ERR_CUDA;
 }
 
 template <typename T, int CODE, int D>

@@ -818,7 +818,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  asm volatile("griddepcontrol.launch_dependents;");
+  begin_behind();  // only then: the joining kernel reads lengths before it waits
   Cursor<NT> cursor;
   long long total;
   if (p.batch <= kLaneRequests) {
@@ -1075,24 +1075,19 @@ int launch(const CachedParams& cp, int max_new, void* ws, unsigned long long ws_
   if (!p.whole && (ws == nullptr || ws_bytes < part_bytes(D, NT) * ctas))
     return ATTN_ERR_WORKSPACE;
   p.ws = static_cast<float*>(ws);
-  split_kernel<T, CODE, D, NT><<<ctas, kThreads, Smem<D, NT>::kBytes, st>>>(map_k, map_v, p);
-  if (cudaGetLastError() != cudaSuccess) return ATTN_ERR_CUDA;
+  if (launch_behind(split_kernel<T, CODE, D, NT>, dim3(static_cast<unsigned>(ctas)), kThreads,
+                    Smem<D, NT>::kBytes, 0, st, map_k, map_v, p) != cudaSuccess)
+    return ATTN_ERR_CUDA;
   if (p.whole || ctas == 1) return ATTN_OK;
   // The joining kernel starts while the first still runs (its search of the
   // cuts overlaps) and waits for it before it reads the parts.
   const bool few = p.batch <= 32 && units <= kFewUnits;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = few ? dim3(static_cast<unsigned>(units), 8 * NT) : dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
   const CachedParams& base = p;
-  const cudaError_t e = few ? cudaLaunchKernelEx(&cfg, join_few_kernel<T, D, NT>, base, ctas)
-                            : cudaLaunchKernelEx(&cfg, join_kernel<T, D, NT>, base);
+  const cudaError_t e =
+      few ? launch_behind(join_few_kernel<T, D, NT>, dim3(static_cast<unsigned>(units), 8 * NT),
+                          256, 0, 0, st, base, ctas)
+          : launch_behind(join_kernel<T, D, NT>, dim3(static_cast<unsigned>(ctas)), 256, 0, 0, st,
+                          base);
   return e == cudaSuccess ? ATTN_OK : ATTN_ERR_CUDA;
 }
 
