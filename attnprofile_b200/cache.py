@@ -29,7 +29,9 @@ BLOCKS = {"OK": 0, "POOL": 1, "ROW": 2, "SLOTS": 3, "NEGATIVE": 4}
 MAX_BATCH = 16384
 _CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+_INT32 = torch.int32
 _workspace_bytes: dict = {}
+_functions: dict = {}
 
 
 def _raw_stream(index: int) -> int:
@@ -39,14 +41,16 @@ def _raw_stream(index: int) -> int:
 # The same without building a Stream object (2 us less per call), where this
 # torch offers it.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+# And the current device (CUDA is initialised: there are tensors).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _stream(device, stream) -> int:
+def _stream(index, stream) -> int:
     """The stream of a call (default: the current one of the tensors' device)."""
     if stream is None:
-        return _raw_stream(device.index)
-    if stream.device != device:
-        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        return _raw_stream(index)
+    if stream.device.index != index:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on cuda:{index}")
     return stream.cuda_stream
 
 
@@ -57,13 +61,16 @@ _APPEND = struct.Struct("@7Q4q7i").pack
 _CACHED = struct.Struct("@11Q5q12if").pack
 
 
-def _call(name, device, *args):
+def _call(name, index, *args):
     """A C entry point with the tensors' device current."""
-    if torch.cuda.current_device() == device.index:
-        rc = getattr(lib(), name)(*args)
+    function = _functions.get(name)
+    if function is None:
+        function = _functions[name] = getattr(lib(), name)
+    if _current_device() == index:
+        rc = function(*args)
     else:
-        with torch.cuda.device(device):
-            rc = getattr(lib(), name)(*args)
+        with torch.cuda.device(index):
+            rc = function(*args)
     if rc:
         _check(rc, name)
 
@@ -78,22 +85,22 @@ def _empty(shape, dtype, device, stream):
     return x
 
 
-def _ints(name, t, device, n):
+def _ints(name, t, index, n):
     """Checks an int32 vector of n; its address."""
-    if t.dtype is not torch.int32:
+    if t.dtype is not _INT32:
         raise TypeError(f"{name} must be int32")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on cuda:{index}")
     if t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of shape ({n},)")
     return t.data_ptr()
 
 
-def _table(tables, device, batch):
-    if tables.dtype is not torch.int32:
+def _table(tables, index, batch):
+    if tables.dtype is not _INT32:
         raise TypeError("tables must be int32")
-    if tables.device != device:
-        raise ValueError(f"tables must be on {device}")
+    if tables.get_device() != index:
+        raise ValueError(f"tables must be on cuda:{index}")
     shape = tables.shape
     if len(shape) != 2 or shape[0] != batch:
         raise ValueError(f"tables must be [{batch}, width]")
@@ -164,8 +171,8 @@ class BlockPool:
         if block_size not in BLOCK_SIZES:
             raise ValueError(f"block_size {block_size} is not one of {BLOCK_SIZES}")
         self.device, self.num_blocks, self.block_size = free.device, free.numel(), block_size
-        _ints("free", free, self.device, free.numel())
-        _ints("free_count", free_count, self.device, 1)
+        _ints("free", free, self.device.index, free.numel())
+        _ints("free_count", free_count, self.device.index, 1)
         self.free, self.free_count = free, free_count
 
     @classmethod
@@ -178,12 +185,30 @@ class BlockPool:
 
 class BlockPlan:
     """What block_tables writes: kv_lens [batch], starts [batch + 1], slots
-    [tokens] and the status word [1] (BLOCKS), all int32."""
+    [tokens] and the status word [1] (BLOCKS), all int32.  They are checked when
+    the plan is first used, and again when one is replaced; they keep their memory
+    meanwhile, as a cache's tensors do."""
 
-    __slots__ = ("kv_lens", "starts", "slots", "status")
+    __slots__ = ("kv_lens", "starts", "slots", "status", "_checked")
 
     def __init__(self, kv_lens, starts, slots, status):
         self.kv_lens, self.starts, self.slots, self.status = kv_lens, starts, slots, status
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_checked", None)
+
+    def _ptrs(self, index, batch, tokens):
+        """Addresses of the four for `batch` requests on device `index`."""
+        checked = self._checked
+        if checked is None or checked[0] != (index, batch, tokens):
+            checked = ((index, batch, tokens),
+                       (_ints("plan.kv_lens", self.kv_lens, index, batch),
+                        _ints("plan.starts", self.starts, index, batch + 1),
+                        _ints("plan.slots", self.slots, index, tokens)),
+                       _ints("plan.status", self.status, index, 1))
+            object.__setattr__(self, "_checked", checked)
+        return checked[1], checked[2]
 
     @classmethod
     def empty(cls, batch: int, tokens: int, device="cuda"):
@@ -202,20 +227,19 @@ def block_tables(pool: BlockPool, lens, new_lens, tables, tokens: int, *, plan=N
     takes it.  All or nothing: plan.status tells (on the device) whether the
     pool, the table rows and the slot map were large enough."""
     device, batch = pool.device, lens.shape[0]
-    s = _stream(device, stream)
+    index = device.index
+    s = _stream(index, stream)
     if plan is None:
         plan = BlockPlan(*(_empty(n, torch.int32, device, stream)
                            for n in (batch, batch + 1, tokens, 1)))
     if free_left is None:
         free_left = pool.free_count
-    t, width, stride = _table(tables, device, batch)
-    _call("attn_block_tables", device, _TABLES(
-        _ints("lens", lens, device, batch), _ints("new_lens", new_lens, device, batch), t,
-        pool.free.data_ptr(), pool.free_count.data_ptr(),
-        _ints("plan.kv_lens", plan.kv_lens, device, batch),
-        _ints("plan.starts", plan.starts, device, batch + 1),
-        _ints("plan.slots", plan.slots, device, tokens), _ints("free_left", free_left, device, 1),
-        _ints("plan.status", plan.status, device, 1), stride, batch, width, pool.num_blocks,
+    t, width, stride = _table(tables, index, batch)
+    written, status = plan._ptrs(index, batch, tokens)
+    _call("attn_block_tables", index, _TABLES(
+        _ints("lens", lens, index, batch), _ints("new_lens", new_lens, index, batch), t,
+        pool.free.data_ptr(), pool.free_count.data_ptr(), *written,
+        _ints("free_left", free_left, index, 1), status, stride, batch, width, pool.num_blocks,
         pool.block_size, tokens), s)
     return plan
 
@@ -227,31 +251,32 @@ def block_trim(pool: BlockPool, lens, keep, tables, *, lens_left=None, free_left
     itself) and free_left (default: pool.free_count); returns the status word
     [1] (BLOCKS; anything but OK: nothing was changed)."""
     device, batch = pool.device, lens.shape[0]
-    s = _stream(device, stream)
+    index = device.index
+    s = _stream(index, stream)
     if lens_left is None:
         lens_left = lens
     if free_left is None:
         free_left = pool.free_count
     if status is None:
         status = _empty(1, torch.int32, device, stream)
-    t, width, stride = _table(tables, device, batch)
-    _call("attn_block_trim", device, _TRIM(
-        _ints("lens", lens, device, batch), _ints("keep", keep, device, batch), t,
+    t, width, stride = _table(tables, index, batch)
+    _call("attn_block_trim", index, _TRIM(
+        _ints("lens", lens, index, batch), _ints("keep", keep, index, batch), t,
         pool.free.data_ptr(), pool.free_count.data_ptr(),
-        _ints("lens_left", lens_left, device, batch), _ints("free_left", free_left, device, 1),
-        _ints("status", status, device, 1), stride, batch, width, pool.num_blocks,
+        _ints("lens_left", lens_left, index, batch), _ints("free_left", free_left, index, 1),
+        _ints("status", status, index, 1), stride, batch, width, pool.num_blocks,
         pool.block_size), s)
     return status
 
 
-def _rows(name, x, device, heads, dim):
+def _rows(name, x, index, heads, dim):
     """Checks a [tokens, heads, D] tensor; its dtype code, shape, and the strides
     of tokens and heads (0 where there is one only, whose stride means nothing)."""
     kind = _DTYPES.get(x.dtype)
     if kind is None:
         raise TypeError(f"unsupported dtype {x.dtype} of {name} (float16 or bfloat16)")
-    if x.device != device:
-        raise ValueError(f"{name} must be on {device}")
+    if x.get_device() != index:
+        raise ValueError(f"{name} must be on cuda:{index}")
     shape = x.shape
     if len(shape) != 3 or shape[2] != dim or (heads and shape[1] != heads):
         raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {dim}]")
@@ -271,27 +296,27 @@ def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
     finite makes that block's k_scale NaN for its head.  The tokens of one
     block follow each other with ascending slots (as block_tables gives them),
     and no block appears twice."""
-    device = cache.device
+    index = cache.device.index
     heads, dim = cache.kv_heads, cache.dim
-    kind, shape, k_token, k_head = _rows("k", k, device, heads, dim)
-    v_kind, v_shape, v_token, v_head = _rows("v", v, device, heads, dim)
+    kind, shape, k_token, k_head = _rows("k", k, index, heads, dim)
+    v_kind, v_shape, v_token, v_head = _rows("v", v, index, heads, dim)
     if v_kind != kind or v_shape != shape:
         raise ValueError("k and v must share one shape and dtype")
     tokens = shape[0]
-    _call("attn_cache_append", device, _APPEND(
-        k.data_ptr(), v.data_ptr(), _ints("slots", slots, device, tokens), *cache.ptrs, k_token,
+    _call("attn_cache_append", index, _APPEND(
+        k.data_ptr(), v.data_ptr(), _ints("slots", slots, index, tokens), *cache.ptrs, k_token,
         k_head, v_token, v_head, tokens, heads, dim, kind, cache.code, cache.num_blocks,
-        cache.block_size), _stream(device, stream))
+        cache.block_size), _stream(index, stream))
 
 
-def _workspace(device, heads, kv_heads, dim, max_new, block_size, width) -> int:
-    key = (device.index, heads, kv_heads, dim, max_new, block_size, width)
+def _workspace(index, heads, kv_heads, dim, max_new, block_size, width) -> int:
+    key = (index, heads, kv_heads, dim, max_new, block_size, width)
     n = _workspace_bytes.get(key)
     if n is None:
         if len(_workspace_bytes) > 4096:
             _workspace_bytes.clear()
         out = ctypes.c_ulonglong()
-        _call("attn_cached_workspace", device, heads, kv_heads, dim, max_new, block_size, width,
+        _call("attn_cached_workspace", index, heads, kv_heads, dim, max_new, block_size, width,
               ctypes.byref(out))
         n = _workspace_bytes[key] = out.value
     return n
@@ -300,7 +325,7 @@ def _workspace(device, heads, kv_heads, dim, max_new, block_size, width) -> int:
 def cached_workspace(cache: PagedCache, heads: int, max_new: int, width: int) -> int:
     """Bytes of workspace that attn_cached needs with `heads` query heads and
     tables of `width` entries, whatever the lengths (0: none)."""
-    return _workspace(cache.device, heads, cache.kv_heads, cache.dim, max_new, cache.block_size,
+    return _workspace(cache.device.index, heads, cache.kv_heads, cache.dim, max_new, cache.block_size,
                       width)
 
 
@@ -321,7 +346,8 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     cached_workspace(...) bytes; calls that may overlap on the GPU need one
     each."""
     device, kv_heads, dim = cache.device, cache.kv_heads, cache.dim
-    kind, shape, q_token, q_head = _rows("q", q, device, 0, dim)
+    index = device.index
+    kind, shape, q_token, q_head = _rows("q", q, index, 0, dim)
     tokens, heads, _ = shape
     if heads == 0 or heads % kv_heads:
         raise ValueError(f"{heads} heads are not a multiple of the cache's {kv_heads}")
@@ -332,28 +358,28 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     if max_new < 0:
         raise ValueError("max_new must not be negative")
     batch = kv_lens.shape[0]
-    t, width, stride = _table(tables, device, batch)
-    lens_ptr = _ints("kv_lens", kv_lens, device, batch)
-    starts_ptr = _ints("starts", starts, device, batch + 1)
-    s = _stream(device, stream)
+    t, width, stride = _table(tables, index, batch)
+    lens_ptr = _ints("kv_lens", kv_lens, index, batch)
+    starts_ptr = _ints("starts", starts, index, batch + 1)
+    s = _stream(index, stream)
     if out is None:
         out = _empty(shape, q.dtype, device, stream)
         o_token, o_head = heads * dim, dim
     else:
-        o_kind, o_shape, o_token, o_head = _rows("out", out, device, heads, dim)
+        o_kind, o_shape, o_token, o_head = _rows("out", out, index, heads, dim)
         if o_kind != kind or o_shape != shape:
             raise ValueError("out must have the shape and dtype of q")
     if workspace is None:
-        need = _workspace(device, heads, kv_heads, dim, max_new, cache.block_size, width)
+        need = _workspace(index, heads, kv_heads, dim, max_new, cache.block_size, width)
         if need:
             workspace = _empty(need, torch.uint8, device, stream)
     else:
         if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
             raise TypeError("workspace must be a contiguous uint8 tensor")
-        if workspace.device != device:
+        if workspace.get_device() != index:
             raise ValueError(f"workspace must be on {device}")
         need = workspace.numel()
-    _call("attn_cached", device, _CACHED(
+    _call("attn_cached", index, _CACHED(
         q.data_ptr(), out.data_ptr(), *cache.ptrs, t, lens_ptr, starts_ptr,
         workspace.data_ptr() if need else 0, need, q_token, q_head, o_token, o_head, stride, tokens, heads, kv_heads, dim, kind,
         cache.code, cache.num_blocks, cache.block_size, width, batch, max_new,
