@@ -791,3 +791,74 @@ def test_steps_of_a_server(ap, code):
             assert batch.trim(ints(keep)).item() == 0
             free, lens, count, _ = ref.trim_ref(lens, keep, tables, free, count, bs)
             assert batch.lens.tolist() == lens and batch.pool.free.tolist()[:count] == free[:count]
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("max_len", [400, 4000])
+def test_calls_that_follow_each_other_at_once(ap, dim, code, max_len):
+    """Steps whose calls are issued without any wait, on one buffer that is
+    overwritten between them, give the bits of steps that wait after every call
+    (up to 512 tokens nothing is joined, beyond that parts are)."""
+    bs, heads, kv_heads, rows = 32, 8, 2, 3
+    most = max_len // 4
+    gen = torch.Generator(device="cuda").manual_seed(max_len)
+    prompts = [[most, most // 2, 1], [1, 1, 1], [2, 1, 3], [most, 7, most // 3]] + [[1, 1, 1]] * 6
+    keeps = {3: [most + 2, 5, most], 7: [0, 9, most + 1]}
+    inputs = [torch.randn(sum(n) + 2, heads + 2 * kv_heads, dim, generator=gen,
+                          device="cuda").half() for n in prompts]
+    new = [ints(n) for n in prompts]
+    keeps = {i: ints(n) for i, n in keeps.items()}
+
+    def run(wait):
+        blocks = rows * (max_len // bs + 1)
+        batch = ap.CacheBatch(ap.BlockPool.full(blocks, bs), rows, max_len, len(inputs[0]))
+        cache = ap.PagedCache.empty(blocks, kv_heads, dim, block_size=bs, dtype=code)
+        buffer, outs = torch.zeros_like(inputs[0]), []
+        torch.cuda.synchronize()
+        for i, x in enumerate(inputs):
+            qkv = buffer[:len(x)]
+            qkv.copy_(x)
+            out = torch.zeros_like(x[:, :heads])
+            wait()
+            batch.advance(new[i], len(x))
+            wait()
+            batch.attend(cache, qkv[:, :heads], qkv[:, heads:heads + kv_heads],
+                         qkv[:, heads + kv_heads:], max_new=max(prompts[i]), out=out)
+            wait()
+            if i in keeps:
+                batch.trim(keeps[i])
+                wait()
+            buffer.fill_(float("nan"))
+            outs.append(out)
+        torch.cuda.synchronize()
+        assert batch.status.item() == 0
+        return outs + [batch.lens, batch.pool.free_count]
+
+    want = run(torch.cuda.synchronize)
+    assert all(torch.isfinite(x).all() for x in want) and any(x.any() for x in want)
+    for _ in range(3):
+        for a, b in zip(run(lambda: None), want):
+            assert torch.equal(a, b)
+
+
+def test_a_plan_is_checked_again_where_it_changed(ap):
+    pool, lens, new = ap.BlockPool.full(8, 16), ints([0, 3]), ints([5, 1])
+    tables, plan = torch.zeros(2, 4, dtype=torch.int32, device="cuda"), ap.BlockPlan.empty(2, 6)
+    for _ in range(2):
+        ap.block_tables(pool, lens, new, tables, 6, plan=plan)
+    with pytest.raises(ValueError, match="plan.slots"):
+        ap.block_tables(pool, lens, new, tables, 7, plan=plan)
+    with pytest.raises(ValueError, match="plan.kv_lens"):
+        ap.block_tables(pool, lens[:1], new[:1], tables[:1], 6, plan=plan)
+    plan.slots = torch.empty(12, dtype=torch.int32, device="cuda")[::2]
+    with pytest.raises(ValueError, match="plan.slots"):
+        ap.block_tables(pool, lens, new, tables, 6, plan=plan)
+    plan.slots = torch.empty(6, dtype=torch.int32, device="cuda")
+    plan.status = torch.empty(1, dtype=torch.int64, device="cuda")
+    with pytest.raises(TypeError, match="plan.status"):
+        ap.block_tables(pool, lens, new, tables, 6, plan=plan)
+    plan.status = torch.full((1,), 9, dtype=torch.int32, device="cuda")
+    plan.slots = slots = torch.full((6,), 77, dtype=torch.int32, device="cuda")
+    ap.block_tables(pool, lens, new, tables, 6, plan=plan)
+    assert plan.status.item() == 0 and (slots >= 0).all() and (slots < 128).all()
