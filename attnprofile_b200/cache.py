@@ -280,10 +280,10 @@ def _rows(name, x, index, heads, dim):
     shape = x.shape
     if len(shape) != 3 or shape[2] != dim or (heads and shape[1] != heads):
         raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {dim}]")
-    strides = x.stride()
-    if strides[2] != 1:
+    token, head, one = x.stride()
+    if one != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    return kind, shape, strides[0] if shape[0] > 1 else 0, strides[1] if shape[1] > 1 else 0
+    return kind, shape, token if shape[0] > 1 else 0, head if shape[1] > 1 else 0
 
 
 def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
@@ -299,9 +299,13 @@ def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
     index = cache.device.index
     heads, dim = cache.kv_heads, cache.dim
     kind, shape, k_token, k_head = _rows("k", k, index, heads, dim)
-    v_kind, v_shape, v_token, v_head = _rows("v", v, index, heads, dim)
-    if v_kind != kind or v_shape != shape:
-        raise ValueError("k and v must share one shape and dtype")
+    if (v.dtype is k.dtype and v.shape == shape and v.get_device() == index
+            and v.stride() == k.stride()):  # the usual: slices of one projection
+        v_token, v_head = k_token, k_head
+    else:
+        v_kind, v_shape, v_token, v_head = _rows("v", v, index, heads, dim)
+        if v_kind != kind or v_shape != shape:
+            raise ValueError("k and v must share one shape and dtype")
     tokens = shape[0]
     _call("attn_cache_append", index, _APPEND(
         k.data_ptr(), v.data_ptr(), _ints("slots", slots, index, tokens), *cache.ptrs, k_token,
