@@ -31,10 +31,15 @@ struct Request {
   int start, n, kv;  // first query row, rows, tokens in the cache
 };
 
+// FROM_L2: for the joining kernels, which ask before they wait for the kernel in
+// front of them; only that wait makes L1 follow what was written since.  (L2 for
+// all: 102 us where this took 91 on 64 requests of 5 to 8191 tokens.)
+template <bool FROM_L2 = false>
 __device__ __forceinline__ Request request_at(const CachedParams& p, int r) {
-  const int a = min(max(p.starts[r], 0), p.tokens);
-  const int b = min(max(p.starts[r + 1], 0), p.tokens);
-  return Request{a, min(max(b - a, 0), p.max_new), min(max(p.kv_lens[r], 0), p.capacity)};
+  auto load = [](const int* x) { return FROM_L2 ? __ldcg(x) : *x; };
+  const int a = min(max(load(p.starts + r), 0), p.tokens);
+  const int b = min(max(load(p.starts + r + 1), 0), p.tokens);
+  return Request{a, min(max(b - a, 0), p.max_new), min(max(load(p.kv_lens + r), 0), p.capacity)};
 }
 
 int codes_map(CUtensorMap* m, const void* codes, const CachedParams& p, int D);

@@ -132,13 +132,13 @@ __device__ __forceinline__ int quotient(long long x, long long y) {
 
 // Sum of all requests' work; a place in it is looked up afterwards: each
 // thread keeps the sum of its share of the requests.
-template <int NT>
+template <int NT, bool FROM_L2 = false>
 __device__ __forceinline__ long long count_work(const CachedParams& p, long long* part) {
   const int each = (p.batch + blockDim.x - 1) / blockDim.x;
   const int first = static_cast<int>(threadIdx.x) * each;
   long long sum = 0;
   for (int r = first; r < min(first + each, p.batch); ++r) {
-    sum += shape_of<NT>(p, request_at(p, r)).work();
+    sum += shape_of<NT>(p, request_at<FROM_L2>(p, r)).work();
   }
   // Inclusive prefix over the threads.
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -158,7 +158,7 @@ __device__ __forceinline__ long long count_work(const CachedParams& p, long long
 }
 
 // The request that holds place `at` (below the total); by one thread.
-template <int NT>
+template <int NT, bool FROM_L2 = false>
 __device__ __forceinline__ Place find_place(const CachedParams& p, const long long* part,
                                             long long at) {
   int lo = -1, hi = static_cast<int>(blockDim.x) - 1;  // first thread whose prefix is above `at`
@@ -169,7 +169,7 @@ __device__ __forceinline__ Place find_place(const CachedParams& p, const long lo
   const int each = (p.batch + blockDim.x - 1) / blockDim.x;
   Place pl{hi * each, hi > 0 ? part[hi - 1] : 0};
   while (true) {
-    const long long w = shape_of<NT>(p, request_at(p, pl.request)).work();
+    const long long w = shape_of<NT>(p, request_at<FROM_L2>(p, pl.request)).work();
     if (pl.before + w > at || pl.request + 1 >= p.batch) return pl;
     pl.before += w;
     ++pl.request;
@@ -182,12 +182,12 @@ constexpr int kLaneRequests = 128;
 struct Lanes {
   long long work, upto;  // of the lane's requests; of all up to and with them
 };
-template <int NT>
+template <int NT, bool FROM_L2 = false>
 __device__ __forceinline__ Lanes count_lanes(const CachedParams& p, long long* total) {
   const int lane = threadIdx.x & 31, each = (p.batch + 31) / 32;
   Lanes x{0, 0};
   for (int r = lane * each; r < min(lane * each + each, p.batch); ++r)
-    x.work += shape_of<NT>(p, request_at(p, r)).work();
+    x.work += shape_of<NT>(p, request_at<FROM_L2>(p, r)).work();
   x.upto = x.work;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -197,13 +197,13 @@ __device__ __forceinline__ Lanes count_lanes(const CachedParams& p, long long* t
   *total = __shfl_sync(~0u, x.upto, 31);
   return x;
 }
-template <int NT>
+template <int NT, bool FROM_L2 = false>
 __device__ __forceinline__ Place place_in(const CachedParams& p, const Lanes& x, long long at) {
   const int each = (p.batch + 31) / 32;
   const int lane = __ffs(__ballot_sync(~0u, x.upto > at)) - 1;
   Place pl{lane * each, __shfl_sync(~0u, x.upto - x.work, lane)};
   for (; pl.request + 1 < min(lane * each + each, p.batch); ++pl.request) {
-    const long long w = shape_of<NT>(p, request_at(p, pl.request)).work();
+    const long long w = shape_of<NT>(p, request_at<FROM_L2>(p, pl.request)).work();
     if (pl.before + w > at) break;
     pl.before += w;
   }
@@ -888,15 +888,15 @@ __global__ void __launch_bounds__(256) join_kernel(const CachedParams p) {
   long long total, each, cut;
   Place pl{0, 0};
   if (p.batch <= kLaneRequests) {
-    const Lanes lanes = count_lanes<NT>(p, &total);
+    const Lanes lanes = count_lanes<NT, true>(p, &total);
     each = work_each(total, gridDim.x);
     cut = each * (blockIdx.x + 1ll);
-    if (cut < total) pl = place_in<NT>(p, lanes, cut);
+    if (cut < total) pl = place_in<NT, true>(p, lanes, cut);
   } else {
-    total = count_work<NT>(p, part_sum);
+    total = count_work<NT, true>(p, part_sum);
     each = work_each(total, gridDim.x);
     cut = each * (blockIdx.x + 1ll);
-    if (threadIdx.x == 0 && cut < total) place = find_place<NT>(p, part_sum, cut);
+    if (threadIdx.x == 0 && cut < total) place = find_place<NT, true>(p, part_sum, cut);
     __syncthreads();
     pl = place;
   }
@@ -948,9 +948,9 @@ __global__ void __launch_bounds__(256) join_few_kernel(const CachedParams p, int
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // Lane r has request r.
   Shape sh{0, 1, 1};
-  if (lane < p.batch) sh = shape_of<NT>(p, request_at(p, lane));
+  if (lane < p.batch) sh = shape_of<NT>(p, request_at<true>(p, lane));
   long long total;
-  const Lanes lanes = count_lanes<NT>(p, &total);
+  const Lanes lanes = count_lanes<NT, true>(p, &total);
   const long long each = work_each(total, ctas);
   // The request that holds this unit.
   int upto = sh.units;

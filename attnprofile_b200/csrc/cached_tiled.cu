@@ -146,6 +146,7 @@ __device__ __forceinline__ int row_limit(const CachedParams& p, const Request& r
 // are short; the heads of a row tile follow each other, so that neighbours share
 // keys in L2.  (More requests than threads, each with a long prompt: in their
 // own order.)  `scratch`: 12 bytes a thread.
+template <bool FROM_L2 = false>
 __device__ bool find_unit(const CachedParams& p, long long at, Unit& u, uint8_t* scratch) {
   long long* units = reinterpret_cast<long long*>(scratch);
   int* keys = reinterpret_cast<int*>(units + kThreads);
@@ -156,7 +157,7 @@ __device__ bool find_unit(const CachedParams& p, long long at, Unit& u, uint8_t*
   long long mine = 0;
   int kv = 0;
   for (int r = first; r < last; ++r) {
-    const Request rq = request_at(p, r);
+    const Request rq = request_at<FROM_L2>(p, r);
     mine += units_of(p, rq);
     kv = rq.kv;
   }
@@ -174,18 +175,18 @@ __device__ bool find_unit(const CachedParams& p, long long at, Unit& u, uint8_t*
     if (at >= before && at < before + mine) {
       int r = first;
       for (; r + 1 < last; ++r) {
-        const long long n = units_of(p, request_at(p, r));
+        const long long n = units_of(p, request_at<FROM_L2>(p, r));
         if (at < before + n) break;
         before += n;
       }
       where[0] = r;
-      where[1] = units_of(p, request_at(p, r)) - 1 - (at - before);
+      where[1] = units_of(p, request_at<FROM_L2>(p, r)) - 1 - (at - before);
     }
   }
   __syncthreads();
   if (where[0] < 0) return false;
   u.request = static_cast<int>(where[0]);
-  u.rq = request_at(p, u.request);
+  u.rq = request_at<FROM_L2>(p, u.request);
   const int in_request = static_cast<int>(where[1]);
   u.kvh = in_request % p.kv_heads;
   u.row0 = in_request / p.kv_heads * kUnit;
@@ -977,7 +978,7 @@ template <typename TQ, int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const TiledParams p) {
   __shared__ __align__(16) uint8_t scratch[12 * kThreads];
   Unit u;
-  const bool there = find_unit(p, blockIdx.x, u, scratch);
+  const bool there = find_unit<true>(p, blockIdx.x, u, scratch);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!there) return;
   const int lane = threadIdx.x & 31, r = 16 * blockIdx.y + (threadIdx.x >> 5);
