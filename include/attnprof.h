@@ -357,8 +357,11 @@ int attn_cache_append(const attn_cache_append_args* args, void* stream);
  * scores (0: 1 / sqrt(D)).  A row that sees no token becomes 0.  Rows behind
  * starts[batch] are left as they were; rows of a request beyond max_new are
  * not computed.  out must not overlap q.  Scales must be positive; V scales and
- * the codes of tokens held must be finite numbers, |v| below 2^100.  What lies in slots that
- * hold no token is never used, whatever it is.  kv_lens is taken as at most
+ * the codes of tokens held must be finite numbers, |v| below 2^100.  For many rows
+ * values are held in f16 relative to the largest V scale of the request and
+ * head: those of a block whose scale is below 2^-22 of it keep an absolute
+ * accuracy of 2^-32 of it only.  What lies in slots that hold no token is never
+ * used, whatever it is.  kv_lens is taken as at most
  * width * block_size, starts as within [0, tokens]; a table entry that is no
  * block of the pool is left out.
  * workspace: 16-byte aligned, attn_cached_workspace(...) bytes (NULL where
