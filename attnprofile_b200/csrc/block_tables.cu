@@ -78,6 +78,12 @@ __device__ __forceinline__ int last_at_most(const int* first, int n, int x) {
   return lo;
 }
 
+// Bits 0 and 1 that any thread of the CTA has.
+__device__ __forceinline__ int any_of(int bad) {
+  if (!__syncthreads_or(bad)) return 0;
+  return (__syncthreads_or(bad & 1) ? 1 : 0) | (__syncthreads_or(bad & 2) ? 2 : 0);
+}
+
 __device__ __forceinline__ void end_of_reading(int ctas) {
   if (ctas > 1)
     ptx::cluster_sync();
@@ -97,6 +103,7 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
   int* len = sm + 2 * p.batch;          // [batch] tokens held before
   __shared__ Counts warp_sum[kThreads / 32];
   begin_behind();
+  const int count = *p.free_count;
   const int ctas = static_cast<int>(gridDim.x);
   const int mask = (1 << p.shift) - 1;
 
@@ -125,8 +132,7 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
       len[r] = l;
     }
   }
-  const int count = *p.free_count;
-  bad = (__syncthreads_or(bad & 1) ? 1 : 0) | (__syncthreads_or(bad & 2) ? 2 : 0);
+  bad = any_of(bad);
   int status = ATTN_BLOCKS_OK;
   if (count < 0 || count > p.num_blocks || total.blocks > count) status = ATTN_BLOCKS_POOL;
   if (bad & 1) status = ATTN_BLOCKS_ROW;
@@ -157,8 +163,9 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
     *p.free_left = count - taken;
     *p.status = status;
   }
-  // New blocks into the tables.
-  for (int j = me; j < taken; j += all) {
+  // New blocks into the tables, by the last threads first: the first ones have
+  // the slots below, and loads of their own to wait for.
+  for (int j = all - 1 - me; j < taken; j += all) {
     const int r = last_at_most(first, p.batch, j);
     const int column = ((len[r] + mask) >> p.shift) + (j - first[r]);
     p.tables[r * p.table_stride + column] = p.free_blocks[count - 1 - j];
@@ -213,6 +220,7 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
   int* left = sm + p.batch;     // [batch] tokens kept
   __shared__ Counts warp_sum[kThreads / 32];
   begin_behind();
+  const int count = *p.free_count;
   const int ctas = static_cast<int>(gridDim.x);
   const int mask = (1 << p.shift) - 1;
 
@@ -237,8 +245,7 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
       left[r] = l;
     }
   }
-  const int count = *p.free_count;
-  bad = (__syncthreads_or(bad & 1) ? 1 : 0) | (__syncthreads_or(bad & 2) ? 2 : 0);
+  bad = any_of(bad);
   int status = ATTN_BLOCKS_OK;
   // More blocks than the pool has: some were given back before.
   if (count < 0 || count + total.blocks > p.num_blocks) status = ATTN_BLOCKS_POOL;
