@@ -15,6 +15,7 @@
 // barrier ends the reading, and then all threads of the cluster write.  The
 // barrier makes in-place calls (kv_lens = lens, free_left = free_count) safe
 // without any scratch memory, atomics or order between CTAs.
+#include <algorithm>
 #include <initializer_list>
 
 #include "cache.cuh"
@@ -36,6 +37,7 @@ struct Counts {
 __device__ __forceinline__ Counts scan_threads(Counts v, Counts carry, Counts* total,
                                                Counts* warp_sum) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int warps = static_cast<int>(blockDim.x) >> 5;
   Counts in = v;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -49,7 +51,7 @@ __device__ __forceinline__ Counts scan_threads(Counts v, Counts carry, Counts* t
   if (lane == 31) warp_sum[warp] = in;
   __syncthreads();
   if (warp == 0) {
-    Counts w = lane < kThreads / 32 ? warp_sum[lane] : Counts{0, 0};
+    Counts w = lane < warps ? warp_sum[lane] : Counts{0, 0};
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const long long a = __shfl_up_sync(~0u, w.tokens, d), b = __shfl_up_sync(~0u, w.blocks, d);
@@ -58,11 +60,11 @@ __device__ __forceinline__ Counts scan_threads(Counts v, Counts carry, Counts* t
         w.blocks += b;
       }
     }
-    if (lane < kThreads / 32) warp_sum[lane] = w;
+    if (lane < warps) warp_sum[lane] = w;
   }
   __syncthreads();
   const Counts before = warp > 0 ? warp_sum[warp - 1] : Counts{0, 0};
-  const Counts all = warp_sum[kThreads / 32 - 1];
+  const Counts all = warp_sum[warps - 1];
   *total = Counts{carry.tokens + all.tokens, carry.blocks + all.blocks};
   return Counts{carry.tokens + before.tokens + in.tokens - v.tokens,
                 carry.blocks + before.blocks + in.blocks - v.blocks};
@@ -104,12 +106,12 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
   __shared__ Counts warp_sum[kThreads / 32];
   begin_behind();
   const int count = *p.free_count;
-  const int ctas = static_cast<int>(gridDim.x);
+  const int ctas = static_cast<int>(gridDim.x), threads = static_cast<int>(blockDim.x);
   const int mask = (1 << p.shift) - 1;
 
   Counts total{0, 0};
   int bad = 0;  // bit 0: a row of the table is too short, bit 1: a negative number
-  for (int base = 0; base < p.batch; base += kThreads) {
+  for (int base = 0; base < p.batch; base += threads) {
     const int r = base + static_cast<int>(threadIdx.x);
     Counts v{0, 0};
     int l = 0;
@@ -144,8 +146,8 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
 
   end_of_reading(ctas);
 
-  const int me = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
-  const int all = ctas * kThreads;
+  const int me = static_cast<int>(blockIdx.x) * threads + static_cast<int>(threadIdx.x);
+  const int all = ctas * threads;
   // The step's lengths and the pool's count: one thread each.
   for (int r = me; r < p.batch; r += all) {
     // (p.lens may be p.kv_lens: len[] has it where it is not negative)
@@ -221,12 +223,12 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
   __shared__ Counts warp_sum[kThreads / 32];
   begin_behind();
   const int count = *p.free_count;
-  const int ctas = static_cast<int>(gridDim.x);
+  const int ctas = static_cast<int>(gridDim.x), threads = static_cast<int>(blockDim.x);
   const int mask = (1 << p.shift) - 1;
 
   Counts total{0, 0};
   int bad = 0;
-  for (int base = 0; base < p.batch; base += kThreads) {
+  for (int base = 0; base < p.batch; base += threads) {
     const int r = base + static_cast<int>(threadIdx.x);
     Counts v{0, 0};
     int l = 0;
@@ -256,8 +258,8 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
 
   end_of_reading(ctas);
 
-  const int me = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
-  const int all = ctas * kThreads;
+  const int me = static_cast<int>(blockIdx.x) * threads + static_cast<int>(threadIdx.x);
+  const int all = ctas * threads;
   for (int r = me; r < p.batch; r += all) {
     if (ok)
       p.lens_left[r] = left[r];
@@ -275,16 +277,22 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
   }
 }
 
-// One CTA where 4 entries a thread do all of the writing, else a cluster.
-int ctas_for(long long entries) { return entries > 4 * kThreads ? kClusterCtas : 1; }
-
+// One CTA where 4 entries a thread do all of the writing, of no more threads
+// than that and the requests need (barriers and the scan of fewer warps are
+// shorter: 256 requests of a token each 4.1 us with 256 threads, 4.8 with 1024);
+// else a cluster.
 template <typename P>
-int launch_cluster(void (*kern)(P), const P& p, int ctas, size_t smem, cudaStream_t st) {
+int launch_cluster(void (*kern)(P), const P& p, long long entries, size_t smem, cudaStream_t st) {
+  const int ctas = entries > 4 * kThreads ? kClusterCtas : 1;
+  const long long wanted = std::max<long long>((entries + 3) / 4, p.batch);
+  const int threads =
+      ctas > 1 ? kThreads
+               : static_cast<int>(std::min<long long>(std::max(wanted, 1ll) + 31, kThreads)) & ~31;
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(smem)) != cudaSuccess)
     return ATTN_ERR_RESOURCE;
-  return launch_behind(kern, dim3(static_cast<unsigned>(ctas)), kThreads, smem, ctas, st, p) ==
+  return launch_behind(kern, dim3(static_cast<unsigned>(ctas)), threads, smem, ctas, st, p) ==
                  cudaSuccess
              ? ATTN_OK
              : ATTN_ERR_CUDA;
@@ -323,7 +331,7 @@ extern "C" int attn_block_tables(const attn_block_tables_args* args, void* strea
                         static_cast<const void*>(a.free_left), static_cast<const void*>(a.status)})
     if (!aligned(x, 4)) return ATTN_ERR_MISALIGNED;
   const TablesParams p{a, shift_of(a.block_size)};
-  return launch_cluster(tables_kernel, p, ctas_for(a.tokens), 3ull * sizeof(int) * a.batch,
+  return launch_cluster(tables_kernel, p, a.tokens, 3ull * sizeof(int) * a.batch,
                         static_cast<cudaStream_t>(stream));
 }
 
@@ -343,6 +351,6 @@ extern "C" int attn_block_trim(const attn_block_trim_args* args, void* stream) {
     if (!aligned(x, 4)) return ATTN_ERR_MISALIGNED;
   const TrimParams p{a, shift_of(a.block_size)};
   const long long most = static_cast<long long>(a.batch) * a.width;
-  return launch_cluster(trim_kernel, p, ctas_for(most < a.num_blocks ? most : a.num_blocks),
+  return launch_cluster(trim_kernel, p, std::min<long long>(most, a.num_blocks),
                         2ull * sizeof(int) * a.batch, static_cast<cudaStream_t>(stream));
 }
