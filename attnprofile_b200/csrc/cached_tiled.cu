@@ -822,30 +822,53 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     const float neg = m == -INFINITY ? 0.f : kLift - m;
     const uint64_t neg2 = ptx::f2_pack(neg, neg);
     uint64_t part[2] = {0ull, 0ull};
+    // A batch's exponentials are asked for before the last batch's are used, and
+    // where P has columns of its own the first 32 wait in registers for the last
+    // step's P V: 70.5 -> 69.4 us on a prompt of 4096, 16 heads of 64 (batches of
+    // 2 pairs 70.4, of 16 69.6); at D = 128 no difference.
+    constexpr int kBatch = 8;  // pairs
+    uint32_t pk[2][16];
+    float before[2 * kBatch];
 #pragma unroll
-    for (int b = 0; b < kBN / 32; ++b) {
-      uint32_t pk[16];
+    for (int at = 0; at <= kBN / 2; at += kBatch) {
+      float x[2 * kBatch];
+      if (at < kBN / 2) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int c0 = 32 * b + 2 * e;
-        const float f = factor[c0 / 16];
-        const uint64_t x2 = ptx::f2_fma(
-            ptx::f2_pack(__uint_as_float(s[c0]), __uint_as_float(s[c0 + 1])), ptx::f2_pack(f, f),
-            neg2);
-        float x0, x1;
-        ptx::f2_unpack(x2, x0, x1);
-        const float p0 = ptx::ex2_approx(x0), p1 = ptx::ex2_approx(x1);
-        part[e & 1] = ptx::f2_add(part[e & 1], ptx::f2_pack(p0, p1));
-        pk[e] = half2_of(p0, p1);
+        for (int e = 0; e < kBatch; ++e) {
+          const int c0 = 2 * (at + e);
+          const float f = factor[c0 / 16];
+          const uint64_t x2 = ptx::f2_fma(
+              ptx::f2_pack(__uint_as_float(s[c0]), __uint_as_float(s[c0 + 1])), ptx::f2_pack(f, f),
+              neg2);
+          ptx::f2_unpack(x2, x[2 * e], x[2 * e + 1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2 * kBatch; ++e) x[e] = ptx::ex2_approx(x[e]);
       }
-      if (b == 0) pv_wait();
-      ptx::tmem_st16(lane_base + p_col + 16 * b, pk);
-      if (b == 1) {  // P V of 64 keys may begin
-        ptx::tmem_wait_st();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(Bar<D>::kP + 2 * i));
+      if (at > 0) {
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) {
+          const int k = at - kBatch + e;
+          part[e & 1] = ptx::f2_add(part[e & 1], ptx::f2_pack(before[2 * e], before[2 * e + 1]));
+          pk[(k / 16) & 1][k % 16] = half2_of(before[2 * e], before[2 * e + 1]);
+        }
+        if (at == 16 && !T::kOwnP) ptx::tmem_st16(lane_base + p_col, pk[0]);
+        if (at == 32) {
+          if (T::kOwnP) {
+            pv_wait();
+            ptx::tmem_st16(lane_base + p_col, pk[0]);
+          }
+          ptx::tmem_st16(lane_base + p_col + 16, pk[1]);
+          ptx::tmem_wait_st();  // P V of 64 keys may begin
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(bar(Bar<D>::kP + 2 * i));
+        }
+        if (at == 48) ptx::tmem_st16(lane_base + p_col + 32, pk[0]);
+        if (at == 64) ptx::tmem_st16(lane_base + p_col + 48, pk[1]);
       }
+#pragma unroll
+      for (int e = 0; e < 2 * kBatch; ++e) before[e] = x[e];
     }
     ptx::tmem_wait_st();
     ptx::tc_fence_before();
