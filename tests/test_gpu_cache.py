@@ -862,3 +862,52 @@ def test_a_plan_is_checked_again_where_it_changed(ap):
     plan.slots = slots = torch.full((6,), 77, dtype=torch.int32, device="cuda")
     ap.block_tables(pool, lens, new, tables, 6, plan=plan)
     assert plan.status.item() == 0 and (slots >= 0).all() and (slots < 128).all()
+
+
+@pytest.mark.parametrize("max_len", [400, 4000])
+def test_captured_behind_copies_and_another_stream(ap, max_len):
+    """A graph in which copies, a cleared buffer and a kernel of another stream
+    come right before the calls gives the bits of calls outside a graph."""
+    bs, heads, kv_heads, dim, rows, most = 16, 4, 2, 64, 2, max_len // 8
+    tokens = 2 * most
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    staged = torch.zeros(tokens, heads + 2 * kv_heads, dim, device="cuda").half()
+    staged_lens, factor = ints([0, 0]), torch.ones(1, device="cuda").half()
+
+    def fresh():
+        blocks = rows * (max_len // bs + 1)
+        batch = ap.CacheBatch(ap.BlockPool.full(blocks, bs), rows, max_len, tokens)
+        cache = ap.PagedCache.empty(blocks, kv_heads, dim, block_size=bs)
+        return batch, cache, torch.zeros_like(staged), torch.zeros_like(staged[:, :heads]), ints([0, 0])
+
+    side = torch.cuda.Stream()
+
+    def step(batch, cache, qkv, out, new):
+        here = torch.cuda.current_stream()
+        qkv.copy_(staged)
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            qkv.mul_(factor)
+        new.copy_(staged_lens)
+        out.zero_()
+        batch.advance(new, tokens)
+        here.wait_stream(side)
+        batch.attend(cache, qkv[:, :heads], qkv[:, heads:heads + kv_heads],
+                     qkv[:, heads + kv_heads:], max_new=most, out=out)
+
+    plain, caught = fresh(), fresh()
+    step(*caught)  # (no tokens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*caught)
+    for new in ([most, 3], [1, most], [1, 1], [2, 1], [most, most], [1, 1]):
+        staged.copy_(torch.randn(staged.shape, generator=gen, device="cuda"))
+        factor.fill_(0.5 + new[0] % 3)
+        staged_lens.copy_(ints(new))
+        step(*plain)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert plain[0].status.item() == 0 and torch.equal(plain[0].lens, caught[0].lens)
+        assert torch.equal(plain[3], caught[3]) and caught[3][:sum(new)].isfinite().all()
+        assert caught[3][:sum(new)].abs().sum() > 0
