@@ -149,9 +149,34 @@ __device__ __forceinline__ int row_limit(const CachedParams& p, const Request& r
 // the last rows (causal: those that see most), so that the last CTAs to start
 // are short; the heads of a row tile follow each other, so that neighbours share
 // keys in L2.  (More requests than threads, each with a long prompt: in their
-// own order.)  `scratch`: 12 bytes a thread.
-template <bool FROM_L2 = false>
-__device__ bool find_unit(const CachedParams& p, long long at, Unit& u, uint8_t* scratch) {
+// own order.)  Up to 32 requests: every warp for itself, a lane a request (without
+// barriers: 68.4 us on one prompt of 4096, 69.5 with them).
+template <bool FROM_L2>
+__device__ __forceinline__ bool find_request_few(const CachedParams& p, long long at, Unit& u,
+                                                 int& in_request) {
+  const int lane = threadIdx.x & 31;
+  Request rq{0, 0, 0};
+  if (lane < p.batch) rq = request_at<FROM_L2>(p, lane);
+  const long long mine = lane < p.batch ? units_of(p, rq) : 0;
+  long long before = 0;
+  for (int i = 0; i < p.batch; ++i) {
+    const int kv = __shfl_sync(~0u, rq.kv, i);
+    const long long n = __shfl_sync(~0u, mine, i);
+    if (kv > rq.kv || (kv == rq.kv && i < lane)) before += n;
+  }
+  const unsigned there = __ballot_sync(~0u, at >= before && at < before + mine);
+  if (there == 0) return false;
+  u.request = __ffs(there) - 1;
+  u.rq = Request{__shfl_sync(~0u, rq.start, u.request), __shfl_sync(~0u, rq.n, u.request),
+                 __shfl_sync(~0u, rq.kv, u.request)};
+  in_request = __shfl_sync(~0u, static_cast<int>(mine - 1 - (at - before)), u.request);
+  return true;
+}
+
+// The same for any number, by the whole CTA.  `scratch`: 12 bytes a thread.
+template <bool FROM_L2>
+__device__ __forceinline__ bool find_request(const CachedParams& p, long long at, Unit& u,
+                                             int& in_request, uint8_t* scratch) {
   long long* units = reinterpret_cast<long long*>(scratch);
   int* keys = reinterpret_cast<int*>(units + kThreads);
   __shared__ long long where[2];
@@ -191,7 +216,16 @@ __device__ bool find_unit(const CachedParams& p, long long at, Unit& u, uint8_t*
   if (where[0] < 0) return false;
   u.request = static_cast<int>(where[0]);
   u.rq = request_at<FROM_L2>(p, u.request);
-  const int in_request = static_cast<int>(where[1]);
+  in_request = static_cast<int>(where[1]);
+  return true;
+}
+
+template <bool FROM_L2 = false>
+__device__ bool find_unit(const CachedParams& p, long long at, Unit& u, uint8_t* scratch) {
+  int in_request;
+  if (!(p.batch <= 32 ? find_request_few<FROM_L2>(p, at, u, in_request)
+                      : find_request<FROM_L2>(p, at, u, in_request, scratch)))
+    return false;
   u.kvh = in_request % p.kv_heads;
   u.row0 = in_request / p.kv_heads * kUnit;
   u.rows_in = u.rq.n * p.group;
