@@ -343,9 +343,9 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     kv_lens[r] tokens lie in the blocks tables[r] (they are in the cache
     already).  Row i of n sees the first kv_lens[r] - n + i + 1 tokens (causal)
     or all of them; a row that sees none becomes 0.  max_new: the most rows of
-    any request.  scale: of the scores, 1 / sqrt(D) by default.  Rows of `out`
-    behind starts[-1] are left as they were (with out=None: undefined); out
-    must not overlap q.  With many rows a block whose V scale is below 2^-22 of
+    any request; n counts those beyond it too.  scale: of the scores,
+    1 / sqrt(D) by default.  Rows of `out` beyond max_new and behind starts[-1]
+    are left as they were (with out=None: undefined); out must not overlap q.  With many rows a block whose V scale is below 2^-22 of
     the request's largest (of that head) keeps an absolute accuracy only, 2^-32
     of that scale.
     workspace: a uint8 tensor to use instead of a new one per call, of

@@ -28,7 +28,8 @@ struct CachedParams {
 
 // A request as the kernels see it, with every number brought into range.
 struct Request {
-  int start, n, kv;  // first query row, rows, tokens in the cache
+  int start, n, kv;  // first query row, rows computed, tokens in the cache
+  int before;        // tokens in front of the first row's own; negative: it has none
 };
 
 // FROM_L2: for the joining kernels, which ask before they wait for the kernel in
@@ -39,7 +40,9 @@ __device__ __forceinline__ Request request_at(const CachedParams& p, int r) {
   auto load = [](const int* x) { return FROM_L2 ? __ldcg(x) : *x; };
   const int a = min(max(load(p.starts + r), 0), p.tokens);
   const int b = min(max(load(p.starts + r + 1), 0), p.tokens);
-  return Request{a, min(max(b - a, 0), p.max_new), min(max(load(p.kv_lens + r), 0), p.capacity)};
+  const int rows = max(b - a, 0), kv = min(max(load(p.kv_lens + r), 0), p.capacity);
+  // All rows count for what a row sees, those beyond max_new too.
+  return Request{a, min(rows, p.max_new), kv, kv - rows};
 }
 
 int codes_map(CUtensorMap* m, const void* codes, const CachedParams& p, int D);

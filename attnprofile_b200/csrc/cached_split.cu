@@ -499,7 +499,7 @@ __device__ void compute_role(const SplitParams& p, Cursor<NT> cursor, uint32_t s
         row_f[nt][j] = __shfl_sync(~0u, mine, (2 * t + j) * 4);
         const int r = x.row0 + 8 * nt + 2 * t + j;
         // (rows behind the last one: zeros that see everything)
-        limit[nt][j] = r < rows_in && p.causal ? rq.kv - rq.n + r / p.group + 1 : rq.kv;
+        limit[nt][j] = r < rows_in && p.causal ? rq.before + r / p.group + 1 : rq.kv;
         limit[nt][j] = min(limit[nt][j], rq.kv);
         least = min(least, limit[nt][j]);
       }

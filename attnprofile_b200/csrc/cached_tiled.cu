@@ -141,7 +141,7 @@ __device__ __forceinline__ long long units_of(const CachedParams& p, const Reque
 
 // Tokens that a row sees.
 __device__ __forceinline__ int row_limit(const CachedParams& p, const Request& rq, int row) {
-  const int last = p.causal ? rq.kv - rq.n + row / p.group + 1 : rq.kv;
+  const int last = p.causal ? rq.before + row / p.group + 1 : rq.kv;
   return min(max(last, 0), rq.kv);
 }
 
@@ -155,7 +155,7 @@ template <bool FROM_L2>
 __device__ __forceinline__ bool find_request_few(const CachedParams& p, long long at, Unit& u,
                                                  int& in_request) {
   const int lane = threadIdx.x & 31;
-  Request rq{0, 0, 0};
+  Request rq{0, 0, 0, 0};
   if (lane < p.batch) rq = request_at<FROM_L2>(p, lane);
   const long long mine = lane < p.batch ? units_of(p, rq) : 0;
   long long before = 0;
@@ -168,7 +168,7 @@ __device__ __forceinline__ bool find_request_few(const CachedParams& p, long lon
   if (there == 0) return false;
   u.request = __ffs(there) - 1;
   u.rq = Request{__shfl_sync(~0u, rq.start, u.request), __shfl_sync(~0u, rq.n, u.request),
-                 __shfl_sync(~0u, rq.kv, u.request)};
+                 __shfl_sync(~0u, rq.kv, u.request), __shfl_sync(~0u, rq.before, u.request)};
   in_request = __shfl_sync(~0u, static_cast<int>(mine - 1 - (at - before)), u.request);
   return true;
 }

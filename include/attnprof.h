@@ -355,10 +355,10 @@ int attn_cache_append(const attn_cache_append_args* args, void* stream);
  * kv head h / (heads / kv_heads).  With causal != 0, row i of n sees the first
  * kv_lens[r] - n + i + 1 tokens, else all kv_lens[r].  scale multiplies the
  * scores (0: 1 / sqrt(D)).  A row that sees no token becomes 0.  Rows behind
- * starts[batch] are left as they were; rows of a request beyond max_new are
- * not computed.  out must not overlap q.  Scales must be positive; V scales and
- * the codes of tokens held must be finite numbers, |v| below 2^100.  For many rows
- * values are held in f16 relative to the largest V scale of the request and
+ * starts[batch] are left as they were; so are rows of a request beyond max_new
+ * (n counts them all the same).  out must not overlap q.  Scales must be
+ * positive; V scales and the codes of tokens held must be finite numbers, |v|
+ * below 2^100.  For many rows values are held in f16 relative to the largest V scale of the request and
  * head: those of a block whose scale is below 2^-22 of it keep an absolute
  * accuracy of 2^-32 of it only.  What lies in slots that hold no token is never
  * used, whatever it is.  kv_lens is taken as at most

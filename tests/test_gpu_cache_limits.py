@@ -1,0 +1,65 @@
+"""The paged 8-bit cache at the limits of what its calls allow: fewer rows than
+requests have, scales far from one and from each other, batches next to the
+shared memory's limits, arrays that are replaced, every call on a stream given
+by name.  Against plain implementations in 64 bits (tests/cache_ref.py)."""
+import math
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests import cache_ref as ref  # noqa: E402
+from tests.test_gpu_cache import CODES, E4M3, INT8, TYPES, ints, make_cache  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+@pytest.fixture(scope="module")
+def ap(engine):
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return engine
+
+
+def rows_of(kv_lens, bs):
+    """Table rows for requests of these lengths, one after the other."""
+    counts = [ref.blocks_of(n, bs) for n in kv_lens]
+    tables, at = [], 0
+    for n in counts:
+        tables.append(list(range(at, at + n)) + [-1] * (max(counts) - n))
+        at += n
+    return tables, at
+
+
+# --------------------------------------------------------------------------- rows beyond max_new
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("dim,heads,kv_heads,max_new,kv_lens,given", [
+    (64, 2, 1, 3, [640], [203]), (128, 4, 1, 2, [300, 77, 5], [9, 2, 5]),   # the split kernel
+    (64, 2, 2, 5, [3000, 64], [12, 1]),                                     # its joining kernels
+    (64, 2, 1, 50, [640], [250]), (128, 2, 1, 50, [400, 90], [120, 3]),     # the tiled kernel
+    (128, 3, 1, 40, [4100], [300]), (64, 2, 2, 150, [700, 400], [400, 150]),
+])
+def test_rows_beyond_max_new_leave_the_others_as_they_are(ap, kind, dim, heads, kv_heads, max_new,
+                                                          kv_lens, given):
+    """Causal rows see the tokens up to their own, however many rows follow them."""
+    bs = 16
+    tables, blocks = rows_of(kv_lens, bs)
+    cache, host = make_cache(ap, blocks, kv_heads, bs, dim, E4M3, dim + max_new)
+    starts = [sum(given[:i]) for i in range(len(given) + 1)]
+    gen = torch.Generator().manual_seed(max_new)
+    q = torch.randn(starts[-1], heads, dim, generator=gen).to(kind)
+    want, tol = ref.attend_ref(q, *host, tables, kv_lens, starts, True)
+    out = torch.full(q.shape, 3.0, dtype=kind, device="cuda")
+    ap.attn_cached(q.cuda(), cache, ints(tables), ints(kv_lens), ints(starts), max_new=max_new,
+                   out=out)
+    got = out.double().cpu()
+    for a, b in zip(starts, starts[1:]):
+        m = min(b, a + max_new)
+        off = (got[a:m] - want[a:m]).abs() / tol[a:m]
+        assert torch.all(off <= 1), f"off by {off.max():.3g} times"
+        assert torch.all(got[m:b] == 3)
