@@ -16,6 +16,7 @@
 // barrier makes in-place calls (kv_lens = lens, free_left = free_count) safe
 // without any scratch memory, atomics or order between CTAs.
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 
 #include "cache.cuh"
@@ -280,18 +281,28 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
 // One CTA where 4 entries a thread do all of the writing, of no more threads
 // than that and the requests need (barriers and the scan of fewer warps are
 // shorter: 256 requests of a token each 4.1 us with 256 threads, 4.8 with 1024);
-// else a cluster.
+// else a cluster.  ints: of shared memory for each request.
 template <typename P>
-int launch_cluster(void (*kern)(P), const P& p, long long entries, size_t smem, cudaStream_t st) {
+int launch_cluster(void (*kern)(P), const P& p, long long entries, int ints, cudaStream_t st) {
   const int ctas = entries > 4 * kThreads ? kClusterCtas : 1;
   const long long wanted = std::max<long long>((entries + 3) / 4, p.batch);
   const int threads =
       ctas > 1 ? kThreads
                : static_cast<int>(std::min<long long>(std::max(wanted, 1ll) + 31, kThreads)) & ~31;
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(smem)) != cudaSuccess)
-    return ATTN_ERR_RESOURCE;
+  // Once per device and kernel (P names it), for the largest batch: the limit
+  // without it counts the kernel's own shared memory too, and a limit that
+  // followed each call's size could be lowered by another thread's.
+  static std::atomic<bool> set_up[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return ATTN_ERR_CUDA;
+  if (dev >= 64 || !set_up[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             ints * static_cast<int>(sizeof(int)) * ATTN_BLOCKS_MAX_BATCH) !=
+        cudaSuccess)
+      return ATTN_ERR_RESOURCE;
+    if (dev < 64) set_up[dev].store(true, std::memory_order_release);
+  }
+  const size_t smem = sizeof(int) * ints * p.batch;
   return launch_behind(kern, dim3(static_cast<unsigned>(ctas)), threads, smem, ctas, st, p) ==
                  cudaSuccess
              ? ATTN_OK
@@ -331,8 +342,7 @@ extern "C" int attn_block_tables(const attn_block_tables_args* args, void* strea
                         static_cast<const void*>(a.free_left), static_cast<const void*>(a.status)})
     if (!aligned(x, 4)) return ATTN_ERR_MISALIGNED;
   const TablesParams p{a, shift_of(a.block_size)};
-  return launch_cluster(tables_kernel, p, a.tokens, 3ull * sizeof(int) * a.batch,
-                        static_cast<cudaStream_t>(stream));
+  return launch_cluster(tables_kernel, p, a.tokens, 3, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int attn_block_trim(const attn_block_trim_args* args, void* stream) {
@@ -351,6 +361,6 @@ extern "C" int attn_block_trim(const attn_block_trim_args* args, void* stream) {
     if (!aligned(x, 4)) return ATTN_ERR_MISALIGNED;
   const TrimParams p{a, shift_of(a.block_size)};
   const long long most = static_cast<long long>(a.batch) * a.width;
-  return launch_cluster(trim_kernel, p, std::min<long long>(most, a.num_blocks),
-                        2ull * sizeof(int) * a.batch, static_cast<cudaStream_t>(stream));
+  return launch_cluster(trim_kernel, p, std::min<long long>(most, a.num_blocks), 2,
+                        static_cast<cudaStream_t>(stream));
 }

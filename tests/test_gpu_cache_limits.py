@@ -63,3 +63,40 @@ def test_rows_beyond_max_new_leave_the_others_as_they_are(ap, kind, dim, heads, 
         off = (got[a:m] - want[a:m]).abs() / tol[a:m]
         assert torch.all(off <= 1), f"off by {off.max():.3g} times"
         assert torch.all(got[m:b] == 3)
+
+
+# --------------------------------------------------------------------------- batches and shared memory
+TABLES_OF = """
+import sys, torch
+sys.path.insert(0, {root!r})
+import attnprofile_b200 as ap
+new = lambda n, x: torch.full((n,), x, dtype=torch.int32, device="cuda")
+for batch in {batches}:
+    pool, tables = ap.BlockPool.full(2 * batch, 16), new(2 * batch, -1).view(batch, 2)
+    lens = new(batch, 0)
+    if {trim}:
+        lens.fill_(32)
+        tables.copy_(torch.arange(2 * batch, device="cuda").view(batch, 2))
+        pool.free_count.fill_(0)
+        status = ap.block_trim(pool, lens, new(batch, 16), tables)
+        ok = bool((lens == 16).all()) and pool.free_count.item() == batch
+        ok &= bool((pool.free[:batch] == tables[:, 1]).all())
+    else:
+        plan = ap.block_tables(pool, lens, new(batch, 1), tables, batch)
+        status = plan.status
+        ok = bool((plan.kv_lens == 1).all()) and pool.free_count.item() == batch
+        ok &= bool((plan.slots == 16 * torch.arange(batch, device="cuda")).all())
+    assert ok and status.item() == 0, batch
+print("fine")
+"""
+
+
+@pytest.mark.parametrize("trim,batches", [
+    (False, [4053, 4054]), (False, [4096]), (False, [4097, 4096, 16384, 4060]),
+    (True, [6080, 6081]), (True, [6144]), (True, [6145, 6144, 16384, 6100]),
+])
+def test_tables_and_trim_of_batches_that_fill_48_kb(ap, trim, batches):
+    """In a process of its own: no larger batch has been there before."""
+    code = TABLES_OF.format(root=str(ROOT), batches=batches, trim=trim)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "fine", r.stderr[-800:]
