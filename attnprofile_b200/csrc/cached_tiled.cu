@@ -370,7 +370,14 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
   ptx::named_bar_sync(1, 128);
   ref = fmaxf(fmaxf(misc[4], misc[5]), fmaxf(misc[6], misc[7]));
   if (!(ref > 0.f)) ref = 1.f;
-  if (warp == 0 && lane == 0) misc[2] = ref / kVLift;  // what O is multiplied by
+  // Scales so small that kVLift / ref would be above the largest f32 (ref below
+  // 2^-120) or ref / kVLift below the least normal one: 2^64 times all of them.
+  const float up = ref < 0x1p-60f ? 0x1p64f : 1.f;
+  ref *= up;
+  if (warp == 0 && lane == 0) {
+    misc[2] = ref / kVLift;  // what O is multiplied by, and then by this:
+    misc[3] = 1.f / up;
+  }
   const float to_v = kVLift / ref;
 
   // A thread's piece `it` of a tile: a row and 16 codes of it, so that the 8
@@ -408,7 +415,7 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
       const float* scale = reinterpret_cast<const float*>(sgen + T::kOffVScale) + 8 * stage;
 #pragma unroll
       for (int it = 0; it < kIters; ++it) {
-        vs[it] = scale[group_of(it)] * to_v;
+        vs[it] = scale[group_of(it)] * up * to_v;
         pow2 &= (__float_as_int(vs[it]) & 0x7fffff) == 0;
       }
       // What lies behind the last token, or where nothing was fetched, may be
@@ -914,7 +921,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
     l = l * alpha + ((sa + sb) + (sc + sd));
   }
 
-  float f = 0.f;
+  float f = 0.f, down = 1.f;
   if (u.steps > 0) {
     if (ok) {
       const bool done = T::kOwnP ? wait_bar(bar(Bar<D>::kPV + i), (c - 1) & 1, w, kSiteODone)
@@ -923,6 +930,7 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
       ptx::tc_fence_after();
     }
     f = reinterpret_cast<const float*>(sgen + T::kOffMisc)[2];
+    down = reinterpret_cast<const float*>(sgen + T::kOffMisc)[3];
   }
   // Two tiles of the same rows: tile 1 hands its sums over in the rings' place,
   // once both have no MMA left that reads there; tile 0 adds them to its own.
@@ -993,6 +1001,10 @@ __device__ void softmax_role(const TiledParams& p, const Unit& u, int i, uint32_
         o[4 * k + 2] = __float_as_uint(fmaf(y.z, other, __uint_as_float(o[4 * k + 2])));
         o[4 * k + 3] = __float_as_uint(fmaf(y.w, other, __uint_as_float(o[4 * k + 3])));
       }
+    }
+    if (down != 1.f) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * down);
     }
     if (p.parts > 1) {
       if (!live) continue;

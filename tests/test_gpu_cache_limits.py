@@ -100,3 +100,36 @@ def test_tables_and_trim_of_batches_that_fill_48_kb(ap, trim, batches):
     code = TABLES_OF.format(root=str(ROOT), batches=batches, trim=trim)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "fine", r.stderr[-800:]
+
+
+# --------------------------------------------------------------------------- scales of V
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dim,heads,kv_lens,new", [
+    (64, 2, [700, 90], [1, 1]), (64, 2, [700, 90], [70, 1]), (128, 2, [300], [200]),
+    (128, 1, [5000], [40]),
+])
+@pytest.mark.parametrize("factor", [2.0 ** -118, 0.37 * 2.0 ** -113, 2.0 ** -130])
+def test_values_of_the_smallest_scales(ap, code, dim, heads, kv_lens, new, factor):
+    """V scales down to the least numbers of 32 bits: results follow them as far
+    as bf16 reaches.  Checked after both sides are multiplied by 2^118, so that
+    the allowance keeps its meaning; it grows by half the least step of bf16
+    (2^-134) and, for scales below 2^-126, by what a product of theirs may be
+    rounded in 32 bits: n tokens' steps of 2^-150 and codes up to 448."""
+    bs = 16
+    tables, blocks = rows_of(kv_lens, bs)
+    cache, host = make_cache(ap, blocks, 1, bs, dim, code, 3)
+    host = list(host)
+    host[3] = host[3] * factor
+    cache.v_scale.copy_(host[3])
+    starts = [sum(new[:i]) for i in range(len(new) + 1)]
+    q = torch.randn(starts[-1], heads, dim, generator=torch.Generator().manual_seed(5)).bfloat16()
+    lift = 2.0 ** 118
+    host[3] = host[3].double() * lift
+    want, tol = ref.attend_ref(q, *host, tables, kv_lens, starts, True)
+    out = ap.attn_cached(q.cuda(), cache, ints(tables), ints(kv_lens), ints(starts),
+                         max_new=max(new))
+    # A sum in 32 bits of p v, each term a multiple of 2^-149 at worst: half a
+    # step for every partial sum of 16 keys and for each later factor.
+    steps = (max(kv_lens) / 16 + 64) * 2.0 ** -150 * lift
+    off = (out.double().cpu() * lift - want).abs() / (tol + 2.0 ** -134 * lift + steps)
+    assert torch.all(off <= 1), f"off by {off.max():.3g} times"
