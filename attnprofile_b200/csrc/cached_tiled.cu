@@ -30,9 +30,9 @@
 // smaller).  V's must act before the sum over keys: V is held as code * s / r
 // * 2^7 (int8: 2^8) in f16, r being the largest V scale of the blocks that the
 // unit sees, found first.  For powers of two that is exact down to s = 2^-22 r
-// (code and factor only meet f16's end below), and what is lost below is under
-// 2^-32 of the largest value that block r could hold; other scales round V to
-// f16 once.  P is rounded to f16 as in the split kernel, held as 2^7 p with p
+// (code and factor only meet f16's end below), and below it the rounding, by
+// half of f16's least step, is 2^-32 r at most (the product is formed in f32
+// where f16 would not hold the factor); other scales round V to f16 once.  P is rounded to f16 as in the split kernel, held as 2^7 p with p
 // up to 2^8 between two moves of the maximum.  bf16 queries become f16 times
 // a power of two per row.
 #include <atomic>
@@ -410,13 +410,13 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
                    : "r"(codes_at + T::codes_at(stage) + it * kRowStep * D)
                    : "memory");
     float vs[kIters];
-    bool pow2 = true;  // all factors are powers of two, or 0
+    bool pow2 = true;  // all factors are powers of two that f16 holds, or 0
     if (is_v) {
       const float* scale = reinterpret_cast<const float*>(sgen + T::kOffVScale) + 8 * stage;
 #pragma unroll
       for (int it = 0; it < kIters; ++it) {
         vs[it] = scale[group_of(it)] * up * to_v;
-        pow2 &= (__float_as_int(vs[it]) & 0x7fffff) == 0;
+        pow2 &= (__float_as_int(vs[it]) & 0x7fffff) == 0 && !(vs[it] > 0.f && vs[it] < 0x1p-24f);
       }
       // What lies behind the last token, or where nothing was fetched, may be
       // any bits: 0 * NaN would reach a sum.  (Among the keys it is masked.)
@@ -465,7 +465,7 @@ __device__ void convert_role(const TiledParams& p, const Unit& u, uint32_t sbase
         for (int i = 0; i < 8; ++i) h[i] = mul_half2(h[i], f2);
         store(it, h);
       }
-    } else {  // scales that the caller brought: one rounding to f16
+    } else {  // scales that the caller brought, or very small ones: one rounding to f16
 #pragma unroll
       for (int it = 0; it < kIters; ++it) {
         uint32_t h[8];

@@ -358,10 +358,12 @@ int attn_cache_append(const attn_cache_append_args* args, void* stream);
  * starts[batch] are left as they were; so are rows of a request beyond max_new
  * (n counts them all the same).  out must not overlap q.  Scales must be
  * positive; V scales and the codes of tokens held must be finite numbers, |v|
- * below 2^100.  For many rows values are held in f16 relative to the largest V scale of the request and
- * head: those of a block whose scale is below 2^-22 of it keep an absolute
- * accuracy of 2^-32 of it only.  What lies in slots that hold no token is never
- * used, whatever it is.  kv_lens is taken as at most
+ * below 2^100.  For many rows values are held in f16 relative to the largest V
+ * scale of the request and head: scales that are no powers of two round a value
+ * once more, by at most 2^-11 of itself, and values of a block whose scale is
+ * below 2^-22 of the largest keep an absolute accuracy of 2^-32 of that one
+ * only.  What lies in slots that hold no token is never used, whatever it is.
+ * kv_lens is taken as at most
  * width * block_size, starts as within [0, tokens]; a table entry that is no
  * block of the pool is left out.
  * workspace: 16-byte aligned, attn_cached_workspace(...) bytes (NULL where

@@ -133,3 +133,35 @@ def test_values_of_the_smallest_scales(ap, code, dim, heads, kv_lens, new, facto
     steps = (max(kv_lens) / 16 + 64) * 2.0 ** -150 * lift
     off = (out.double().cpu() * lift - want).abs() / (tol + 2.0 ** -134 * lift + steps)
     assert torch.all(off <= 1), f"off by {off.max():.3g} times"
+
+
+# --------------------------------------------------------------------------- scales of V far apart
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("power", [20, 22, 24, 25, 27, 30, 33])
+def test_values_far_below_the_largest_scale(ap, code, dim, new, power):
+    """All weight lies on blocks whose V scale is 2^-power of the largest one's:
+    values keep the stated absolute accuracy, 2^-32 of the largest scale."""
+    bs, n_kv, r = 16, 64, 2.0 ** 6
+    cache, host = make_cache(ap, 4, 1, bs, dim, code, power)
+    k, v, ks, vs = host
+    k.zero_()
+    k[0, :, :, 0] = -100  # block 0: scores of -100 * 8 * D^-1/2, no weight is left
+    ks.fill_(1.0)
+    v.copy_(v.float().abs().clamp(min=64).to(v.dtype))
+    vs.fill_(r * 2.0 ** -power)
+    vs[0] = r
+    for mine, x in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), host):
+        mine.copy_(x)
+    q = torch.zeros(new, 1, dim).bfloat16()
+    q[:, 0, 0] = 8.0
+    want, tol = ref.attend_ref(q, *host, [[0, 1, 2, 3]], [n_kv], [0, new], False)
+    out = ap.attn_cached(q.cuda(), cache, ints([[0, 1, 2, 3]]), ints([n_kv]), ints([0, new]),
+                         max_new=new, causal=False)
+    # (the allowance of the reference has an absolute part of 2^-25, which values
+    # of 2^-27 and more may not hide behind)
+    tol = tol - 2.0 ** -25 + 2.0 ** -32 * r
+    assert torch.all(want[:, 0] > 64 * r * 2.0 ** -power * 0.99)
+    off = (out.double().cpu() - want).abs() / tol
+    assert torch.all(off <= 1), f"off by {off.max():.3g} times"
