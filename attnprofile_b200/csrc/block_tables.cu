@@ -289,20 +289,21 @@ int launch_cluster(void (*kern)(P), const P& p, long long entries, int ints, cud
   const int threads =
       ctas > 1 ? kThreads
                : static_cast<int>(std::min<long long>(std::max(wanted, 1ll) + 31, kThreads)) & ~31;
-  // Once per device and kernel (P names it), for the largest batch: the limit
-  // without it counts the kernel's own shared memory too, and a limit that
-  // followed each call's size could be lowered by another thread's.
-  static std::atomic<bool> set_up[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return ATTN_ERR_CUDA;
-  if (dev >= 64 || !set_up[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             ints * static_cast<int>(sizeof(int)) * ATTN_BLOCKS_MAX_BATCH) !=
-        cudaSuccess)
-      return ATTN_ERR_RESOURCE;
-    if (dev < 64) set_up[dev].store(true, std::memory_order_release);
-  }
   const size_t smem = sizeof(int) * ints * p.batch;
+  if (smem > 40 * 1024) {  // (the 48 KB of other launches hold the kernel's own too)
+    // Once per device and kernel (P names it), for the largest batch: a limit
+    // that followed each call's size could be lowered by another thread's.
+    static std::atomic<bool> set_up[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return ATTN_ERR_CUDA;
+    if (dev >= 64 || !set_up[dev].load(std::memory_order_acquire)) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               ints * static_cast<int>(sizeof(int)) * ATTN_BLOCKS_MAX_BATCH) !=
+          cudaSuccess)
+        return ATTN_ERR_RESOURCE;
+      if (dev < 64) set_up[dev].store(true, std::memory_order_release);
+    }
+  }
   return launch_behind(kern, dim3(static_cast<unsigned>(ctas)), threads, smem, ctas, st, p) ==
                  cudaSuccess
              ? ATTN_OK
