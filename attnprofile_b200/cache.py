@@ -46,9 +46,7 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 
 
 def _stream(index, stream) -> int:
-    """The stream of a call (default: the current one of the tensors' device)."""
-    if stream is None:
-        return _raw_stream(index)
+    """The handle of a stream that a call was given."""
     if stream.device.index != index:
         raise ValueError(f"the stream is on {stream.device}, the tensors on cuda:{index}")
     return stream.cuda_stream
@@ -63,14 +61,13 @@ _CACHED = struct.Struct("@11Q5q12if").pack
 
 def _call(name, index, *args):
     """A C entry point with the tensors' device current."""
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return _call(name, index, *args)
     function = _functions.get(name)
     if function is None:
         function = _functions[name] = getattr(lib(), name)
-    if _current_device() == index:
-        rc = function(*args)
-    else:
-        with torch.cuda.device(index):
-            rc = function(*args)
+    rc = function(*args)
     if rc:
         _check(rc, name)
 
@@ -111,28 +108,61 @@ def _table(tables, index, batch):
     return tables.data_ptr(), width, row if batch > 1 else width
 
 
-class PagedCache:
+class _Checked:
+    """Tensors that are checked when they are first used, and again once one was
+    replaced or has other memory."""
+
+    __slots__ = ("_seen", "_at", "_held")
+
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        object.__setattr__(self, "_seen", None)
+        object.__setattr__(self, "_held", None)
+
+    def _keep(self, tensors, *seen):
+        """Remembers what a check gave, the tensors' addresses last.  It holds as
+        long as _at, which reads them, gives the same: their memory is held until
+        then, so that no other tensor can get the same address."""
+        seen += (tuple(t.data_ptr() for t in tensors),)
+        object.__setattr__(self, "_seen", seen)
+        object.__setattr__(self, "_at", tuple(t.data_ptr for t in tensors))
+        object.__setattr__(self, "_held", tuple(t.untyped_storage() for t in tensors))
+        return seen
+
+
+class PagedCache(_Checked):
     """Keys and values of one layer in a pool of blocks.
 
     k, v: codes [num_blocks, kv_heads, block_size, D], float8_e4m3fn or int8;
     k_scale, v_scale: float32 [num_blocks, kv_heads], all contiguous CUDA
     tensors of one device.  A code c of block b, head h stands for
-    c * scale[b, h].  The object holds the tensors and nothing else."""
+    c * scale[b, h].  The object holds the tensors and nothing else; they may
+    be replaced by others (all that belong together, before the next call)."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "num_blocks", "kv_heads", "block_size", "dim",
-                 "device", "code", "ptrs")
+    __slots__ = ("k", "v", "k_scale", "v_scale")
 
     def __init__(self, k, v, k_scale, v_scale):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._now()
+
+    def _now(self):
+        """(device index, num_blocks, kv_heads, block_size, D, code, addresses)."""
+        seen = self._seen
+        if seen is not None:
+            k, v, k_scale, v_scale = self._at
+            if seen[6] == (k(), v(), k_scale(), v_scale()):
+                return seen
+        k, v, k_scale, v_scale = tensors = self.k, self.v, self.k_scale, self.v_scale
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v must share one [num_blocks, kv_heads, block_size, D] shape "
                              "and dtype")
         if k.dtype not in _CODES:
             raise TypeError(f"unsupported codes {k.dtype} (float8_e4m3fn or int8)")
-        self.num_blocks, self.kv_heads, self.block_size, self.dim = k.shape
-        if self.block_size not in BLOCK_SIZES:
-            raise ValueError(f"block_size {self.block_size} is not one of {BLOCK_SIZES}")
-        if self.dim not in (64, 128):
-            raise ValueError(f"D = {self.dim} is not 64 or 128")
+        num_blocks, kv_heads, block_size, dim = k.shape
+        if block_size not in BLOCK_SIZES:
+            raise ValueError(f"block_size {block_size} is not one of {BLOCK_SIZES}")
+        if dim not in (64, 128):
+            raise ValueError(f"D = {dim} is not 64 or 128")
         if not k.is_cuda:
             raise ValueError("k must be a CUDA tensor")
         for name, t in (("k", k), ("v", v), ("k_scale", k_scale), ("v_scale", v_scale)):
@@ -145,9 +175,16 @@ class PagedCache:
                 raise TypeError(f"{name} must be float32")
             if t.shape != k.shape[:2]:
                 raise ValueError(f"{name} must be [num_blocks, kv_heads]")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device, self.code = k.device, _CODES[k.dtype]
-        self.ptrs = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        return self._keep(tensors, k.get_device(), num_blocks, kv_heads, block_size, dim,
+                          _CODES[k.dtype])
+
+    device = property(lambda self: self.k.device)
+    num_blocks = property(lambda self: self._now()[1])
+    kv_heads = property(lambda self: self._now()[2])
+    block_size = property(lambda self: self._now()[3])
+    dim = property(lambda self: self._now()[4])
+    code = property(lambda self: self._now()[5])
+    ptrs = property(lambda self: self._now()[6])
 
     @classmethod
     def empty(cls, num_blocks: int, kv_heads: int, dim: int, *, block_size: int = 32,
@@ -159,21 +196,35 @@ class PagedCache:
         return cls(k, v, ks, vs)
 
 
-class BlockPool:
+class BlockPool(_Checked):
     """The free blocks of a pool: the stack free[0 : free_count[0]] of block
     ids (int32, capacity = the number of blocks)."""
 
-    __slots__ = ("free", "free_count", "block_size", "num_blocks", "device")
+    __slots__ = ("free", "free_count", "block_size")
 
     def __init__(self, free, free_count, block_size: int):
+        self.free, self.free_count, self.block_size = free, free_count, block_size
+        self._now()
+
+    def _now(self):
+        """(device index, num_blocks, block_size, addresses of free and free_count)."""
+        seen = self._seen
+        if seen is not None:
+            free, free_count = self._at
+            if seen[3] == (free(), free_count()):
+                return seen
+        free, free_count, block_size = self.free, self.free_count, self.block_size
         if not free.is_cuda or free.dim() != 1 or free.numel() == 0:
             raise ValueError("free must be a CUDA tensor [num_blocks]")
         if block_size not in BLOCK_SIZES:
             raise ValueError(f"block_size {block_size} is not one of {BLOCK_SIZES}")
-        self.device, self.num_blocks, self.block_size = free.device, free.numel(), block_size
-        _ints("free", free, self.device.index, free.numel())
-        _ints("free_count", free_count, self.device.index, 1)
-        self.free, self.free_count = free, free_count
+        index, num_blocks = free.get_device(), free.numel()
+        _ints("free", free, index, num_blocks)
+        _ints("free_count", free_count, index, 1)
+        return self._keep((free, free_count), index, num_blocks, block_size)
+
+    device = property(lambda self: self.free.device)
+    num_blocks = property(lambda self: self._now()[1])
 
     @classmethod
     def full(cls, num_blocks: int, block_size: int, device="cuda"):
@@ -183,32 +234,27 @@ class BlockPool:
                    block_size)
 
 
-class BlockPlan:
+class BlockPlan(_Checked):
     """What block_tables writes: kv_lens [batch], starts [batch + 1], slots
-    [tokens] and the status word [1] (BLOCKS), all int32.  They are checked when
-    the plan is first used, and again when one is replaced; they keep their memory
-    meanwhile, as a cache's tensors do."""
+    [tokens] and the status word [1] (BLOCKS), all int32."""
 
-    __slots__ = ("kv_lens", "starts", "slots", "status", "_checked")
+    __slots__ = ("kv_lens", "starts", "slots", "status")
 
     def __init__(self, kv_lens, starts, slots, status):
         self.kv_lens, self.starts, self.slots, self.status = kv_lens, starts, slots, status
 
-    def __setattr__(self, name, value):
-        object.__setattr__(self, name, value)
-        object.__setattr__(self, "_checked", None)
-
     def _ptrs(self, index, batch, tokens):
         """Addresses of the four for `batch` requests on device `index`."""
-        checked = self._checked
-        if checked is None or checked[0] != (index, batch, tokens):
-            checked = ((index, batch, tokens),
-                       (_ints("plan.kv_lens", self.kv_lens, index, batch),
-                        _ints("plan.starts", self.starts, index, batch + 1),
-                        _ints("plan.slots", self.slots, index, tokens)),
-                       _ints("plan.status", self.status, index, 1))
-            object.__setattr__(self, "_checked", checked)
-        return checked[1], checked[2]
+        seen, want = self._seen, (index, batch, tokens)
+        if seen is not None and seen[0] == want:
+            kv_lens, starts, slots, status = self._at
+            if seen[1] == (kv_lens(), starts(), slots(), status()):
+                return seen[1]
+        _ints("plan.kv_lens", self.kv_lens, index, batch)
+        _ints("plan.starts", self.starts, index, batch + 1)
+        _ints("plan.slots", self.slots, index, tokens)
+        _ints("plan.status", self.status, index, 1)
+        return self._keep((self.kv_lens, self.starts, self.slots, self.status), want)[1]
 
     @classmethod
     def empty(cls, batch: int, tokens: int, device="cuda"):
@@ -226,21 +272,19 @@ def block_tables(pool: BlockPool, lens, new_lens, tables, tokens: int, *, plan=N
     pool.free_count becomes what is left, or keeps its value if free_left
     takes it.  All or nothing: plan.status tells (on the device) whether the
     pool, the table rows and the slot map were large enough."""
-    device, batch = pool.device, lens.shape[0]
-    index = device.index
-    s = _stream(index, stream)
+    index, num_blocks, block_size, stack = pool._now()
+    batch = lens.shape[0]
+    s = _raw_stream(index) if stream is None else _stream(index, stream)
     if plan is None:
-        plan = BlockPlan(*(_empty(n, torch.int32, device, stream)
+        plan = BlockPlan(*(_empty(n, torch.int32, pool.device, stream)
                            for n in (batch, batch + 1, tokens, 1)))
-    if free_left is None:
-        free_left = pool.free_count
+    left = stack[1] if free_left is None else _ints("free_left", free_left, index, 1)
     t, width, stride = _table(tables, index, batch)
-    written, status = plan._ptrs(index, batch, tokens)
+    kv_lens, starts, slots, status = plan._ptrs(index, batch, tokens)
     _call("attn_block_tables", index, _TABLES(
         _ints("lens", lens, index, batch), _ints("new_lens", new_lens, index, batch), t,
-        pool.free.data_ptr(), pool.free_count.data_ptr(), *written,
-        _ints("free_left", free_left, index, 1), status, stride, batch, width, pool.num_blocks,
-        pool.block_size, tokens), s)
+        *stack, kv_lens, starts, slots, left, status, stride, batch, width, num_blocks,
+        block_size, tokens), s)
     return plan
 
 
@@ -250,40 +294,39 @@ def block_trim(pool: BlockPool, lens, keep, tables, *, lens_left=None, free_left
     behind them go back to the pool.  Writes lens_left (default: `lens`
     itself) and free_left (default: pool.free_count); returns the status word
     [1] (BLOCKS; anything but OK: nothing was changed)."""
-    device, batch = pool.device, lens.shape[0]
-    index = device.index
-    s = _stream(index, stream)
+    index, num_blocks, block_size, stack = pool._now()
+    batch = lens.shape[0]
+    s = _raw_stream(index) if stream is None else _stream(index, stream)
     if lens_left is None:
         lens_left = lens
-    if free_left is None:
-        free_left = pool.free_count
+    left = stack[1] if free_left is None else _ints("free_left", free_left, index, 1)
     if status is None:
-        status = _empty(1, torch.int32, device, stream)
+        status = _empty(1, torch.int32, pool.device, stream)
     t, width, stride = _table(tables, index, batch)
     _call("attn_block_trim", index, _TRIM(
         _ints("lens", lens, index, batch), _ints("keep", keep, index, batch), t,
-        pool.free.data_ptr(), pool.free_count.data_ptr(),
-        _ints("lens_left", lens_left, index, batch), _ints("free_left", free_left, index, 1),
-        _ints("status", status, index, 1), stride, batch, width, pool.num_blocks,
-        pool.block_size), s)
+        *stack, _ints("lens_left", lens_left, index, batch), left,
+        _ints("status", status, index, 1), stride, batch, width, num_blocks, block_size), s)
     return status
 
 
 def _rows(name, x, index, heads, dim):
-    """Checks a [tokens, heads, D] tensor; its dtype code, shape, and the strides
-    of tokens and heads (0 where there is one only, whose stride means nothing)."""
+    """Checks a [tokens, heads, D] tensor; its dtype code, shape, strides, and the
+    strides of tokens and heads (0 where there is one only, whose stride means
+    nothing)."""
     kind = _DTYPES.get(x.dtype)
     if kind is None:
         raise TypeError(f"unsupported dtype {x.dtype} of {name} (float16 or bfloat16)")
     if x.get_device() != index:
         raise ValueError(f"{name} must be on cuda:{index}")
     shape = x.shape
-    if len(shape) != 3 or shape[2] != dim or (heads and shape[1] != heads):
+    tokens, many, last = shape if len(shape) == 3 else (0, 0, 0)
+    if last != dim or (heads and many != heads):
         raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {dim}]")
-    token, head, one = x.stride()
+    token, head, one = strides = x.stride()
     if one != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    return kind, shape, token if shape[0] > 1 else 0, head if shape[1] > 1 else 0
+    return kind, shape, strides, token if tokens > 1 else 0, head if many > 1 else 0
 
 
 def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
@@ -296,21 +339,20 @@ def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
     finite makes that block's k_scale NaN for its head.  The tokens of one
     block follow each other with ascending slots (as block_tables gives them),
     and no block appears twice."""
-    index = cache.device.index
-    heads, dim = cache.kv_heads, cache.dim
-    kind, shape, k_token, k_head = _rows("k", k, index, heads, dim)
+    index, num_blocks, heads, block_size, dim, code, ptrs = cache._now()
+    kind, shape, strides, k_token, k_head = _rows("k", k, index, heads, dim)
     if (v.dtype is k.dtype and v.shape == shape and v.get_device() == index
-            and v.stride() == k.stride()):  # the usual: slices of one projection
+            and v.stride() == strides):  # the usual: slices of one projection
         v_token, v_head = k_token, k_head
     else:
-        v_kind, v_shape, v_token, v_head = _rows("v", v, index, heads, dim)
+        v_kind, v_shape, _, v_token, v_head = _rows("v", v, index, heads, dim)
         if v_kind != kind or v_shape != shape:
             raise ValueError("k and v must share one shape and dtype")
     tokens = shape[0]
     _call("attn_cache_append", index, _APPEND(
-        k.data_ptr(), v.data_ptr(), _ints("slots", slots, index, tokens), *cache.ptrs, k_token,
-        k_head, v_token, v_head, tokens, heads, dim, kind, cache.code, cache.num_blocks,
-        cache.block_size), _stream(index, stream))
+        k.data_ptr(), v.data_ptr(), _ints("slots", slots, index, tokens), *ptrs, k_token, k_head,
+        v_token, v_head, tokens, heads, dim, kind, code, num_blocks, block_size),
+        _raw_stream(index) if stream is None else _stream(index, stream))
 
 
 def _workspace(index, heads, kv_heads, dim, max_new, block_size, width) -> int:
@@ -329,8 +371,8 @@ def _workspace(index, heads, kv_heads, dim, max_new, block_size, width) -> int:
 def cached_workspace(cache: PagedCache, heads: int, max_new: int, width: int) -> int:
     """Bytes of workspace that attn_cached needs with `heads` query heads and
     tables of `width` entries, whatever the lengths (0: none)."""
-    return _workspace(cache.device.index, heads, cache.kv_heads, cache.dim, max_new, cache.block_size,
-                      width)
+    index, _, kv_heads, block_size, dim, _, _ = cache._now()
+    return _workspace(index, heads, kv_heads, dim, max_new, block_size, width)
 
 
 def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
@@ -351,9 +393,8 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     workspace: a uint8 tensor to use instead of a new one per call, of
     cached_workspace(...) bytes; calls that may overlap on the GPU need one
     each."""
-    device, kv_heads, dim = cache.device, cache.kv_heads, cache.dim
-    index = device.index
-    kind, shape, q_token, q_head = _rows("q", q, index, 0, dim)
+    index, num_blocks, kv_heads, block_size, dim, code, ptrs = cache._now()
+    kind, shape, _, q_token, q_head = _rows("q", q, index, 0, dim)
     tokens, heads, _ = shape
     if heads == 0 or heads % kv_heads:
         raise ValueError(f"{heads} heads are not a multiple of the cache's {kv_heads}")
@@ -367,29 +408,28 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     t, width, stride = _table(tables, index, batch)
     lens_ptr = _ints("kv_lens", kv_lens, index, batch)
     starts_ptr = _ints("starts", starts, index, batch + 1)
-    s = _stream(index, stream)
+    s = _raw_stream(index) if stream is None else _stream(index, stream)
     if out is None:
-        out = _empty(shape, q.dtype, device, stream)
+        out = _empty(shape, q.dtype, q.device, stream)
         o_token, o_head = heads * dim, dim
     else:
-        o_kind, o_shape, o_token, o_head = _rows("out", out, index, heads, dim)
+        o_kind, o_shape, _, o_token, o_head = _rows("out", out, index, heads, dim)
         if o_kind != kind or o_shape != shape:
             raise ValueError("out must have the shape and dtype of q")
     if workspace is None:
-        need = _workspace(index, heads, kv_heads, dim, max_new, cache.block_size, width)
+        need = _workspace(index, heads, kv_heads, dim, max_new, block_size, width)
         if need:
-            workspace = _empty(need, torch.uint8, device, stream)
+            workspace = _empty(need, torch.uint8, q.device, stream)
     else:
         if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
             raise TypeError("workspace must be a contiguous uint8 tensor")
         if workspace.get_device() != index:
-            raise ValueError(f"workspace must be on {device}")
+            raise ValueError(f"workspace must be on {q.device}")
         need = workspace.numel()
     _call("attn_cached", index, _CACHED(
-        q.data_ptr(), out.data_ptr(), *cache.ptrs, t, lens_ptr, starts_ptr,
+        q.data_ptr(), out.data_ptr(), *ptrs, t, lens_ptr, starts_ptr,
         workspace.data_ptr() if need else 0, need, q_token, q_head, o_token, o_head, stride, tokens, heads, kv_heads, dim, kind,
-        cache.code, cache.num_blocks, cache.block_size, width, batch, max_new,
-        1 if causal else 0, scale), s)
+        code, num_blocks, block_size, width, batch, max_new, 1 if causal else 0, scale), s)
     return out
 
 

@@ -165,3 +165,101 @@ def test_values_far_below_the_largest_scale(ap, code, dim, new, power):
     assert torch.all(want[:, 0] > 64 * r * 2.0 ** -power * 0.99)
     off = (out.double().cpu() - want).abs() / tol
     assert torch.all(off <= 1), f"off by {off.max():.3g} times"
+
+
+# --------------------------------------------------------------------------- arrays that are replaced
+def other_cache(ap, blocks, seed):
+    return make_cache(ap, blocks, 2, 16, 64, E4M3, seed)[0]
+
+
+@pytest.mark.parametrize("how", ["attribute", "set_"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_cache_follows_tensors_that_are_replaced(ap, how, new):
+    """Every call reads and writes the tensors that the cache has now."""
+    cache, want_from = other_cache(ap, 6, 1), other_cache(ap, 20, 2)
+    kept = [x.detach() for x in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    before = [x.clone() for x in kept]
+    for name in cache.__slots__:
+        mine = getattr(want_from, name).clone()
+        if how == "attribute":
+            setattr(cache, name, mine)
+        else:
+            getattr(cache, name).set_(mine)
+    assert cache.num_blocks == 20
+    q = torch.randn(new, 4, 64, device="cuda").half()
+    args = ints([list(range(19, 3, -1))]), ints([250]), ints([0, new])
+    got = ap.attn_cached(q, cache, *args, max_new=new)
+    assert torch.equal(got, ap.attn_cached(q, want_from, *args, max_new=new))
+    k, v = (torch.randn(3, 2, 64, device="cuda").half() for _ in range(2))
+    for c in (cache, want_from):
+        ap.cache_append(c, k, v, ints([16 * 18, 16 * 18 + 1, 0]))
+    for name in cache.__slots__:
+        assert torch.equal(getattr(cache, name).float(), getattr(want_from, name).float())
+    for x, y in zip(kept, before):
+        assert torch.equal(x.float(), y.float())
+
+
+def test_a_cache_of_tensors_that_do_not_belong_together_is_refused(ap):
+    cache = other_cache(ap, 6, 1)
+    q = torch.randn(1, 4, 64, device="cuda").half()
+    args = ints([[0, 1]]), ints([20]), ints([0, 1])
+    first = cache.k
+    cache.k = other_cache(ap, 7, 2).k
+    with pytest.raises(ValueError, match="share one"):
+        ap.attn_cached(q, cache, *args, max_new=1)
+    with pytest.raises(ValueError, match="share one"):
+        ap.cache_append(cache, q[:, :2], q[:, :2], ints([0]))
+    cache.k = first
+    cache.v_scale = cache.v_scale[:5]
+    with pytest.raises(ValueError, match="v_scale"):
+        ap.attn_cached(q, cache, *args, max_new=1)
+    cache.v_scale = torch.ones(6, 2, device="cuda", dtype=torch.float64)
+    with pytest.raises(TypeError, match="v_scale"):
+        ap.attn_cached(q, cache, *args, max_new=1)
+    cache.v_scale = torch.ones(6, 2, device="cuda")
+    ap.attn_cached(q, cache, *args, max_new=1)
+    with pytest.raises(AttributeError):
+        cache.num_blocks = 9
+
+
+@pytest.mark.parametrize("how", ["attribute", "set_"])
+def test_a_pool_follows_a_list_that_is_replaced(ap, how):
+    """A shorter free list takes no more blocks than it has room for."""
+    pool = ap.BlockPool.full(32, 16)
+    kept = pool.free.detach()
+    buffer = torch.full((32,), -5, dtype=torch.int32, device="cuda")
+    if how == "attribute":
+        pool.free = buffer[:4]
+    else:
+        pool.free.set_(buffer[:4])
+    assert pool.num_blocks == 4
+    pool.free_count = ints([0])
+    lens, tables = ints([90]), ints([[9, 8, 7, 6, 5, 4]])
+    assert ap.block_trim(pool, lens, ints([0]), tables).item() == 1
+    assert (buffer == -5).all() and kept[0].item() == 31 and lens.item() == 90
+    lens.fill_(60)
+    assert ap.block_trim(pool, lens, ints([0]), tables).item() == 0
+    assert buffer[:4].tolist() == [9, 8, 7, 6] and (buffer[4:] == -5).all()
+    pool.block_size = 32
+    pool.free, pool.free_count = ints([3, 2, 1, 0]), ints([4])
+    plan = ap.block_tables(pool, ints([0]), ints([33]), ints([[-1, -1]]), 33)
+    assert plan.slots[32].item() == 32 and pool.free_count.item() == 2
+    pool.free = torch.zeros(4, dtype=torch.int64, device="cuda")
+    with pytest.raises(TypeError, match="free"):
+        ap.block_tables(pool, ints([0]), ints([0]), ints([[-1]]), 0)
+
+
+def test_a_plan_follows_memory_that_is_replaced(ap):
+    pool, lens, new = ap.BlockPool.full(8, 16), ints([0, 3]), ints([5, 1])
+    tables, plan = torch.zeros(2, 4, dtype=torch.int32, device="cuda"), ap.BlockPlan.empty(2, 6)
+    ap.block_tables(pool, lens, new, tables, 6, plan=plan)
+    kept = plan.slots.detach()
+    buffer = torch.full((12,), -5, dtype=torch.int32, device="cuda")
+    plan.slots.set_(buffer[:4])
+    with pytest.raises(ValueError, match="plan.slots"):
+        ap.block_tables(pool, lens, new, tables, 6, plan=plan)
+    kept.fill_(-9)
+    plan.slots.set_(buffer[4:10])
+    ap.block_tables(pool, lens, new, tables, 6, plan=plan)
+    assert (kept == -9).all() and (buffer[4:10] >= 0).all()
+    assert (buffer[:4] == -5).all() and (buffer[10:] == -5).all()
