@@ -400,8 +400,8 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
         raise ValueError(f"{heads} heads are not a multiple of the cache's {kv_heads}")
     if scale is None:
         scale = 0.0
-    elif not scale > 0:
-        raise ValueError("scale must be positive")
+    elif not scale > 2.0 ** -150:  # (in 32 bits that is 0, which stands for the default)
+        raise ValueError("scale must be positive in 32 bits")
     if max_new < 0:
         raise ValueError("max_new must not be negative")
     batch = kv_lens.shape[0]

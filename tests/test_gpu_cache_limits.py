@@ -167,6 +167,22 @@ def test_values_far_below_the_largest_scale(ap, code, dim, new, power):
     assert torch.all(off <= 1), f"off by {off.max():.3g} times"
 
 
+# --------------------------------------------------------------------------- scale of the scores
+@pytest.mark.parametrize("new", [1, 50])
+def test_a_scale_of_the_scores_is_never_taken_for_none(ap, new):
+    """A scale that is 0 in 32 bits would mean 1 / sqrt(D): it is refused; the
+    least one that is not makes all weights alike."""
+    cache, host = make_cache(ap, 3, 1, 16, 64, E4M3, 4)
+    q = torch.randn(new, 1, 64, device="cuda").half()
+    args = (q, cache, ints([[0, 1, 2]]), ints([48]), ints([0, new]))
+    for scale in (1e-46, 2.0 ** -150, 0.0, -1.0, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            ap.attn_cached(*args, max_new=new, scale=scale)
+    want, tol = ref.attend_ref(q.cpu(), *host, [[0, 1, 2]], [48], [0, new], False, 2.0 ** -149)
+    out = ap.attn_cached(*args, max_new=new, causal=False, scale=2.0 ** -149)
+    assert torch.all((out.double().cpu() - want).abs() <= tol)
+
+
 # --------------------------------------------------------------------------- arrays that are replaced
 def other_cache(ap, blocks, seed):
     return make_cache(ap, blocks, 2, 16, 64, E4M3, seed)[0]
