@@ -52,11 +52,12 @@ def _stream(index, stream) -> int:
     return stream.cuda_stream
 
 
-# The argument structs of include/attnprof.h, field by field in their order.
-_TABLES = struct.Struct("@10Qq5i").pack
-_TRIM = struct.Struct("@8Qq4i").pack
-_APPEND = struct.Struct("@7Q4q7i").pack
-_CACHED = struct.Struct("@11Q5q12if").pack
+# The argument structs of include/attnprof.h, field by field in their order ("0q":
+# and the padding behind the last one).
+_TABLES = struct.Struct("@10Qq5i0q").pack
+_TRIM = struct.Struct("@8Qq4i0q").pack
+_APPEND = struct.Struct("@7Q4q7i0q").pack
+_CACHED = struct.Struct("@11Q5q12if0q").pack
 
 
 def _call(name, index, *args):

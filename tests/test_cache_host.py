@@ -1,6 +1,9 @@
 """Argument checks of the paged cache: every call here is refused on the host
 (or has nothing to do), so no GPU is needed."""
 import ctypes
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 
@@ -139,3 +142,20 @@ def test_python_face_refuses_cpu_tensors_and_shapes(engine):
         engine.PagedCache(k, k[:2], s, s)
     with pytest.raises(ValueError, match="CUDA"):
         engine.BlockPool(torch.zeros(4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 16)
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="no C compiler")
+def test_argument_structs_are_as_long_as_the_header_s(tmp_path):
+    """The C side may copy a struct whole, its padding too."""
+    packs = {"attn_block_tables_args": (cache._TABLES, TABLES),
+             "attn_block_trim_args": (cache._TRIM, TRIM),
+             "attn_cache_append_args": (cache._APPEND, APPEND),
+             "attn_cached_args": (cache._CACHED, ATTN)}
+    source, exe = tmp_path / "sizes.c", tmp_path / "sizes"
+    source.write_text('#include <stdio.h>\n#include "attnprof.h"\nint main(void) {\n' + "".join(
+        f'  printf("%zu\\n", sizeof({name}));\n' for name in packs) + "  return 0;\n}\n")
+    include = Path(__file__).resolve().parent.parent / "include"
+    subprocess.run(["gcc", "-std=c99", "-I", str(include), str(source), "-o", str(exe)], check=True)
+    sizes = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
+    for size, (name, (pack, good)) in zip(sizes, packs.items()):
+        assert len(pack(*good.values())) == int(size), name
