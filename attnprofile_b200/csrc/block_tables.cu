@@ -81,6 +81,14 @@ __device__ __forceinline__ int last_at_most(const int* first, int n, int x) {
   return lo;
 }
 
+// Blocks of n >= 0 tokens, up to the largest n: the sum may pass 31 bits.
+__device__ __forceinline__ int blocks_of(int n, int shift) {
+  return static_cast<int>((static_cast<unsigned>(n) + (1u << shift) - 1) >> shift);
+}
+__device__ __forceinline__ long long blocks_of(long long n, int shift) {
+  return (n + (1 << shift) - 1) >> shift;
+}
+
 // Bits 0 and 1 that any thread of the CTA has.
 __device__ __forceinline__ int any_of(int bad) {
   if (!__syncthreads_or(bad)) return 0;
@@ -123,9 +131,9 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
         bad |= 2;
         l = 0;
       } else {
-        const long long after = (static_cast<long long>(l) + n + mask) >> p.shift;
+        const long long after = blocks_of(static_cast<long long>(l) + n, p.shift);
         if (after > p.width || static_cast<long long>(l) + n > INT_MAX) bad |= 1;
-        v = Counts{n, after - ((static_cast<long long>(l) + mask) >> p.shift)};
+        v = Counts{n, after - blocks_of(l, p.shift)};
       }
     }
     const Counts at = scan_threads(v, total, &total, warp_sum);
@@ -170,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
   // the slots below, and loads of their own to wait for.
   for (int j = all - 1 - me; j < taken; j += all) {
     const int r = last_at_most(first, p.batch, j);
-    const int column = ((len[r] + mask) >> p.shift) + (j - first[r]);
+    const int column = blocks_of(len[r], p.shift) + (j - first[r]);
     p.tables[r * p.table_stride + column] = p.free_blocks[count - 1 - j];
   }
   // Slots, four tokens a thread: one search, then a walk.  A block that the
@@ -193,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) tables_kernel(const TablesParams p) 
         const int pos = len[r] + (t - start[r]);
         const int b = pos >> p.shift;
         if (b != block_rank) {
-          const int held = (len[r] + mask) >> p.shift;
+          const int held = blocks_of(len[r], p.shift);
           id = b < held ? p.tables[r * p.table_stride + b]
                         : p.free_blocks[count - 1 - (first[r] + b - held)];
           block_rank = b;
@@ -225,7 +233,6 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
   begin_behind();
   const int count = *p.free_count;
   const int ctas = static_cast<int>(gridDim.x), threads = static_cast<int>(blockDim.x);
-  const int mask = (1 << p.shift) - 1;
 
   Counts total{0, 0};
   int bad = 0;
@@ -237,10 +244,10 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
       l = p.lens[r];
       const int k = p.keep[r];
       if (l < 0 || k < 0) bad |= 2;
-      const long long held = (static_cast<long long>(max(l, 0)) + mask) >> p.shift;
+      const int held = blocks_of(max(l, 0), p.shift);
       if (held > p.width) bad |= 1;
       l = max(0, min(l, k));
-      v.blocks = held - ((static_cast<long long>(l) + mask) >> p.shift);
+      v.blocks = held - blocks_of(l, p.shift);
     }
     const Counts at = scan_threads(v, total, &total, warp_sum);
     if (r < p.batch) {
@@ -273,7 +280,7 @@ __global__ void __launch_bounds__(kThreads) trim_kernel(const TrimParams p) {
   }
   for (int j = me; j < back; j += all) {
     const int r = last_at_most(first, p.batch, j);
-    const int column = ((left[r] + mask) >> p.shift) + (j - first[r]);
+    const int column = blocks_of(left[r], p.shift) + (j - first[r]);
     p.free_blocks[count + j] = p.tables[r * p.table_stride + column];
   }
 }

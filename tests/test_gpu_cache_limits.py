@@ -279,3 +279,34 @@ def test_a_plan_follows_memory_that_is_replaced(ap):
     ap.block_tables(pool, lens, new, tables, 6, plan=plan)
     assert (kept == -9).all() and (buffer[4:10] >= 0).all()
     assert (buffer[:4] == -5).all() and (buffer[10:] == -5).all()
+
+
+# --------------------------------------------------------------------------- the longest requests
+def test_tables_and_trim_of_the_longest_requests(ap):
+    """Lengths up to the last that 31 bits hold, in a table of 2^24 entries."""
+    bs, width = 128, 2 ** 24
+    tables = torch.full((1, width), 7, dtype=torch.int32, device="cuda")
+    tables[0, -1] = 250
+    pool = ap.BlockPool(torch.arange(300, dtype=torch.int32, device="cuda"), ints([5]), bs)
+    lens, new = ints([2 ** 31 - 10]), ints([9])
+    plan = ap.block_tables(pool, lens, new, tables, 10)  # all in the last block, which is held
+    assert plan.status.item() == 0 and pool.free_count.item() == 5
+    assert plan.kv_lens.item() == 2 ** 31 - 1
+    assert plan.slots.tolist() == [250 * bs + 118 + i for i in range(9)] + [-1]
+    new.fill_(10)
+    plan = ap.block_tables(pool, lens, new, tables, 10)  # one token too many
+    assert plan.status.item() == 2 and plan.slots.tolist() == [-1] * 10
+    lens.fill_(2 ** 31 - 131)
+    new.fill_(7)
+    plan = ap.block_tables(pool, lens, new, tables, 7)  # over the border into a new block
+    assert plan.status.item() == 0 and pool.free_count.item() == 4
+    assert plan.slots.tolist() == [7 * bs + 125 + i for i in range(3)] + [4 * bs + i for i in range(4)]
+    assert tables[0, -2:].tolist() == [7, 4]
+    lens.fill_(2 ** 31 - 1)
+    assert ap.block_trim(pool, lens, ints([2 ** 31 - 128]), tables).item() == 0
+    assert pool.free[:5].tolist() == [0, 1, 2, 3, 4] and pool.free_count.item() == 5
+    assert lens.item() == 2 ** 31 - 128
+    lens.fill_(2 ** 31 - 1)
+    assert ap.block_trim(pool, lens, ints([2 ** 31 - 2]), tables).item() == 0
+    assert pool.free_count.item() == 5 and lens.item() == 2 ** 31 - 2
+    assert ap.block_trim(pool, lens, ints([0]), tables).item() == 1  # more than the pool has
