@@ -10,6 +10,7 @@ device cannot run it, every call raises.
 from __future__ import annotations
 
 import ctypes
+from importlib.util import find_spec
 from pathlib import Path
 
 from ._build import LIB_PATH, build  # noqa: F401
@@ -20,8 +21,6 @@ __all__ = [
     "attn_sharded",
     "shard_range", "set_split", "set_schedule", "plan_split", "plan_schedule", "query_split",
     "set_correction",
-    "PagedCache", "BlockPool", "BlockPlan", "CacheBatch", "block_tables", "block_trim",
-    "cache_append", "attn_cached", "cached_workspace",
 ]
 
 ERR = {
@@ -296,6 +295,8 @@ def shard_range(units: int, n_dev: int, g: int) -> tuple[int, int]:
 
 _CACHE_NAMES = ("PagedCache", "BlockPool", "BlockPlan", "CacheBatch", "block_tables", "block_trim",
                 "cache_append", "attn_cached", "cached_workspace")
+if find_spec("torch"):  # (a star import asks for every name)
+    __all__ += _CACHE_NAMES
 
 
 def __getattr__(name):

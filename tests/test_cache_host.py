@@ -3,6 +3,7 @@
 import ctypes
 import shutil
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -159,3 +160,15 @@ def test_argument_structs_are_as_long_as_the_header_s(tmp_path):
     sizes = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()
     for size, (name, (pack, good)) in zip(sizes, packs.items()):
         assert len(pack(*good.values())) == int(size), name
+
+
+@pytest.mark.parametrize("torch_there", [True, False])
+def test_names_that_a_star_import_brings(torch_there):
+    """Without torch the dense engine's names come, with it the cache's too."""
+    root = Path(__file__).resolve().parent.parent
+    code = ("import sys\n" + ("" if torch_there else "sys.modules['torch'] = None\n") +
+            f"sys.path.insert(0, {str(root)!r})\nfrom attnprofile_b200 import *\n"
+            "print('attn' in globals(), 'attn_cached' in globals())\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-800:]
+    assert r.stdout.split() == ["True", str(torch_there)]
