@@ -470,6 +470,11 @@ class CacheBatch:
         self.trim_status = torch.zeros(1, dtype=torch.int32, device=device)
         self.plan = None
 
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        if name in ("lens", "starts", "slots", "status"):  # a plan holds these
+            self.plan = None
+
     def advance(self, new_lens, tokens: int, *, stream=None) -> BlockPlan:
         """new_lens[r] tokens more for request r, in a slot map of `tokens`."""
         if not 0 <= tokens <= self.slots.shape[0]:

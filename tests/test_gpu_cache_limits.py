@@ -281,6 +281,25 @@ def test_a_plan_follows_memory_that_is_replaced(ap):
     assert (buffer[:4] == -5).all() and (buffer[10:] == -5).all()
 
 
+@pytest.mark.parametrize("name", ["lens", "starts", "slots", "status"])
+def test_a_batch_follows_arrays_that_are_replaced(ap, name):
+    """The next step writes into the array that the batch has now."""
+    batch = ap.CacheBatch(ap.BlockPool.full(20, 16), rows=2, max_len=64, max_tokens=8)
+    cache = ap.PagedCache.empty(20, 1, 64, block_size=16)
+    x = torch.randn(8, 1, 64, device="cuda").half()
+    batch.advance(ints([5, 3]), 8)
+    batch.attend(cache, x, x, x, max_new=5)
+    old = getattr(batch, name)
+    was = old.clone()
+    setattr(batch, name, old.clone() if name == "lens" else torch.full_like(old, -5))
+    with pytest.raises(RuntimeError, match="advance"):
+        batch.attend(cache, x, x, x, max_new=5)
+    batch.advance(ints([2, 6]), 8)
+    assert batch.lens.tolist() == [7, 9] and batch.starts.tolist() == [0, 2, 8]
+    assert batch.slots.tolist() == [5, 6] + [16 + i for i in range(3, 9)]
+    assert batch.status.item() == 0 and torch.equal(old, was)
+
+
 # --------------------------------------------------------------------------- the longest requests
 def test_tables_and_trim_of_the_longest_requests(ap):
     """Lengths up to the last that 31 bits hold, in a table of 2^24 entries."""
