@@ -337,9 +337,10 @@ def cache_append(cache: PagedCache, k, v, slots, *, stream=None) -> None:
     A block's scale per head is the least power of two that holds its largest
     number; it grows when new tokens need that, and the block's older codes are
     rounded again.  Negative slots (padding) are skipped.  A number that is not
-    finite makes that block's k_scale NaN for its head.  The tokens of one
-    block follow each other with ascending slots (as block_tables gives them),
-    and no block appears twice."""
+    finite makes that block's k_scale NaN for its head.  The tokens of
+    one block follow each other with consecutive slots, as block_tables gives
+    them: no gap, no skipped token between them, and no block twice (pieces of a
+    block go into calls of their own)."""
     index, num_blocks, heads, block_size, dim, code, ptrs = cache._now()
     kind, shape, strides, k_token, k_head = _rows("k", k, index, heads, dim)
     if (v.dtype is k.dtype and v.shape == shape and v.get_device() == index

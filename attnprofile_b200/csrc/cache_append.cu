@@ -18,7 +18,8 @@
 // a sum; a NaN among the values would instead spread to masked rows as 0 * NaN.
 //
 // Tokens that follow each other into one block (a run) share its scale, so the
-// unit of work is one run and one head.  A CTA of 2 to 8 warps looks at `chunk`
+// unit of work is one run and one head; nothing orders two runs, so a call may
+// have only one for a block.  A CTA of 2 to 8 warps looks at `chunk`
 // consecutive tokens of one head and takes the runs that begin there: a short
 // run (single tokens, drafts) by one warp, so that several go at once, a longer
 // one by the whole CTA, which holds it in registers between finding its largest

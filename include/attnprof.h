@@ -333,8 +333,10 @@ int attn_block_trim(const attn_block_trim_args* args, void* stream);
  * A number that is not finite makes the block's k_scale NaN for that head
  * (and its own code 0), so that rows attending to the block become NaN and no
  * others, until the block is written from its first slot again.
- * The tokens of one block must follow each other in the call with ascending
- * slots, as attn_block_tables gives them; a block must not appear twice.
+ * The tokens of one block must follow each other in the call with consecutive
+ * slots, as attn_block_tables gives them: no gap, no skipped token between them,
+ * and no block twice.  (Pieces of one block are worked on at the same time, each
+ * with the scale that it finds: append them in calls of their own.)
  * Asynchronous; needs no scratch.
  */
 typedef struct {

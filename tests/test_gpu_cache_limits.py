@@ -12,7 +12,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from tests import cache_ref as ref  # noqa: E402
-from tests.test_gpu_cache import CODES, E4M3, INT8, TYPES, ints, make_cache  # noqa: E402
+from tests.test_gpu_cache import CODES, E4M3, TYPES, check_append, ints, make_cache  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -329,3 +329,18 @@ def test_tables_and_trim_of_the_longest_requests(ap):
     assert ap.block_trim(pool, lens, ints([2 ** 31 - 2]), tables).item() == 0
     assert pool.free_count.item() == 5 and lens.item() == 2 ** 31 - 2
     assert ap.block_trim(pool, lens, ints([0]), tables).item() == 1  # more than the pool has
+
+
+# --------------------------------------------------------------------------- pieces of a block
+@pytest.mark.parametrize("code", CODES)
+def test_pieces_of_a_block_in_calls_of_their_own(ap, code):
+    """Slots with a gap, or with padding between them, are appended piece by
+    piece; each piece finds the scale that the one before it left."""
+    bs, dim = 16, 64
+    cache, host = make_cache(ap, 3, 2, bs, dim, code, 5)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for i, slots in enumerate(([16, 17, -1, 32], [-1, 18, 35], [21, 22, -1], [23, 37, 38, 39])):
+        k, v = ((torch.randn(len(slots), 2, dim, generator=gen, device="cuda") * 4 ** i).half()
+                for _ in range(2))
+        check_append(cache, host, k, v, slots, bs, code)
+        host = tuple(x.cpu() for x in (cache.k, cache.v, cache.k_scale, cache.v_scale))
