@@ -344,3 +344,82 @@ def test_pieces_of_a_block_in_calls_of_their_own(ap, code):
                 for _ in range(2))
         check_append(cache, host, k, v, slots, bs, code)
         host = tuple(x.cpu() for x in (cache.k, cache.v, cache.k_scale, cache.v_scale))
+
+
+# --------------------------------------------------------------------------- streams given by name
+def test_every_call_on_a_stream_given_by_name(ap):
+    """A step of single calls, and of CacheBatch, on a stream that waits behind
+    a long kernel of its own while the current stream is idle: the results are
+    those of the current stream, and are there once the named one has ended."""
+    bs, heads, kv_heads, dim, rows = 16, 4, 2, 64, 3
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    new = [70, 1, 40]
+    tokens = sum(new) + 2
+    qkv = torch.randn(tokens, heads + 2 * kv_heads, dim, generator=gen, device="cuda").half()
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+    new_t, keep = ints(new), ints([66, 0, 40])
+    side = torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device="cuda")
+
+    def single(stream):
+        pool, lens = ap.BlockPool.full(30, bs), ints([0] * rows)
+        tables = torch.full((rows, 9), -1, dtype=torch.int32, device="cuda")
+        cache = ap.PagedCache.empty(30, kv_heads, dim, block_size=bs)
+        out = torch.zeros(tokens, heads, dim, device="cuda").half()
+        torch.cuda.synchronize()
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                for _ in range(8):
+                    torch.mm(busy, busy)
+        plan = ap.block_tables(pool, lens, new_t, tables, tokens, stream=stream)
+        ap.cache_append(cache, k, v, plan.slots, stream=stream)
+        ap.attn_cached(q, cache, tables, plan.kv_lens, plan.starts, max_new=70, out=out,
+                       stream=stream)
+        status = ap.block_trim(pool, plan.kv_lens, keep, tables, stream=stream)
+        (stream or torch.cuda.current_stream()).synchronize()
+        n = int(pool.free_count)
+        return [plan.kv_lens, plan.starts, plan.slots, plan.status, status, tables, pool.free[:n],
+                cache.k_scale[tables[2, :3].long()], cache.v_scale[tables[2, :3].long()], out]
+
+    def batch(stream):
+        b = ap.CacheBatch(ap.BlockPool.full(30, bs), rows, 9 * bs, tokens)
+        cache = ap.PagedCache.empty(30, kv_heads, dim, block_size=bs)
+        out = torch.zeros(tokens, heads, dim, device="cuda").half()
+        torch.cuda.synchronize()
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                for _ in range(8):
+                    torch.mm(busy, busy)
+        b.advance(new_t, tokens, stream=stream)
+        b.attend(cache, q, k, v, max_new=70, out=out, stream=stream)
+        got = b.attend(cache, q, k, v, max_new=70, stream=stream)  # (a second layer, with a new output)
+        status = b.trim(keep, stream=stream)
+        (stream or torch.cuda.current_stream()).synchronize()
+        return [b.lens, b.starts, b.slots, b.status, status, b.tables,
+                b.pool.free[:int(b.pool.free_count)], out, got[:sum(new)]]
+
+    for step in (single, batch):
+        want = step(None)
+        for a, b in zip(step(side), want):
+            assert torch.equal(a, b)
+        assert want[4].item() == 0 and want[3].item() == 0
+        assert want[-1][:sum(new)].abs().sum() > 0
+
+
+def test_a_stream_of_the_tensors_device_is_asked_for(ap):
+    """(with one device: a stream that says it is another's)"""
+    class Other:
+        device = torch.device("cuda", 7)
+        cuda_stream = 0
+    batch = ap.CacheBatch(ap.BlockPool.full(4, 16), 1, 64, 4)
+    cache = ap.PagedCache.empty(4, 1, 64, block_size=16)
+    x = torch.zeros(4, 1, 64, device="cuda").half()
+    batch.advance(ints([4]), 4)
+    for call in (lambda: batch.advance(ints([0]), 4, stream=Other),
+                 lambda: batch.trim(ints([0]), stream=Other),
+                 lambda: ap.cache_append(cache, x, x, batch.slots, stream=Other),
+                 lambda: ap.attn_cached(x, cache, batch.tables, batch.lens, batch.starts, max_new=4,
+                                        stream=Other)):
+        with pytest.raises(ValueError, match="stream"):
+            call()
+    assert batch.lens.tolist() == [4]
