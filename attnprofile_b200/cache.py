@@ -294,7 +294,9 @@ def block_trim(pool: BlockPool, lens, keep, tables, *, lens_left=None, free_left
     """Request r keeps its first min(lens[r], keep[r]) tokens; the blocks
     behind them go back to the pool.  Writes lens_left (default: `lens`
     itself) and free_left (default: pool.free_count); returns the status word
-    [1] (BLOCKS; anything but OK: nothing was changed)."""
+    [1] (BLOCKS; anything but OK: nothing was changed).  A block that is kept in
+    part keeps its scale, which the tokens given up may have made larger, or
+    NaN (where they were not finite), until it is begun anew."""
     index, num_blocks, block_size, stack = pool._now()
     batch = lens.shape[0]
     s = _raw_stream(index) if stream is None else _stream(index, stream)
@@ -383,15 +385,17 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     """Attention of each request's newest tokens over its cache; returns out.
 
     q, out: [tokens, heads, D], heads a multiple of the cache's; rows
-    starts[r] .. starts[r + 1) are the last tokens of request r, whose
-    kv_lens[r] tokens lie in the blocks tables[r] (they are in the cache
-    already).  Row i of n sees the first kv_lens[r] - n + i + 1 tokens (causal)
-    or all of them; a row that sees none becomes 0.  max_new: the most rows of
-    any request; n counts those beyond it too.  scale: of the scores,
+    starts[r] .. starts[r + 1) (starts may not decrease) are the last tokens of
+    request r, whose kv_lens[r] tokens lie in the blocks tables[r] (they are in
+    the cache already).  Row i of n sees the first kv_lens[r] - n + i + 1 tokens
+    (causal) or all of them; a row that sees none becomes 0.  max_new: the most
+    rows of any request; n counts those beyond it too.  scale: of the scores,
     1 / sqrt(D) by default.  Rows of `out` beyond max_new and behind starts[-1]
-    are left as they were (with out=None: undefined); out must not overlap q.  With many rows a block whose V scale is below 2^-22 of
-    the request's largest (of that head) keeps an absolute accuracy only, 2^-32
-    of that scale.
+    are left as they were (with out=None: undefined); out must not overlap q.
+    With many rows values are rounded once more, by up to 2^-11 of themselves,
+    where the V scales are no powers of two, and those of a block whose V scale is
+    below 2^-22 of the request's largest (of that head) keep an absolute accuracy
+    only, 2^-32 of that scale.
     workspace: a uint8 tensor to use instead of a new one per call, of
     cached_workspace(...) bytes; calls that may overlap on the GPU need one
     each."""
@@ -487,7 +491,9 @@ class CacheBatch:
 
     def attend(self, cache: PagedCache, q, k, v, *, max_new: int, causal: bool = True,
                scale: float | None = None, out=None, stream=None):
-        """Appends k and v of the step's tokens, then attends with q."""
+        """Appends k and v of the step's tokens, then attends with q.  With
+        out=None the rows of padding, of a refused step and beyond max_new are
+        undefined."""
         if self.plan is None:
             raise RuntimeError("advance() first")
         if cache.block_size != self.pool.block_size or cache.num_blocks != self.pool.num_blocks:
@@ -497,6 +503,7 @@ class CacheBatch:
                            causal=causal, scale=scale, out=out, stream=stream)
 
     def trim(self, keep, *, stream=None):
-        """Requests keep their first keep[r] tokens; returns the status word."""
+        """Requests keep their first keep[r] tokens; returns the status word.
+        (See block_trim for the scales of blocks that are kept in part.)"""
         return block_trim(self.pool, self.lens, keep, self.tables, status=self.trim_status,
                           stream=stream)

@@ -309,7 +309,9 @@ int attn_block_tables(const attn_block_tables_args* args, void* stream);
  * (may be lens), free_left (may be free_count) and status; when that is not
  * OK, lens_left = lens and the stack is unchanged.  The tables keep their
  * entries, which mean nothing behind lens_left.  A block that several requests
- * share must be given back by one of them only.
+ * share must be given back by one of them only.  The scale of a block that is
+ * kept in part stays as attn_cache_append left it, for the tokens given up too
+ * (larger than the others need, or NaN), until the block is begun anew.
  */
 typedef struct {
   const int *lens, *keep, *tables;
@@ -366,8 +368,9 @@ int attn_cache_append(const attn_cache_append_args* args, void* stream);
  * below 2^-22 of the largest keep an absolute accuracy of 2^-32 of that one
  * only.  What lies in slots that hold no token is never used, whatever it is.
  * kv_lens is taken as at most
- * width * block_size, starts as within [0, tokens]; a table entry that is no
- * block of the pool is left out.
+ * width * block_size, starts as within [0, tokens]; starts must not decrease
+ * (where they do, rows are left out); a table entry that is no block of the pool
+ * is left out.
  * workspace: 16-byte aligned, attn_cached_workspace(...) bytes (NULL where
  * that is 0), needs no initial value; calls that may overlap need one each.
  * Asynchronous; like attn_fwd's, its waits are bounded (attn_set_timeout_ns)
