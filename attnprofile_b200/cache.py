@@ -117,8 +117,8 @@ class _Checked:
 
     def __setattr__(self, name, value):
         object.__setattr__(self, name, value)
-        object.__setattr__(self, "_seen", None)
-        object.__setattr__(self, "_held", None)
+        for kept in _Checked.__slots__:  # (the memory of the tensor before too)
+            object.__setattr__(self, kept, None)
 
     def _keep(self, tensors, *seen):
         """Remembers what a check gave, the tensors' addresses last.  It holds as

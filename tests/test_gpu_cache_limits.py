@@ -281,6 +281,20 @@ def test_a_plan_follows_memory_that_is_replaced(ap):
     assert (buffer[:4] == -5).all() and (buffer[10:] == -5).all()
 
 
+def test_a_tensor_that_was_replaced_is_not_held(ap):
+    pool = ap.BlockPool.full(1 << 20, 16)
+    cache = ap.PagedCache.empty(64, 8, 128, block_size=128)
+    size = cache.k.numel()
+    ap.cache_append(cache, *torch.zeros(2, 1, 8, 128, device="cuda").half(), ints([0]))
+    before = torch.cuda.memory_allocated()
+    cache.v = cache.k
+    assert torch.cuda.memory_allocated() <= before - size
+    ap.block_trim(pool, ints([0]), ints([0]), ints([[0]]))
+    before = torch.cuda.memory_allocated()
+    pool.free = pool.free[:4].clone()
+    assert torch.cuda.memory_allocated() <= before - (4 << 20) + 512
+
+
 @pytest.mark.parametrize("name", ["lens", "starts", "slots", "status"])
 def test_a_batch_follows_arrays_that_are_replaced(ap, name):
     """The next step writes into the array that the batch has now."""
