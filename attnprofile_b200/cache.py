@@ -392,7 +392,8 @@ def attn_cached(q, cache: PagedCache, tables, kv_lens, starts, *, max_new: int,
     rows of any request; n counts those beyond it too.  scale: of the scores,
     1 / sqrt(D) by default.  Rows of `out` beyond max_new and behind starts[-1]
     are left as they were (with out=None: undefined); out must not overlap q.
-    With many rows values are rounded once more, by up to 2^-11 of themselves,
+    Weights are rounded to f16, by up to 2^-11 of themselves or 2^-32 of the
+    row's largest.  With many rows values are rounded once more, by up to 2^-11 of themselves,
     where the V scales are no powers of two, and those of a block whose V scale is
     below 2^-22 of the request's largest (of that head) keep an absolute accuracy
     only, 2^-32 of that scale.

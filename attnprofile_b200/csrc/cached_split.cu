@@ -30,7 +30,8 @@
 // sum of p v in f32, so no scale is rounded.  P is rounded to f16, by at most
 // 2^-11 of itself as an f16 result is (a bf16 result by 2^-8): it is held as
 // 2^7 p (p up to 2^8 between two moves of the maximum), so that also weights down
-// to 2^-21 of the largest keep all their bits.  Maximum, sum and O are f32.
+// to 2^-21 of the largest keep all their bits, and smaller ones an absolute
+// accuracy of 2^-32 of it.  Maximum, sum and O are f32.
 // bf16 queries become f16 times a power of two per row: elements down to 2^-31
 // of the row's largest keep all their bits, smaller ones an absolute accuracy of
 // 2^-39 of it.

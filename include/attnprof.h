@@ -362,7 +362,8 @@ int attn_cache_append(const attn_cache_append_args* args, void* stream);
  * starts[batch] are left as they were; so are rows of a request beyond max_new
  * (n counts them all the same).  out must not overlap q.  Scales must be
  * positive; V scales and the codes of tokens held must be finite numbers, |v|
- * below 2^100.  For many rows values are held in f16 relative to the largest V
+ * below 2^100.  Softmax weights are rounded to f16: by at most 2^-11 of
+ * themselves, or 2^-32 of the row's largest.  For many rows values are held in f16 relative to the largest V
  * scale of the request and head: scales that are no powers of two round a value
  * once more, by at most 2^-11 of itself, and values of a block whose scale is
  * below 2^-22 of the largest keep an absolute accuracy of 2^-32 of that one

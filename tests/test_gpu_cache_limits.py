@@ -437,3 +437,32 @@ def test_a_stream_of_the_tensors_device_is_asked_for(ap):
         with pytest.raises(ValueError, match="stream"):
             call()
     assert batch.lens.tolist() == [4]
+
+
+# --------------------------------------------------------------------------- weights far below the largest
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 70])
+def test_weights_far_below_the_largest(ap, code, dim, new):
+    """The largest weight lies on values of 2^-20 of the others': what the small
+    weights add keeps the stated accuracy, 2^-32 of the largest weight each."""
+    bs, n_kv = 16, 160
+    cache, host = make_cache(ap, 10, 1, bs, dim, code, dim)
+    k, v, ks, vs = host
+    k.zero_()
+    k[:, 0, :, 0] = (-torch.arange(1.0, n_kv + 1).view(10, bs)).clamp(min=-120).to(k.dtype)
+    k[0, 0, 0, 0] = 0
+    ks.fill_(2.0 ** -2)   # scores of 0 and about -0.25, -0.5, ... -30 (weights down to 2^-43)
+    vs.fill_(1.0)
+    vs[0] = 2.0 ** -20
+    for mine, x in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), host):
+        mine.copy_(x)
+    q = torch.zeros(new, 1, dim).bfloat16()
+    q[:, 0, 0] = 1.0
+    table = [list(range(10))]
+    want, tol = ref.attend_ref(q, *host, table, [n_kv], [0, new], False, 1.0)
+    tol = tol - 2.0 ** -25 + 2.0 ** -32 * (v.double() * vs.double()[:, :, None, None]).abs().sum((0, 2))
+    out = ap.attn_cached(q.cuda(), cache, ints(table), ints([n_kv]), ints([0, new]), max_new=new,
+                         causal=False, scale=1.0)
+    off = (out.double().cpu() - want).abs() / tol
+    assert torch.all(off <= 1), f"off by {off.max():.3g} times"
